@@ -16,7 +16,7 @@ from typing import Dict, List, Sequence, Tuple
 
 import numpy as np
 
-from . import numerics
+from . import numerics, operators
 
 FLOAT = {"f16", "bf16", "f32", "f64", "f8E4M3FN", "f8E5M2"}
 INT_BITS = {"i1": 1, "i8": 8, "i16": 16, "i32": 32, "i64": 64, "ui8": 8, "ui16": 16, "ui32": 32, "ui64": 64}
@@ -519,6 +519,13 @@ def _eval_op(op: str, rest: str, env, dot_precision: str) -> Tuple[np.ndarray, s
         return normalize(np.broadcast_to(np.asarray(v), out_shape), out_dt), out_dt
     if op == "scatter":
         return _scatter(rest, env, dot_precision)
+    if op == "custom_call":
+        # `@target(%a, %b) {..., backend_config = {...}} : (types) -> types`: one of the plugin's own operators
+        target, names = re.match(r"@([\w.]+)\((.*?)\)", rest).groups()
+        vals = operators.OPERATORS[target]([env[x][0] for x in re.findall(r"%[\w.$#-]+", names)], operators.config(rest))
+        types = _types(ty[ty.rfind("->"):])
+        vals = [(normalize(np.asarray(v).reshape(shape), dt), dt) for v, (shape, dt) in zip(vals, types)]
+        return vals if len(vals) > 1 else vals[0]
     if op == "concatenate":
         # manipulation.rs:778-822: the inputs one after another along `dim`, in operand order
         head = rest.split(":")[0]

@@ -51,6 +51,8 @@ enum class Op : uint8_t {
   Reverse, Scatter,
   // contractions and reductions
   DotGeneral, Reduce,
+  // custom_call of one of the plugin's own operators (custom_call.cc)
+  CustomCall,
 };
 const char* op_name(Op op);
 bool op_is_elementwise(Op op);  // one output element depends on the same-index elements of its operands
@@ -104,6 +106,11 @@ struct Node {
   // N values folded in), its results the N new accumulated values.
   int result_index = 0;
   std::shared_ptr<const Graph> body;
+  // custom_call: the operator and its backend_config (truth values as 0 / 1). The op's results are a node each, sharing
+  // operands, `call` (one number per op) and config; `result_index` names the result.
+  std::string call_target;
+  std::map<std::string, double> config;
+  int call = -1;
   int param_index = -1;
   // constant payload: raw little-endian bytes in `type.dtype`; splat constants hold one element
   std::vector<uint8_t> literal;

@@ -341,4 +341,74 @@ struct ScatterArgs {
   int64_t win_elems;   // elements per update window
 };
 
+// ------------------------------------------------------------------------------------------------ decoding operators
+// ryft.rope_append (k_rope_append.hip): per token t and head h, y = x · rsqrt(mean(x²) + eps) · weight (with weights),
+// then with angle a_i = positions[t] · inv_freq[i], i < R / 2, the pair (y[i], y[i + R/2]) (interleaved: (y[2i],
+// y[2i + 1])) turned by a_i and scaled by `magnitude`; values from R on stay. Queries go to q_out, keys and values
+// (values as they are) to slot s = slots[t] of the caches [pages][Hkv][P][D], page s / P, row s % P; a slot outside
+// [0, pages · P) is not written.
+struct RopeAppendArgs {
+  const void* q;  // [T, Hq, D] and k, v [T, Hkv, D]: unit stride along D, 16-byte aligned rows
+  const void* k;
+  const void* v;
+  const int32_t* positions;
+  const int32_t* slots;
+  const float* inv_freq;
+  const void* q_weight;  // [D] of dtype (null: no norm)
+  const void* k_weight;
+  void* q_out;           // [T, Hq, D] row-major
+  void* k_cache;
+  void* v_cache;
+  int64_t T, pages;
+  int64_t qs[2], ks[2], vs[2];  // element strides of (token, head)
+  int32_t Hq, Hkv, D, R, P;
+  int32_t dtype;
+  int32_t interleaved;
+  float eps, magnitude;
+  int32_t pad_;
+};
+
+// ryft.paged_attention (k_paged_attention.hip): sequence b has the queries starts[b] .. starts[b+1]-1 of q [T, Hq, D],
+// its last n_b of lengths[b] positions, and key position p in row p % P of page table[b][p / P] of the caches
+// [pages][Hkv][P][D]. Query head h reads key head h / (Hq / Hkv). With s = scale · q·k, capped to softcap · tanh(s /
+// softcap) and, with slopes, s += slopes[h] · (p_k - p_q): o = Σ softmax(s) v over the visible keys: p_k < lengths[b],
+// p_k <= p_q (causal), p_q - p_k < window (window > 0), a page inside [0, pages). A query that sees no key, or belongs
+// to no sequence, gets zeros. starts are clamped to [0, T] and lengths to [0, M · P].
+struct PagedAttnArgs {
+  const void* q;        // [T, Hq, D]: unit stride along D, 16-byte aligned rows
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* table;   // [B, M]
+  const int32_t* starts;  // [B + 1]
+  const int32_t* lengths; // [B]
+  const float* slopes;    // [Hq] or null
+  void* o;                // [T, Hq, D] row-major
+  int64_t T, pages;
+  int64_t qs[2];          // element strides of (token, head)
+  int32_t B, M, Hq, Hkv, D, P;
+  int32_t dtype;
+  int32_t causal, window;
+  float scale, softcap;
+  int32_t pad_;
+};
+
+// ryft.sample (k_sample.hip): for each row of logits [B, V], in 64 bits, w_i = exp((x_i - max x) / temperature); of the
+// tokens with w_i > 0, those among the top_k largest (0: all; equal logits: the lower index first), with w_i >= min_p
+// (relative to the largest), and preceded in that order by less than top_p of the weight left so far; then token = the
+// first index whose running sum of kept weights exceeds uniform · their total, logprob = log(w / total). temperature 0
+// is the largest logit. NaN logits are never drawn; a row without any logit above -inf gives token -1, logprob -inf.
+struct SampleArgs {
+  const void* logits;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* uniform;
+  int32_t* token;
+  float* logprob;
+  int64_t B, V;
+  int32_t dtype;
+  int32_t pad_;
+};
+
 }  // namespace ryft

@@ -25,6 +25,9 @@ void launch_window(const WindowArgs& a, hipStream_t stream, hipEvent_t done = nu
 void launch_gather(const GatherArgs& a, hipStream_t stream, hipEvent_t done = nullptr);
 void launch_pack(const PackArgs& a, hipStream_t stream, hipEvent_t done = nullptr);
 void launch_scatter(const ScatterArgs& a, hipStream_t stream, hipEvent_t done = nullptr);
+void launch_rope_append(const RopeAppendArgs& a, hipStream_t stream, hipEvent_t done = nullptr);
+void launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done = nullptr);
+void launch_sample(const SampleArgs& a, hipStream_t stream, hipEvent_t done = nullptr);
 
 // Operands of these GEMM arguments (bit 0: A, 1: B, 2: B2) whose layout keeps them from the MFMA kernels (0: the
 // MFMA kernels run them as they are; -1: their element types or epilogue have no MFMA kernel whatever the layout).

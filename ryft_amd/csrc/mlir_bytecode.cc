@@ -629,6 +629,15 @@ class BytecodeParser {
          {{"indices_are_sorted", false, {BAttr::INT}},
           {"scatter_dimension_numbers", true, {BAttr::SCATTER_DIMS}},
           {"unique_indices", false, {BAttr::INT}}}},
+        {"stablehlo.custom_call",
+         {{"api_version", false, {BAttr::INT}},
+          {"backend_config", false, {BAttr::DICT, BAttr::STRING}},
+          {"call_target_name", true, {BAttr::STRING}},
+          {"called_computations", false, {BAttr::ARRAY}},
+          {"has_side_effect", false, {BAttr::INT}},
+          {"operand_layouts", false, {BAttr::ARRAY}},
+          {"output_operand_aliases", false, {BAttr::ARRAY}},
+          {"result_layouts", false, {BAttr::ARRAY}}}},
         {"stablehlo.pad", {{"edge_padding_high", true, {BAttr::DENSE_ARRAY}}, {"edge_padding_low", true, {BAttr::DENSE_ARRAY}},
                            {"interior_padding", true, {BAttr::DENSE_ARRAY}}}},
         {"stablehlo.compare",
@@ -654,6 +663,9 @@ class BytecodeParser {
     if (op == "stablehlo.dot_general") return pick({"dot_dimension_numbers", "precision_config", "algorithm"});
     if (op == "stablehlo.gather") return pick({"dimension_numbers", "slice_sizes", "indices_are_sorted"});
     if (op == "stablehlo.scatter") return pick({"scatter_dimension_numbers", "indices_are_sorted", "unique_indices"});
+    if (op == "stablehlo.custom_call")
+      return pick({"call_target_name", "has_side_effect", "backend_config", "api_version", "called_computations",
+                   "operand_layouts", "result_layouts", "output_operand_aliases"});
     // (slice and pad: three fields of one kind, so another order could not be told apart; sorted only)
     return sorted;
   }
@@ -827,15 +839,21 @@ class BytecodeParser {
     --depth_;
   }
 
-  const BOp* find_function(const BBlock& b, const std::string& entry) {
-    for (const BOp& op : b.ops) {
+  BOp* find_function(BBlock& b, const std::string& entry) {
+    for (BOp& op : b.ops) {
       if (op.name == "func.func") {
         auto it = op.attrs.find("sym_name");
         if (it != op.attrs.end() && attr(it->second).str == entry) return &op;
+        // the other property order's reading, where the first one takes another string for the name
+        it = op.alt_attrs.find("sym_name");
+        if (op.has_alt && it != op.alt_attrs.end() && attr(it->second).str == entry) {
+          op.attrs.swap(op.alt_attrs);
+          return &op;
+        }
       }
-      for (const BRegion& reg : op.regions)
-        for (const BBlock& inner : reg.blocks)
-          if (const BOp* f = find_function(inner, entry)) return f;
+      for (BRegion& reg : op.regions)
+        for (BBlock& inner : reg.blocks)
+          if (BOp* f = find_function(inner, entry)) return f;
     }
     return nullptr;
   }
@@ -966,6 +984,27 @@ class BytecodeParser {
     return g;
   }
 
+  // backend_config of a custom_call: numbers and truth values by name
+  std::map<std::string, double> call_config(const BAttr& c) {
+    if (c.kind == BAttr::TEXT) return mlir_config_text(c.str);
+    if (c.kind == BAttr::STRING) {
+      if (!c.str.empty()) invalid("custom_call: backend_config must be a dictionary (api_version 4)");
+      return {};
+    }
+    std::map<std::string, double> config;
+    for (auto& kv : c.dict) {
+      const BAttr& v = attr(kv.second);
+      double x = 0;
+      if (v.kind == BAttr::INT) x = (double)v.i;
+      else if (v.kind == BAttr::FLOAT) x = v.f;
+      else if (v.kind == BAttr::UNIT) x = 1;
+      else if (v.kind == BAttr::TEXT) x = mlir_config_text("{" + kv.first + " = " + v.str + "}").begin()->second;
+      else invalid("custom_call: backend_config value of '" + kv.first + "' is no number");
+      config[kv.first] = x;
+    }
+    return config;
+  }
+
   // The ops of one block into `g`, up to its return (whose operands become g's results).
   void build_ops(const BBlock& body, Graph& g, std::map<int64_t, int>& node_of) {
     auto add = [&](Node n) {
@@ -1018,6 +1057,23 @@ class BytecodeParser {
         const std::shared_ptr<Graph> body = build_region(op.regions[0]);
         node_of[op.results[0]] =
             mlir_inline_map(g, inputs, tensor_type(op.result_types[0]), int_list(op, "dimensions"), *body);
+        continue;
+      }
+      if (nm == "custom_call") {
+        Node n;
+        n.debug = "%" + std::to_string(g.nodes.size());
+        for (int64_t v : op.operands) n.operands.push_back(value(v));
+        std::vector<TensorType> results;
+        for (int t : op.result_types) results.push_back(tensor_type(t));
+        const BAttr* side = get(op, "has_side_effect");
+        if (side && (side->kind == BAttr::TEXT ? side->str.rfind("true", 0) == 0 : side->i != 0))
+          unimplemented("custom_call with side effects is not supported");
+        if (const BAttr* c = get(op, "backend_config")) n.config = call_config(*c);
+        std::string target = need(op, "call_target_name").str;
+        if (target.size() >= 2 && target.front() == '"' && target.back() == '"') target = target.substr(1, target.size() - 2);
+        std::vector<Node> nodes = custom_call_nodes(g, n, target, results);
+        if (op.results.size() != nodes.size()) invalid("custom_call: result count mismatch");
+        for (size_t i = 0; i < nodes.size(); ++i) node_of[op.results[i]] = add(std::move(nodes[i]));
         continue;
       }
       if (nm == "reduce") {

@@ -2,6 +2,7 @@
 // mlir_bytecode.cc): textual type / attribute forms and the node checks both apply.
 #pragma once
 
+#include <map>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -38,6 +39,12 @@ std::vector<int> mlir_select_branches(Graph& g, const std::string& nm, const std
 // map: the body's ops copied into `g` over the result's shape; returns the node of the body's result.
 int mlir_inline_map(Graph& g, const std::vector<int>& inputs, const TensorType& result, const std::vector<int64_t>& dims,
                     const Graph& body);
+// backend_config of a custom_call as text: `{eps = 1.0e-06 : f32, interleaved = false}` (numbers and truth values)
+std::map<std::string, double> mlir_config_text(const std::string& raw);
+// The nodes of one custom_call, one per result (`proto` holds the operands and the config), after the checks of the
+// operator that `target` names (custom_call.cc). Throws UNIMPLEMENTED for a target the plugin does not provide.
+std::vector<Node> custom_call_nodes(const Graph& g, const Node& proto, const std::string& target,
+                                    const std::vector<TensorType>& results);
 std::vector<Node> mlir_reduce_nodes(const Graph& g, const Node& proto, const std::vector<TensorType>& results,
                                     const std::string& applies, std::shared_ptr<const Graph> body);
 

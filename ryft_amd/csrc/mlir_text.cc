@@ -114,6 +114,7 @@ const char* op_name(Op op) {
     case Op::Iota: return "iota";
     case Op::Reverse: return "reverse";
     case Op::Scatter: return "scatter";
+    case Op::CustomCall: return "custom_call";
     case Op::BitcastConvert: return "bitcast_convert";
     case Op::ReducePrecision: return "reduce_precision";
     case Op::DotGeneral: return "dot_general";
@@ -901,6 +902,17 @@ class Parser {
       os.type = parse_fn_or_types(c_);
       return;
     }
+    if (n == "custom_call") {
+      // stablehlo.custom_call @target(%a, %b) {attributes} : (types) -> types
+      os.attrs["call_target_name"] = c_.sigil_name('@');
+      c_.expect("(");
+      operand_list();
+      c_.expect(")");
+      if (c_.try_consume("{")) parse_attr_dict(os.attrs);
+      c_.expect(":");
+      os.type = parse_fn_or_types(c_);
+      return;
+    }
     operand_list();
     // keyword attributes before the ':' (dims = [...], batching_dims = [..] x [..], precision = [...], algorithm = <...>)
     for (;;) {
@@ -1087,6 +1099,19 @@ class Parser {
         invalid("reduce: " + std::to_string(nodes.size()) + " results, " + std::to_string(os.results.size()) + " names");
       for (size_t i = 0; i < nodes.size(); ++i) names_[os.results[i]] = add(std::move(nodes[i]));
       return;
+    } else if (nm == "custom_call") {
+      std::string target = get("call_target_name");
+      if (!target.empty() && target[0] == '@') target = target.substr(1);
+      if (target.size() >= 2 && target.front() == '"' && target.back() == '"') target = target.substr(1, target.size() - 2);
+      if (get("has_side_effect").rfind("true", 0) == 0) unimplemented("custom_call with side effects is not supported");
+      n.config = mlir_config_text(get("backend_config"));
+      std::vector<TensorType> results = os.type.results;
+      if (results.empty()) results.push_back(result_type(os));
+      std::vector<Node> nodes = custom_call_nodes(graph_, n, target, results);
+      if (os.results.size() != nodes.size())
+        invalid("custom_call: " + std::to_string(nodes.size()) + " results, " + std::to_string(os.results.size()) + " names");
+      for (size_t i = 0; i < nodes.size(); ++i) names_[os.results[i]] = add(std::move(nodes[i]));
+      return;
     } else if (nm == "dot_general") {
       n.op = Op::DotGeneral;
       std::string dd = get("dot_dimension_numbers");
@@ -1262,6 +1287,65 @@ void mlir_dense_text(const std::string& text, const TensorType& tt, Node& n) {
   Cursor vc(text);
   vc.set_pos(d + 6);
   parse_dense(vc.angle_body(), tt, n);
+}
+std::map<std::string, double> mlir_config_text(const std::string& raw) {
+  std::map<std::string, double> config;
+  size_t b = 0, e = raw.size();
+  while (b < e && isspace((unsigned char)raw[b])) ++b;
+  while (e > b && isspace((unsigned char)raw[e - 1])) --e;
+  const std::string s = raw.substr(b, e - b);
+  if (s.empty() || s == "\"\"") return config;
+  if (s.size() < 2 || s.front() != '{' || s.back() != '}')
+    invalid("custom_call: backend_config must be a dictionary (api_version 4), got '" + s.substr(0, 80) + "'");
+  size_t p = 1;
+  const size_t end = s.size() - 1;
+  auto ws = [&]() { while (p < end && isspace((unsigned char)s[p])) ++p; };
+  for (ws(); p < end; ws()) {
+    std::string key, val;
+    if (s[p] == '"') {
+      for (++p; p < end && s[p] != '"'; ++p) key += s[p];
+      ++p;
+    } else {
+      for (; p < end && (isalnum((unsigned char)s[p]) || s[p] == '_' || s[p] == '.' || s[p] == '$'); ++p) key += s[p];
+    }
+    ws();
+    if (key.empty()) invalid("custom_call: malformed backend_config '" + s.substr(0, 80) + "'");
+    if (p < end && s[p] == '=') {
+      for (++p; p < end && s[p] != ','; ++p) val += s[p];
+    } else {
+      val = "true";  // a unit attribute
+    }
+    if (p < end && s[p] == ',') ++p;
+    std::string type;
+    const size_t colon = val.find(':');
+    if (colon != std::string::npos) type = val.substr(colon + 1), val = val.substr(0, colon);
+    auto trim = [](std::string& t) {
+      while (!t.empty() && isspace((unsigned char)t.front())) t.erase(t.begin());
+      while (!t.empty() && isspace((unsigned char)t.back())) t.pop_back();
+    };
+    trim(val), trim(type);
+    double x = 0;
+    if (val == "true") x = 1;
+    else if (val == "false") x = 0;
+    else {
+      char* stop = nullptr;
+      if (val.rfind("0x", 0) == 0 && (type == "f32" || type == "f64")) {  // a float that has no short decimal form
+        const uint64_t bits = strtoull(val.c_str(), &stop, 16);
+        if (type == "f64") memcpy(&x, &bits, 8);
+        else {
+          const uint32_t w = (uint32_t)bits;
+          float f;
+          memcpy(&f, &w, 4);
+          x = f;
+        }
+      } else {
+        x = strtod(val.c_str(), &stop);
+      }
+      if (val.empty() || !stop || *stop) invalid("custom_call: backend_config value '" + val + "' of '" + key + "' is no number");
+    }
+    if (!config.emplace(key, x).second) invalid("custom_call: backend_config names '" + key + "' twice");
+  }
+  return config;
 }
 CmpDir mlir_cmp_dir_text(const std::string& raw) { return Parser::parse_dir(raw); }
 CmpType mlir_cmp_type_text(const std::string& raw) { return Parser::parse_cmp_type(raw); }

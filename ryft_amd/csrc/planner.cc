@@ -176,6 +176,9 @@ class Planner {
   void emit_dynamic_slice(int node, int target);
   void emit_dynamic_update_slice(int node, int target);
   void emit_gather(int node, int target);
+  void emit_custom_call(int node, int target);
+  View row_view(int node);
+  int updated_operand(int operand, int out);
   void push_window_step(const char* name, int mode, int src, int dst, const std::vector<int>& idx,
                         const TensorType& big, const std::vector<int64_t>& win, DType idx_dtype);
   void push_strided_step(ExprBuilder& b, const char* name, int out, int64_t out_offset,
@@ -615,6 +618,9 @@ int Planner::materialize(int node, int target) {
     case Op::Scatter:
       emit_scatter(node, target);
       break;
+    case Op::CustomCall:
+      emit_custom_call(node, target);
+      break;
     case Op::Reshape: {
       int s = materialize(n.operands[0]);
       if (target >= 0) {
@@ -793,6 +799,145 @@ void Planner::emit_concatenate(int node, int target) {
   mat_[node] = out;
 }
 
+// The value that a step is about to write parts of, put into the step's result slot `out`: computed straight into it
+// only when nothing else reads it (the write would change it under its other readers); otherwise it gets a slot of its
+// own and is copied. For a parameter that is a copy, which an execution that donates it into `out` skips.
+int Planner::updated_operand(int operand, int out) {
+  if (users_[operand].size() > 1 || results_.count(operand))
+    emit_copy(materialize(operand), 0, out, g_.nodes[operand].type.bytes());
+  else materialize(operand, out);
+  return out;
+}
+
+// A [tokens, heads, head dim] operand as rows of contiguous elements at 16-byte aligned addresses: the strided view
+// where its rows are that (a slice of a fused projection), else a contiguous copy. Rows of a contiguous operand that
+// are no multiple of 16 bytes stay as they are; the kernels read those an element at a time.
+View Planner::row_view(int node) {
+  View v = view_of(node);
+  const Node& n = g_.nodes[node];
+  const auto dense = row_major_strides(n.type.shape);
+  const int64_t es = (int64_t)dtype_size(v.dtype);
+  const bool whole = v.offset == 0 && v.strides == dense;
+  const bool rows = v.strides[2] == 1 && v.offset * es % 16 == 0 && v.strides[0] * es % 16 == 0 && v.strides[1] * es % 16 == 0;
+  if (whole || rows) return v;
+  v.slot = canonical_copy(node, {0, 1, 2});
+  v.offset = 0;
+  v.strides = dense;
+  return v;
+}
+
+// One of the plugin's operators (custom_call.cc): all results of the op written by one step, each straight into the
+// buffer of the function result it is, if it is one. rope_append's caches are copied into their results first and then
+// written at their slots, so that an execution whose cache argument is donated into the result, or is the result's own
+// memory, writes the new tokens only.
+void Planner::emit_custom_call(int node, int target) {
+  const Node n = g_.nodes[node];
+  std::vector<int> res;  // the op's result nodes
+  for (size_t k = 0; k < g_.nodes.size(); ++k)
+    if (g_.nodes[k].op == Op::CustomCall && g_.nodes[k].call == n.call) res.push_back((int)k);
+  auto out_slot = [&](int i) {
+    const int r = res[i];
+    int slot = r == node ? target : -1;
+    for (size_t k = 0; k < g_.results.size() && slot < 0; ++k)
+      if (g_.results[k] == r) slot = plan_.output_slots[k];
+    if (slot < 0) slot = new_slot(Slot::TEMP, g_.nodes[r].type);
+    mat_[r] = slot;
+    return slot;
+  };
+  auto type = [&](int i) -> const TensorType& { return g_.nodes[n.operands[i]].type; };
+  auto num = [&](const char* k) { return n.config.at(k); };
+  Step st{};
+  st.name = n.call_target.substr(5);  // (after "ryft.")
+  auto read = [&](size_t field, int i) { st.patches.push_back({field, materialize(n.operands[i])}); };
+  auto read_rows = [&](size_t field, const void** ptr, int64_t* strides, int i) {
+    const View v = row_view(n.operands[i]);
+    *ptr = (const void*)(uintptr_t)(v.offset * (int64_t)dtype_size(v.dtype));
+    strides[0] = v.strides[0];
+    strides[1] = v.strides[1];
+    st.patches.push_back({field, v.slot});
+  };
+  if (n.call_target == "ryft.rope_append") {
+    st.kind = Step::ROPE_APPEND;
+    RopeAppendArgs& a = st.rope;
+    const TensorType &q = type(0), &kc = type(6);
+    a.T = q.shape[0];
+    a.Hq = (int32_t)q.shape[1];
+    a.D = (int32_t)q.shape[2];
+    a.R = (int32_t)(2 * type(5).shape[0]);
+    a.pages = kc.shape[0];
+    a.Hkv = (int32_t)kc.shape[1];
+    a.P = (int32_t)kc.shape[2];
+    a.dtype = (int32_t)q.dtype;
+    a.interleaved = num("interleaved") != 0;
+    a.eps = (float)num("eps");
+    a.magnitude = (float)num("magnitude");
+    read_rows(offsetof(RopeAppendArgs, q), &a.q, a.qs, 0);
+    read_rows(offsetof(RopeAppendArgs, k), &a.k, a.ks, 1);
+    read_rows(offsetof(RopeAppendArgs, v), &a.v, a.vs, 2);
+    read(offsetof(RopeAppendArgs, positions), 3);
+    read(offsetof(RopeAppendArgs, slots), 4);
+    read(offsetof(RopeAppendArgs, inv_freq), 5);
+    double weights = 0;
+    if (n.operands.size() == 10) {
+      read(offsetof(RopeAppendArgs, q_weight), 8);
+      read(offsetof(RopeAppendArgs, k_weight), 9);
+      weights = 2.0 * (double)type(8).bytes();
+    }
+    const int qo = out_slot(0), ko = out_slot(1), vo = out_slot(2);
+    updated_operand(n.operands[6], ko);
+    updated_operand(n.operands[7], vo);
+    st.patches.push_back({offsetof(RopeAppendArgs, q_out), qo});
+    st.patches.push_back({offsetof(RopeAppendArgs, k_cache), ko});
+    st.patches.push_back({offsetof(RopeAppendArgs, v_cache), vo});
+    st.bytes = 2.0 * (double)(q.bytes() + 2 * type(1).bytes()) + 8.0 * (double)a.T + 2.0 * a.R + weights;
+    st.flops = (double)a.T * (a.Hq + a.Hkv) * (4.0 * a.R + (weights ? 4.0 * a.D : 0.0));
+  } else if (n.call_target == "ryft.paged_attention") {
+    st.kind = Step::PAGED_ATTENTION;
+    PagedAttnArgs& a = st.paged;
+    const TensorType &q = type(0), &kc = type(1), &tab = type(3);
+    a.T = q.shape[0];
+    a.Hq = (int32_t)q.shape[1];
+    a.D = (int32_t)q.shape[2];
+    a.pages = kc.shape[0];
+    a.Hkv = (int32_t)kc.shape[1];
+    a.P = (int32_t)kc.shape[2];
+    a.B = (int32_t)tab.shape[0];
+    a.M = (int32_t)tab.shape[1];
+    a.dtype = (int32_t)q.dtype;
+    a.causal = num("causal") != 0;
+    a.window = (int32_t)num("window");
+    a.scale = (float)num("scale");
+    a.softcap = (float)num("softcap");
+    read_rows(offsetof(PagedAttnArgs, q), &a.q, a.qs, 0);
+    read(offsetof(PagedAttnArgs, k_cache), 1);
+    read(offsetof(PagedAttnArgs, v_cache), 2);
+    read(offsetof(PagedAttnArgs, table), 3);
+    read(offsetof(PagedAttnArgs, starts), 4);
+    read(offsetof(PagedAttnArgs, lengths), 5);
+    if (n.operands.size() == 7) read(offsetof(PagedAttnArgs, slopes), 6);
+    st.patches.push_back({offsetof(PagedAttnArgs, o), out_slot(0)});
+    // how many keys are read is known on the device only: the queries and the result
+    st.bytes = 2.0 * (double)q.bytes();
+  } else {
+    st.kind = Step::SAMPLE;
+    SampleArgs& a = st.sample;
+    const TensorType& x = type(0);
+    a.B = x.shape[0];
+    a.V = x.shape[1];
+    a.dtype = (int32_t)x.dtype;
+    read(offsetof(SampleArgs, logits), 0);
+    read(offsetof(SampleArgs, temperature), 1);
+    read(offsetof(SampleArgs, top_k), 2);
+    read(offsetof(SampleArgs, top_p), 3);
+    read(offsetof(SampleArgs, min_p), 4);
+    read(offsetof(SampleArgs, uniform), 5);
+    st.patches.push_back({offsetof(SampleArgs, token), out_slot(0)});
+    st.patches.push_back({offsetof(SampleArgs, logprob), out_slot(1)});
+    st.bytes = (double)x.bytes() + 28.0 * (double)a.B;
+  }
+  plan_.steps.push_back(std::move(st));
+}
+
 // One window step (kernels/k_window.hip): mode WIN_READ copies the window of `src` (a tensor of type `big`) into
 // `dst`, WIN_WRITE copies `src` into the window of `dst`; the window origin is read from the start-index slots `idx`.
 void Planner::push_window_step(const char* name, int mode, int src, int dst, const std::vector<int>& idx,
@@ -848,11 +993,7 @@ void Planner::emit_dynamic_update_slice(int node, int target) {
   for (size_t k = 2; k < n.operands.size(); ++k) idx.push_back(materialize(n.operands[k]));
   const int upd = materialize(n.operands[1]);
   const int out = temp_or(target, n.type);
-  // the operand's value is computed straight into the result only when nothing else reads it (the window write
-  // would change it under its other readers); otherwise it gets a slot of its own and is copied
-  const int xo = n.operands[0];
-  if (users_[xo].size() > 1 || results_.count(xo)) emit_copy(materialize(xo), 0, out, n.type.bytes());
-  else materialize(xo, out);
+  updated_operand(n.operands[0], out);
   const DType it = n.type.rank() ? g_.nodes[n.operands[2]].type.dtype : DType::S32;
   push_window_step("dynamic_update_slice", WIN_WRITE, upd, out, idx, n.type, un.type.shape, it);
   mat_[node] = out;
@@ -2332,6 +2473,22 @@ bool Planner::in_place(int ps, int os) const {
       if (pt.second == os) {
         if (writer >= 0 && writer != (int)i) {
           const Step& w = steps[i];
+          // attention over the updated cache only reads the result
+          if (w.kind == Step::PAGED_ATTENTION &&
+              std::all_of(w.patches.begin(), w.patches.end(), [&](const std::pair<size_t, int>& q) {
+                return q.second != ps && (q.second != os || q.first != offsetof(PagedAttnArgs, o));
+              }))
+            continue;
+          // so does a write of new tokens into a cache (rope_append) that has the result in that place alone
+          const bool append = w.kind == Step::ROPE_APPEND &&
+                              std::none_of(w.patches.begin(), w.patches.end(), [&](const std::pair<size_t, int>& q) {
+                                return q.second == ps || (q.second == os && q.first != offsetof(RopeAppendArgs, k_cache) &&
+                                                          q.first != offsetof(RopeAppendArgs, v_cache));
+                              });
+          if (append) {
+            if (windows.empty() || windows.back() != (int)i) windows.push_back((int)i);
+            continue;
+          }
           // a later window write into the result that reads neither the parameter nor the result elsewhere
           const bool window = w.kind == Step::WINDOW && w.win.mode == WIN_WRITE && w.patches[1].second == os &&
                               std::none_of(w.patches.begin(), w.patches.end(), [&](const std::pair<size_t, int>& q) {
@@ -2423,6 +2580,14 @@ std::string Plan::describe() const {
       os << " window=" << s.win.total << " of rank " << s.win.rank;
     } else if (s.kind == Step::GATHER) {
       os << " elems=" << s.gat.total << " index_vector=" << s.gat.n_map;
+    } else if (s.kind == Step::ROPE_APPEND) {
+      os << " tokens=" << s.rope.T << " heads=" << s.rope.Hq << "+" << s.rope.Hkv << " D=" << s.rope.D << " rotated=" << s.rope.R
+         << (s.rope.interleaved ? " interleaved" : "") << " page=" << s.rope.P;
+    } else if (s.kind == Step::PAGED_ATTENTION) {
+      os << " tokens=" << s.paged.T << " sequences=" << s.paged.B << " heads=" << s.paged.Hq << "/" << s.paged.Hkv
+         << " D=" << s.paged.D << " page=" << s.paged.P << " causal=" << s.paged.causal << " window=" << s.paged.window;
+    } else if (s.kind == Step::SAMPLE) {
+      os << " rows=" << s.sample.B << " vocab=" << s.sample.V;
     } else if (s.kind == Step::SCATTER) {
       os << " windows=" << s.sca.n_windows << " window_elems=" << s.sca.win_elems << " kind=" << s.sca.kind
          << (s.sca.serial ? " serial" : " parallel");

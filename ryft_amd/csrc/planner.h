@@ -18,7 +18,8 @@ struct Slot {
 };
 
 struct Step {
-  enum Kind { ELEMENTWISE, REDUCE, GEMM, ATTENTION, COPY, ROW, WINDOW, GATHER, REDUCE_BODY, SCATTER, PACK } kind;
+  enum Kind { ELEMENTWISE, REDUCE, GEMM, ATTENTION, COPY, ROW, WINDOW, GATHER, REDUCE_BODY, SCATTER, PACK,
+              ROPE_APPEND, PAGED_ATTENTION, SAMPLE } kind;
   std::string name;  // kernel family ("gemm_bf16_mfma_256x256", "attention_fwd", ...)
   std::string timing_name;  // label in kernel timings and profiles: the name, or an edge GEMM's own tile and K ranges
   EwProgram ew;
@@ -31,6 +32,9 @@ struct Step {
   ScatterArgs sca;
   ReduceBodyArgs rbody;
   PackArgs pack;
+  RopeAppendArgs rope;
+  PagedAttnArgs paged;
+  SampleArgs sample;
   struct { int64_t bytes; int64_t src_offset; } copy;  // src_offset: bytes into the source slot
   // Pointer fields inside the args block that refer to slots: (byte offset of the pointer field, slot). The
   // field's initial value is a byte offset into the slot's buffer.
@@ -49,6 +53,9 @@ struct Step {
       case SCATTER: return &sca;
       case REDUCE_BODY: return &rbody;
       case PACK: return &pack;
+      case ROPE_APPEND: return &rope;
+      case PAGED_ATTENTION: return &paged;
+      case SAMPLE: return &sample;
       default: return nullptr;
     }
   }

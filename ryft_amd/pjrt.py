@@ -1251,6 +1251,30 @@ class LoadedExecutable(_OwnedHandle, _Owned):
             results.append(ExecutionDeviceOutputs(outs, done))
         return results
 
+    def execute_into(self, inputs: Sequence[Tuple[int, int]], outputs: Sequence[Tuple[int, int]], stream: int = 0):
+        """One execution on the caller's device memory and stream (RyftMi355x_ExecuteNoAlloc, include/ryft_mi355x.h; no
+        counterpart in ryft): (device address, bytes) of every parameter and of every result, 256-byte aligned, and a
+        hipStream_t (0: the null stream). Enqueues and returns; allocates nothing. A result that the program aliases to
+        a parameter it updates in place (`tf.aliasing_output`) may have that parameter's address. Calls that overlap on
+        one GPU share its scratch memory and race."""
+        handle = self.handle
+        if not handle:
+            raise PjrtError(ErrorCode.INVALID_ARGUMENT, "the executable is null: it was destroyed with its client")
+        ni, no = len(inputs), len(outputs)
+        try:  # the arrays' types, made once for a number of arguments
+            fn, ptrs_i, sizes_i, ptrs_o, sizes_o = self._local.into[ni, no]
+        except (AttributeError, KeyError):
+            fn = self.client.plugin.lib.RyftMi355x_ExecuteNoAlloc
+            fn.restype = C.c_int
+            fn.argtypes = [_vp, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_size_t, _vp, C.c_void_p]
+            ptrs_i, sizes_i, ptrs_o, sizes_o = _vp * ni, C.c_size_t * ni, _vp * no, C.c_size_t * no
+            self._local.__dict__.setdefault("into", {})[ni, no] = (fn, ptrs_i, sizes_i, ptrs_o, sizes_o)
+        message = C.c_char_p()
+        code = fn(handle, ptrs_i(*[p for p, _ in inputs]), sizes_i(*[n for _, n in inputs]), ni,
+                  ptrs_o(*[p for p, _ in outputs]), sizes_o(*[n for _, n in outputs]), no, stream, C.byref(message))
+        if code:
+            raise PjrtError(ErrorCode(code), (message.value or b"").decode())
+
     def _prepare(self, buffers, launch_id: int, output_count: int):
         """The argument block of an execution on `buffers` (one device, every input non-donatable)."""
         n = len(buffers)

@@ -1,0 +1,437 @@
+"""The decoding operators on the GPU against the oracle in 64 bits, through PJRT_LoadedExecutable_Execute and, where
+noted, through execute_into.
+
+Tolerances. A result is rounded once to its type: half a step of it, `HALF_STEP`, relative to the value. rope_append
+computes in f32: a row's values, their norm, the cosine and the sine are each a few roundings of 2^-24 off, together
+below 2^-19 of the largest value of the row. paged_attention weighs the values by probabilities that may be rounded to
+the operands' 16-bit type (half a step of it each, in the sum and in its norm: twice that, of the largest value seen),
+and whose scores are f32 sums of D products: below D · 2^-24 · Σ|q||k| · scale, 2^-11 for the inputs here (f32: 2^-14,
+by the same count)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from oracle import operators as oo
+from oracle import stablehlo as sh
+from ryft_amd import operators, pjrt
+from tests import operator_programs as op
+from tests.helpers import run_pjrt
+
+pytestmark = pytest.mark.gpu
+
+
+def run(client, module, ins, dtypes):
+    got, exe = run_pjrt(client, module, ins)
+    return [sh.from_raw(g.view(np.uint16) if d == "f16" else g, d) for g, d in zip(got, dtypes)], exe
+
+
+def close(got, want, dtype, extra, what):
+    assert got.shape == want.shape
+    bad = ~(np.abs(got - want) <= op.HALF_STEP[dtype] * np.abs(want) + extra)
+    bad &= ~((got == want) | (np.isnan(got) & np.isnan(want)))
+    assert not bad.any(), (what, int(bad.sum()), np.argwhere(bad)[:4], got[bad][:4], want[bad][:4])
+
+
+# ------------------------------------------------------------------------------------------------ rope_append
+APPEND = [
+    # tokens, hq, hkv, d, rotated, page, pages
+    (1, 4, 2, 128, 128, 16, 2), (1, 1, 1, 64, 64, 1, 1), (37, 32, 8, 128, 128, 16, 5), (130, 5, 1, 64, 32, 64, 3),
+    (9, 12, 12, 64, 64, 48, 2), (20, 8, 4, 256, 256, 16, 3), (33, 6, 2, 80, 20, 16, 4), (17, 3, 3, 96, 96, 16, 2),
+    (5, 2, 1, 7, 6, 4, 3), (8, 4, 4, 128, 0, 16, 1), (70, 40, 2, 128, 64, 32, 3), (600, 8, 1, 64, 16, 16, 40),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("shape", APPEND, ids=str)
+def test_rope_append(gpu_client, shape, interleaved, dtype):
+    seed = sum(shape) * 2 + interleaved
+    norm = sum(shape) % 2 == 0
+    module, ins = op.append_case(*shape, dtype, norm=norm, interleaved=interleaved, start=sum(shape) * 1000,
+                                 bad_slots=shape[0] > 8, magnitude=1.25 if shape[1] % 2 else 1.0, seed=seed)
+    (q, kc, vc), _ = run(gpu_client, module, ins, [dtype] * 3)
+    x = op.values(ins)
+    wq, wk, wv = oo.rope_append(x, op.config_of(module))
+    big = lambda w: 2.0 ** -19 * np.abs(w).max(axis=-1, keepdims=True)  # noqa: E731
+    close(q, wq, dtype, big(wq), "q")
+    close(kc, wk, dtype, big(wk), "keys")
+    assert np.array_equal(vc, wv)                                     # values are stored as they are
+    untouched = np.all(wk == x[6], axis=-1)
+    assert np.array_equal(kc[untouched], x[6][untouched])             # and nothing else is written
+
+
+def test_rope_append_far_positions(gpu_client):
+    # positions up to 2^31 - 4: an f32 angle would be off by whole turns
+    module, ins = op.append_case(4, 2, 2, 64, 64, 16, 1, "f32", norm=False, interleaved=False, start=2 ** 31 - 4, seed=5)
+    (q, kc, _), _ = run(gpu_client, module, ins, ["f32"] * 3)
+    wq, wk, _ = oo.rope_append(op.values(ins), op.config_of(module))
+    close(q, wq, "f32", 2.0 ** -18, "q")
+    close(kc, wk, "f32", 2.0 ** -18, "keys")
+
+
+def test_rope_append_strided_projection(gpu_client):
+    # q, k and v as slices of one projection, read in place; and heads that a slice leaves unaligned, copied first
+    for first, width in ((0, 64), (0, 72), (3, 80)):
+        t, hq, hkv, d, pages = 11, 4, 2, 64, 2
+        r = np.random.RandomState(first + width)
+        a, q3, k3 = f"tensor<{t}x{hq + 2 * hkv}x{width}xbf16>", f"tensor<{t}x{hq}x{d}xbf16>", f"tensor<{t}x{hkv}x{d}xbf16>"
+        c, i, f = f"tensor<{pages}x{hkv}x16x{d}xbf16>", f"tensor<{t}xi32>", "tensor<32xf32>"
+        cut = "".join(f"    %{n} = stablehlo.slice %a [0:{t}, {lo}:{hi}, {first}:{first + d}] : ({a}) -> {ty}\n"
+                      for n, lo, hi, ty in (("q", 0, hq, q3), ("k", hq, hq + hkv, k3), ("v", hq + hkv, hq + 2 * hkv, k3)))
+        call = operators.rope_append("%r", [("%q", q3), ("%k", k3), ("%v", k3), ("%p", i), ("%s", i), ("%f", f), ("%kc", c), ("%vc", c)])
+        module = (f"module {{\n  func.func @main(%a: {a}, %p: {i}, %s: {i}, %f: {f}, %kc: {c}, %vc: {c}) -> ({q3}, {c}, {c}) {{\n"
+                  f"{cut}{call}    return %r#0, %r#1, %r#2 : {q3}, {c}, {c}\n  }}\n}}\n")
+        cache = (pages, hkv, 16, d)
+        ins = [op.host(r.randn(t, hq + 2 * hkv, width), "bf16"), op.host(np.arange(t), "i32"), op.host(r.permutation(32)[:t], "i32"),
+               op.host(10000.0 ** (-np.arange(32) / 32), "f32"), op.host(r.randn(*cache), "bf16"), op.host(r.randn(*cache), "bf16")]
+        (q, kc, vc), _ = run(gpu_client, module, ins, ["bf16"] * 3)
+        x = op.values(ins)
+        part = x[0][:, :, first:first + d]
+        wq, wk, wv = oo.rope_append([part[:, :hq], part[:, hq:hq + hkv], part[:, hq + hkv:], *x[1:]], op.config_of(module))
+        close(q, wq, "bf16", 2.0 ** -17, "q")
+        close(kc, wk, "bf16", 2.0 ** -17, "keys")
+        assert np.array_equal(vc, wv)
+
+
+# ------------------------------------------------------------------------------------------------ paged_attention
+ATTENTION = {
+    # new tokens and total lengths of each sequence, query / key heads, head dim, page size, options
+    "one": dict(new=[1], lengths=[1], heads=(1, 1, 64), page=16),
+    "decode": dict(new=[1] * 7, lengths=[1, 2, 63, 64, 65, 300, 129], heads=(8, 2, 128), page=16),
+    "decode_mha": dict(new=[1] * 3, lengths=[500, 17, 1000], heads=(4, 4, 64), page=32),
+    "decode_wide_group": dict(new=[1] * 3, lengths=[77, 1, 513], heads=(40, 2, 128), page=64),
+    "long": dict(new=[1], lengths=[9001], heads=(8, 1, 128), page=16),
+    "verify": dict(new=[4, 1, 8, 3], lengths=[100, 1, 8, 700], heads=(8, 2, 128), page=16),
+    "prompt": dict(new=[200, 1, 64, 65, 130], lengths=[200, 1, 64, 65, 130], heads=(4, 2, 128), page=16),
+    "prompt_64": dict(new=[257, 31], lengths=[257, 31], heads=(6, 3, 64), page=64),
+    "prompt_group5": dict(new=[150, 33], lengths=[150, 33], heads=(5, 1, 128), page=16),
+    "chunk": dict(new=[100, 7, 33], lengths=[1000, 777, 33], heads=(4, 1, 64), page=16),
+    "mixed": dict(new=[1, 140, 1, 1, 3], lengths=[900, 140, 33, 64, 500], heads=(8, 2, 128), page=16),
+    "window": dict(new=[1, 150, 4], lengths=[900, 400, 64], heads=(4, 2, 128), page=16, window=100),
+    "window_one": dict(new=[1, 40], lengths=[200, 100], heads=(2, 2, 64), page=16, window=1),
+    "softcap": dict(new=[1, 90], lengths=[300, 200], heads=(4, 2, 128), page=16, softcap=5.0, spread=2.0),
+    "slopes": dict(new=[1, 90], lengths=[300, 200], heads=(6, 2, 64), page=16, slopes=True),
+    "all": dict(new=[1, 90], lengths=[300, 200], heads=(8, 2, 128), page=32, softcap=5.0, window=130, slopes=True),
+    "not_causal": dict(new=[1, 70, 5], lengths=[300, 70, 200], heads=(4, 2, 128), page=16, causal=False),
+    "empty": dict(new=[0, 1, 0, 3], lengths=[50, 0, 0, 2], heads=(4, 2, 64), page=16, spare=3),
+    "before_the_start": dict(new=[40, 5], lengths=[10, 0], heads=(4, 2, 128), page=16),
+    "odd_pages": dict(new=[1, 60], lengths=[300, 131], heads=(4, 2, 128), page=24),
+    "page_of_one": dict(new=[1, 20], lengths=[70, 20], heads=(2, 1, 64), page=1),
+    "page_large": dict(new=[1, 20], lengths=[700, 120], heads=(4, 2, 64), page=512),
+    "bad_pages": dict(new=[1, 1, 70, 2], lengths=[300, 10, 200, 64], heads=(4, 2, 128), page=16, bad_pages=True),
+    "poison": dict(new=[1, 70, 1, 3], lengths=[301, 200, 64, 70], heads=(4, 2, 128), page=16, poison=True),
+    "poison_64": dict(new=[1, 70], lengths=[301, 201], heads=(4, 2, 64), page=64, poison=True, bad_pages=True),
+    "head_80": dict(new=[1, 30], lengths=[200, 90], heads=(4, 2, 80), page=16),
+    "head_256": dict(new=[1, 30], lengths=[200, 90], heads=(4, 2, 256), page=16, softcap=20.0),
+    "head_7": dict(new=[1, 3], lengths=[20, 9], heads=(2, 1, 7), page=4),
+}
+
+
+def attention_error(x, dtype):
+    """What rounding may do beside the result's own (see the module's docstring)."""
+    v = x[2][np.isfinite(x[2])]
+    return (2 * (op.HALF_STEP[dtype] if dtype != "f32" else 0.0) + (2.0 ** -14 if dtype == "f32" else 2.0 ** -11)) * np.abs(v).max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("name", ATTENTION)
+def test_paged_attention(gpu_client, name, dtype):
+    c = dict(ATTENTION[name])
+    new, lengths, (hq, hkv, d), page = (c.pop(k) for k in ("new", "lengths", "heads", "page"))
+    module, ins = op.attention_case(new, lengths, hq, hkv, d, page, dtype, seed=len(name), **c)
+    (got,), _ = run(gpu_client, module, ins, [dtype])
+    x = op.values(ins)
+    want, = oo.paged_attention(x, op.config_of(module))
+    assert np.isfinite(want).all()
+    close(got, want, dtype, attention_error(x, dtype), name)
+    for b, (n, length) in enumerate(zip(new, lengths)):               # rows that see nothing are exactly zero
+        start = sum(new[:b])
+        if c.get("causal", True) and length < n:
+            assert not got[start:start + n - length].any()
+    assert not got[sum(new):].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads", [(4, 2, 128), (2, 1, 64)], ids=str)
+def test_paged_attention_later_tokens_do_not_reach_back(gpu_client, heads, dtype):
+    # NaN and infinite keys and values of later tokens, and of tokens before the window, in the blocks of the visible ones
+    hq, hkv, d = heads
+    module, ins = op.attention_case([80, 3], [80, 200], hq, hkv, d, 16, dtype, window=50, seed=3)
+    x = op.values(ins)
+    kc, vc, table = x[1], x[2], x[3]
+    for c, junk in ((kc, [np.nan, np.inf]), (vc, [np.inf, np.nan])):
+        for b, p, bad in ((0, 40, 0), (0, 79, 1), (1, 140, 0)):
+            c[table[b, p // 16], :, p % 16] = junk[bad]
+    ins[1], ins[2] = op.host(kc, dtype), op.host(vc, dtype)
+    (got,), _ = run(gpu_client, module, ins, [dtype])
+    want, = oo.paged_attention(x, op.config_of(module))
+    assert np.isfinite(want[:40]).all() and np.isfinite(want[80:]).all() and np.isnan(want[40:80]).any()
+    extra = attention_error(x, dtype)
+    close(got[:40], want[:40], dtype, extra, "before")
+    close(got[80:], want[80:], dtype, extra, "other sequence")
+    assert (np.isfinite(got) == np.isfinite(want)).all()
+
+
+def test_paged_attention_large_scores(gpu_client):
+    # scores of hundreds: the softmax is one-hot or a tie, and nothing overflows
+    for new, lengths in (([1, 1], [300, 40]), ([70], [200])):
+        module, ins = op.attention_case(new, lengths, 4, 2, 128, 16, "bf16", seed=8, spread=8.0)
+        (got,), _ = run(gpu_client, module, ins, ["bf16"])
+        x = op.values(ins)
+        want, = oo.paged_attention(x, op.config_of(module))
+        # scores up to 64 · 40: their f32 sums are D · 2^-24 · Σ|q||k| · scale = 0.01 off, which a probability shows
+        close(got, want, "bf16", attention_error(x, "bf16") + 0.02 * np.abs(x[2]).max(), "large")
+
+
+def test_paged_attention_bad_starts_stay_in_bounds(gpu_client):
+    # starts and lengths outside their ranges are clamped: zeros or numbers, in rows that exist
+    module, ins = op.attention_case([2, 2, 2], [30, 20, 10], 4, 2, 64, 16, "bf16", seed=4)
+    ins[4] = op.host([-5, 2, 4, 1000], "i32")
+    ins[5] = op.host([-3, 2 ** 31 - 1, 20], "i32")
+    (got,), _ = run(gpu_client, module, ins, ["bf16"])
+    want, = oo.paged_attention(op.values(ins), op.config_of(module))
+    close(got, want, "bf16", attention_error(op.values(ins), "bf16"), "clamped")
+
+
+# ------------------------------------------------------------------------------------------------ sample
+def check_sample(client, logits, dtype, **kw):
+    args = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, uniform=0.5)
+    args.update(kw)
+    module, ins = op.sample_case(logits, dtype, **args)
+    (token, logprob), _ = run(client, module, ins, ["i32", "f32"])
+    wt, wl = oo.sample(op.values(ins), {})
+    assert np.array_equal(token, wt), (np.flatnonzero(token != wt)[:5], token[token != wt][:5], wt[token != wt][:5])
+    # one rounding to f32 of a logarithm whose weight and total are 64-bit values
+    finite = np.isfinite(wl)
+    assert np.array_equal(finite, np.isfinite(logprob))
+    assert np.all(np.abs(logprob - wl)[finite] <= 2.0 ** -23 * np.abs(wl[finite]) + 2.0 ** -30)
+    return token
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 1000, 4097, 50257, 131073])
+def test_sample(gpu_client, vocab, dtype):
+    r = np.random.RandomState(vocab)
+    rows = 12 if vocab < 60000 else 6
+    kind = np.arange(rows) % 6
+    check_sample(gpu_client, r.randn(rows, vocab) * 3, dtype, temperature=np.where(kind == 4, 0.0, r.uniform(0.4, 1.5, rows)),
+                 top_k=np.where((kind == 1) | (kind == 5), r.randint(1, 60, rows), 0),
+                 top_p=np.where((kind == 2) | (kind == 5), r.uniform(0.3, 0.99, rows), 1.0),
+                 min_p=np.where((kind == 3) | (kind == 5), r.uniform(0.01, 0.2, rows), 0.0),
+                 uniform=np.float32(r.uniform(0, 1, rows)))
+
+
+def test_sample_uniform_ends(gpu_client):
+    r = np.random.RandomState(2)
+    x = r.randn(8, 3001)
+    u = np.array([0.0, 1.0 - 2.0 ** -24, 2.0 ** -30, 0.5, 0.0, 1.0 - 2.0 ** -24, 2.0 ** -30, 0.5])
+    check_sample(gpu_client, x, "f32", uniform=u, top_p=np.repeat([1.0, 0.9], 4))
+
+
+def test_sample_ties(gpu_client):
+    # 16-bit logits tie in their hundreds: at the border of top_k and of top_p the lower indexes win
+    r = np.random.RandomState(3)
+    x = np.round(r.randn(40, 5000) * 2) / 2
+    check_sample(gpu_client, x, "bf16", top_k=np.arange(1, 41) * 37, uniform=r.uniform(0, 1, 40))
+    check_sample(gpu_client, x, "bf16", top_p=np.linspace(0.01, 0.99, 40), uniform=r.uniform(0, 1, 40))
+    check_sample(gpu_client, np.zeros((6, 777)), "f32", top_k=[0, 1, 2, 776, 777, 778], uniform=0.9999)
+    check_sample(gpu_client, np.tile([0.0, -0.0, 1.0, -1.0], (4, 100)), "f32", top_k=[150, 250, 0, 0],
+                 top_p=[1.0, 1.0, 0.6, 0.9], uniform=[0.3, 0.9, 0.5, 0.99])
+
+
+def test_sample_all_filters_together(gpu_client):
+    r = np.random.RandomState(4)
+    rows = 64
+    check_sample(gpu_client, r.randn(rows, 2048) * r.uniform(0.1, 6, (rows, 1)), "f32", temperature=r.uniform(0.2, 2, rows),
+                 top_k=r.randint(0, 2100, rows), top_p=r.uniform(0, 1.1, rows), min_p=r.uniform(0, 0.3, rows) ** 2,
+                 uniform=np.float32(r.uniform(0, 1, rows)))
+
+
+def test_sample_unusual_logits(gpu_client):
+    r = np.random.RandomState(5)
+    x = r.randn(14, 900)
+    x[0] = -np.inf                                   # nothing to draw: -1
+    x[1] = np.nan
+    x[2, ::2] = -np.inf                              # masked tokens
+    x[3, ::2] = np.nan
+    x[4, 17] = x[4, 500] = np.inf                    # an infinite logit takes all
+    x[5] = -np.inf
+    x[5, 899] = -1000.0                              # the only one
+    x[6] = 3.4e38
+    x[7] = -3.4e38
+    x[8] = np.where(np.arange(900) == 5, 3.4e38, -3.4e38)
+    x[9] *= 1e-38
+    x[10], x[11] = -np.inf, np.nan
+    x[10, 3] = x[11, 4] = 0.0
+    t = np.ones(14)
+    t[10:12] = 0.0
+    t[12], t[13] = 1e-30, 1e30
+    check_sample(gpu_client, x, "f32", temperature=t, uniform=r.uniform(0, 1, 14))
+    check_sample(gpu_client, x, "f32", temperature=t, uniform=r.uniform(0, 1, 14), top_k=20, top_p=0.7, min_p=0.1)
+
+
+def test_sample_follows_the_distribution(gpu_client):
+    # evenly spaced uniforms give every token its probability, to within one draw
+    r = np.random.RandomState(6)
+    x, n = r.randn(50) * 2, 4096
+    token = check_sample(gpu_client, np.tile(x, (n, 1)), "f32", temperature=0.8, uniform=(np.arange(n) + 0.5) / n)
+    p = np.exp(np.float32(x).astype(np.float64) / 0.8)
+    assert np.all(np.abs(np.bincount(token, minlength=50) / n - p / p.sum()) <= 1.0 / n)
+
+
+# ------------------------------------------------------------------------------------------------ repeated, captured, in place
+def device_buffers(client, ins):
+    bufs = [client.buffer(x.data, x.type, x.dims) for x in ins]
+    for b in bufs:
+        b.ready_event().await_()
+    return bufs
+
+
+def span(b):
+    return b.unsafe_pointer(), b.on_device_size_in_bytes()
+
+
+def sync():
+    lib = C.CDLL("libamdhip64.so")
+    assert lib.hipDeviceSynchronize() == 0
+
+
+CASES = {
+    "rope_append": lambda: op.append_case(37, 32, 8, 128, 128, 16, 5, "bf16", norm=True, interleaved=False, seed=1),
+    "decode": lambda: op.attention_case([1] * 5, [4000, 1, 63, 2000, 129], 16, 2, 128, 16, "bf16", seed=1),
+    "chunk": lambda: op.attention_case([100, 7, 200], [3000, 777, 200], 8, 2, 128, 16, "bf16", softcap=20.0, seed=2),
+    "sample": lambda: op.sample_case(np.random.RandomState(1).randn(5, 100000), "f32", 0.9, [0, 50, 0, 9, 0],
+                                     [1, 1, .9, .8, 1], [0, 0, 0, .05, .1], [.1, .2, .3, .4, .5]),
+}
+
+
+@pytest.mark.parametrize("name", CASES)
+def test_execute_into_gives_the_same_bits_every_time(gpu_client, name):
+    module, ins = CASES[name]()
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    bufs = device_buffers(gpu_client, ins)
+    ref = exe.execute([bufs])[0]
+    ref.done.await_()
+    want = [o.to_numpy() for o in ref.outputs]
+    outs = [gpu_client.uninitialized_buffer(o.element_type(), o.dimensions()) for o in ref.outputs]
+    for _ in range(4):
+        exe.execute_into([span(b) for b in bufs], [span(o) for o in outs])
+        sync()
+        for o, w in zip(outs, want):
+            assert np.array_equal(o.to_numpy().view(np.uint8), w.view(np.uint8))
+
+
+def test_execute_into_updates_caches_in_place(gpu_client):
+    module, ins = CASES["rope_append"]()
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    bufs = device_buffers(gpu_client, ins)
+    ref = exe.execute([bufs])[0]
+    ref.done.await_()
+    want = [o.to_numpy() for o in ref.outputs]
+    q = gpu_client.uninitialized_buffer(pjrt.BufferType.BF16, ins[0].dims)
+    exe.execute_into([span(b) for b in bufs], [span(q), span(bufs[6]), span(bufs[7])])
+    sync()
+    for got, w in zip((q, bufs[6], bufs[7]), want):
+        assert np.array_equal(got.to_numpy(), w)
+    # and through a donated argument
+    bufs = device_buffers(gpu_client, ins)
+    at = [b.unsafe_pointer() for b in bufs[6:8]]
+    bufs[6:8] = device_buffers(gpu_client, ins[6:8])
+    donated = [pjrt.ExecutionInput(b, donatable=n in (6, 7)) for n, b in enumerate(bufs)]
+    out = exe.execute([donated])[0]
+    out.done.await_()
+    for got, w in zip(out.outputs, want):
+        assert np.array_equal(got.to_numpy(), w)
+    assert bufs[6].is_deleted() and bufs[7].is_deleted() and not bufs[0].is_deleted()
+
+
+@pytest.mark.parametrize("name", ["decode", "chunk", "sample"])
+def test_replayed_from_a_graph(gpu_client, name):
+    # captured on a stream of torch's, replayed with eager work of the program's own in between
+    import torch
+    module, ins = CASES[name]()
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    bufs = device_buffers(gpu_client, ins)
+    ref = exe.execute([bufs])[0]
+    ref.done.await_()
+    want = [o.to_numpy() for o in ref.outputs]
+    outs = [gpu_client.uninitialized_buffer(o.element_type(), o.dimensions()) for o in ref.outputs]
+    other = exe.execute([bufs])[0]
+    other.done.await_()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        exe.execute_into([span(b) for b in bufs], [span(o) for o in outs], torch.cuda.current_stream().cuda_stream)
+    scratch = torch.zeros(1 << 16, device="cuda")
+    for i in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert np.array_equal(o.to_numpy().view(np.uint8), w.view(np.uint8)), i
+        scratch.add_(1.0)
+        again = exe.execute([bufs])[0]
+        again.done.await_()
+        assert all(np.array_equal(o.to_numpy(), w) for o, w in zip(again.outputs, want))
+
+
+# ------------------------------------------------------------------------------------------------ together
+def test_decoder_generates_as_the_oracle_does(gpu_client):
+    """A prompt of each of three sequences and then single tokens, through a two-layer decoder whose caches stay on the
+    device: every step's tokens and caches, given the same inputs, are the oracle's."""
+    cfg = dict(vocab=300, layers=2, d_model=128, q_heads=4, kv_heads=2, head_dim=64, ffn=192, pages=12, page_size=16,
+               pages_per_sequence=4)
+    r = np.random.RandomState(9)
+    prompts = [list(r.randint(0, 300, n)) for n in (21, 1, 9)]
+    table = r.permutation(12).reshape(3, 4)
+    weights, state = {}, None
+    history = [list(p) for p in prompts]
+    done = [0, 0, 0]
+    caches = want_caches = None
+    for step in range(3):
+        new = [p[d:] for p, d in zip(history, done)]
+        t = sum(map(len, new))
+        module, params = operators.decoder_module(tokens=t, sequences=3, **cfg)
+        positions = np.concatenate([np.arange(d, d + len(n)) for n, d in zip(new, done)])
+        seq = np.concatenate([np.full(len(n), b) for b, n in enumerate(new)])
+        small = {
+            "ids": np.concatenate(new), "positions": positions, "slots": table[seq, positions // 16] * 16 + positions % 16,
+            "table": table, "starts": np.cumsum([0] + [len(n) for n in new]), "lengths": [len(h) for h in history],
+            "last": np.cumsum([len(n) for n in new]) - 1, "temperature": [0.0, 0.8, 1.0], "top_k": [0, 20, 0],
+            "top_p": [1.0, 1.0, 0.9], "min_p": [0.0, 0.0, 0.02], "uniform": r.uniform(0, 1, 3),
+            "inv_freq": 10000.0 ** (-np.arange(32) / 32)}
+        ins = []
+        for name, shape, dt in params:
+            if name not in small and name not in weights:
+                scale = 1.0 if name == "embed" or name.endswith(("norm", "norm1", "norm2", "qw", "kw")) else shape[0] ** -0.5
+                x = 1 + 0.1 * r.randn(*shape) if len(shape) == 1 else r.randn(*shape) * scale
+                weights[name] = op.host(np.zeros(shape) if name.endswith(("_k", "_v")) else x, dt)
+            ins.append(op.host(np.asarray(small[name]).reshape(shape), dt) if name in small else weights[name])
+        names = [p[0] for p in params]
+        exe = gpu_client.compile(pjrt.Program.mlir(module))
+        bufs = device_buffers(gpu_client, ins)
+        where = [i for i, n in enumerate(names) if n.startswith("l") and n.endswith(("_k", "_v"))]
+        if caches is not None:
+            for i, c in zip(where, caches):
+                bufs[i] = c
+        vals = op.values(ins)
+        if want_caches is not None:
+            for i, c in zip(where, want_caches):
+                vals[i] = c
+        out = exe.execute([[pjrt.ExecutionInput(b, donatable=i in where) for i, b in enumerate(bufs)]])[0]
+        out.done.await_()
+        # the logits carry the rounding of two layers of bf16 activations, which moves the running sum of the kept
+        # probabilities by less than 0.1: the token lies between the oracle's for uniform numbers 0.1 less and more
+        token = sh.from_raw(out.outputs[0].to_numpy(), "i32")
+        u = vals[names.index("uniform")]
+        want = sh.evaluate(module, vals)
+        lo, hi = (sh.evaluate(module, [np.clip(u + d, 0, 1 - 2.0 ** -24) if n == "uniform" else v for n, v in zip(names, vals)])[0][0]
+                  for d in (-0.1, 0.1))
+        assert np.all((lo <= token) & (token <= hi)), (step, token, lo, hi)
+        assert token[0] == want[0][0][0]                              # the greedy one
+        caches, want_caches = out.outputs[2:], [w for w, _ in want[2:]]
+        for c, w in zip(caches, want_caches):
+            assert sh.rel_error(sh.from_raw(c.to_numpy(), "bf16"), w) < 3e-2
+        for b in range(3):
+            done[b] = len(history[b])
+            history[b].append(int(token[b]))
