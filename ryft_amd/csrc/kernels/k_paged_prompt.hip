@@ -1,0 +1,468 @@
+// ryft.paged_attention with many rows a sequence (prompts, chunks of prompts, wide groups), bf16 and f16, head dim 64 or
+// 128: a tile is 128 rows (query, head of a group) of a sequence that share a key head, 32 a wavefront; blocks of 64 keys
+// and values stream through LDS, two stages, loaded straight from the rows of the cache that the page table names.
+//
+// Scores come transposed, S = K · Qᵀ, so that a lane has one row and half its keys: the running maximum and sum take one
+// exchange between the half-waves, and the probabilities, packed, are the second operand of Oᵀ = Vᵀ · Pᵀ as they are.
+// The matrix products and the exponentials bound it (a wavefront's float instructions and matrix instructions add up):
+// the exponent reference moves only when a block exceeds it by 2^8, and masks are applied only in the blocks that need
+// one. Two workgroups share a CU, so that one's waits for LDS are the other's work.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "../common.h"
+#include "kernels.h"
+#include "launch.h"
+#include "paged_attention.h"
+#include "paged_prompt.h"
+
+namespace ryft {
+
+namespace {
+
+constexpr int BKV = 64;  // keys a block
+constexpr int kMaxParts = 16;
+
+template <int D>
+struct PromptCfg {
+  static constexpr int RB = 2 * D;              // bytes a row
+  static constexpr int KBYTES = BKV * RB;       // a block of keys (or values)
+  static constexpr int STAGE = 2 * KBYTES;
+  static constexpr int PPW = KBYTES / 4096;     // wave-wide loads of 1 KB a wavefront and tensor
+  static constexpr int PROWS = 4096 / RB;       // rows between a wavefront's consecutive loads
+  static constexpr int OP = D + 4;              // pitch of staged output rows, floats
+  static constexpr int LDS = 2 * STAGE > kPromptRows * OP * 4 ? 2 * STAGE : kPromptRows * OP * 4;
+};
+
+// LDS position of 16-byte chunk c of key row r: c ^ prompt_swz(r). Key fragments (16 rows, one chunk) need a bijection of
+// r mod 16, value fragments (4 rows, 4 chunks) the rows' quads on distinct banks.
+template <int D>
+__device__ __forceinline__ int prompt_swz(int r) {
+  if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+
+typedef __attribute__((address_space(3))) void prompt_lds;
+typedef const __attribute__((address_space(1))) void prompt_glb;
+
+// Key fragments of four k-steps for both 32-key tiles (T2: bytes from one to the other), waited for in the statement.
+template <int T2>
+__device__ __forceinline__ void prompt_read_k(u32x4p (&f)[8], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n ds_read_b128 %1, %8 offset:%12\n ds_read_b128 %2, %9\n ds_read_b128 %3, %9 offset:%12\n"
+      "ds_read_b128 %4, %10\n ds_read_b128 %5, %10 offset:%12\n ds_read_b128 %6, %11\n ds_read_b128 %7, %11 offset:%12\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7])
+      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "i"(T2)
+      : "memory");
+}
+// Transposed value fragments: two reads (keys 4 and 8 + 4 rows on) of four 32-column tiles at one k-step (head dim 128),
+// or of two at two k-steps (64).
+__device__ __forceinline__ void prompt_read_v(u32x2p (&f)[8], const uint32_t (&a)[8]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n ds_read_b64_tr_b16 %1, %9\n ds_read_b64_tr_b16 %2, %10\n ds_read_b64_tr_b16 %3, %11\n"
+      "ds_read_b64_tr_b16 %4, %12\n ds_read_b64_tr_b16 %5, %13\n ds_read_b64_tr_b16 %6, %14\n ds_read_b64_tr_b16 %7, %15\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7])
+      : "memory");
+}
+
+// GENERAL: scores may be capped or biased by distance.
+template <class X, class E, int D, bool GENERAL>
+__global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArgs A) {
+  typedef PromptCfg<D> C;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float row_ml[kPromptRows][2];
+  __shared__ PagedRowLds row_lds;
+  __shared__ uint32_t bad_rows[4];
+  __shared__ int last_word;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = A.Hq / A.Hkv;
+  const PagedScore score(A);
+
+  // rows of no sequence
+  for (int64_t t = blockIdx.x; t < A.T; t += gridDim.x) {
+    if (t >= paged_start(A, 0) && t < paged_start(A, A.B)) continue;
+    for (int64_t i = tid; i < (int64_t)A.Hq * D; i += 256) ((uint16_t*)A.o)[t * A.Hq * D + i] = 0;
+  }
+
+  // Workgroup x has range x % splits of row tile x / splits / Hkv from the end (a sequence's last tiles see most keys and
+  // come first), of key head x / splits % Hkv: with 8 key heads each XCD (x mod 8) reads one head's keys.
+  const int x = blockIdx.x;
+  const int split = A.splits > 1 ? x / A.Hkv % A.splits : 0;
+  const int want = A.splits > 1 ? x / (A.Hkv * A.splits) : x / A.Hkv;
+  PagedTile t;
+  t.hk = x % A.Hkv;
+  int sum = 0, found = -1, tiles_of = 0, s0 = 0, s1 = 0;
+  auto tiles = [&](int b) {
+    if (b >= A.B) return 0;
+    s0 = paged_start(A, b);
+    s1 = max(s0, paged_start(A, b + 1));
+    return (int)(((uint32_t)(s1 - s0) * (uint32_t)G + kPromptRows - 1) / kPromptRows);
+  };
+  // from the last sequence to the first, 64 at a time, a lane a sequence
+  for (int b1 = A.B; b1 > 0 && found < 0; b1 -= 64) {
+    const int b = b1 - 1 - lane;
+    tiles_of = b >= 0 ? tiles(b) : 0;
+    int incl = tiles_of;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(incl, off, 64);
+      if (lane >= off) incl += o;
+    }
+    const uint64_t here = __builtin_amdgcn_ballot_w64(sum + incl > want);
+    if (here) {
+      found = __builtin_ctzll(here);
+      t.b = b1 - 1 - found;
+      t.s0 = __builtin_amdgcn_readlane(s0, found);
+      t.n = __builtin_amdgcn_readlane(s1, found) - t.s0;
+      t.row0 = (sum + __builtin_amdgcn_readlane(incl, found) - 1 - want) * kPromptRows;
+    } else {
+      sum += __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  if (found < 0) return;
+  t.len = __builtin_amdgcn_readfirstlane(paged_length(A, t.b));
+  t.pos0 = t.len - t.n;
+  const int rows = min(kPromptRows, t.n * G - t.row0);
+  auto last_key = [&](int q) { return A.causal ? min(t.len - 1, t.pos0 + q) : t.len - 1; };
+  auto first_key = [&](int q) { return A.window > 0 ? (int)max((int64_t)0, (int64_t)t.pos0 + q - A.window + 1) : 0; };
+  const int q_first = __builtin_amdgcn_readfirstlane(t.row0 / G), q_last = __builtin_amdgcn_readfirstlane((t.row0 + rows - 1) / G);
+  // this range's blocks [j0, j1) of 64 keys
+  const int any_hi = last_key(q_last);
+  const int jfirst = first_key(q_first) / BKV, blocks = max(0, any_hi / BKV + (any_hi >= 0 ? 1 : 0) - jfirst);
+  const int parts = max(1, min((int)A.splits, blocks / 4));
+  if (split >= parts) return;
+  const int each = (blocks + parts - 1) / parts;
+  const int j0 = jfirst + min(blocks, split * each), j1 = jfirst + min(blocks, (split + 1) * each);
+
+  // this wavefront's rows, and this lane's
+  const int wrows = min(32, rows - 32 * wave);
+  const bool wlive = wrows > 0;
+  const int wq0 = __builtin_amdgcn_readfirstlane((t.row0 + 32 * wave) / G);
+  const int wq1 = __builtin_amdgcn_readfirstlane((t.row0 + 32 * wave + max(wrows, 1) - 1) / G);
+  const int w_all_hi = last_key(wq0), w_any_hi = last_key(wq1), w_all_lo = first_key(wq1), w_any_lo = first_key(wq0);
+  const int flat = t.row0 + min(32 * wave + (lane & 31), rows - 1), qi = flat / G, h = t.hk * G + (flat - qi * G);
+  const int pos = t.pos0 + qi, hi = last_key(qi), lo = first_key(qi);
+  const float slope = GENERAL && A.slopes ? A.slopes[h] * kLog2e : 0.f;
+  u32x4p qf[D / 16];
+  const uint16_t* const qg = (const uint16_t*)A.q + (int64_t)(t.s0 + qi) * A.qs[0] + h * A.qs[1] + 8 * half;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) qf[s] = *(const u32x4p*)(qg + 16 * s);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // (waited for inside the loop, the wait would run every iteration)
+
+  // Blocks into LDS: a wave-wide load fills 1 KB, the lane that fills chunk position c of row r takes chunk c ^ swz(r).
+  // (The swizzle depends on r mod 16, the same for all loads of a lane.)
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(prompt_lds*)smem;
+  const int r0 = (wave * 1024 + lane * 16) / C::RB;
+  const uint32_t c0 = 16 * (lane % (C::RB / 16) ^ prompt_swz<D>(r0));
+  const int32_t* const table = A.table + (int64_t)t.b * A.M;
+  int page0 = -64, entry = -1;   // entries [page0, page0 + 64) of the page table, one a lane
+  uint64_t bad = 0;              // keys of the block whose page is outside the cache
+  auto fetch = [&](int j) {
+    const int key = min(j * BKV + lane, any_hi);
+    const int pi = page_of(A, key);
+    const int p_first = __builtin_amdgcn_readlane(pi, 0), p_last = __builtin_amdgcn_readlane(pi, 63);
+    if (p_last >= page0 + 64) {
+      page0 = p_first;
+      entry = page0 + lane < A.M ? table[page0 + lane] : -1;
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // (waited for at its use, it would be waited for in every iteration)
+    }
+    const int page = __shfl(entry, pi - page0, 64);
+    const bool ok = page >= 0 && page < A.pages;
+    bad = __builtin_amdgcn_ballot_w64(!ok);
+    const uint32_t cache_row = ok ? ((uint32_t)page * A.Hkv + t.hk) * A.P + (key - pi * A.P) : 0;
+    char* const to = smem + (j & 1) * C::STAGE + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < C::PPW; ++i) {
+      const uint64_t at = (uint64_t)(uint32_t)__shfl(cache_row, r0 + i * C::PROWS, 64) * C::RB + c0;
+      __builtin_amdgcn_global_load_lds((prompt_glb*)((const char*)A.k_cache + at), (prompt_lds*)(to + i * 4096), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((prompt_glb*)((const char*)A.v_cache + at), (prompt_lds*)(to + C::KBYTES + i * 4096), 16, 0, 0);
+    }
+  };
+  auto arrived = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+  };
+
+  // key fragment: row t·32 + l % 32, chunk 2 s + l / 32: byte k_lane ^ 32 s (+ 32 rows)
+  const uint32_t k_lane = (lane & 31) * C::RB + 16 * (prompt_swz<D>(lane & 15) ^ half);
+  // value fragment: rows 16 s + vr (+ 8), chunk 4 dt + vc: byte v_lane ^ 64 dt, plus 16 s rows
+  const int vr = 4 * half + ((lane & 15) >> 2), vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const uint32_t v_lo = vr * C::RB + 16 * (vc ^ prompt_swz<D>(vr)) + 8 * (lane & 1);
+  const uint32_t v_hi = (vr + 8) * C::RB + 16 * (vc ^ prompt_swz<D>(vr + 8)) + 8 * (lane & 1);
+
+  // m: the row's exponent reference (log2), -inf until its first visible score
+  float m = -INFINITY, l = 0.f;
+  f32x16p o[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) o[d] = f32x16p{};
+
+  if (j0 < j1) fetch(j0);
+  arrived();
+  for (int j = j0; j < j1; ++j) {
+    const uint64_t bad_now = bad;
+    if (j + 1 < j1) fetch(j + 1);
+    const int kb = j * BKV;
+    // a wavefront without rows, or none of whose rows sees a key of this block, only takes part in the loads
+    if (!wlive || kb > w_any_hi || kb + BKV <= w_any_lo) {
+      arrived();
+      continue;
+    }
+    const uint32_t sk = lds0 + (j & 1) * C::STAGE, sv = sk + C::KBYTES;
+    f32x16p st[2] = {f32x16p{}, f32x16p{}};
+#pragma unroll
+    for (int s4 = 0; s4 < D / 64; ++s4) {
+      u32x4p f[8];
+      const int s = 4 * s4;
+      prompt_read_k<32 * C::RB>(f, sk + (k_lane ^ (32 * s)), sk + (k_lane ^ (32 * s + 32)), sk + (k_lane ^ (32 * s + 64)),
+                                sk + (k_lane ^ (32 * s + 96)));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) st[tt] = X::mma32(f[2 * i + tt], qf[s + i], st[tt]);
+    }
+    // exponents relative to the reference, masked; key of register r: kb + 32 tt + 8 (r / 4) + 4 half + r % 4
+    const float ref = m == -INFINITY ? 0.f : m;
+    if constexpr (GENERAL) {
+      if (score.cap2 > 0.f) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) st[tt][r] = score.capped(st[tt][r]);
+      } else {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) st[tt][r] *= score.sl2;
+      }
+      const float base = slope * (float)(kb + 4 * half - pos) - ref;
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[tt][r] += __builtin_fmaf(slope, (float)(32 * tt + 8 * (r >> 2) + (r & 3)), base);
+    } else {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[tt][r] = __builtin_fmaf(st[tt][r], score.sl2, -ref);
+    }
+    if (kb + BKV - 1 > w_all_hi || kb < w_all_lo) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kb + 4 * half + 32 * tt + 8 * (r >> 2) + (r & 3);
+          st[tt][r] = key <= hi && key >= lo ? st[tt][r] : -INFINITY;
+        }
+    }
+    if (bad_now) {
+      const uint64_t bits = bad_now >> (4 * half);
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          st[tt][r] = (uint32_t)(bits >> (32 * tt)) >> (8 * (r >> 2) + (r & 3)) & 1 ? -INFINITY : st[tt][r];
+    }
+    // The largest exponent, as signed integers over the bit patterns: in order among positive floats, and every negative
+    // one is a negative integer, so it tells whether any exceeds 8 (integer instructions run beside another wavefront's
+    // matrix instructions, float ones do not)
+    int top = (int)0x80000000u;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = max(top, (int)__float_as_uint(st[tt][r]));
+    {
+      const auto sw = __builtin_amdgcn_permlane32_swap((uint32_t)top, (uint32_t)top, false, false);
+      top = max((int)sw[0], (int)sw[1]);
+    }
+    // the reference moves when a row's block exceeds it by more than 8, or with its first visible score
+    if (__builtin_amdgcn_ballot_w64((top > (int)0x41000000) | (m == -INFINITY))) {
+      float mb = -INFINITY;
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mb = fmaxf(mb, st[tt][r]);
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mb), __float_as_uint(mb), false, false);
+      mb = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+      const bool move = (mb > 8.f) | ((m == -INFINITY) & (mb != -INFINITY));
+      const float shift = move ? mb - X::LIFT : 0.f, mn = move ? ref + shift : m;
+      const float alpha = move ? __builtin_amdgcn_exp2f(m - mn) : 1.f;  // (0 from -inf)
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[tt][r] -= shift;
+    }
+    // probabilities of 16 keys a k-step, in the accumulator's key order (16 s + 8 (e / 4) + 4 half + e % 4)
+    u32x4p pf[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = __builtin_amdgcn_exp2f(st[s >> 1][8 * (s & 1) + 2 * i]);
+        const float b = __builtin_amdgcn_exp2f(st[s >> 1][8 * (s & 1) + 2 * i + 1]);
+        pf[s][i] = X::pack(a, b);
+        l = X::sum2(pf[s][i], l);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s += 128 / D) {
+      u32x2p f[8];
+      uint32_t a[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int dt = i % (D / 32), ss = s + i / (D / 32);
+        a[2 * i] = sv + (v_lo ^ (64 * dt)) + 16 * ss * C::RB;
+        a[2 * i + 1] = sv + (v_hi ^ (64 * dt)) + 16 * ss * C::RB;
+      }
+      prompt_read_v(f, a);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int dt = i % (D / 32), ss = s + i / (D / 32);
+        o[dt] = X::mma32(u32x4p{f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y}, pf[ss], o[dt]);
+      }
+    }
+    arrived();
+  }
+
+  // rows through LDS: unnormalised outputs [128][OP], (maximum, sum) beside them
+  float* const so = (float*)smem;
+  {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    const int row = 32 * wave + (lane & 31);
+    if (half == 0) row_ml[row][0] = m, row_ml[row][1] = l;
+    if (tid < 4) bad_rows[tid] = 0;
+    bool finite = true;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const f32x4p v = {o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+        *(f32x4p*)(so + row * C::OP + 32 * d + 2 * r + 4 * half) = v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) finite &= fabsf(v[e]) < INFINITY;
+      }
+    __syncthreads();
+    if (!finite && row < rows) atomicOr(&bad_rows[wave], 1u << (lane & 31));
+    __syncthreads();
+  }
+  // A value that a row does not see has probability 0, which an infinity or NaN in it would still turn into NaN: rows with
+  // such outputs are computed again from what they see alone.
+  for (int w = 0; w < 4; ++w) {
+    uint32_t again = bad_rows[w];
+    while (again) {
+      const int row = 32 * w + __builtin_ctz(again);
+      again &= again - 1;
+      const int f = t.row0 + row, q = f / G;
+      const int k0 = max(first_key(q), j0 * BKV), k1 = min(last_key(q) + 1, j1 * BKV);
+      float rm, rl;
+      const float v = paged_row<E>(A, t.b, t.s0 + q, t.hk * G + (f - q * G), t.pos0 + q, k0, max(k1, 0), row_lds, &rm, &rl);
+      if (tid < D) so[row * C::OP + tid] = v;
+      if (tid == 0) row_ml[row][0] = rm, row_ml[row][1] = rl;
+      __syncthreads();
+    }
+  }
+  if (parts == 1) {
+    for (int i = tid; i < rows * (D / 4); i += 256) {
+      const int r = i / (D / 4), d = 4 * (i % (D / 4));
+      const float sum_r = row_ml[r][1];
+      paged_store4<X, D>(A, t, r, d, *(const f32x4p*)(so + r * C::OP + d) * (sum_r == 0.f ? 0.f : 1.f / sum_r));
+    }
+    return;
+  }
+  const __amdgpu_buffer_rsrc_t ws = paged_ws(A);
+  const int tile = want * A.Hkv + t.hk;
+  if (tile >= A.max_tiles) return;
+  constexpr uint32_t PART = kPromptRows * (D + 2) * 4;  // bytes of a part
+  const uint32_t slot = (uint32_t)(tile * A.splits + split) * PART;
+  for (int i = tid; i < rows * (D / 4); i += 256) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    agent_put4(ws, slot + (r * D + d) * 4, *(const f32x4p*)(so + r * C::OP + d));
+  }
+  for (int r = tid; r < rows; r += 256) agent_put2(ws, slot + (kPromptRows * D + 2 * r) * 4, row_ml[r][0], row_ml[r][1]);
+  if (!paged_arrive(A.counters + tile, parts, &last_word)) return;
+  // the last range to arrive joins them all: weights of the parts first, so that the loads of the rows overlap
+  const uint32_t first = (uint32_t)(tile * A.splits) * PART;
+  float(*const join_ml)[kPromptRows][2] = (float(*)[kPromptRows][2])smem;
+  for (int i = tid; i < parts * rows; i += 256) {
+    const int p = i / rows, r = i - p * rows;
+    const float2 v = agent_get2(ws, first + p * PART + (kPromptRows * D + 2 * r) * 4);
+    join_ml[p][r][0] = v.x, join_ml[p][r][1] = v.y;
+  }
+  __syncthreads();
+  for (int r = tid; r < rows; r += 256) {
+    float mt = -INFINITY, lt = 0.f;
+    for (int p = 0; p < parts; ++p) mt = fmaxf(mt, join_ml[p][r][0]);
+    const float rf = mt == -INFINITY ? 0.f : mt;
+    for (int p = 0; p < parts; ++p) {
+      const float w = __builtin_amdgcn_exp2f(join_ml[p][r][0] - rf);
+      lt = __builtin_fmaf(join_ml[p][r][1], w, lt);
+      join_ml[p][r][0] = w;
+    }
+    row_ml[r][1] = lt == 0.f ? 0.f : 1.f / lt;
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * (D / 4); i += 256) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    f32x4p v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+      const f32x4p y = agent_get4(ws, first + p * PART + (r * D + d) * 4);
+      const float w = join_ml[p][r][0];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(y[e], w, v[e]);
+    }
+    paged_store4<X, D>(A, t, r, d, v * row_ml[r][1]);
+  }
+}
+
+template <class X, class E, int D>
+void launch_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
+  constexpr int lds = PromptCfg<D>::LDS;
+  const dim3 grid((unsigned)a.groups), block(256);
+  auto go = [&](auto kernel) {
+    // (per device and kernel, so asked for at every launch: it costs no device work)
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("paged_attention LDS attribute: ") + hipGetErrorString(e));
+    launch_k(done, kernel, grid, block, lds, stream, a);
+  };
+  if (a.softcap > 0.f || a.slopes) go(paged_prompt_kernel<X, E, D, true>);
+  else go(paged_prompt_kernel<X, E, D, false>);
+}
+
+}  // namespace
+
+void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counters) {
+  const int64_t tiles = (a.T * (a.Hq / a.Hkv) / kPromptRows + a.B) * a.Hkv;
+  if (a.T * a.Hq > INT32_MAX || tiles > INT32_MAX / kMaxParts) return;
+  a.tile_rows = kPromptRows;
+  a.max_tiles = (int32_t)tiles;
+  // Ranges of keys where the tiles alone leave the chip short of two workgroups a CU. (An upper bound of the tiles:
+  // ranges that a tile has no use for end at once.)
+  a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, kMaxParts, ((int64_t)a.M * a.P + 255) / 256}));
+  a.groups = (int32_t)(tiles * a.splits);
+  if (a.splits > 1) {
+    *ws_floats = tiles * a.splits * paged_part_floats(kPromptRows, a.D);
+    *counters = tiles;
+  }
+}
+
+void launch_paged_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
+  if (a.splits > 1 && (!a.ws || !a.counters)) fail(PJRT_Error_Code_INTERNAL, "paged_attention ranges without a workspace");
+  if (a.dtype == DT_BF16) a.D == 128 ? launch_prompt<MmaBF16, ElemBF16, 128>(a, stream, done) : launch_prompt<MmaBF16, ElemBF16, 64>(a, stream, done);
+  else a.D == 128 ? launch_prompt<MmaF16, ElemF16, 128>(a, stream, done) : launch_prompt<MmaF16, ElemF16, 64>(a, stream, done);
+}
+
+}  // namespace ryft

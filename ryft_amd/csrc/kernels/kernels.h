@@ -58,5 +58,8 @@ const char* attention_kernel_name(const AttnArgs& a);
 // Number of key ranges launch_attention runs these arguments in when given a workspace of
 // B·H × ranges × Sq × (D + 2) floats and B·H zeroed counters (1: it needs neither).
 int attention_plan_splits(const AttnArgs& a);
+// Chooses the kernel of a paged_attention and its split from the sizes (the operands' pointers are not looked at):
+// floats of workspace and zeroed counters that its launch needs.
+void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counters);
 
 }  // namespace ryft

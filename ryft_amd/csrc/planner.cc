@@ -179,6 +179,8 @@ class Planner {
   void emit_custom_call(int node, int target);
   View row_view(int node);
   int updated_operand(int operand, int out);
+  int shared_workspace(int64_t bytes);
+  int shared_counters(int64_t count);
   void push_window_step(const char* name, int mode, int src, int dst, const std::vector<int>& idx,
                         const TensorType& big, const std::vector<int64_t>& win, DType idx_dtype);
   void push_strided_step(ExprBuilder& b, const char* name, int out, int64_t out_offset,
@@ -198,6 +200,7 @@ class Planner {
   std::set<int> results_;
   Plan plan_;
   std::map<int, int> mat_;  // node → slot holding it contiguously (row-major)
+  int workspace_ = -1, counters_ = -1;  // slots that the operators' steps share
 };
 
 // ------------------------------------------------------------------------------------------------ ExprBuilder
@@ -826,6 +829,22 @@ View Planner::row_view(int node) {
   return v;
 }
 
+// The workspace of the operators' steps, which run one after the other: one slot, as large as the largest needs.
+int Planner::shared_workspace(int64_t bytes) {
+  if (workspace_ < 0) workspace_ = new_slot(Slot::TEMP, TensorType{DType::U8, {0}});
+  int64_t& n = plan_.slots[workspace_].type.shape[0];
+  n = std::max(n, bytes);
+  return workspace_;
+}
+// Their arrival counters: part of the executable, zeroed once when it is loaded; each launch leaves them at zero.
+int Planner::shared_counters(int64_t count) {
+  if (counters_ < 0) counters_ = new_slot(Slot::CONSTANT, TensorType{DType::S32, {0}});
+  Slot& s = plan_.slots[counters_];
+  s.type.shape[0] = std::max(s.type.shape[0], count);
+  s.literal.assign((size_t)s.type.bytes(), 0);
+  return counters_;
+}
+
 // One of the plugin's operators (custom_call.cc): all results of the op written by one step, each straight into the
 // buffer of the function result it is, if it is one. rope_append's caches are copied into their results first and then
 // written at their slots, so that an execution whose cache argument is donated into the result, or is the result's own
@@ -916,6 +935,10 @@ void Planner::emit_custom_call(int node, int target) {
     read(offsetof(PagedAttnArgs, lengths), 5);
     if (n.operands.size() == 7) read(offsetof(PagedAttnArgs, slopes), 6);
     st.patches.push_back({offsetof(PagedAttnArgs, o), out_slot(0)});
+    int64_t ws = 0, counters = 0;
+    paged_attention_plan(a, &ws, &counters);
+    if (ws) st.patches.push_back({offsetof(PagedAttnArgs, ws), shared_workspace(4 * ws)});
+    if (counters) st.patches.push_back({offsetof(PagedAttnArgs, counters), shared_counters(counters)});
     // how many keys are read is known on the device only: the queries and the result
     st.bytes = 2.0 * (double)q.bytes();
   } else {
