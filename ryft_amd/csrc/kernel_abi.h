@@ -417,7 +417,12 @@ struct SampleArgs {
   float* logprob;
   int64_t B, V;
   int32_t dtype;
+  // set by sample_plan
+  int32_t chunks;     // workgroups a row (0: one, and no list)
+  int32_t rows;       // rows of a launch, which share the workspace
   int32_t pad_;
+  int64_t row0;       // first row of a launch
+  void* ws;           // the chunks' results; each one that is read was written by the same call
 };
 
 }  // namespace ryft

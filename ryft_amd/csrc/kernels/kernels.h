@@ -61,5 +61,7 @@ int attention_plan_splits(const AttnArgs& a);
 // Chooses the kernel of a paged_attention and its split from the sizes (the operands' pointers are not looked at):
 // floats of workspace and zeroed counters that its launch needs.
 void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counters);
+// The split of a sample: bytes of workspace that its launches need.
+void sample_plan(SampleArgs& a, int64_t* ws_bytes);
 
 }  // namespace ryft

@@ -956,6 +956,9 @@ void Planner::emit_custom_call(int node, int target) {
     read(offsetof(SampleArgs, uniform), 5);
     st.patches.push_back({offsetof(SampleArgs, token), out_slot(0)});
     st.patches.push_back({offsetof(SampleArgs, logprob), out_slot(1)});
+    int64_t ws = 0;
+    sample_plan(a, &ws);
+    if (ws) st.patches.push_back({offsetof(SampleArgs, ws), shared_workspace(ws)});
     st.bytes = (double)x.bytes() + 28.0 * (double)a.B;
   }
   plan_.steps.push_back(std::move(st));
