@@ -76,6 +76,8 @@ struct FewCfg {
   static constexpr int PIECE_ROWS = 1024 / RB;  // rows of a wave-wide load
   static constexpr int WAVE = 16384;            // bytes of LDS a wavefront
   static constexpr int OP = D + 4;              // pitch of staged output rows, floats
+  static constexpr int STAGE_ROWS = 7 * 128 / D;  // rows of all wavefronts that fit beside the blocks, with two workgroups a CU
+  static constexpr int LDS = FEW_WAVES * (WAVE + STAGE_ROWS * OP * 4);
 };
 
 // All fragments of a 16-key tile: D / 32 reads, waited for in the same statement.
@@ -106,28 +108,61 @@ __device__ __forceinline__ void few_read_v(u32x2p (&f)[8], uint32_t a0, uint32_t
       : "memory");
 }
 
+// A barrier that waits for this wavefront's LDS accesses and no others: __syncthreads would wait for the blocks on their way.
+__device__ __forceinline__ void few_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// LDS accesses while blocks are on their way: the compiler, which cannot tell their places apart, would wait for the blocks
+// before each of its own. Reads are waited for in their statement, writes by few_barrier.
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+__device__ __forceinline__ void lds_put4(uint32_t a, f32x4p v) { asm volatile("ds_write_b128 %0, %1" ::"v"(a), "v"(v) : "memory"); }
+__device__ __forceinline__ void lds_put2(uint32_t a, float x, float y) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  asm volatile("ds_write_b64 %0, %1" ::"v"(a), "v"(f2{x, y}) : "memory");
+}
+__device__ __forceinline__ void lds_put1(uint32_t a, uint32_t v) { asm volatile("ds_write_b32 %0, %1" ::"v"(a), "v"(v) : "memory"); }
+__device__ __forceinline__ uint32_t lds_get1(uint32_t a) {
+  uint32_t v;
+  asm volatile("ds_read_b32 %0, %1\n s_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(a) : "memory");
+  return v;
+}
+// (maximum, sum) and four elements of a row from each of the four wavefronts, `ml` and `o` bytes apart
+__device__ __forceinline__ void lds_get_parts(f32x4p (&v)[4], f32x2p (&w)[4], uint32_t a, uint32_t o, uint32_t b, uint32_t ml) {
+  asm volatile(
+      "ds_read_b64 %4, %12\n ds_read_b64 %5, %13\n ds_read_b64 %6, %14\n ds_read_b64 %7, %15\n"
+      "ds_read_b128 %0, %8\n ds_read_b128 %1, %9\n ds_read_b128 %2, %10\n ds_read_b128 %3, %11\n s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3])
+      : "v"(a), "v"(a + o), "v"(a + 2 * o), "v"(a + 3 * o), "v"(b), "v"(b + ml), "v"(b + 2 * ml), "v"(b + 3 * ml)
+      : "memory");
+}
+
 typedef __attribute__((address_space(3))) void few_lds;
 typedef const __attribute__((address_space(1))) void few_glb;
 
-// A value that is the same in all lanes, in scalar registers.
+// A value that is the same in all lanes, in a scalar register.
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uni(int64_t x) {
-  return (int64_t)((uint64_t)(uint32_t)uni((int)(x >> 32)) << 32 | (uint32_t)uni((int)x));
-}
-__device__ __forceinline__ int64_t lane64(int64_t x, int lane) {
-  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
-                   (uint32_t)__builtin_amdgcn_readlane((int)x, lane));
-}
 
-// What a lane knows of its sequence: how many units its tiles are together.
+// What a lane knows of its sequence: its tiles, and the units of each.
 struct FewSeq {
-  int s0, n, len, units, tiles;  // units: of one tile
-  __device__ int64_t total() const { return (int64_t)units * tiles; }
+  int s0, n, len, units, tiles;
 };
-// (a 64-bit division is some hundred instructions: taken only where it is needed)
-__device__ __forceinline__ int64_t few_div(int64_t a, int64_t b) {
-  return (a | b) >> 32 ? (int64_t)((uint64_t)a / (uint64_t)b) : (int64_t)((uint32_t)a / (uint32_t)b);
-}
+// A stretch's part of a tile: the units [u0, u1) of it.
+struct FewRange {
+  PagedTile t;
+  int rows, kfirst;       // its rows, the key that its units count from
+  int units, u0, u1;
+  int at, index;          // its first unit on the line, its number
+};
+// A part that waits to be joined: the rows' place, the workgroups [w0, w0 + parts) that have the others, its counter.
+struct FewPart {
+  PagedTile t;
+  int rows, w0, parts, index;
+};
 
 template <class X, class E, int D, int NR>
 __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const PagedAttnArgs A) {
@@ -162,81 +197,173 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
     }
     return s;
   };
-  auto scan = [&](int64_t v) {  // inclusive, over the wavefront
+  auto scan = [&](int v) {  // inclusive, over the wavefront
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int64_t o = __shfl_up(v, off, 64);
+      const int o = __shfl_up(v, off, 64);
       if (lane >= off) v += o;
     }
     return v;
   };
-  // the whole line's length, then this workgroup's stretch [at, end) of it
+  auto last_lane = [&](int v) { return __builtin_amdgcn_readlane(v, 63); };
+  // The whole line's length (paged_attention_plan keeps it below 2^30); workgroup w has [w q + min(w, r), ...) of it, a
+  // unit more where w < r, and none where the stretches would fall below the least.
   FewSeq seq = sequence(lane);
-  int64_t incl = scan(seq.total());
-  int64_t all = lane64(incl, 63);
-  for (int b0 = 64; b0 < A.B; b0 += 64) all += lane64(scan(sequence(b0 + lane).total()), 63);
-  const int64_t per = uni(max(few_div(all + W - 1, W), (int64_t)A.min_units));
-  int64_t at = (int64_t)blockIdx.x * per;
-  const int64_t end = min(all, at + per);
-  int b0 = 0;
-  int64_t before = 0;  // units of the sequences before b0
-  int64_t tiles_before = 0;
-  while (at < end) {
-    // the sequence, its tile and the unit within it (the same in every wavefront)
-    int64_t here = lane64(incl, 63);
+  int incl = scan(seq.units * seq.tiles), tiles_incl = scan(seq.tiles);
+  int all = last_lane(incl);
+  for (int b = 64; b < A.B; b += 64) {
+    const FewSeq s = sequence(b + lane);
+    all += last_lane(scan(s.units * s.tiles));
+  }
+  const int working = uni(max(1, min(W, all / A.min_units)));
+  const int q_units = uni(all / working), r_units = all - q_units * working;
+  const int w = blockIdx.x;
+  if (w >= working) return;
+  auto owner = [&](int unit) {
+    const int wide = r_units * (q_units + 1);
+    return uni(unit < wide ? unit / (q_units + 1) : r_units + (unit - wide) / q_units);
+  };
+  int at = w * q_units + min(w, r_units);
+  const int end = at + q_units + (w < r_units ? 1 : 0);
+  if (at >= end) return;
+  int b0 = 0, before = 0, tiles_before = 0;  // units and tiles of the sequences before b0
+  auto next_range = [&]() {  // (the same in every wavefront)
+    FewRange R;
+    R.rows = 0;
+    int here = last_lane(incl);
     while (at >= before + here) {
+      if (b0 + 64 >= A.B) {  // (starts that decrease: their sums may have overflowed)
+        at = end;
+        return R;
+      }
       before += here;
-      tiles_before += lane64(scan(seq.tiles), 63);
+      tiles_before += last_lane(tiles_incl);
       b0 += 64;
       seq = sequence(b0 + lane);
-      incl = scan(seq.total());
-      here = lane64(incl, 63);
+      incl = scan(seq.units * seq.tiles), tiles_incl = scan(seq.tiles);
+      here = last_lane(incl);
     }
-    const int64_t tiles_incl = scan(seq.tiles);
-    const uint64_t mine = __builtin_amdgcn_ballot_w64(before + incl > at);
-    const int who = __builtin_ctzll(mine);
-    PagedTile t;
+    PagedTile& t = R.t;
+    const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + incl > at));
     t.b = b0 + who;
     t.s0 = __builtin_amdgcn_readlane(seq.s0, who);
     t.n = __builtin_amdgcn_readlane(seq.n, who);
     t.len = __builtin_amdgcn_readlane(seq.len, who);
     t.pos0 = t.len - t.n;
-    const int units = __builtin_amdgcn_readlane(seq.units, who);
+    R.units = __builtin_amdgcn_readlane(seq.units, who);
     const int tiles = __builtin_amdgcn_readlane(seq.tiles, who);
-    const int64_t r = at - (before + lane64(incl, who) - (int64_t)tiles * units);
-    const int tile = uni((int)few_div(r, units)), u0 = (int)(r - (int64_t)tile * units);
-    const int64_t tile_index = tiles_before + lane64(tiles_incl, who) - tiles + tile;
-    const int64_t tile_at = at - u0;
-    const int u1 = (int)min((int64_t)units, u0 + (end - at));
-    at += u1 - u0;
-    t.hk = uni(tile % A.Hkv);
-    t.row0 = uni(tile / A.Hkv) * TR;
-    const int rows = (int)min((int64_t)TR, (int64_t)t.n * G - t.row0);
-    const int kfirst = A.window > 0 ? (int)max((int64_t)0, (int64_t)t.pos0 - A.window + 1) / C::KB * C::KB : 0;
+    const int r = at - (before + __builtin_amdgcn_readlane(incl, who) - tiles * R.units), tile = uni(r / R.units);
+    R.index = tiles_before + __builtin_amdgcn_readlane(tiles_incl, who) - tiles + tile;
+    R.u0 = r - tile * R.units;
+    R.u1 = min(R.units, R.u0 + (end - at));
+    R.at = at - R.u0;
+    at += R.u1 - R.u0;
+    const int group = uni(tile / A.Hkv);
+    t.hk = tile - group * A.Hkv;
+    t.row0 = group * TR;
+    R.rows = min(TR, t.n * G - t.row0);
+    R.kfirst = A.window > 0 ? (int)max((int64_t)0, (int64_t)t.pos0 - A.window + 1) / C::KB * C::KB : 0;
+    return R;
+  };
+  auto last_key = [&](const PagedTile& t, int q) { return A.causal ? min(t.len - 1, t.pos0 + q) : t.len - 1; };
+  auto first_key = [&](const PagedTile& t, int q) { return A.window > 0 ? (int)max((int64_t)0, (int64_t)t.pos0 + q - A.window + 1) : 0; };
 
+  // this wavefront's blocks of a range, first key kfirst + (4 u + wave) · KB, and what it needs to load them
+  char* const lds = smem + wave * C::WAVE;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(few_lds*)lds;
+  const int prow = lane / (C::RB / 16);
+  int kstart = 0, blocks = 0, any_hi = 0, hk = 0;
+  const int32_t* table = nullptr;
+  int page0 = -64, entry = -1;  // entries [page0, page0 + 64) of the page table, one a lane
+  uint64_t bad = 0;             // keys of the block whose page is outside the cache
+  uint32_t row[8];              // cache row of each of the lane's eight loads
+  auto locate = [&](int kb) {   // (the lane of key kb + lane)
+    const int key = min(kb + (lane & (C::KB - 1)), any_hi);
+    const int pi = page_of(A, key);
+    const int p_first = __builtin_amdgcn_readlane(pi, 0), p_last = __builtin_amdgcn_readlane(pi, C::KB - 1);
+    if (p_last >= page0 + 64) {
+      page0 = p_first;
+      entry = page0 + lane < A.M ? table[page0 + lane] : -1;
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // (waited for at its use, it would be waited for in every iteration)
+    }
+    const int page = __shfl(entry, pi - page0, 64);
+    const bool ok = page >= 0 && page < A.pages;
+    bad = __builtin_amdgcn_ballot_w64(!ok);
+    const uint32_t cache_row = ok ? ((uint32_t)page * A.Hkv + hk) * A.P + (key - pi * A.P) : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row[i] = __shfl(cache_row, i * C::PIECE_ROWS + prow, 64);
+  };
+  // Eight wave-wide loads of 1 KB; the lane that fills chunk position c of row r takes chunk c ^ few_swz(r).
+  auto fetch = [&](const void* cache, int to) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * C::PIECE_ROWS + prow, c = lane % (C::RB / 16) ^ few_swz<D>(r);
+      const char* const src = (const char*)cache + (uint64_t)row[i] * C::RB + 16 * c;
+      __builtin_amdgcn_global_load_lds((few_glb*)src, (few_lds*)(lds + to + i * 1024), 16, 0, 0);
+    }
+  };
+  // A range's queries, then its first block on its way: everything that was loaded before has arrived when it returns.
+  auto begin = [&](const FewRange& R, u32x4p (&qn)[NR][D / 32]) {
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+      const int r = 16 * k + l16, flat = R.t.row0 + r, qi = flat / G, h = R.t.hk * G + (flat - qi * G);
+      const uint16_t* const qg = (const uint16_t*)A.q + (int64_t)(R.t.s0 + qi) * A.qs[0] + h * A.qs[1] + 8 * g16;
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) qn[k][s] = r < R.rows ? *(const u32x4p*)(qg + 32 * s) : u32x4p{0, 0, 0, 0};
+    }
+    hk = R.t.hk;
+    table = A.table + (int64_t)R.t.b * A.M;
+    page0 = -64;
+    any_hi = last_key(R.t, uni((R.t.row0 + R.rows - 1) / G));
+    const int64_t first = (int64_t)R.kfirst + (int64_t)R.u0 * C::UNIT + wave * C::KB;
+    const int64_t limit = min((int64_t)any_hi + 1, (int64_t)R.kfirst + (int64_t)R.u1 * C::UNIT);
+    blocks = limit > first ? (int)((limit - first + C::UNIT - 1) / C::UNIT) : 0;
+    kstart = (int)first;
+    if (blocks > 0) locate(kstart);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    // (the queries pass through a statement, or they would be waited for at their use, in every iteration)
+#pragma unroll
+    for (int k = 0; k < NR; ++k)
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) asm volatile("" : "+v"(qn[k][s]));
+    if (blocks > 0) {
+      fetch(A.k_cache, 0);
+      fetch(A.v_cache, 8192);
+    }
+  };
+  uint32_t ka[D / 32];
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) ka[s] = lds0 + l16 * C::RB + 16 * ((4 * s + g16) ^ few_swz<D>(l16));
+  const int vrow = 4 * g16 + (l16 >> 2), vc = (l16 & 3) >> 1;
+  const uint32_t va = lds0 + 8192 + vrow * C::RB + 8 * (l16 & 1);
+  const int vsw = few_swz<D>(vrow);
+
+  FewPart part[2];
+  int parts = 0;
+  u32x4p qf[NR][D / 32];
+  FewRange R = next_range();
+  if (R.rows <= 0) return;
+  begin(R, qf);
+  while (true) {
+    const PagedTile t = R.t;
+    const int rows = R.rows;
     // this lane's rows: one a 16-row tile
     int lo[NR], hi[NR], pos[NR];
     float slope[NR];
-    u32x4p qf[NR][D / 32];
 #pragma unroll
     for (int k = 0; k < NR; ++k) {
-      const int row = 16 * k + l16, flat = t.row0 + row, qi = flat / G, h = t.hk * G + (flat - qi * G);
-      const bool live = row < rows;
+      const int r = 16 * k + l16, flat = t.row0 + r, qi = flat / G;
       pos[k] = t.pos0 + qi;
-      hi[k] = live ? (A.causal ? min(t.len - 1, pos[k]) : t.len - 1) : -1;
-      lo[k] = A.window > 0 ? (int)max((int64_t)0, (int64_t)pos[k] - A.window + 1) : 0;
-      slope[k] = A.slopes && live ? A.slopes[h] * kLog2e : 0.f;
-      const uint16_t* const qg = (const uint16_t*)A.q + (int64_t)(t.s0 + qi) * A.qs[0] + h * A.qs[1] + 8 * g16;
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) qf[k][s] = live ? *(const u32x4p*)(qg + 32 * s) : u32x4p{0, 0, 0, 0};
+      hi[k] = r < rows ? last_key(t, qi) : -1;
+      lo[k] = first_key(t, qi);
+      slope[k] = 0.f;
+      if (A.slopes) {
+        slope[k] = A.slopes[r < rows ? t.hk * G + (flat - qi * G) : 0] * kLog2e;
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+      }
     }
-    // the keys that every row sees, and those that any does
-    const int q_first = uni(t.row0 / G), q_last = uni((t.row0 + rows - 1) / G);
-    const int all_hi = A.causal ? min(t.len - 1, t.pos0 + q_first) : t.len - 1;
-    const int any_hi = A.causal ? min(t.len - 1, t.pos0 + q_last) : t.len - 1;
-    const int all_lo = A.window > 0 ? (int)max((int64_t)0, (int64_t)t.pos0 + q_last - A.window + 1) : 0;
-
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // the queries: waited for inside the loop, the wait would run every iteration
+    // the keys that every row sees
+    const int all_hi = last_key(t, uni(t.row0 / G)), all_lo = first_key(t, uni((t.row0 + rows - 1) / G));
 
     float m[NR], l[NR];
     f32x4p o[NR][D / 16];
@@ -247,59 +374,8 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       for (int d = 0; d < D / 16; ++d) o[k][d] = f32x4p{0.f, 0.f, 0.f, 0.f};
     }
 
-    // blocks of this wavefront: first key kfirst + (4 u + wave) · KB
-    const int64_t kstart = (int64_t)kfirst + (int64_t)u0 * C::UNIT + wave * C::KB;
-    const int64_t klimit = min((int64_t)any_hi + 1, (int64_t)kfirst + (int64_t)u1 * C::UNIT);
-    const int blocks = klimit > kstart ? (int)((klimit - kstart + C::UNIT - 1) / C::UNIT) : 0;
-
-    char* const lds = smem + wave * C::WAVE;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(few_lds*)lds;
-    // entries [page0, page0 + 64) of the page table, one a lane
-    const int32_t* const table = A.table + (int64_t)t.b * A.M;
-    int page0 = -64, entry = -1;
-    uint64_t bad = 0;             // keys of the block whose page is outside the cache
-    uint32_t row[8];              // cache row of each of the lane's eight loads
-    const int prow = lane / (C::RB / 16);
-    auto locate = [&](int kb) {   // (the lane of key kb + lane)
-      const int key = min(kb + (lane & (C::KB - 1)), any_hi);
-      const int pi = page_of(A, key);
-      const int p_first = __builtin_amdgcn_readlane(pi, 0), p_last = __builtin_amdgcn_readlane(pi, C::KB - 1);
-      if (p_last >= page0 + 64) {
-        page0 = p_first;
-        entry = page0 + lane < A.M ? table[page0 + lane] : -1;
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // (waited for at its use, it would be waited for in every iteration)
-      }
-      const int page = __shfl(entry, pi - page0, 64);
-      const bool ok = page >= 0 && page < A.pages;
-      bad = __builtin_amdgcn_ballot_w64(!ok);
-      const uint32_t cache_row = ok ? ((uint32_t)page * A.Hkv + t.hk) * A.P + (key - pi * A.P) : 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) row[i] = __shfl(cache_row, i * C::PIECE_ROWS + prow, 64);
-    };
-    // Eight wave-wide loads of 1 KB; the lane that fills chunk position c of row r takes chunk c ^ few_swz(r). (r of a
-    // load: a multiple of 16 of rows, or 4, 8 or 12 more.)
-    auto fetch = [&](const void* cache, int to) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * C::PIECE_ROWS + prow, c = lane % (C::RB / 16) ^ few_swz<D>(r);
-        const char* const src = (const char*)cache + (uint64_t)row[i] * C::RB + 16 * c;
-        __builtin_amdgcn_global_load_lds((few_glb*)src, (few_lds*)(lds + to + i * 1024), 16, 0, 0);
-      }
-    };
-    uint32_t ka[D / 32];
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) ka[s] = lds0 + l16 * C::RB + 16 * ((4 * s + g16) ^ few_swz<D>(l16));
-    const int vrow = 4 * g16 + (l16 >> 2), vc = (l16 & 3) >> 1;
-    const uint32_t va = lds0 + 8192 + vrow * C::RB + 8 * (l16 & 1);
-    const int vsw = few_swz<D>(vrow);
-
-    if (blocks > 0) {
-      locate((int)kstart);
-      fetch(A.k_cache, 0);
-      fetch(A.v_cache, 8192);
-    }
     for (int j = 0; j < blocks; ++j) {
-      const int kb = (int)kstart + j * C::UNIT;
+      const int kb = kstart + j * C::UNIT;
       const bool more = j + 1 < blocks;
       const uint64_t bad_now = bad;
       asm volatile("" ::: "memory");
@@ -413,101 +489,136 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       if (more) fetch(A.v_cache, 8192);
     }
 
-    // join the wavefronts, 16 rows at a time: staged outputs [wave][16][OP], then the joined rows [16][OP] in place of the
-    // first wavefront's
-    const bool whole = u0 == 0 && u1 == units;
+    // The next range's first block is on its way before the wavefronts join this one's rows, where the rows fit beside the
+    // ring: waiting for each other, for the workspace and for that block one after the other took as long as two blocks.
+    const bool early = rows <= C::STAGE_ROWS;
+    bool more_ranges = at < end;
+    const FewRange cur = R;
+    u32x4p qn[NR][D / 32];
+    if (more_ranges) {
+      R = next_range();
+      more_ranges = R.rows > 0;
+    }
+    if (NR == 1 && early && more_ranges) begin(R, qn);
+    // 16 rows at a time: staged outputs [wave][rows][OP], summed by all threads
+    const bool whole = cur.u0 == 0 && cur.u1 == cur.units;
     const __amdgpu_buffer_rsrc_t ws = paged_ws(A);
-    const uint32_t slot = 2 * blockIdx.x + (u0 == 0 ? 1 : 0);
-    const uint32_t slot_byte = slot * (uint32_t)paged_part_floats(TR, D) * 4;
-    float* const so = (float*)smem;
+    const uint32_t slot_byte = (2 * (uint32_t)w + (cur.u0 == 0 ? 1 : 0)) * (uint32_t)paged_part_floats(TR, D) * 4;
+    float* const so = (float*)(NR == 1 && early ? smem + FEW_WAVES * C::WAVE : smem);
 #pragma unroll
     for (int k = 0; k < NR; ++k) l[k] = sum_rows16(l[k]);
-    __syncthreads();
-    if (tid == 0) bad_rows = 0;
+    few_barrier();
+    if (tid == 0) lds_put1(lds_at(&bad_rows), 0);
 #pragma unroll
     for (int k = 0; k < NR; ++k)
-      if (g16 == 0) part_ml[wave][16 * k + l16][0] = m[k], part_ml[wave][16 * k + l16][1] = l[k];
+      if (g16 == 0) lds_put2(lds_at(part_ml[wave][16 * k + l16]), m[k], l[k]);
 #pragma unroll
     for (int k = 0; k < NR; ++k) {
       if (16 * k >= rows) break;
-      float* const mine_o = so + (wave * 16 + l16) * C::OP + 4 * g16;
+      const int n = min(16, rows - 16 * k);
+      if (l16 < n) {
+        const uint32_t mine_o = lds_at(so + (wave * n + l16) * C::OP + 4 * g16);
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) *(f32x4p*)(mine_o + 16 * d) = o[k][d];
-      __syncthreads();
+        for (int d = 0; d < D / 16; ++d) lds_put4(mine_o + 64 * d, o[k][d]);
+      }
+      few_barrier();
       f32x4p x[D / 64];
       float mt[D / 64], lt[D / 64];
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
         const int idx = tid + 256 * i, r = idx / (D / 4), d = 4 * (idx % (D / 4));
         float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-        for (int w = 0; w < FEW_WAVES; ++w) mm = fmaxf(mm, part_ml[w][16 * k + r][0]);
-        const float ref = mm == -INFINITY ? 0.f : mm;
         f32x4p v = {0.f, 0.f, 0.f, 0.f};
+        if (r < n) {
+          f32x4p y[4];
+          f32x2p ml[4];
+          lds_get_parts(y, ml, lds_at(so + r * C::OP + d), n * C::OP * 4, lds_at(part_ml[0][16 * k + r]), sizeof(part_ml[0]));
 #pragma unroll
-        for (int w = 0; w < FEW_WAVES; ++w) {
-          const float f = __builtin_amdgcn_exp2f(part_ml[w][16 * k + r][0] - ref);
-          ll = __builtin_fmaf(part_ml[w][16 * k + r][1], f, ll);
-          const f32x4p y = *(const f32x4p*)(so + (w * 16 + r) * C::OP + d);
+          for (int u = 0; u < FEW_WAVES; ++u) mm = fmaxf(mm, ml[u].x);
+          const float ref = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(y[e], f, v[e]);
+          for (int u = 0; u < FEW_WAVES; ++u) {
+            const float f = __builtin_amdgcn_exp2f(ml[u].x - ref);
+            ll = __builtin_fmaf(ml[u].y, f, ll);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(y[u][e], f, v[e]);
+          }
+          bool finite = true;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) finite &= fabsf(v[e]) < INFINITY;
+          if (!finite) asm volatile("ds_or_b32 %0, %1" ::"v"(lds_at(&bad_rows)), "v"(1u << r) : "memory");
         }
         x[i] = v, mt[i] = mm, lt[i] = ll;
-        const bool finite = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))) < INFINITY &&
-                            !(v.x != v.x) && !(v.y != v.y) && !(v.z != v.z) && !(v.w != v.w);
-        if (!finite && 16 * k + r < rows) atomicOr(&bad_rows, 1u << r);
       }
-      __syncthreads();
+      few_barrier();
       // A value that a row does not see has probability 0, which an infinity or NaN in it would still turn into NaN:
       // rows with such outputs are computed again from what they see alone.
-      uint32_t again = bad_rows;
+      uint32_t again = uni((int)lds_get1(lds_at(&bad_rows)));
       while (again) {
         const int r = __builtin_ctz(again);
         again &= again - 1;
-        const int flat = t.row0 + 16 * k + r, qi = flat / G, p = t.pos0 + qi;
-        const int64_t first = max((int64_t)kfirst + (int64_t)u0 * C::UNIT, A.window > 0 ? (int64_t)p - A.window + 1 : 0);
-        const int64_t last = min((int64_t)kfirst + (int64_t)u1 * C::UNIT, (int64_t)(A.causal ? min(t.len, p + 1) : t.len));
+        const int flat = t.row0 + 16 * k + r, qi = flat / G;
+        const int64_t first = max((int64_t)cur.kfirst + (int64_t)cur.u0 * C::UNIT, (int64_t)first_key(t, qi));
+        const int64_t last = min((int64_t)cur.kfirst + (int64_t)cur.u1 * C::UNIT, (int64_t)last_key(t, qi) + 1);
         float rm, rl;
-        const float v = paged_row<E>(A, t.b, t.s0 + qi, t.hk * G + (flat - qi * G), p, (int)max(first, (int64_t)0), (int)max(last, (int64_t)0),
-                                     *(PagedRowLds*)smem, &rm, &rl);
-        __syncthreads();
-        if (tid < D) so[tid] = v;
+        const float v = paged_row<E>(A, t.b, t.s0 + qi, t.hk * G + (flat - qi * G), t.pos0 + qi, (int)first, (int)max(last, (int64_t)0),
+                                     *(PagedRowLds*)so, &rm, &rl);
+        float* const one = so + sizeof(PagedRowLds) / 4;
+        if (tid < D) one[tid] = v;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
           const int idx = tid + 256 * i, d = 4 * (idx % (D / 4));
-          if (idx / (D / 4) == r) x[i] = *(const f32x4p*)(so + d), mt[i] = rm, lt[i] = rl;
+          if (idx / (D / 4) == r) x[i] = *(const f32x4p*)(one + d), mt[i] = rm, lt[i] = rl;
         }
         __syncthreads();
-        if (tid == 0) bad_rows = 0;
+        if (tid == 0) lds_put1(lds_at(&bad_rows), 0);
       }
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
-        const int idx = tid + 256 * i, r = 16 * k + idx / (D / 4), d = 4 * (idx % (D / 4));
-        if (r < rows) {
+        const int idx = tid + 256 * i, r = idx / (D / 4), d = 4 * (idx % (D / 4)), rk = 16 * k + r;
+        if (r < n) {
           if (whole) {
-            paged_store4<X, D>(A, t, r, d, x[i] * (lt[i] == 0.f ? 0.f : 1.f / lt[i]));
+            paged_store4<X, D>(A, t, rk, d, x[i] * (lt[i] == 0.f ? 0.f : 1.f / lt[i]));
           } else {
-            agent_put4(ws, slot_byte + (r * D + d) * 4, x[i]);
-            if (d == 0) agent_put2(ws, slot_byte + (TR * D + 2 * r) * 4, mt[i], lt[i]);
+            agent_put4(ws, slot_byte + (rk * D + d) * 4, x[i]);
+            if (d == 0) agent_put2(ws, slot_byte + (TR * D + 2 * rk) * 4, mt[i], lt[i]);
           }
         }
       }
-      __syncthreads();
+      few_barrier();
     }
-    if (!whole && tile_index < A.max_tiles) {
-      // the workgroups of this tile's parts: the first has it from its beginning, the others in their first slot
-      const int w0 = uni((int)few_div(tile_at, per)), w1 = uni((int)few_div(tile_at + units - 1, per)), parts = w1 - w0 + 1;
-      if (paged_arrive(A.counters + tile_index, parts, &last_word))
-        paged_join<X, D, TR>(A, t, rows, parts, [&](int i) { return 2 * (w0 + i) + (i == 0 ? 1 : 0); }, so);
-      __syncthreads();
+    if (!whole && cur.index < A.max_tiles) {
+      // (its first range and its last: no workgroup has more parts than two)
+      const int w0 = owner(cur.at), w1 = owner(cur.at + cur.units - 1);
+      const FewPart P{t, rows, w0, w1 - w0 + 1, cur.index};
+      if (parts == 0) part[0] = P;
+      else part[1] = P;
+      ++parts;
     }
+    if (!more_ranges) break;
+    if (NR == 1 && early) {
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) qf[0][s] = qn[0][s];
+    } else {
+      begin(R, qf);
+    }
+  }
+  // The workgroup of a tile that arrives last joins its parts: the first workgroup has it from its beginning, the others in
+  // their first slot.
+  for (int p = 0; p < parts; ++p) {
+    const FewPart P = p == 0 ? part[0] : part[1];
+    if (paged_arrive(A.counters + P.index, P.parts, &last_word))
+      paged_join<X, D, TR>(A, P.t, P.rows, P.parts, [&](int i) { return 2 * (P.w0 + i) + (i == 0 ? 1 : 0); }, (float*)smem);
+    __syncthreads();
   }
 }
 
 template <class X, class E, int D, int NR>
 void launch_few(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
-  constexpr int lds = FEW_WAVES * FewCfg<D>::WAVE;
+  constexpr int lds = FewCfg<D>::LDS;
+  const hipError_t e = hipFuncSetAttribute((const void*)paged_attention_few_kernel<X, E, D, NR>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("paged_attention LDS attribute: ") + hipGetErrorString(e));
   launch_k(done, paged_attention_few_kernel<X, E, D, NR>, dim3((unsigned)a.groups), dim3(256), lds, stream, a);
 }
 
@@ -538,7 +649,8 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
   const int unit = a.D == 128 ? 128 : 256;
   a.min_units = 512 / unit;
   const int64_t tiles = (a.T * G / a.tile_rows + a.B) * a.Hkv;
-  if (a.T * a.Hq > INT32_MAX || tiles > INT32_MAX) { a.tile_rows = 0; return; }
+  // (units are counted in 32 bits)
+  if (a.T * a.Hq > INT32_MAX || tiles > (1 << 30) / ((int64_t)a.M * a.P / unit + 1)) { a.tile_rows = 0; return; }
   a.max_tiles = (int32_t)tiles;
   // two workgroups a CU, fewer if even the longest sequences have no work for them
   const int64_t most = tiles * (((int64_t)a.M * a.P + 511) / 512 + 1);

@@ -9,6 +9,7 @@ namespace ryft {
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef float f32x4p __attribute__((ext_vector_type(4)));
+typedef float f32x2p __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2p __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4p __attribute__((ext_vector_type(4)));
 typedef float f32x16p __attribute__((__vector_size__(16 * sizeof(float))));
@@ -229,11 +230,11 @@ __device__ __forceinline__ void paged_store4(const PagedAttnArgs& A, const Paged
 }
 
 // Joins the partial results of a tile's `parts` ranges (slot(i): the workspace slot of range i) into its output rows.
-// Maxima and sums of 32 ranges at a time come to LDS first (`sh`: 2 · 32 · ROWS floats), so that the loads of the rows
-// depend on nothing and overlap.
+// Maxima and sums of as many ranges as LDS holds (`sh`: 64 KB) come there first, so that the loads of the rows depend on
+// nothing: 16 of a thread's are in flight (112 parts of 8 rows × 128: 40 us with 8 in flight and 32 ranges at a time).
 template <class E, int D, int ROWS, class F>
 __device__ __forceinline__ void paged_join(const PagedAttnArgs& A, const PagedTile& t, int rows, int parts, F&& slot, float* sh) {
-  constexpr int CH = 32;
+  constexpr int CH = 8192 / ROWS;
   const __amdgpu_buffer_rsrc_t ws = paged_ws(A);
   const int tid = threadIdx.x;
   const uint32_t part_bytes = (uint32_t)paged_part_floats(ROWS, D) * 4;
@@ -262,7 +263,7 @@ __device__ __forceinline__ void paged_join(const PagedAttnArgs& A, const PagedTi
       m[k] = mn;
       l[k] *= alpha;
       o[k] *= alpha;
-#pragma unroll 8
+#pragma unroll 16
       for (int p = 0; p < np; ++p) {
         const f32x4p v = agent_get4(ws, (uint32_t)slot(p0 + p) * part_bytes + (r * D + d) * 4);
         const float w = __builtin_amdgcn_exp2f(sh[2 * (p * ROWS + r)] - ref);
