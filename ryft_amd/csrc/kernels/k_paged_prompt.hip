@@ -70,6 +70,29 @@ __device__ __forceinline__ void prompt_read_v(u32x2p (&f)[8], const uint32_t (&a
       : "memory");
 }
 
+// Sums and maxima over the wavefront in scalar registers (DPP, no LDS), and an inclusive scan.
+template <int CTRL, int MASK>
+__device__ __forceinline__ int dpp_int(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, MASK, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_int<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += dpp_int<0x112, 0xf>(v);
+  v += dpp_int<0x114, 0xf>(v);
+  v += dpp_int<0x118, 0xf>(v);
+  v += dpp_int<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
+  v += dpp_int<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+__device__ __forceinline__ int wave_max(int v) {  // (of values of at least 0)
+  v = max(v, dpp_int<0x111, 0xf>(v));
+  v = max(v, dpp_int<0x112, 0xf>(v));
+  v = max(v, dpp_int<0x114, 0xf>(v));
+  v = max(v, dpp_int<0x118, 0xf>(v));
+  v = max(v, dpp_int<0x142, 0xa>(v));
+  v = max(v, dpp_int<0x143, 0xc>(v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 // GENERAL: scores may be capped or biased by distance.
 template <class X, class E, int D, bool GENERAL>
 __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArgs A) {
@@ -83,6 +106,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = A.Hq / A.Hkv;
   const PagedScore score(A);
+  const float cap_scale = A.softcap > 0.f ? A.scale / A.softcap : 0.f;
 
   // rows of no sequence
   for (int64_t t = blockIdx.x; t < A.T; t += gridDim.x) {
@@ -90,42 +114,73 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     for (int64_t i = tid; i < (int64_t)A.Hq * D; i += 256) ((uint16_t*)A.o)[t * A.Hq * D + i] = 0;
   }
 
-  // Workgroup x has range x % splits of row tile x / splits / Hkv from the end (a sequence's last tiles see most keys and
-  // come first), of key head x / splits % Hkv: with 8 key heads each XCD (x mod 8) reads one head's keys.
+  // Workgroup x has range x / Hkv % splits of row tile x / Hkv / splits, of key head x % Hkv: with 8 key heads each XCD
+  // (x mod 8) reads one head's keys. Row tiles are taken in falling order of the blocks of keys they see, over all
+  // sequences, so that the chip does not wait for long ones that began late (four causal prompts of 875 to 1824 tokens:
+  // the last workgroup ended 26% after the mean). The place in that order is found without a sort: a sequence a lane, the
+  // number of blocks that as many tiles reach by bisection, then the tile among those of that number.
   const int x = blockIdx.x;
   const int split = A.splits > 1 ? x / A.Hkv % A.splits : 0;
   const int want = A.splits > 1 ? x / (A.Hkv * A.splits) : x / A.Hkv;
   PagedTile t;
   t.hk = x % A.Hkv;
-  int sum = 0, found = -1, tiles_of = 0, s0 = 0, s1 = 0;
-  auto tiles = [&](int b) {
-    if (b >= A.B) return 0;
-    s0 = paged_start(A, b);
-    s1 = max(s0, paged_start(A, b + 1));
-    return (int)(((uint32_t)(s1 - s0) * (uint32_t)G + kPromptRows - 1) / kPromptRows);
+  int s0 = 0, n = 0, len = 0, tiles = 0;
+  auto sequence = [&](int b) {
+    s0 = 0, n = 0, len = 0;
+    if (b >= 0 && b < A.B) {
+      s0 = paged_start(A, b);
+      n = max(0, paged_start(A, b + 1) - s0);
+      len = paged_length(A, b);
+    }
+    tiles = (int)(((uint32_t)n * (uint32_t)G + kPromptRows - 1) / kPromptRows);
   };
-  // from the last sequence to the first, 64 at a time, a lane a sequence
-  for (int b1 = A.B; b1 > 0 && found < 0; b1 -= 64) {
-    const int b = b1 - 1 - lane;
-    tiles_of = b >= 0 ? tiles(b) : 0;
-    int incl = tiles_of;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += o;
+  if (A.B <= 64) {
+    sequence(lane);
+    // blocks of a tile: to its last query's key, at most those of a window and the tile's own queries
+    const int most = A.window > 0 ? A.window / BKV + kPromptRows / G / BKV + 2 : INT32_MAX;
+    const int all = A.causal ? 0 : tiles;  // (not causal: every tile sees all)
+    auto reach = [&](int c) {  // tiles that see c blocks or more
+      if (c > most) return 0;
+      if (!A.causal) return (len + BKV - 1) / BKV >= c ? all : 0;
+      const int q = BKV * (c - 1) - (len - n);  // the first query that does
+      if (q <= 0) return tiles;
+      return q >= n ? 0 : tiles - (int)(((uint32_t)G * q + kPromptRows) / kPromptRows) + 1;
+    };
+    if (want >= wave_total(tiles)) return;
+    int lo = 0, hi = wave_max(min((len + BKV - 1) / BKV, most)) + 1;  // more than `want` tiles see lo blocks, not more see hi
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (wave_total(reach(mid)) > want) lo = mid;
+      else hi = mid;
     }
-    const uint64_t here = __builtin_amdgcn_ballot_w64(sum + incl > want);
-    if (here) {
-      found = __builtin_ctzll(here);
-      t.b = b1 - 1 - found;
-      t.s0 = __builtin_amdgcn_readlane(s0, found);
-      t.n = __builtin_amdgcn_readlane(s1, found) - t.s0;
-      t.row0 = (sum + __builtin_amdgcn_readlane(incl, found) - 1 - want) * kPromptRows;
-    } else {
-      sum += __builtin_amdgcn_readlane(incl, 63);
+    const int above = reach(hi), equal = reach(lo) - above;
+    const int incl = wave_scan(equal), rest = want - wave_total(above);
+    const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > rest));
+    t.b = who;
+    t.s0 = __builtin_amdgcn_readlane(s0, who);
+    t.n = __builtin_amdgcn_readlane(n, who);
+    // (the last `above` tiles of a sequence see more, the `equal` before those as many)
+    const int tile = __builtin_amdgcn_readlane(tiles - above - equal + rest - (incl - equal), who);
+    t.row0 = tile * kPromptRows;
+  } else {
+    // from the last sequence to the first, 64 at a time, each from its last tile
+    int sum = 0, found = -1;
+    for (int b1 = A.B; b1 > 0 && found < 0; b1 -= 64) {
+      sequence(b1 - 1 - lane);
+      const int incl = wave_scan(tiles);
+      const uint64_t here = __builtin_amdgcn_ballot_w64(sum + incl > want);
+      if (here) {
+        found = __builtin_ctzll(here);
+        t.b = b1 - 1 - found;
+        t.s0 = __builtin_amdgcn_readlane(s0, found);
+        t.n = __builtin_amdgcn_readlane(n, found);
+        t.row0 = (sum + __builtin_amdgcn_readlane(incl, found) - 1 - want) * kPromptRows;
+      } else {
+        sum += __builtin_amdgcn_readlane(incl, 63);
+      }
     }
+    if (found < 0) return;
   }
-  if (found < 0) return;
   t.len = __builtin_amdgcn_readfirstlane(paged_length(A, t.b));
   t.pos0 = t.len - t.n;
   const int rows = min(kPromptRows, t.n * G - t.row0);
@@ -149,11 +204,6 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
   const int flat = t.row0 + min(32 * wave + (lane & 31), rows - 1), qi = flat / G, h = t.hk * G + (flat - qi * G);
   const int pos = t.pos0 + qi, hi = last_key(qi), lo = first_key(qi);
   const float slope = GENERAL && A.slopes ? A.slopes[h] * kLog2e : 0.f;
-  u32x4p qf[D / 16];
-  const uint16_t* const qg = (const uint16_t*)A.q + (int64_t)(t.s0 + qi) * A.qs[0] + h * A.qs[1] + 8 * half;
-#pragma unroll
-  for (int s = 0; s < D / 16; ++s) qf[s] = *(const u32x4p*)(qg + 16 * s);
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // (waited for inside the loop, the wait would run every iteration)
 
   // Blocks into LDS: a wave-wide load fills 1 KB, the lane that fills chunk position c of row r takes chunk c ^ swz(r).
   // (The swizzle depends on r mod 16, the same for all loads of a lane.)
@@ -204,7 +254,14 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
   for (int d = 0; d < D / 32; ++d) o[d] = f32x16p{};
 
   if (j0 < j1) fetch(j0);
+  u32x4p qf[D / 16];
+  const uint16_t* const qg = (const uint16_t*)A.q + (int64_t)(t.s0 + qi) * A.qs[0] + h * A.qs[1] + 8 * half;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) qf[s] = *(const u32x4p*)(qg + 16 * s);
   arrived();
+  // (they pass through a statement here, or they would be waited for at their use, in every iteration)
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) asm volatile("" : "+v"(qf[s]));
   for (int j = j0; j < j1; ++j) {
     const uint64_t bad_now = bad;
     if (j + 1 < j1) fetch(j + 1);
@@ -230,22 +287,45 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     // exponents relative to the reference, masked; key of register r: kb + 32 tt + 8 (r / 4) + 4 half + r % 4
     const float ref = m == -INFINITY ? 0.f : m;
     if constexpr (GENERAL) {
-      if (score.cap2 > 0.f) {
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) st[tt][r] = score.capped(st[tt][r]);
-      } else {
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) st[tt][r] *= score.sl2;
-      }
       const float base = slope * (float)(kb + 4 * half - pos) - ref;
+      auto scores = [&](auto&& bias) {  // (the last operation of every form adds the bias: none costs one for it)
+        if (!(score.cap2 > 0.f)) {
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
+          for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st[tt][r] += __builtin_fmaf(slope, (float)(32 * tt + 8 * (r >> 2) + (r & 3)), base);
+            for (int r = 0; r < 16; ++r) st[tt][r] = __builtin_fmaf(st[tt][r], score.sl2, bias(tt, r));
+          return;
+        }
+        // tanh z = z P(z²) to 2^-25 for |z| <= 1/2, a polynomial that interpolates at Chebyshev nodes: 28 cycles a score
+        // instead of 48, in the blocks where no score reaches half the cap (four prompts of up to 2048 tokens 136 -> 120 us)
+        float top = 0.f;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[tt][r]));
+        if (__builtin_amdgcn_ballot_w64(!(top * fabsf(cap_scale) <= 0.5f))) {
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float e = __builtin_amdgcn_exp2f(st[tt][r] * score.capz);
+              st[tt][r] = __builtin_fmaf(-2.f * score.cap2, __builtin_amdgcn_rcpf(e + 1.f), score.cap2 + bias(tt, r));
+            }
+        } else {
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float z = st[tt][r] * cap_scale, zz = z * z;
+              float p = __builtin_fmaf(zz, 0x1.18d7e8p-6f, -0x1.b2167ep-5f);
+              p = __builtin_fmaf(zz, p, 0x1.10e47ap-3f);
+              p = __builtin_fmaf(zz, p, -0x1.5554a6p-2f);
+              st[tt][r] = __builtin_fmaf(__builtin_fmaf(zz, p, 1.f), z * score.cap2, bias(tt, r));
+            }
+        }
+      };
+      if (A.slopes) scores([&](int tt, int r) { return __builtin_fmaf(slope, (float)(32 * tt + 8 * (r >> 2) + (r & 3)), base); });
+      else scores([&](int, int) { return -ref; });
     } else {
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
@@ -375,10 +455,15 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     }
   }
   if (parts == 1) {
-    for (int i = tid; i < rows * (D / 4); i += 256) {
-      const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    // (a row is a query and a head of the group; the thread's next one is 1024 / D on: no division a row)
+    constexpr int STEP = 1024 / D;
+    const int d = 4 * (tid % (D / 4)), dq = STEP / G, dg = STEP - dq * G;
+    int q = (t.row0 + tid / (D / 4)) / G, g = t.row0 + tid / (D / 4) - q * G;
+    for (int r = tid / (D / 4); r < rows; r += STEP) {
       const float sum_r = row_ml[r][1];
-      paged_store4<X, D>(A, t, r, d, *(const f32x4p*)(so + r * C::OP + d) * (sum_r == 0.f ? 0.f : 1.f / sum_r));
+      paged_put4<X>(A, D, t.s0 + q, t.hk * G + g, d, *(const f32x4p*)(so + r * C::OP + d) * (sum_r == 0.f ? 0.f : 1.f / sum_r));
+      q += dq, g += dg;
+      if (g >= G) g -= G, ++q;
     }
     return;
   }
@@ -449,7 +534,8 @@ void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counters) 
   if (a.T * a.Hq > INT32_MAX || tiles > INT32_MAX / kMaxParts) return;
   a.tile_rows = kPromptRows;
   a.max_tiles = (int32_t)tiles;
-  // Ranges of keys where the tiles alone leave the chip short of two workgroups a CU. (An upper bound of the tiles:
+  // Ranges of keys where the tiles alone leave the chip short of two workgroups a CU (80 tiles of head dim 64: 42 us in 6
+  // ranges, 50 in 9, which run one after the other). (An upper bound of the tiles:
   // ranges that a tile has no use for end at once.)
   a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, kMaxParts, ((int64_t)a.M * a.P + 255) / 256}));
   a.groups = (int32_t)(tiles * a.splits);

@@ -222,11 +222,14 @@ __device__ __forceinline__ bool paged_arrive(int32_t* counter, int parts, int* l
 __host__ __device__ inline int64_t paged_part_floats(int rows, int D) { return (int64_t)rows * (D + 2); }
 
 // Four elements of a finished row.
+template <class E>
+__device__ __forceinline__ void paged_put4(const PagedAttnArgs& A, int D, int64_t token, int head, int d, f32x4p v) {
+  *(u32x2p*)((uint16_t*)A.o + (token * A.Hq + head) * D + d) = u32x2p{E::pack(v.x, v.y), E::pack(v.z, v.w)};
+}
 template <class E, int D>
 __device__ __forceinline__ void paged_store4(const PagedAttnArgs& A, const PagedTile& t, int row, int d, f32x4p v) {
   const int G = A.Hq / A.Hkv, flat = t.row0 + row, q = flat / G, g = flat - q * G;
-  uint16_t* const o = (uint16_t*)A.o + ((int64_t)(t.s0 + q) * A.Hq + t.hk * G + g) * D + d;
-  *(u32x2p*)o = u32x2p{E::pack(v.x, v.y), E::pack(v.z, v.w)};
+  paged_put4<E>(A, D, t.s0 + q, t.hk * G + g, d, v);
 }
 
 // Joins the partial results of a tile's `parts` ranges (slot(i): the workspace slot of range i) into its output rows.
