@@ -644,7 +644,7 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
   if (a.pages * a.Hkv * a.P > (int64_t)UINT32_MAX || (a.qs[0] | a.qs[1]) & 7) return;
   const int G = a.Hq / a.Hkv;
   const double rows = (double)a.T * G / a.B;  // rows a sequence has of a key head, on average
-  if (rows > 32) return paged_prompt_plan(a, ws_floats, counters);
+  if (rows > 32) return paged_prompt_plan(a, ws_floats);
   a.tile_rows = rows > 16 ? 32 : 16;
   const int unit = a.D == 128 ? 128 : 256;
   a.min_units = 512 / unit;

@@ -23,7 +23,12 @@ namespace ryft {
 namespace {
 
 constexpr int BKV = 64;  // keys a block
-constexpr int kMaxParts = 16;
+constexpr int kRanges = 512;  // workgroups where tiles are cut into ranges of keys: two a CU
+
+// The workspace of a launch with ranges: the parts (workgroup slots of kPromptRows rows), {ranges, tiles}, and for each
+// tile {first token of its sequence, first flat row, rows, parts}.
+__host__ __device__ inline int64_t prompt_part(int D) { return paged_part_floats(kPromptRows, D); }
+__device__ __forceinline__ int32_t* prompt_head(const PagedAttnArgs& A, int D) { return (int32_t*)(A.ws + (int64_t)kRanges * prompt_part(D)); }
 
 template <int D>
 struct PromptCfg {
@@ -101,7 +106,6 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
   __shared__ float row_ml[kPromptRows][2];
   __shared__ PagedRowLds row_lds;
   __shared__ uint32_t bad_rows[4];
-  __shared__ int last_word;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = A.Hq / A.Hkv;
@@ -120,8 +124,6 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
   // the last workgroup ended 26% after the mean). The place in that order is found without a sort: a sequence a lane, the
   // number of blocks that as many tiles reach by bisection, then the tile among those of that number.
   const int x = blockIdx.x;
-  const int split = A.splits > 1 ? x / A.Hkv % A.splits : 0;
-  const int want = A.splits > 1 ? x / (A.Hkv * A.splits) : x / A.Hkv;
   PagedTile t;
   t.hk = x % A.Hkv;
   int s0 = 0, n = 0, len = 0, tiles = 0;
@@ -134,8 +136,31 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     }
     tiles = (int)(((uint32_t)n * (uint32_t)G + kPromptRows - 1) / kPromptRows);
   };
+  sequence(lane);
+  int splits = 1;
+  if (A.splits > 1) {
+    int total = wave_total(tiles);
+    for (int b = 64; b < A.B; b += 64) {
+      sequence(b + lane);
+      total += wave_total(tiles);
+    }
+    splits = max(1, min((int)A.splits, kRanges / max(1, total * A.Hkv)));
+    if (x == 0 && tid == 0) {
+      int32_t* const head = prompt_head(A, D);
+      head[0] = splits, head[1] = max(0, min(total * A.Hkv, kRanges));
+    }
+    if (A.B > 64) sequence(lane);
+  }
+  const int split = splits > 1 ? x / A.Hkv % splits : 0;
+  const int want = splits > 1 ? x / (A.Hkv * splits) : x / A.Hkv;
+  const int tile_no = want * A.Hkv + t.hk;
+  auto describe = [&](int rows, int parts) {  // for the join
+    if (A.splits > 1 && split == 0 && tid == 0 && tile_no < kRanges) {
+      int32_t* const at = prompt_head(A, D) + 4 + 4 * tile_no;
+      at[0] = t.s0, at[1] = t.row0, at[2] = rows, at[3] = parts;
+    }
+  };
   if (A.B <= 64) {
-    sequence(lane);
     // blocks of a tile: to its last query's key, at most those of a window and the tile's own queries
     const int most = A.window > 0 ? A.window / BKV + kPromptRows / G / BKV + 2 : INT32_MAX;
     const int all = A.causal ? 0 : tiles;  // (not causal: every tile sees all)
@@ -179,7 +204,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
         sum += __builtin_amdgcn_readlane(incl, 63);
       }
     }
-    if (found < 0) return;
+    if (found < 0) return describe(0, 0);
   }
   t.len = __builtin_amdgcn_readfirstlane(paged_length(A, t.b));
   t.pos0 = t.len - t.n;
@@ -190,7 +215,8 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
   // this range's blocks [j0, j1) of 64 keys
   const int any_hi = last_key(q_last);
   const int jfirst = first_key(q_first) / BKV, blocks = max(0, any_hi / BKV + (any_hi >= 0 ? 1 : 0) - jfirst);
-  const int parts = max(1, min((int)A.splits, blocks / 4));
+  const int parts = max(1, min(splits, blocks / 4));
+  describe(rows, parts);
   if (split >= parts) return;
   const int each = (blocks + parts - 1) / parts;
   const int j0 = jfirst + min(blocks, split * each), j1 = jfirst + min(blocks, (split + 1) * each);
@@ -467,50 +493,79 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     }
     return;
   }
-  const __amdgpu_buffer_rsrc_t ws = paged_ws(A);
-  const int tile = want * A.Hkv + t.hk;
-  if (tile >= A.max_tiles) return;
-  constexpr uint32_t PART = kPromptRows * (D + 2) * 4;  // bytes of a part
-  const uint32_t slot = (uint32_t)(tile * A.splits + split) * PART;
+  const int slot = tile_no * splits + split;
+  if (slot >= kRanges) return;  // (starts that decrease)
+  float* const part = A.ws + (int64_t)slot * prompt_part(D);
   for (int i = tid; i < rows * (D / 4); i += 256) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
-    agent_put4(ws, slot + (r * D + d) * 4, *(const f32x4p*)(so + r * C::OP + d));
+    *(f32x4p*)(part + r * D + d) = *(const f32x4p*)(so + r * C::OP + d);
   }
-  for (int r = tid; r < rows; r += 256) agent_put2(ws, slot + (kPromptRows * D + 2 * r) * 4, row_ml[r][0], row_ml[r][1]);
-  if (!paged_arrive(A.counters + tile, parts, &last_word)) return;
-  // the last range to arrive joins them all: weights of the parts first, so that the loads of the rows overlap
-  const uint32_t first = (uint32_t)(tile * A.splits) * PART;
-  float(*const join_ml)[kPromptRows][2] = (float(*)[kPromptRows][2])smem;
-  for (int i = tid; i < parts * rows; i += 256) {
-    const int p = i / rows, r = i - p * rows;
-    const float2 v = agent_get2(ws, first + p * PART + (kPromptRows * D + 2 * r) * 4);
-    join_ml[p][r][0] = v.x, join_ml[p][r][1] = v.y;
-  }
-  __syncthreads();
-  for (int r = tid; r < rows; r += 256) {
-    float mt = -INFINITY, lt = 0.f;
-    for (int p = 0; p < parts; ++p) mt = fmaxf(mt, join_ml[p][r][0]);
-    const float rf = mt == -INFINITY ? 0.f : mt;
-    for (int p = 0; p < parts; ++p) {
-      const float w = __builtin_amdgcn_exp2f(join_ml[p][r][0] - rf);
-      lt = __builtin_fmaf(join_ml[p][r][1], w, lt);
-      join_ml[p][r][0] = w;
-    }
-    row_ml[r][1] = lt == 0.f ? 0.f : 1.f / lt;
-  }
-  __syncthreads();
-  for (int i = tid; i < rows * (D / 4); i += 256) {
-    const int r = i / (D / 4), d = 4 * (i % (D / 4));
-    f32x4p v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      const f32x4p y = agent_get4(ws, first + p * PART + (r * D + d) * 4);
-      const float w = join_ml[p][r][0];
+  for (int r = tid; r < rows; r += 256) *(f32x2p*)(part + kPromptRows * D + 2 * r) = f32x2p{row_ml[r][0], row_ml[r][1]};
+}
+
+// Joins the parts of every tile: four elements of a row a thread, or of a quarter of its parts (PG = 4). In a launch of its
+// own: joined by the range that arrived last, 16 parts of 128 rows took one workgroup 25 us.
+template <class X, int D, int PG>
+__global__ void __launch_bounds__(256) paged_prompt_join_kernel(const PagedAttnArgs A) {
+  constexpr int ITEMS = 256 / PG, CHUNKS = kPromptRows * D / 4 / ITEMS, U = 8;
+  __shared__ f32x4p join_o[PG][ITEMS];
+  __shared__ f32x2p join_ml[PG][ITEMS];
+  const int tid = threadIdx.x, tile = blockIdx.x / CHUNKS, item = blockIdx.x % CHUNKS * ITEMS + tid % ITEMS, pg = tid / ITEMS;
+  const int r = item / (D / 4), d = 4 * (item % (D / 4));
+  const int32_t* const head = prompt_head(A, D);
+  const int splits = head[0], tiles = head[1];
+  PagedTile t;
+  t.hk = tile % A.Hkv;
+  t.s0 = head[4 + 4 * tile], t.row0 = head[5 + 4 * tile];
+  const int rows = head[6 + 4 * tile], parts = head[7 + 4 * tile];
+  if (splits < 2 || tile >= tiles || parts < 2 || (tile + 1) * splits > kRanges) return;
+  float m = -INFINITY, l = 0.f;
+  f32x4p o = {0.f, 0.f, 0.f, 0.f};
+  if (r < rows) {
+    const float* const first = A.ws + (int64_t)tile * splits * prompt_part(D);
+    for (int p0 = pg; p0 < parts; p0 += PG * U) {
+      f32x4p v[U];
+      f32x2p w[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(y[e], w, v[e]);
+      for (int u = 0; u < U; ++u) {
+        const float* const part = first + (int64_t)min(p0 + PG * u, parts - 1) * prompt_part(D);
+        v[u] = *(const f32x4p*)(part + r * D + d);
+        w[u] = *(const f32x2p*)(part + kPromptRows * D + 2 * r);
+        if (p0 + PG * u >= parts) w[u].x = -INFINITY, v[u] = f32x4p{0.f, 0.f, 0.f, 0.f};
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, w[u].x);
+      const float ref = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - ref);
+      m = mn, l *= alpha, o *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float f = __builtin_amdgcn_exp2f(w[u].x - ref);
+        l = __builtin_fmaf(w[u].y, f, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[u][e], f, o[e]);
+      }
     }
-    paged_store4<X, D>(A, t, r, d, v * row_ml[r][1]);
   }
+  if constexpr (PG > 1) {
+    join_o[pg][tid % ITEMS] = o;
+    join_ml[pg][tid % ITEMS] = f32x2p{m, l};
+    __syncthreads();
+    if (pg) return;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < PG; ++g) mt = fmaxf(mt, join_ml[g][tid].x);
+    const float ref = mt == -INFINITY ? 0.f : mt;
+    l = 0.f, o = f32x4p{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < PG; ++g) {
+      const float f = __builtin_amdgcn_exp2f(join_ml[g][tid].x - ref);
+      l = __builtin_fmaf(join_ml[g][tid].y, f, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(join_o[g][tid][e], f, o[e]);
+    }
+  }
+  if (r < rows) paged_store4<X, D>(A, t, r, d, o * (l == 0.f ? 0.f : 1.f / l));
 }
 
 template <class X, class E, int D>
@@ -521,32 +576,33 @@ void launch_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) 
     // (per device and kernel, so asked for at every launch: it costs no device work)
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("paged_attention LDS attribute: ") + hipGetErrorString(e));
-    launch_k(done, kernel, grid, block, lds, stream, a);
+    launch_k(a.splits > 1 ? nullptr : done, kernel, grid, block, lds, stream, a);
   };
   if (a.softcap > 0.f || a.slopes) go(paged_prompt_kernel<X, E, D, true>);
   else go(paged_prompt_kernel<X, E, D, false>);
+  if (a.splits <= 1) return;
+  const unsigned tiles = (unsigned)std::min(a.max_tiles, kRanges / 2), chunks = kPromptRows * D / 4 / 256;
+  if (tiles <= 32) launch_k(done, paged_prompt_join_kernel<X, D, 4>, dim3(tiles * chunks * 4), block, 0, stream, a);
+  else launch_k(done, paged_prompt_join_kernel<X, D, 1>, dim3(tiles * chunks), block, 0, stream, a);
 }
 
 }  // namespace
 
-void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counters) {
-  const int64_t tiles = (a.T * (a.Hq / a.Hkv) / kPromptRows + a.B) * a.Hkv;
-  if (a.T * a.Hq > INT32_MAX || tiles > INT32_MAX / kMaxParts) return;
+void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats) {
+  const int64_t tiles = (a.T * (a.Hq / a.Hkv) / kPromptRows + a.B) * a.Hkv;  // (at most)
+  if (a.T * a.Hq > INT32_MAX || tiles > INT32_MAX) return;
   a.tile_rows = kPromptRows;
   a.max_tiles = (int32_t)tiles;
-  // Ranges of keys where the tiles alone leave the chip short of two workgroups a CU (80 tiles of head dim 64: 42 us in 6
-  // ranges, 50 in 9, which run one after the other). (An upper bound of the tiles:
-  // ranges that a tile has no use for end at once.)
-  a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, kMaxParts, ((int64_t)a.M * a.P + 255) / 256}));
-  a.groups = (int32_t)(tiles * a.splits);
-  if (a.splits > 1) {
-    *ws_floats = tiles * a.splits * paged_part_floats(kPromptRows, a.D);
-    *counters = tiles;
-  }
+  // Ranges of keys where the tiles alone may leave the chip short of two workgroups a CU; the kernel, which knows the
+  // tiles, chooses how many (80 tiles of head dim 64: 42 us in 6 ranges, 50 in 9, which run one after the other; one
+  // tile of 85 rows × 31072 keys of two heads: 76 us in 16 ranges, 25 in 121). Of four blocks at least.
+  a.splits = tiles <= kRanges ? (int32_t)std::max<int64_t>(1, std::min<int64_t>(kRanges, (int64_t)a.M * a.P / 256)) : 1;
+  a.groups = a.splits > 1 ? kRanges : (int32_t)tiles;
+  if (a.splits > 1) *ws_floats = kRanges * prompt_part((int)a.D) + 4 + 4 * kRanges;
 }
 
 void launch_paged_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
-  if (a.splits > 1 && (!a.ws || !a.counters)) fail(PJRT_Error_Code_INTERNAL, "paged_attention ranges without a workspace");
+  if (a.splits > 1 && !a.ws) fail(PJRT_Error_Code_INTERNAL, "paged_attention ranges without a workspace");
   if (a.dtype == DT_BF16) a.D == 128 ? launch_prompt<MmaBF16, ElemBF16, 128>(a, stream, done) : launch_prompt<MmaBF16, ElemBF16, 64>(a, stream, done);
   else a.D == 128 ? launch_prompt<MmaF16, ElemF16, 128>(a, stream, done) : launch_prompt<MmaF16, ElemF16, 64>(a, stream, done);
 }
