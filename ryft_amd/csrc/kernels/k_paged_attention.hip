@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAtt
 }
 
 // ------------------------------------------------------------------------------------------------ few rows a sequence
-// A decoding step: a tile is the 16 or 32 rows (query, head of a group) of a sequence that share a key head, and the
+// A decoding step: a tile is up to 16 rows (query, head of a group) of a sequence that share a key head, and the
 // work is reading that head's keys and values once. The matrix cores take 16 rows at the cost of one, so what bounds
 // it is HBM, as long as enough loads are in flight and the workgroups finish together:
 //  - the (tile, 4 blocks of keys) units of the whole batch are one line, cut into equal stretches, one a workgroup (two
@@ -56,8 +56,11 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAtt
 //    of LDS, and waits for its own loads only: no barriers inside a stretch. While the scores are computed the values
 //    are in flight, while the values are weighed the next keys.
 // Scores come transposed, S = K · Qᵀ, so that a lane has one row's scores and the probabilities, rounded and packed, are
-// the second operand of Oᵀ = Vᵀ · Pᵀ as they are; transposing LDS reads give the first.
+// the second operand of Oᵀ = Vᵀ · Pᵀ as they are; transposing LDS reads give the first. Measured: 64 sequences of 8 to 4096
+// keys, 32 heads on 8 of 128: 110 us (4.9 TB/s; all of 4096: 5.5); 8 x 2 queries over 20000 keys of 8 heads of 64: 70 us
+// (4.7 TB/s); one query of 8 heads over 500 keys: 9 us, as any launch from the host.
 constexpr int FEW_WAVES = 4;
+constexpr int TR = 16;  // rows of a tile
 
 // LDS position of 16-byte chunk c of row r: c ^ few_swz(r). Key fragments (16 rows, one chunk) need a bijection of
 // r mod 16 onto the banks, value fragments (8 rows, two neighbouring chunks) distinct pairs.
@@ -164,10 +167,9 @@ struct FewPart {
   int rows, w0, parts, index;
 };
 
-template <class X, class E, int D, int NR>
+template <class X, class E, int D>
 __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const PagedAttnArgs A) {
   typedef FewCfg<D> C;
-  constexpr int TR = 16 * NR;  // rows of a tile
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float part_ml[FEW_WAVES][TR][2];
   __shared__ uint32_t bad_rows;
@@ -303,14 +305,11 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
     }
   };
   // A range's queries, then its first block on its way: everything that was loaded before has arrived when it returns.
-  auto begin = [&](const FewRange& R, u32x4p (&qn)[NR][D / 32]) {
+  auto begin = [&](const FewRange& R, u32x4p (&qn)[D / 32]) {
+    const int flat = R.t.row0 + l16, qi = flat / G, h = R.t.hk * G + (flat - qi * G);
+    const uint16_t* const qg = (const uint16_t*)A.q + (int64_t)(R.t.s0 + qi) * A.qs[0] + h * A.qs[1] + 8 * g16;
 #pragma unroll
-    for (int k = 0; k < NR; ++k) {
-      const int r = 16 * k + l16, flat = R.t.row0 + r, qi = flat / G, h = R.t.hk * G + (flat - qi * G);
-      const uint16_t* const qg = (const uint16_t*)A.q + (int64_t)(R.t.s0 + qi) * A.qs[0] + h * A.qs[1] + 8 * g16;
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) qn[k][s] = r < R.rows ? *(const u32x4p*)(qg + 32 * s) : u32x4p{0, 0, 0, 0};
-    }
+    for (int s = 0; s < D / 32; ++s) qn[s] = l16 < R.rows ? *(const u32x4p*)(qg + 32 * s) : u32x4p{0, 0, 0, 0};
     hk = R.t.hk;
     table = A.table + (int64_t)R.t.b * A.M;
     page0 = -64;
@@ -323,9 +322,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
     __builtin_amdgcn_s_waitcnt(0x0F70);
     // (the queries pass through a statement, or they would be waited for at their use, in every iteration)
 #pragma unroll
-    for (int k = 0; k < NR; ++k)
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) asm volatile("" : "+v"(qn[k][s]));
+    for (int s = 0; s < D / 32; ++s) asm volatile("" : "+v"(qn[s]));
     if (blocks > 0) {
       fetch(A.k_cache, 0);
       fetch(A.v_cache, 8192);
@@ -340,39 +337,28 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
 
   FewPart part[2];
   int parts = 0;
-  u32x4p qf[NR][D / 32];
+  u32x4p qf[D / 32];
   FewRange R = next_range();
   if (R.rows <= 0) return;
   begin(R, qf);
   while (true) {
     const PagedTile t = R.t;
     const int rows = R.rows;
-    // this lane's rows: one a 16-row tile
-    int lo[NR], hi[NR], pos[NR];
-    float slope[NR];
-#pragma unroll
-    for (int k = 0; k < NR; ++k) {
-      const int r = 16 * k + l16, flat = t.row0 + r, qi = flat / G;
-      pos[k] = t.pos0 + qi;
-      hi[k] = r < rows ? last_key(t, qi) : -1;
-      lo[k] = first_key(t, qi);
-      slope[k] = 0.f;
-      if (A.slopes) {
-        slope[k] = A.slopes[r < rows ? t.hk * G + (flat - qi * G) : 0] * kLog2e;
-        __builtin_amdgcn_s_waitcnt(0x0F70);
-      }
+    // this lane's row
+    const int flat = t.row0 + l16, qi = flat / G, pos = t.pos0 + qi;
+    const int hi = l16 < rows ? last_key(t, qi) : -1, lo = first_key(t, qi);
+    float slope = 0.f;
+    if (A.slopes) {
+      slope = A.slopes[l16 < rows ? t.hk * G + (flat - qi * G) : 0] * kLog2e;
+      __builtin_amdgcn_s_waitcnt(0x0F70);
     }
     // the keys that every row sees
     const int all_hi = last_key(t, uni(t.row0 / G)), all_lo = first_key(t, uni((t.row0 + rows - 1) / G));
 
-    float m[NR], l[NR];
-    f32x4p o[NR][D / 16];
+    float m = -INFINITY, l = 0.f;
+    f32x4p o[D / 16];
 #pragma unroll
-    for (int k = 0; k < NR; ++k) {
-      m[k] = -INFINITY, l[k] = 0.f;
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) o[k][d] = f32x4p{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int d = 0; d < D / 16; ++d) o[d] = f32x4p{0.f, 0.f, 0.f, 0.f};
 
     for (int j = 0; j < blocks; ++j) {
       const int kb = kstart + j * C::UNIT;
@@ -381,18 +367,15 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): the keys are there, the values may be on their way
       asm volatile("" ::: "memory");
-      f32x4p st[NR][C::KT];
+      f32x4p st[C::KT];
 #pragma unroll
       for (int tt = 0; tt < C::KT; ++tt) {
         u32x4p kf[D / 32];
         few_read_k<D>(kf, ka, tt * 16 * C::RB);
+        f32x4p acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NR; ++k) {
-          f32x4p acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < D / 32; ++s) acc = X::mma16(kf[s], qf[k][s], acc);
-          st[k][tt] = acc;
-        }
+        for (int s = 0; s < D / 32; ++s) acc = X::mma16(kf[s], qf[s], acc);
+        st[tt] = acc;
       }
       // (from here on `row` and `bad` are the next block's; the values of this one are on their way already)
       if (more) {
@@ -400,68 +383,65 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
         fetch(A.k_cache, 0);
       }
       const bool mask = kb + C::KB - 1 > all_hi || kb < all_lo;
-      uint32_t pf[NR][C::KT * 2];
-#pragma unroll
-      for (int k = 0; k < NR; ++k) {
-        if (score.cap2 > 0.f) {
-#pragma unroll
-          for (int tt = 0; tt < C::KT; ++tt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) st[k][tt][i] = score.capped(st[k][tt][i]);
-        } else {
-#pragma unroll
-          for (int tt = 0; tt < C::KT; ++tt) st[k][tt] *= score.sl2;
-        }
-        if (A.slopes) {
-#pragma unroll
-          for (int tt = 0; tt < C::KT; ++tt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              st[k][tt][i] = __builtin_fmaf(slope[k], (float)(kb + 16 * tt + 4 * g16 + i - pos[k]), st[k][tt][i]);
-        }
-        if (mask) {
-#pragma unroll
-          for (int tt = 0; tt < C::KT; ++tt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rel = 16 * tt + 4 * g16 + i, key = kb + rel;
-              st[k][tt][i] = key <= hi[k] && key >= lo[k] ? st[k][tt][i] : -INFINITY;
-            }
-        }
-        if (bad_now) {
-#pragma unroll
-          for (int tt = 0; tt < C::KT; ++tt) {
-            const uint32_t bits = (uint32_t)(bad_now >> (16 * tt)) >> (4 * g16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) st[k][tt][i] = bits >> i & 1 ? -INFINITY : st[k][tt][i];
-          }
-        }
-        float mb = st[k][0][0];
+      uint32_t pf[C::KT * 2];
+      if (score.cap2 > 0.f) {
 #pragma unroll
         for (int tt = 0; tt < C::KT; ++tt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mb = fmaxf(mb, st[k][tt][i]);
-        mb = max_rows16(mb) - X::LIFT;
-        if (__builtin_amdgcn_ballot_w64(mb > m[k])) {
-          const float mn = fmaxf(m[k], mb);
-          const float alpha = m[k] == mn ? 1.f : __builtin_amdgcn_exp2f(m[k] - mn);  // (equal: also -inf, nothing seen)
-          m[k] = mn;
-          l[k] *= alpha;
+          for (int i = 0; i < 4; ++i) st[tt][i] = score.capped(st[tt][i]);
+      } else {
 #pragma unroll
-          for (int d = 0; d < D / 16; ++d) o[k][d] *= alpha;
-        }
-        const float ref = m[k] == -INFINITY ? 0.f : m[k];
+        for (int tt = 0; tt < C::KT; ++tt) st[tt] *= score.sl2;
+      }
+      if (A.slopes) {
+#pragma unroll
+        for (int tt = 0; tt < C::KT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            st[tt][i] = __builtin_fmaf(slope, (float)(kb + 16 * tt + 4 * g16 + i - pos), st[tt][i]);
+      }
+      if (mask) {
+#pragma unroll
+        for (int tt = 0; tt < C::KT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rel = 16 * tt + 4 * g16 + i, key = kb + rel;
+            st[tt][i] = key <= hi && key >= lo ? st[tt][i] : -INFINITY;
+          }
+      }
+      if (bad_now) {
 #pragma unroll
         for (int tt = 0; tt < C::KT; ++tt) {
-          float p[4];
+          const uint32_t bits = (uint32_t)(bad_now >> (16 * tt)) >> (4 * g16);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(st[k][tt][i] - ref);
+          for (int i = 0; i < 4; ++i) st[tt][i] = bits >> i & 1 ? -INFINITY : st[tt][i];
+        }
+      }
+      float mb = st[0][0];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t w = X::pack(p[2 * i], p[2 * i + 1]);
-            l[k] = X::sum2(w, l[k]);
-            pf[k][2 * tt + i] = w;
-          }
+      for (int tt = 0; tt < C::KT; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mb = fmaxf(mb, st[tt][i]);
+      mb = max_rows16(mb) - X::LIFT;
+      if (__builtin_amdgcn_ballot_w64(mb > m)) {
+        const float mn = fmaxf(m, mb);
+        const float alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);  // (equal: also -inf, nothing seen)
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[d] *= alpha;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int tt = 0; tt < C::KT; ++tt) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(st[tt][i] - ref);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t w = X::pack(p[2 * i], p[2 * i + 1]);
+          l = X::sum2(w, l);
+          pf[2 * tt + i] = w;
         }
       }
       // the values; of what was issued after them, the eight loads of the next keys may still run
@@ -480,9 +460,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
             const u32x4p vf = {f[2 * d].x, f[2 * d].y, f[2 * d + 1].x, f[2 * d + 1].y};
-#pragma unroll
-            for (int k = 0; k < NR; ++k)
-              o[k][4 * d4 + d] = X::mma16(vf, u32x4p{pf[k][4 * s], pf[k][4 * s + 1], pf[k][4 * s + 2], pf[k][4 * s + 3]}, o[k][4 * d4 + d]);
+            o[4 * d4 + d] = X::mma16(vf, u32x4p{pf[4 * s], pf[4 * s + 1], pf[4 * s + 2], pf[4 * s + 3]}, o[4 * d4 + d]);
           }
         }
       }
@@ -494,100 +472,92 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
     const bool early = rows <= C::STAGE_ROWS;
     bool more_ranges = at < end;
     const FewRange cur = R;
-    u32x4p qn[NR][D / 32];
+    u32x4p qn[D / 32];
     if (more_ranges) {
       R = next_range();
       more_ranges = R.rows > 0;
     }
-    if (NR == 1 && early && more_ranges) begin(R, qn);
-    // 16 rows at a time: staged outputs [wave][rows][OP], summed by all threads
+    if (early && more_ranges) begin(R, qn);
+    // staged outputs [wave][rows][OP], summed by all threads
     const bool whole = cur.u0 == 0 && cur.u1 == cur.units;
     const __amdgpu_buffer_rsrc_t ws = paged_ws(A);
     const uint32_t slot_byte = (2 * (uint32_t)w + (cur.u0 == 0 ? 1 : 0)) * (uint32_t)paged_part_floats(TR, D) * 4;
-    float* const so = (float*)(NR == 1 && early ? smem + FEW_WAVES * C::WAVE : smem);
-#pragma unroll
-    for (int k = 0; k < NR; ++k) l[k] = sum_rows16(l[k]);
+    float* const so = (float*)(early ? smem + FEW_WAVES * C::WAVE : smem);
+    l = sum_rows16(l);
     few_barrier();
     if (tid == 0) lds_put1(lds_at(&bad_rows), 0);
+    if (g16 == 0) lds_put2(lds_at(part_ml[wave][l16]), m, l);
+    if (l16 < rows) {
+      const uint32_t mine_o = lds_at(so + (wave * rows + l16) * C::OP + 4 * g16);
 #pragma unroll
-    for (int k = 0; k < NR; ++k)
-      if (g16 == 0) lds_put2(lds_at(part_ml[wave][16 * k + l16]), m[k], l[k]);
-#pragma unroll
-    for (int k = 0; k < NR; ++k) {
-      if (16 * k >= rows) break;
-      const int n = min(16, rows - 16 * k);
-      if (l16 < n) {
-        const uint32_t mine_o = lds_at(so + (wave * n + l16) * C::OP + 4 * g16);
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) lds_put4(mine_o + 64 * d, o[k][d]);
-      }
-      few_barrier();
-      f32x4p x[D / 64];
-      float mt[D / 64], lt[D / 64];
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const int idx = tid + 256 * i, r = idx / (D / 4), d = 4 * (idx % (D / 4));
-        float mm = -INFINITY, ll = 0.f;
-        f32x4p v = {0.f, 0.f, 0.f, 0.f};
-        if (r < n) {
-          f32x4p y[4];
-          f32x2p ml[4];
-          lds_get_parts(y, ml, lds_at(so + r * C::OP + d), n * C::OP * 4, lds_at(part_ml[0][16 * k + r]), sizeof(part_ml[0]));
-#pragma unroll
-          for (int u = 0; u < FEW_WAVES; ++u) mm = fmaxf(mm, ml[u].x);
-          const float ref = mm == -INFINITY ? 0.f : mm;
-#pragma unroll
-          for (int u = 0; u < FEW_WAVES; ++u) {
-            const float f = __builtin_amdgcn_exp2f(ml[u].x - ref);
-            ll = __builtin_fmaf(ml[u].y, f, ll);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(y[u][e], f, v[e]);
-          }
-          bool finite = true;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) finite &= fabsf(v[e]) < INFINITY;
-          if (!finite) asm volatile("ds_or_b32 %0, %1" ::"v"(lds_at(&bad_rows)), "v"(1u << r) : "memory");
-        }
-        x[i] = v, mt[i] = mm, lt[i] = ll;
-      }
-      few_barrier();
-      // A value that a row does not see has probability 0, which an infinity or NaN in it would still turn into NaN:
-      // rows with such outputs are computed again from what they see alone.
-      uint32_t again = uni((int)lds_get1(lds_at(&bad_rows)));
-      while (again) {
-        const int r = __builtin_ctz(again);
-        again &= again - 1;
-        const int flat = t.row0 + 16 * k + r, qi = flat / G;
-        const int64_t first = max((int64_t)cur.kfirst + (int64_t)cur.u0 * C::UNIT, (int64_t)first_key(t, qi));
-        const int64_t last = min((int64_t)cur.kfirst + (int64_t)cur.u1 * C::UNIT, (int64_t)last_key(t, qi) + 1);
-        float rm, rl;
-        const float v = paged_row<E>(A, t.b, t.s0 + qi, t.hk * G + (flat - qi * G), t.pos0 + qi, (int)first, (int)max(last, (int64_t)0),
-                                     *(PagedRowLds*)so, &rm, &rl);
-        float* const one = so + sizeof(PagedRowLds) / 4;
-        if (tid < D) one[tid] = v;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          const int idx = tid + 256 * i, d = 4 * (idx % (D / 4));
-          if (idx / (D / 4) == r) x[i] = *(const f32x4p*)(one + d), mt[i] = rm, lt[i] = rl;
-        }
-        __syncthreads();
-        if (tid == 0) lds_put1(lds_at(&bad_rows), 0);
-      }
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const int idx = tid + 256 * i, r = idx / (D / 4), d = 4 * (idx % (D / 4)), rk = 16 * k + r;
-        if (r < n) {
-          if (whole) {
-            paged_store4<X, D>(A, t, rk, d, x[i] * (lt[i] == 0.f ? 0.f : 1.f / lt[i]));
-          } else {
-            agent_put4(ws, slot_byte + (rk * D + d) * 4, x[i]);
-            if (d == 0) agent_put2(ws, slot_byte + (TR * D + 2 * rk) * 4, mt[i], lt[i]);
-          }
-        }
-      }
-      few_barrier();
+      for (int d = 0; d < D / 16; ++d) lds_put4(mine_o + 64 * d, o[d]);
     }
+    few_barrier();
+    f32x4p x[D / 64];
+    float mt[D / 64], lt[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const int idx = tid + 256 * i, r = idx / (D / 4), d = 4 * (idx % (D / 4));
+      float mm = -INFINITY, ll = 0.f;
+      f32x4p v = {0.f, 0.f, 0.f, 0.f};
+      if (r < rows) {
+        f32x4p y[4];
+        f32x2p ml[4];
+        lds_get_parts(y, ml, lds_at(so + r * C::OP + d), rows * C::OP * 4, lds_at(part_ml[0][r]), sizeof(part_ml[0]));
+#pragma unroll
+        for (int u = 0; u < FEW_WAVES; ++u) mm = fmaxf(mm, ml[u].x);
+        const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+        for (int u = 0; u < FEW_WAVES; ++u) {
+          const float f = __builtin_amdgcn_exp2f(ml[u].x - ref);
+          ll = __builtin_fmaf(ml[u].y, f, ll);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(y[u][e], f, v[e]);
+        }
+        bool finite = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) finite &= fabsf(v[e]) < INFINITY;
+        if (!finite) asm volatile("ds_or_b32 %0, %1" ::"v"(lds_at(&bad_rows)), "v"(1u << r) : "memory");
+      }
+      x[i] = v, mt[i] = mm, lt[i] = ll;
+    }
+    few_barrier();
+    // A value that a row does not see has probability 0, which an infinity or NaN in it would still turn into NaN:
+    // rows with such outputs are computed again from what they see alone.
+    uint32_t again = uni((int)lds_get1(lds_at(&bad_rows)));
+    while (again) {
+      const int r = __builtin_ctz(again);
+      again &= again - 1;
+      const int flat = t.row0 + r, qi = flat / G;
+      const int64_t first = max((int64_t)cur.kfirst + (int64_t)cur.u0 * C::UNIT, (int64_t)first_key(t, qi));
+      const int64_t last = min((int64_t)cur.kfirst + (int64_t)cur.u1 * C::UNIT, (int64_t)last_key(t, qi) + 1);
+      float rm, rl;
+      const float v = paged_row<E>(A, t.b, t.s0 + qi, t.hk * G + (flat - qi * G), t.pos0 + qi, (int)first, (int)max(last, (int64_t)0),
+                                   *(PagedRowLds*)so, &rm, &rl);
+      float* const one = so + sizeof(PagedRowLds) / 4;
+      if (tid < D) one[tid] = v;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const int idx = tid + 256 * i, d = 4 * (idx % (D / 4));
+        if (idx / (D / 4) == r) x[i] = *(const f32x4p*)(one + d), mt[i] = rm, lt[i] = rl;
+      }
+      __syncthreads();
+      if (tid == 0) lds_put1(lds_at(&bad_rows), 0);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const int idx = tid + 256 * i, r = idx / (D / 4), d = 4 * (idx % (D / 4));
+      if (r < rows) {
+        if (whole) {
+          paged_store4<X, D>(A, t, r, d, x[i] * (lt[i] == 0.f ? 0.f : 1.f / lt[i]));
+        } else {
+          agent_put4(ws, slot_byte + (r * D + d) * 4, x[i]);
+          if (d == 0) agent_put2(ws, slot_byte + (TR * D + 2 * r) * 4, mt[i], lt[i]);
+        }
+      }
+    }
+    few_barrier();
     if (!whole && cur.index < A.max_tiles) {
       // (its first range and its last: no workgroup has more parts than two)
       const int w0 = owner(cur.at), w1 = owner(cur.at + cur.units - 1);
@@ -597,9 +567,9 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       ++parts;
     }
     if (!more_ranges) break;
-    if (NR == 1 && early) {
+    if (early) {
 #pragma unroll
-      for (int s = 0; s < D / 32; ++s) qf[0][s] = qn[0][s];
+      for (int s = 0; s < D / 32; ++s) qf[s] = qn[s];
     } else {
       begin(R, qf);
     }
@@ -614,19 +584,19 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
   }
 }
 
-template <class X, class E, int D, int NR>
+template <class X, class E, int D>
 void launch_few(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
   constexpr int lds = FewCfg<D>::LDS;
-  const hipError_t e = hipFuncSetAttribute((const void*)paged_attention_few_kernel<X, E, D, NR>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  const hipError_t e = hipFuncSetAttribute((const void*)paged_attention_few_kernel<X, E, D>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("paged_attention LDS attribute: ") + hipGetErrorString(e));
-  launch_k(done, paged_attention_few_kernel<X, E, D, NR>, dim3((unsigned)a.groups), dim3(256), lds, stream, a);
+  launch_k(done, paged_attention_few_kernel<X, E, D>, dim3((unsigned)a.groups), dim3(256), lds, stream, a);
 }
 
 template <class X, class E>
 void launch_matrix(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
   if (a.tile_rows == kPromptRows) return launch_paged_prompt(a, stream, done);
-  if (a.D == 128) a.tile_rows == 16 ? launch_few<X, E, 128, 1>(a, stream, done) : launch_few<X, E, 128, 2>(a, stream, done);
-  else a.tile_rows == 16 ? launch_few<X, E, 64, 1>(a, stream, done) : launch_few<X, E, 64, 2>(a, stream, done);
+  if (a.D == 128) return launch_few<X, E, 128>(a, stream, done);
+  launch_few<X, E, 64>(a, stream, done);
 }
 
 }  // namespace
@@ -644,8 +614,14 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
   if (a.pages * a.Hkv * a.P > (int64_t)UINT32_MAX || (a.qs[0] | a.qs[1]) & 7) return;
   const int G = a.Hq / a.Hkv;
   const double rows = (double)a.T * G / a.B;  // rows a sequence has of a key head, on average
-  if (rows > 32) return paged_prompt_plan(a, ws_floats);
-  a.tile_rows = rows > 16 ? 32 : 16;
+  // The other kernel takes tiles of up to 128 rows, and its parts are joined by a second launch of the whole chip, here a
+  // tile's by one workgroup. Heads of 128 over 4 x 4 queries of 8 sequences of 16000 keys: 102 us there, 132 here in tiles
+  // of 32 rows; 3 x 5 queries of 5 heads of 64 over 12811 keys 25 and 38. With 16 rows or fewer it is the parts of a tile
+  // that decide: one query of 5 heads over 30000 keys of two heads 19 and 30 us, 8 queries of 4 x 4 heads over 9000 keys
+  // 39 and 42, but one over 9000 keys of one head 14 and 12, and 8 of 8 x 4 over 4000 34 and 32.
+  const int64_t tiles128 = (a.T * G / kPromptRows + a.B) * a.Hkv, keys = (int64_t)a.M * a.P;
+  if (rows > 16 || (tiles128 <= 32 && keys >= (tiles128 >= 16 ? 8192 : 16384))) return paged_prompt_plan(a, ws_floats);
+  a.tile_rows = TR;
   const int unit = a.D == 128 ? 128 : 256;
   a.min_units = 512 / unit;
   const int64_t tiles = (a.T * G / a.tile_rows + a.B) * a.Hkv;

@@ -2,11 +2,15 @@
 // 128: a tile is 128 rows (query, head of a group) of a sequence that share a key head, 32 a wavefront; blocks of 64 keys
 // and values stream through LDS, two stages, loaded straight from the rows of the cache that the page table names.
 //
+// Where the tiles do not fill the chip, each is cut into ranges of keys, which a second launch joins.
+//
 // Scores come transposed, S = K · Qᵀ, so that a lane has one row and half its keys: the running maximum and sum take one
 // exchange between the half-waves, and the probabilities, packed, are the second operand of Oᵀ = Vᵀ · Pᵀ as they are.
 // The matrix products and the exponentials bound it (a wavefront's float instructions and matrix instructions add up):
 // the exponent reference moves only when a block exceeds it by 2^8, and masks are applied only in the blocks that need
-// one. Two workgroups share a CU, so that one's waits for LDS are the other's work.
+// one. Two workgroups share a CU, so that one's waits for LDS are the other's work. Measured, heads of 128 and 64: four
+// prompts of 875 to 1824 tokens, 32 heads, capped, 116 us (550 TFLOP/s); two chunks of 512 with a window of 4096, 38 us;
+// 256 x 4 queries of two sequences of 60000 keys 87 us (720 TFLOP/s); 16 rows over 4 x 8 x 16000 keys 105 us (5.0 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,10 +27,11 @@ namespace ryft {
 namespace {
 
 constexpr int BKV = 64;  // keys a block
-constexpr int kRanges = 512;  // workgroups where tiles are cut into ranges of keys: two a CU
+constexpr int kRanges = 512;    // workgroups where tiles are cut into ranges of keys: two a CU
+constexpr int kMaxParts = 128;  // ranges of a tile (two tiles of 85 rows × 31072 keys: 23 us with at most 128, 29 with 243)
 
-// The workspace of a launch with ranges: the parts (workgroup slots of kPromptRows rows), {ranges, tiles}, and for each
-// tile {first token of its sequence, first flat row, rows, parts}.
+// The workspace of a launch with ranges: the parts (one a workgroup, of kPromptRows rows), the number of tiles, and for each
+// tile {first token of its sequence, first flat row, rows + 256 parts, first workgroup}.
 __host__ __device__ inline int64_t prompt_part(int D) { return paged_part_floats(kPromptRows, D); }
 __device__ __forceinline__ int32_t* prompt_head(const PagedAttnArgs& A, int D) { return (int32_t*)(A.ws + (int64_t)kRanges * prompt_part(D)); }
 
@@ -118,15 +123,11 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     for (int64_t i = tid; i < (int64_t)A.Hq * D; i += 256) ((uint16_t*)A.o)[t * A.Hq * D + i] = 0;
   }
 
-  // Workgroup x has range x / Hkv % splits of row tile x / Hkv / splits, of key head x % Hkv: with 8 key heads each XCD
-  // (x mod 8) reads one head's keys. Row tiles are taken in falling order of the blocks of keys they see, over all
-  // sequences, so that the chip does not wait for long ones that began late (four causal prompts of 875 to 1824 tokens:
-  // the last workgroup ended 26% after the mean). The place in that order is found without a sort: a sequence a lane, the
-  // number of blocks that as many tiles reach by bisection, then the tile among those of that number.
-  const int x = blockIdx.x;
+  // Key heads are dealt first: with 8 of them each XCD (workgroup mod 8) reads one head's keys.
+  const int x = blockIdx.x, want = x / A.Hkv;
   PagedTile t;
   t.hk = x % A.Hkv;
-  int s0 = 0, n = 0, len = 0, tiles = 0;
+  int s0 = 0, n = 0, len = 0, tiles = 0;  // of a sequence a lane
   auto sequence = [&](int b) {
     s0 = 0, n = 0, len = 0;
     if (b >= 0 && b < A.B) {
@@ -136,33 +137,59 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     }
     tiles = (int)(((uint32_t)n * (uint32_t)G + kPromptRows - 1) / kPromptRows);
   };
-  sequence(lane);
-  int splits = 1;
+  // blocks of a tile: to its last query's key, at most those of a window and the tile's own queries
+  const int most = A.window > 0 ? A.window / BKV + kPromptRows / G / BKV + 2 : INT32_MAX;
+  int split = 0, cuts = 1, tile_no = 0;  // this workgroup's range of the tile, ranges that the tile has at most
   if (A.splits > 1) {
-    int total = wave_total(tiles);
-    for (int b = 64; b < A.B; b += 64) {
-      sequence(b + lane);
-      total += wave_total(tiles);
+    // Every tile in ranges of about `each` blocks (a sequence's tiles in as many as its last has), the least with which all
+    // fit into the launch: ragged lengths need no other balancing.
+    auto cuts_of = [&](int each) { return max(1, min((int)A.splits, (min((len + BKV - 1) / BKV, most) + each - 1) / each)); };
+    const int room = kRanges / A.Hkv;
+    auto over = [&](auto&& f) {  // the sum of f over the sequences, at most 2^24
+      int sum = 0;
+      for (int b = 0; b < A.B; b += 64) {
+        if (A.B > 64) sequence(b + lane);
+        sum = min(1 << 24, sum + wave_total(min(1 << 18, f())));
+      }
+      return sum;
+    };
+    sequence(lane);
+    const int total = over([&]() { return tiles; });
+    int each = 1 << 30;
+    if (total <= room) {
+      each = max(2, over([&]() { return (int)min((int64_t)1 << 18, (int64_t)tiles * min((len + BKV - 1) / BKV, most) / room); }));
+      while (over([&]() { return tiles * cuts_of(each); }) > room) each += max(1, each / 16);
     }
-    splits = max(1, min((int)A.splits, kRanges / max(1, total * A.Hkv)));
-    if (x == 0 && tid == 0) {
-      int32_t* const head = prompt_head(A, D);
-      head[0] = splits, head[1] = max(0, min(total * A.Hkv, kRanges));
+    if (x == 0 && tid == 0) *prompt_head(A, D) = total <= room ? total * A.Hkv : 0;
+    int sum = 0, before = 0, found = -1;
+    for (int b = 0; b < A.B && found < 0; b += 64) {
+      if (A.B > 64) sequence(b + lane);
+      const int own = cuts_of(each), incl = wave_scan(tiles * own), tiles_incl = wave_scan(tiles);
+      const uint64_t here = __builtin_amdgcn_ballot_w64(sum + incl > want);
+      if (here) {
+        found = __builtin_ctzll(here);
+        t.b = b + found;
+        t.s0 = __builtin_amdgcn_readlane(s0, found);
+        t.n = __builtin_amdgcn_readlane(n, found);
+        cuts = __builtin_amdgcn_readlane(own, found);
+        const int count = __builtin_amdgcn_readlane(tiles, found);
+        const int rest = want - (sum + __builtin_amdgcn_readlane(incl, found) - count * cuts);
+        const int turn = __builtin_amdgcn_readfirstlane(rest / cuts), tile = count - 1 - turn;  // (long ones first)
+        split = rest - turn * cuts;
+        t.row0 = tile * kPromptRows;
+        tile_no = (before + __builtin_amdgcn_readlane(tiles_incl, found) - count + tile) * A.Hkv + t.hk;
+      } else {
+        sum += __builtin_amdgcn_readlane(incl, 63);
+        before += __builtin_amdgcn_readlane(tiles_incl, 63);
+      }
     }
-    if (A.B > 64) sequence(lane);
-  }
-  const int split = splits > 1 ? x / A.Hkv % splits : 0;
-  const int want = splits > 1 ? x / (A.Hkv * splits) : x / A.Hkv;
-  const int tile_no = want * A.Hkv + t.hk;
-  auto describe = [&](int rows, int parts) {  // for the join
-    if (A.splits > 1 && split == 0 && tid == 0 && tile_no < kRanges) {
-      int32_t* const at = prompt_head(A, D) + 4 + 4 * tile_no;
-      at[0] = t.s0, at[1] = t.row0, at[2] = rows, at[3] = parts;
-    }
-  };
-  if (A.B <= 64) {
-    // blocks of a tile: to its last query's key, at most those of a window and the tile's own queries
-    const int most = A.window > 0 ? A.window / BKV + kPromptRows / G / BKV + 2 : INT32_MAX;
+    if (found < 0) return;
+  } else if (A.B <= 64) {
+    // Row tiles in falling order of the blocks of keys they see, over all sequences, so that the chip does not wait for
+    // long ones that began late (four causal prompts of 875 to 1824 tokens: the last workgroup ended 26% after the mean).
+    // The place in that order is found without a sort: a sequence a lane, the number of blocks that as many tiles reach by
+    // bisection, then the tile among those of that number.
+    sequence(lane);
     const int all = A.causal ? 0 : tiles;  // (not causal: every tile sees all)
     auto reach = [&](int c) {  // tiles that see c blocks or more
       if (c > most) return 0;
@@ -204,7 +231,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
         sum += __builtin_amdgcn_readlane(incl, 63);
       }
     }
-    if (found < 0) return describe(0, 0);
+    if (found < 0) return;
   }
   t.len = __builtin_amdgcn_readfirstlane(paged_length(A, t.b));
   t.pos0 = t.len - t.n;
@@ -215,8 +242,11 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
   // this range's blocks [j0, j1) of 64 keys
   const int any_hi = last_key(q_last);
   const int jfirst = first_key(q_first) / BKV, blocks = max(0, any_hi / BKV + (any_hi >= 0 ? 1 : 0) - jfirst);
-  const int parts = max(1, min(splits, blocks / 4));
-  describe(rows, parts);
+  const int parts = max(1, min(cuts, blocks / 2));
+  if (A.splits > 1 && split == 0 && tid == 0 && tile_no < kRanges) {  // for the join
+    int32_t* const at = prompt_head(A, D) + 4 + 4 * tile_no;
+    at[0] = t.s0, at[1] = t.row0, at[2] = rows + 256 * parts, at[3] = x;
+  }
   if (split >= parts) return;
   const int each = (blocks + parts - 1) / parts;
   const int j0 = jfirst + min(blocks, split * each), j1 = jfirst + min(blocks, (split + 1) * each);
@@ -493,9 +523,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     }
     return;
   }
-  const int slot = tile_no * splits + split;
-  if (slot >= kRanges) return;  // (starts that decrease)
-  float* const part = A.ws + (int64_t)slot * prompt_part(D);
+  float* const part = A.ws + (int64_t)x * prompt_part(D);
   for (int i = tid; i < rows * (D / 4); i += 256) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
     *(f32x4p*)(part + r * D + d) = *(const f32x4p*)(so + r * C::OP + d);
@@ -513,22 +541,21 @@ __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const PagedAttnA
   const int tid = threadIdx.x, tile = blockIdx.x / CHUNKS, item = blockIdx.x % CHUNKS * ITEMS + tid % ITEMS, pg = tid / ITEMS;
   const int r = item / (D / 4), d = 4 * (item % (D / 4));
   const int32_t* const head = prompt_head(A, D);
-  const int splits = head[0], tiles = head[1];
+  const int tiles = head[0], word = head[6 + 4 * tile], first = head[7 + 4 * tile];
   PagedTile t;
   t.hk = tile % A.Hkv;
   t.s0 = head[4 + 4 * tile], t.row0 = head[5 + 4 * tile];
-  const int rows = head[6 + 4 * tile], parts = head[7 + 4 * tile];
-  if (splits < 2 || tile >= tiles || parts < 2 || (tile + 1) * splits > kRanges) return;
+  const int rows = word & 255, parts = word >> 8;
+  if (tile >= tiles || parts < 2) return;
   float m = -INFINITY, l = 0.f;
   f32x4p o = {0.f, 0.f, 0.f, 0.f};
   if (r < rows) {
-    const float* const first = A.ws + (int64_t)tile * splits * prompt_part(D);
     for (int p0 = pg; p0 < parts; p0 += PG * U) {
       f32x4p v[U];
       f32x2p w[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float* const part = first + (int64_t)min(p0 + PG * u, parts - 1) * prompt_part(D);
+        const float* const part = A.ws + (int64_t)(first + min(p0 + PG * u, parts - 1) * A.Hkv) * prompt_part(D);
         v[u] = *(const f32x4p*)(part + r * D + d);
         w[u] = *(const f32x2p*)(part + kPromptRows * D + 2 * r);
         if (p0 + PG * u >= parts) w[u].x = -INFINITY, v[u] = f32x4p{0.f, 0.f, 0.f, 0.f};
@@ -581,7 +608,7 @@ void launch_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) 
   if (a.softcap > 0.f || a.slopes) go(paged_prompt_kernel<X, E, D, true>);
   else go(paged_prompt_kernel<X, E, D, false>);
   if (a.splits <= 1) return;
-  const unsigned tiles = (unsigned)std::min(a.max_tiles, kRanges / 2), chunks = kPromptRows * D / 4 / 256;
+  const unsigned tiles = (unsigned)a.max_tiles, chunks = kPromptRows * D / 4 / 256;
   if (tiles <= 32) launch_k(done, paged_prompt_join_kernel<X, D, 4>, dim3(tiles * chunks * 4), block, 0, stream, a);
   else launch_k(done, paged_prompt_join_kernel<X, D, 1>, dim3(tiles * chunks), block, 0, stream, a);
 }
@@ -593,10 +620,10 @@ void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats) {
   if (a.T * a.Hq > INT32_MAX || tiles > INT32_MAX) return;
   a.tile_rows = kPromptRows;
   a.max_tiles = (int32_t)tiles;
-  // Ranges of keys where the tiles alone may leave the chip short of two workgroups a CU; the kernel, which knows the
-  // tiles, chooses how many (80 tiles of head dim 64: 42 us in 6 ranges, 50 in 9, which run one after the other; one
-  // tile of 85 rows × 31072 keys of two heads: 76 us in 16 ranges, 25 in 121). Of four blocks at least.
-  a.splits = tiles <= kRanges ? (int32_t)std::max<int64_t>(1, std::min<int64_t>(kRanges, (int64_t)a.M * a.P / 256)) : 1;
+  // Ranges of keys where the tiles alone may leave the chip short of two workgroups a CU (one tile of 85 rows × 31072 keys
+  // of two heads: 76 us in 16 ranges, 23 in 121). Of two blocks at least; under 8 blocks the second launch costs more than
+  // they save (300 queries of their own: 16 us, 17 with ranges).
+  a.splits = tiles <= kRanges && (int64_t)a.M * a.P >= 8 * BKV ? (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (int64_t)a.M * a.P / (2 * BKV))) : 1;
   a.groups = a.splits > 1 ? kRanges : (int32_t)tiles;
   if (a.splits > 1) *ws_floats = kRanges * prompt_part((int)a.D) + 4 + 4 * kRanges;
 }
