@@ -11,6 +11,7 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch  # (before the plugin: both then use one HIP runtime)
 
 from oracle import operators as oo
 from oracle import stablehlo as sh
@@ -349,7 +350,6 @@ def test_execute_into_updates_caches_in_place(gpu_client):
 @pytest.mark.parametrize("name", ["decode", "chunk", "sample"])
 def test_replayed_from_a_graph(gpu_client, name):
     # captured on a stream of torch's, replayed with eager work of the program's own in between
-    import torch
     module, ins = CASES[name]()
     exe = gpu_client.compile(pjrt.Program.mlir(module))
     bufs = device_buffers(gpu_client, ins)
