@@ -54,12 +54,54 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
 }
 __device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
-  return (uint32_t)__shfl_xor((int)(uint32_t)v, m, 64) | (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), m, 64) << 32;
+// Running results over a wavefront's lanes (inclusive; all lanes take part), by moves between lanes inside the registers: a
+// search is little else than these, and each took six trips through LDS (one filtered row of 32000 logits 24 us, 20 so; 64 mixed rows of 128256 70 and 58).
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T from_lane(T v, T none) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+  } else {
+    const uint64_t a = __builtin_bit_cast(uint64_t, v), b = __builtin_bit_cast(uint64_t, none);
+    const uint32_t lo = __builtin_amdgcn_update_dpp((int)(uint32_t)b, (int)(uint32_t)a, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp((int)(b >> 32), (int)(a >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+  }
 }
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-  for (int m = 32; m; m >>= 1) v += shfl_xor64(v, m);
+template <class T, class F>
+__device__ __forceinline__ T running(T v, T none, F&& op) {
+  v = op(v, from_lane<0x111, 0xf>(v, none));  // from 1, 2, 4 and 8 lanes below, in rows of 16
+  v = op(v, from_lane<0x112, 0xf>(v, none));
+  v = op(v, from_lane<0x114, 0xf>(v, none));
+  v = op(v, from_lane<0x118, 0xf>(v, none));
+  v = op(v, from_lane<0x142, 0xa>(v, none));  // from lane 15 of the row below, for rows 1 and 3
+  v = op(v, from_lane<0x143, 0xc>(v, none));  // from lane 31, for rows 2 and 3
   return v;
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32;
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+  return __builtin_bit_cast(double, lane64(__builtin_bit_cast(uint64_t, v), lane));
+}
+__device__ __forceinline__ uint64_t scan64(uint64_t v) {
+  return running(v, (uint64_t)0, [](uint64_t a, uint64_t b) { return a + b; });
+}
+__device__ __forceinline__ int scan32(int v) {
+  return running(v, 0, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ double scan_f64(double v) {
+  return running(v, 0.0, [](double a, double b) { return a + b; });
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return lane64(scan64(v), 63); }
+__device__ __forceinline__ uint64_t wave_min(uint64_t v) {
+  return lane64(running(v, ~(uint64_t)0, [](uint64_t a, uint64_t b) { return min(a, b); }), 63);
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+  return lane64(running(v, (uint64_t)0, [](uint64_t a, uint64_t b) { return max(a, b); }), 63);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  return __builtin_amdgcn_readlane((int)running(v, 0u, [](uint32_t a, uint32_t b) { return max(a, b); }), 63);
 }
 
 // 2^y for y <= 0, scaled by 2^bits and rounded to a whole number (2^y 2^bits < 2^52): a polynomial that interpolates
@@ -263,12 +305,7 @@ __device__ __forceinline__ int find_index(const SampleArgs& A, int64_t row, int 
     begin = min(end, begin + w * part);
     end = min(end, begin + part);
   }
-  uint64_t s = begin + lane < end ? f(begin + lane, E::get(x[begin + lane])) : 0;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = (uint32_t)__shfl_up((int)(uint32_t)s, off, 64) | (uint64_t)(uint32_t)__shfl_up((int)(s >> 32), off, 64) << 32;
-    if (lane >= off) s += o;
-  }
+  const uint64_t s = scan64(begin + lane < end ? f(begin + lane, E::get(x[begin + lane])) : 0);
   const uint64_t past = __builtin_amdgcn_ballot_w64(s > target);
   return past ? min(last, begin + __builtin_ctzll(past)) : last;
 }
@@ -407,28 +444,6 @@ __device__ __attribute__((noinline)) uint32_t lowest_of_weight(uint32_t top, dou
   return lowest_key_near(logit_key((float)(at + (double)log2f((float)minp) / c)), top, [&](uint32_t key) { return !(w.real(key_logit(key)) < minp); });
 }
 
-__device__ __forceinline__ uint64_t scan64(uint64_t v) {  // inclusive, over the wavefront
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = (uint32_t)__shfl_up((int)(uint32_t)v, off, 64) | (uint64_t)(uint32_t)__shfl_up((int)(v >> 32), off, 64) << 32;
-    if (lane >= off) v += o;
-  }
-  return v;
-}
-__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
-  return (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
-         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32;
-}
-__device__ __forceinline__ int scan32(int v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(v, off, 64);
-    if (lane >= off) v += o;
-  }
-  return v;
-}
 // Room for `mine` entries of each lane in a list of *n so far: where this lane's begin. One atomic a wavefront.
 __device__ __forceinline__ int list_room(int* n, int mine) {
   const int incl = scan32(mine);
@@ -448,7 +463,7 @@ __device__ __attribute__((noinline)) uint64_t list_select(SampleLds& sh, uint64_
     const uint64_t e = sh.list[i];
     if (e >= cut) low = min(low, e & mask), high = max(high, e & mask);
   }
-  for (int m = 32; m; m >>= 1) low = min(low, shfl_xor64(low, m)), high = max(high, shfl_xor64(high, m));
+  low = wave_min(low), high = wave_max(high);
   __syncthreads();
   if (lane == 0) sh.low[tid >> 6] = low, sh.high[tid >> 6] = high;
   __syncthreads();
@@ -588,8 +603,8 @@ __global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs A)
   };
   float best = -INFINITY;
   each([&](int, float x) { best = fmaxf(best, x); });
-  for (int m = 32; m; m >>= 1) best = fmaxf(best, __shfl_xor(best, m, 64));
-  if (lane == 0) sh.top[wave] = logit_key(best);
+  const uint32_t wave_top = wave_max(logit_key(best));
+  if (lane == 0) sh.top[wave] = wave_top;
   if (want.filtered) sh.mass[tid] = 0, sh.count[tid] = 0;
   if (tid == 0) sh.index = row.V, sh.n = 0;
   __syncthreads();
@@ -666,16 +681,6 @@ __global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs A)
     ws.stats[1] = (uint32_t)picked | (uint64_t)(uint32_t)sh.n << 32;
     ws.stats[2] = usual;
   }
-}
-
-__device__ __forceinline__ double scan_f64(double m) {  // inclusive, over the wavefront
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double o = __shfl_up(m, off, 64);
-    if (lane >= off) m += o;
-  }
-  return m;
 }
 
 // The place down to which a filtered row's tokens are kept, in sh.kept each chunk's kept weights; or 0, and the draw is
@@ -869,9 +874,7 @@ __global__ void __launch_bounds__(ST, 2) sample_draw_kernel(const SampleArgs A) 
     for (int w = 0; w < SW; ++w) kept += ws[4 + w];
   }
   const uint32_t top = (uint32_t)head;
-  uint32_t key_top = top;
-  for (int m = 32; m; m >>= 1) key_top = max(key_top, (uint32_t)__shfl_xor((int)key_top, m, 64));
-  key_top = __builtin_amdgcn_readfirstlane(key_top);
+  const uint32_t key_top = wave_max(top);
   if (key_top == 0 || want.greedy) {
     const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(top == key_top));
     const int index = __builtin_amdgcn_readlane((int)(head >> 32), who);
@@ -883,7 +886,7 @@ __global__ void __launch_bounds__(ST, 2) sample_draw_kernel(const SampleArgs A) 
   const Weights rw{(double)ftop, want.c, 0};  // relative to the row's maximum
   const float ctop = key_logit(top);
   const double factor = top ? rw.real(ctop) : 0.0;
-  double running = scan_f64((double)kept * unit * factor), all = __shfl(running, 63, 64);
+  double upto = scan_f64((double)kept * unit * factor), all = lane_f64(upto, 63);
 
   uint64_t cut = (uint64_t)1 << 32;  // kept: entries key << 32 | ~index of at least this
   if (want.filtered) {
@@ -896,19 +899,19 @@ __global__ void __launch_bounds__(ST, 2) sample_draw_kernel(const SampleArgs A) 
     cut = filtered<E>(A, r, key_top, all, sh);
     if (!cut) return;
     kept = sh.kept[lane];
-    running = scan_f64((double)kept * unit * factor);
-    all = __shfl(running, 63, 64);
+    upto = scan_f64((double)kept * unit * factor);
+    all = lane_f64(upto, 63);
   }
 
   // ---- the draw: the chunk whose running sum passes the uniform number, its stretch, and the index in that
   const double aim = uniform * all;
   const bool none = !(aim > 0);  // the first that has any weight, however little
   const bool cut_off = cut > (uint64_t)1 << 32;
-  const uint64_t passed = __builtin_amdgcn_ballot_w64(running > aim), some = __builtin_amdgcn_ballot_w64(kept > 0 && factor > 0);
+  const uint64_t passed = __builtin_amdgcn_ballot_w64(upto > aim), some = __builtin_amdgcn_ballot_w64(kept > 0 && factor > 0);
   // (none passed: rounding of the sums alone)
   int at = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
   const uint64_t have = lane64(kept, at);
-  const double in = (aim - (at ? __shfl(running, at - 1, 64) : 0.0)) / (unit * __shfl(factor, at, 64));
+  const double in = (aim - (at ? lane_f64(upto, at - 1) : 0.0)) / (unit * lane_f64(factor, at));
   uint64_t target = none ? 0 : !passed ? have - 1 : in > 0 ? min((uint64_t)in, have - 1) : 0;
   for (at = none ? 0 : at; at < C; ++at) {
     const FastWeights w(key_logit(__builtin_amdgcn_readlane(top, at)), want.c);
@@ -974,7 +977,7 @@ __global__ void __launch_bounds__(ST) sample_whole_kernel(const SampleArgs A) {
   const int64_t r = blockIdx.x;
   uint32_t top = 0;
   for (int i = tid; i < V; i += ST) top = max(top, logit_key(E::get(((const typename E::raw*)A.logits)[r * A.V + i])));
-  for (int m = 32; m; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
+  top = wave_max(top);
   if ((tid & 63) == 0) sh.high[tid >> 6] = top;
   __syncthreads();
   for (int w = 0; w < SW; ++w) top = max(top, (uint32_t)sh.high[w]);
