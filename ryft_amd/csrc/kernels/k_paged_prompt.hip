@@ -8,7 +8,7 @@
 // exchange between the half-waves, and the probabilities, packed, are the second operand of Oᵀ = Vᵀ · Pᵀ as they are.
 // The matrix products and the exponentials bound it (a wavefront's float instructions and matrix instructions add up):
 // the exponent reference moves only when a block exceeds it by 2^8, and masks are applied only in the blocks that need
-// one. Two workgroups share a CU, so that one's waits for LDS are the other's work. Measured, heads of 128 and 64: four
+// one. Two or three workgroups share a CU, so that one's waits for LDS are the others' work. Measured, heads of 128 and 64: four
 // prompts of 875 to 1824 tokens, 32 heads, capped, 116 us (550 TFLOP/s); two chunks of 512 with a window of 4096, 38 us;
 // 256 x 4 queries of two sequences of 60000 keys 87 us (720 TFLOP/s); 16 rows over 4 x 8 x 16000 keys 105 us (5.0 TB/s).
 #include <hip/hip_runtime.h>
@@ -27,13 +27,17 @@ namespace ryft {
 namespace {
 
 constexpr int BKV = 64;  // keys a block
-constexpr int kRanges = 512;    // workgroups where tiles are cut into ranges of keys: two a CU
+// Workgroups that share a CU, by registers and LDS (2048 queries of two heads of 64 over 65000 keys: 99 us with three, 111
+// with two; capped or biased scores take registers that three do not have: a chunk of such 41 us with three, 38 with two).
+__host__ __device__ constexpr int prompt_shares(int D, bool general) { return D == 64 && !general ? 3 : 2; }
+// Workgroups where tiles are cut into ranges of keys, at most
+__host__ __device__ constexpr int prompt_ranges(int D) { return 256 * prompt_shares(D, false); }
 constexpr int kMaxParts = 128;  // ranges of a tile (two tiles of 85 rows × 31072 keys: 23 us with at most 128, 29 with 243)
 
 // The workspace of a launch with ranges: the parts (one a workgroup, of kPromptRows rows), the number of tiles, and for each
 // tile {first token of its sequence, first flat row, rows + 256 parts, first workgroup}.
 __host__ __device__ inline int64_t prompt_part(int D) { return paged_part_floats(kPromptRows, D); }
-__device__ __forceinline__ int32_t* prompt_head(const PagedAttnArgs& A, int D) { return (int32_t*)(A.ws + (int64_t)kRanges * prompt_part(D)); }
+__device__ __forceinline__ int32_t* prompt_head(const PagedAttnArgs& A, int D) { return (int32_t*)(A.ws + (int64_t)prompt_ranges(D) * prompt_part(D)); }
 
 template <int D>
 struct PromptCfg {
@@ -105,7 +109,7 @@ __device__ __forceinline__ int wave_max(int v) {  // (of values of at least 0)
 
 // GENERAL: scores may be capped or biased by distance.
 template <class X, class E, int D, bool GENERAL>
-__global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArgs A) {
+__global__ void __launch_bounds__(256, prompt_shares(D, GENERAL)) paged_prompt_kernel(const PagedAttnArgs A) {
   typedef PromptCfg<D> C;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float row_ml[kPromptRows][2];
@@ -144,7 +148,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     // Every tile in ranges of about `each` blocks (a sequence's tiles in as many as its last has), the least with which all
     // fit into the launch: ragged lengths need no other balancing.
     auto cuts_of = [&](int each) { return max(1, min((int)A.splits, (min((len + BKV - 1) / BKV, most) + each - 1) / each)); };
-    const int room = kRanges / A.Hkv;
+    int room = 256 * prompt_shares(D, GENERAL) / A.Hkv;
     auto over = [&](auto&& f) {  // the sum of f over the sequences, at most 2^24
       int sum = 0;
       for (int b = 0; b < A.B; b += 64) {
@@ -157,10 +161,14 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     const int total = over([&]() { return tiles; });
     int each = 1 << 30;
     if (total <= room) {
-      each = max(2, over([&]() { return (int)min((int64_t)1 << 18, (int64_t)tiles * min((len + BKV - 1) / BKV, most) / room); }));
+      const int work = over([&]() { return (int)min((int64_t)1 << 18, (int64_t)tiles * min((len + BKV - 1) / BKV, most)); });
+      // (a third workgroup a CU where that leaves ranges of four blocks: two times 4 x 5 rows over 16000 keys of 4 heads 18
+      // us, 19 with it)
+      if (work / room < 4 && total <= 512 / A.Hkv) room = min(room, 512 / A.Hkv);
+      each = max(2, work / room);
       while (over([&]() { return tiles * cuts_of(each); }) > room) each += max(1, each / 16);
     }
-    if (x == 0 && tid == 0) *prompt_head(A, D) = total <= room ? total * A.Hkv : 0;
+    if (x == 0 && tid == 0) *prompt_head(A, D) = total <= room ? min(total * A.Hkv, prompt_ranges(D)) : 0;
     int sum = 0, before = 0, found = -1;
     for (int b = 0; b < A.B && found < 0; b += 64) {
       if (A.B > 64) sequence(b + lane);
@@ -243,7 +251,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
   const int any_hi = last_key(q_last);
   const int jfirst = first_key(q_first) / BKV, blocks = max(0, any_hi / BKV + (any_hi >= 0 ? 1 : 0) - jfirst);
   const int parts = max(1, min(cuts, blocks / 2));
-  if (A.splits > 1 && split == 0 && tid == 0 && tile_no < kRanges) {  // for the join
+  if (A.splits > 1 && split == 0 && tid == 0 && tile_no < prompt_ranges(D)) {  // for the join
     int32_t* const at = prompt_head(A, D) + 4 + 4 * tile_no;
     at[0] = t.s0, at[1] = t.row0, at[2] = rows + 256 * parts, at[3] = x;
   }
@@ -617,15 +625,16 @@ void launch_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) 
 
 void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats) {
   const int64_t tiles = (a.T * (a.Hq / a.Hkv) / kPromptRows + a.B) * a.Hkv;  // (at most)
+  const int ranges = prompt_ranges((int)a.D);
   if (a.T * a.Hq > INT32_MAX || tiles > INT32_MAX) return;
   a.tile_rows = kPromptRows;
   a.max_tiles = (int32_t)tiles;
   // Ranges of keys where the tiles alone may leave the chip short of two workgroups a CU (one tile of 85 rows × 31072 keys
   // of two heads: 76 us in 16 ranges, 23 in 121). Of two blocks at least; under 8 blocks the second launch costs more than
   // they save (300 queries of their own: 16 us, 17 with ranges).
-  a.splits = tiles <= kRanges && (int64_t)a.M * a.P >= 8 * BKV ? (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (int64_t)a.M * a.P / (2 * BKV))) : 1;
-  a.groups = a.splits > 1 ? kRanges : (int32_t)tiles;
-  if (a.splits > 1) *ws_floats = kRanges * prompt_part((int)a.D) + 4 + 4 * kRanges;
+  a.splits = tiles <= 512 && (int64_t)a.M * a.P >= 8 * BKV ? (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (int64_t)a.M * a.P / (2 * BKV))) : 1;
+  a.groups = a.splits > 1 ? ranges : (int32_t)tiles;  // (of ranges, those that the kernel has no room for end at once)
+  if (a.splits > 1) *ws_floats = ranges * prompt_part((int)a.D) + 4 + 4 * ranges;
 }
 
 void launch_paged_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
