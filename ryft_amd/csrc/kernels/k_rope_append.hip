@@ -96,99 +96,89 @@ __global__ void __launch_bounds__(256) rope_append_any_kernel(const RopeAppendAr
 // 16-bit heads of 16, 32, 64, 128 or 256 values, the rotated part a multiple of 16: a lane has 16 values of a head in two
 // 16-byte loads, the two halves of its pairs (half layout: 8 c and R / 2 + 8 c on; interleaved: 16 c and 16 c + 8 on; past
 // the rotated part the same), so that a rotation needs no other lane, and D / 16 lanes have a head, 64 · 16 / D heads a
-// pass of a wavefront. It moves each value in and out once and is bound by HBM where there are many tokens (8192 of 48
-// heads of 128, half of each rotated, 201 MB) and by latency where there are few. A wavefront turns its lane number into
-// one rotation of its token, and the lanes take theirs from LDS: with N passes of a token for one of them. N = 3 where the
-// tokens alone fill the chip, all loads first; else 1, for the shortest way through.
+// wavefront. It moves each value in and out once and is bound by HBM where there are many tokens (8192 of 48 heads of 128,
+// half of each rotated, 201 MB: 42 us, 4.8 TB/s; with three times as many heads a wavefront, all loads first, 48; a
+// workgroup a token with a value a lane, 97) and by latency where there are few (256 tokens of the same 10 us and 17). A
+// wavefront turns its lane number into one rotation of its token, and the lanes take theirs from LDS.
 typedef uint32_t u32x4r __attribute__((ext_vector_type(4)));
-template <class E, int N>
-__global__ void __launch_bounds__(256) rope_append_rows_kernel(const RopeAppendArgs A, int parts) {
+template <class E>
+__global__ void __launch_bounds__(256) rope_append_rows_kernel(const RopeAppendArgs A, int passes) {
   typedef typename E::raw raw;
   __shared__ float2 turns[4][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = (int64_t)blockIdx.x * 4 + wave, t = id / parts;
-  const int part = (int)(id - t * parts);
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave, t = id / passes;
+  const int pass = (int)(id - t * passes);
   if (t >= A.T) return;
   const int D = A.D, R = A.R, half = R / 2, lph = D / 16, heads = A.Hq + 2 * A.Hkv;
   const int c = lane % lph, per = 64 / lph;
   const bool turned = 16 * c < R;
   const int a0 = turned && !A.interleaved ? 8 * c : 16 * c, a1 = turned && !A.interleaved ? half + 8 * c : 16 * c + 8;
-  u32x4r x0[N], x1[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int h = (part + n * parts) * per + lane / lph;
-    if (h < heads) {
-      const raw* const x = rope_in<E>(A, t, h);
-      x0[n] = *(const u32x4r*)(x + a0), x1[n] = *(const u32x4r*)(x + a1);
-    }
+  const int h = pass * per + lane / lph;
+  const bool live = h < heads, value = h >= A.Hq + A.Hkv, key = h >= A.Hq;
+  u32x4r x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+  if (live) {
+    const raw* const x = rope_in<E>(A, t, h);
+    x0 = *(const u32x4r*)(x + a0), x1 = *(const u32x4r*)(x + a1);
   }
   const int position = A.positions[t], slot = A.slots[t];
   for (int i = lane; i < half; i += 64) turns[wave][i] = rotation(position, A.inv_freq[i], A.magnitude);
   float2 cs[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) cs[i] = turned ? turns[wave][8 * c + i] : float2{1.f, 0.f};
+  raw* const y = live ? rope_out<E>(A, t, h, slot) : nullptr;
+  float f[16];
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int h = (part + n * parts) * per + lane / lph;
-    const bool live = h < heads, value = h >= A.Hq + A.Hkv, key = h >= A.Hq;
-    raw* const y = live ? rope_out<E>(A, t, h, slot) : nullptr;
-    float f[16];
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = E::get((raw)x0[i]), f[2 * i + 1] = E::get((raw)(x0[i] >> 16));
+    f[8 + 2 * i] = E::get((raw)x1[i]), f[8 + 2 * i + 1] = E::get((raw)(x1[i] >> 16));
+  }
+  if (A.q_weight) {
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sq = __builtin_fmaf(f[i], f[i], sq);
+    for (int m = 1; m < lph; m <<= 1) sq += __shfl_xor(sq, m, 64);
+    const raw* const w = (const raw*)(key ? A.k_weight : A.q_weight);
+    const u32x4r w0 = *(const u32x4r*)(w + a0), w1 = *(const u32x4r*)(w + a1);
+    const float inv = rsqrtf(sq / (float)D + A.eps);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f[2 * i] = E::get((raw)x0[n][i]), f[2 * i + 1] = E::get((raw)(x0[n][i] >> 16));
-      f[8 + 2 * i] = E::get((raw)x1[n][i]), f[8 + 2 * i + 1] = E::get((raw)(x1[n][i] >> 16));
+      f[2 * i] *= inv * E::get((raw)w0[i]), f[2 * i + 1] *= inv * E::get((raw)(w0[i] >> 16));
+      f[8 + 2 * i] *= inv * E::get((raw)w1[i]), f[8 + 2 * i + 1] *= inv * E::get((raw)(w1[i] >> 16));
     }
-    if (A.q_weight) {
-      float sq = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sq = __builtin_fmaf(f[i], f[i], sq);
-      for (int m = 1; m < lph; m <<= 1) sq += __shfl_xor(sq, m, 64);
-      const raw* const w = (const raw*)(key ? A.k_weight : A.q_weight);
-      const u32x4r w0 = *(const u32x4r*)(w + a0), w1 = *(const u32x4r*)(w + a1);
-      const float inv = rsqrtf(sq / (float)D + A.eps);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[2 * i] *= inv * E::get((raw)w0[i]), f[2 * i + 1] *= inv * E::get((raw)(w0[i] >> 16));
-        f[8 + 2 * i] *= inv * E::get((raw)w1[i]), f[8 + 2 * i + 1] *= inv * E::get((raw)(w1[i] >> 16));
-      }
-    }
-    if (!y) continue;
-    u32x4r y0 = x0[n], y1 = x1[n];
-    if (!value && (turned || A.q_weight)) {
-      // pairs (p, q) → (p c - q s, q c + p s)
-      if (turned && A.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = f[2 * i], q = f[2 * i + 1];
-          f[2 * i] = p * cs[i].x - q * cs[i].y, f[2 * i + 1] = q * cs[i].x + p * cs[i].y;
-        }
-      } else if (turned) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = f[i], q = f[8 + i];
-          f[i] = p * cs[i].x - q * cs[i].y, f[8 + i] = q * cs[i].x + p * cs[i].y;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y0[i] = (uint32_t)E::put(f[2 * i]) | (uint32_t)E::put(f[2 * i + 1]) << 16;
-        y1[i] = (uint32_t)E::put(f[8 + 2 * i]) | (uint32_t)E::put(f[8 + 2 * i + 1]) << 16;
-      }
-    }
-    *(u32x4r*)(y + a0) = y0;
-    *(u32x4r*)(y + a1) = y1;
   }
+  if (!y) return;
+  u32x4r y0 = x0, y1 = x1;
+  if (!value && (turned || A.q_weight)) {
+    // pairs (p, q) → (p c - q s, q c + p s)
+    if (turned && A.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p = f[2 * i], q = f[2 * i + 1];
+        f[2 * i] = p * cs[i].x - q * cs[i].y, f[2 * i + 1] = q * cs[i].x + p * cs[i].y;
+      }
+    } else if (turned) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p = f[i], q = f[8 + i];
+        f[i] = p * cs[i].x - q * cs[i].y, f[8 + i] = q * cs[i].x + p * cs[i].y;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y0[i] = (uint32_t)E::put(f[2 * i]) | (uint32_t)E::put(f[2 * i + 1]) << 16;
+      y1[i] = (uint32_t)E::put(f[8 + 2 * i]) | (uint32_t)E::put(f[8 + 2 * i + 1]) << 16;
+    }
+  }
+  *(u32x4r*)(y + a0) = y0;
+  *(u32x4r*)(y + a1) = y1;
 }
 
 template <class E>
 void launch_rows(const RopeAppendArgs& a, hipStream_t stream, hipEvent_t done) {
   const int per = 64 / (a.D / 16), passes = (a.Hq + 2 * a.Hkv + per - 1) / per;
-  const bool many = a.T * passes >= 3 * 4096;  // (four wavefronts a SIMD with three passes each)
-  const int parts = many ? (passes + 2) / 3 : passes;
-  const int64_t blocks = (a.T * parts + 3) / 4;
+  const int64_t blocks = (a.T * passes + 3) / 4;
   if (blocks > INT32_MAX) fail(PJRT_Error_Code_INTERNAL, "rope_append of too many tokens");
-  if (many) launch_k(done, rope_append_rows_kernel<E, 3>, dim3((unsigned)blocks), dim3(256), 0, stream, a, parts);
-  else launch_k(done, rope_append_rows_kernel<E, 1>, dim3((unsigned)blocks), dim3(256), 0, stream, a, parts);
+  launch_k(done, rope_append_rows_kernel<E>, dim3((unsigned)blocks), dim3(256), 0, stream, a, passes);
 }
 
 bool rows_supported(const RopeAppendArgs& a) {

@@ -42,7 +42,7 @@ constexpr int NB = 512;        // bins of a chunk: 64 octaves below its top; wha
 constexpr int kPicks = 1024;   // a chunk's picks, at most
 constexpr int kList = 3840;    // tokens that LDS holds
 constexpr int kAll = 1024;     // tokens up to which all that is kept is listed, if it need not be (3800: 29 us, as one bin 17)
-constexpr int kFew = 1024;     // top_k up to which the counts alone lead to a list of all that is kept
+constexpr int kFew = 1024;     // top_k up to which the counts alone lead to a list of all that is kept (64 rows 33 us; sums too: 41)
 constexpr int kStretch = kChunk / SW;
 constexpr int kStats = 4 + SW; // words of a chunk's results before its bins
 
@@ -55,7 +55,8 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
 __device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
 // Running results over a wavefront's lanes (inclusive; all lanes take part), by moves between lanes inside the registers: a
-// search is little else than these, and each took six trips through LDS (one filtered row of 32000 logits 24 us, 20 so; 64 mixed rows of 128256 70 and 58).
+// search is little else than these, and each took six trips through LDS (one filtered row of 32000 logits 24 us, 20 so; 64
+// mixed rows of 128256 70 and 58).
 template <int CTRL, int ROWS, class T>
 __device__ __forceinline__ T from_lane(T v, T none) {
   if constexpr (sizeof(T) == 4) {
@@ -1002,10 +1003,11 @@ int64_t rows_at_once(const SampleArgs& a) {
 
 void sample_plan(SampleArgs& a, int64_t* ws_bytes) {
   const int64_t vec = 16 / (a.dtype == DT_F32 ? 4 : 2);
-  // Chunks that LDS holds (with room for a row that begins and ends inside 16 bytes); of few rows, more and smaller ones
+  // As few chunks as LDS holds (with room for a row that begins and ends inside 16 bytes). Of few rows, up to 256 smaller ones
+  // are no faster: the search is longer by them (one row of 128256 logits, all filters: 22 us in 16 chunks, 25 in 31). A
+  // workgroup a row, for vocabularies that need more than 64, takes much longer: that row 773 us, 64 of them 1.1 ms and 33 us.
   const int64_t least = (a.V + 2 * vec + kChunk - 1) / kChunk;
-  const int64_t want = a.B ? std::min<int64_t>((256 + a.B - 1) / a.B, a.V / 4096) : 1;
-  a.chunks = least > kMaxChunks || a.B * a.V < vec ? 0 : (int32_t)std::max(least, std::min<int64_t>(want, kMaxChunks));
+  a.chunks = least > kMaxChunks || a.B * a.V < vec ? 0 : (int32_t)least;
   a.rows = (int32_t)rows_at_once(a);
   *ws_bytes = a.chunks ? a.rows * (int64_t)a.chunks * 8 * kChunkWords : 0;
 }
