@@ -221,7 +221,7 @@ struct Rows {
   // the chunk that an index lies in
   __device__ __forceinline__ int chunk(int i) const { return (int)(((off + i) / VEC - v0) / per); }
   // 16 bytes v (read as the operand's last whole ones where they end past it)
-  __device__ __forceinline__ u32x4s load(int v) const { return ((const u32x4s*)x)[min(v0 + v, end - 1)]; }
+  __device__ __forceinline__ u32x4s load(int v) const { return ((const __attribute__((address_space(1))) u32x4s*)x)[min(v0 + v, end - 1)]; }
   __device__ __forceinline__ float get(const u32x4s& w, int e) const {
     if constexpr (ES == 4) return __uint_as_float(w[e]);
     else return E::get((raw)(w[e / 2] >> (16 * (e % 2))));
@@ -519,41 +519,55 @@ __device__ __attribute__((noinline)) uint64_t list_select(SampleLds& sh, uint64_
   return prefix;
 }
 
+// i & bit ? a : b, as one instruction (the compiler makes an array in memory of a tree of these)
+__device__ __forceinline__ float select_bit(int i, int bit, float a, float b) {
+  float y;
+  asm("v_cndmask_b32 %0, %1, %2, %3" : "=v"(y) : "v"(b), "v"(a), "s"(__builtin_amdgcn_ballot_w64(i & bit)));
+  return y;
+}
 // The list: the row's tokens with keys in [from, to), by a pass over the row, 32 logits a thread in flight.
 template <class E>
 __device__ __attribute__((noinline)) void list_row(const SampleArgs& A, int64_t r, SampleLds& sh, uint32_t from, uint32_t to) {
   constexpr int VEC = Rows<E>::VEC;
   const Rows<E> row(A, r);
   const int tid = threadIdx.x;
+  const float least = key_logit(from), past = key_logit(to);  // (NaN: past +inf)
   // (between the row's first and last 16 bytes)
   constexpr int U = 32 / VEC;
-  for (int b = 1; b < row.vecs - 1; b += U * ST) {
-    u32x4s w[U];
+  u32x4s next[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = row.load(min(b + u * ST + tid, row.vecs - 1));
+  for (int u = 0; u < U; ++u) next[u] = row.load(min(1 + u * ST + tid, row.vecs - 1));
+  for (int b = 1; b < row.vecs - 1; b += U * ST) {
+    float x[32];
     uint32_t hits = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint32_t bits = 0;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const uint32_t key = logit_key(row.get(w[u], e));
-        bits |= (key >= from && key < to ? 1u : 0u) << e;
+        x[u * VEC + e] = row.get(next[u], e);
+        bits |= (x[u * VEC + e] >= least && !(x[u * VEC + e] >= past) ? 1u : 0u) << e;
       }
       if (b + u * ST + tid < row.vecs - 1) hits |= bits << (u * VEC);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = row.load(min(b + (U + u) * ST + tid, row.vecs - 1));
     int at = list_room(&sh.n, __builtin_popcount(hits));
-    // (from the registers: read again, every token waited for memory: 57 us for 3800 of 128256)
+    // (from the registers, by a tree of selections: a branch for each logit took 3 us a pass, read again every token waited
+    // for memory)
+    while (hits) {
+      const int i = __builtin_ctz(hits);
+      hits &= hits - 1;
+      float y[16];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (hits >> (u * VEC) & ((1u << VEC) - 1)) {
+      for (int k = 0; k < 16; ++k) y[k] = select_bit(i, 16, x[k + 16], x[k]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (hits >> (u * VEC + e) & 1) {
-            if (at < kList) sh.list[at] = (uint64_t)logit_key(row.get(w[u], e)) << 32 | (uint32_t)~(row.index(b + u * ST + tid) + e);
-            ++at;
-          }
-      }
+      for (int half = 8; half; half >>= 1)
+#pragma unroll
+        for (int k = 0; k < half; ++k) y[k] = select_bit(i, half, y[k + half], y[k]);
+      if (at < kList) sh.list[at] = (uint64_t)logit_key(y[0]) << 32 | (uint32_t)~(row.index(b + i / VEC * ST + tid) + i % VEC);
+      ++at;
+    }
   }
   if (tid < 64) {
     const int i = tid < VEC ? row.index(0) + tid : row.vecs > 1 && tid < 2 * VEC ? row.index(row.vecs - 1) + tid - VEC : -1;
@@ -707,9 +721,15 @@ __device__ __forceinline__ uint64_t filtered(const SampleArgs& A, int64_t r, uin
 #pragma unroll
     for (int u = 0; u < 16; ++u) {
       const int i = min(i0 + u, C - 1), b = min(max(tid - sh.shift[i], 0), NB - 1);
-      w[u] = want.few ? 0 : ws.mass[i * NB + b];
       q[u] = ws.count[i * NB + b];
+      w[u] = 0;
     }
+    if (!want.few)  // (a branch for all of them: with one each they followed each other)
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int i = min(i0 + u, C - 1);
+        w[u] = ws.mass[i * NB + min(max(tid - sh.shift[i], 0), NB - 1)];
+      }
 #pragma unroll
     for (int u = 0; u < 16; ++u) {
       const int i = min(i0 + u, C - 1);
