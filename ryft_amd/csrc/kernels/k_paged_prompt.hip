@@ -9,7 +9,7 @@
 // The matrix products and the exponentials bound it (a wavefront's float instructions and matrix instructions add up):
 // the exponent reference moves only when a block exceeds it by 2^8, and masks are applied only in the blocks that need
 // one. Two or three workgroups share a CU, so that one's waits for LDS are the others' work. Measured, heads of 128 and 64: four
-// prompts of 875 to 1824 tokens, 32 heads, capped, 116 us (550 TFLOP/s); two chunks of 512 with a window of 4096, 38 us;
+// prompts of 875 to 1824 tokens, 32 heads, capped, 116 us (550 TFLOP/s); two chunks of 512 with a window of 4096, 36 us;
 // 256 x 4 queries of two sequences of 60000 keys 87 us (720 TFLOP/s); 16 rows over 4 x 8 x 16000 keys 105 us (5.0 TB/s).
 #include <hip/hip_runtime.h>
 
@@ -28,10 +28,11 @@ namespace {
 
 constexpr int BKV = 64;  // keys a block
 // Workgroups that share a CU, by registers and LDS (2048 queries of two heads of 64 over 65000 keys: 99 us with three, 111
-// with two; capped or biased scores take registers that three do not have: a chunk of such 41 us with three, 38 with two).
-__host__ __device__ constexpr int prompt_shares(int D, bool general) { return D == 64 && !general ? 3 : 2; }
+// with two; two chunks of 512, biased, 36 and 38). Caps and biases in kernels of their own are what leaves room for it: in
+// one kernel they spilled, 41 us.
+__host__ __device__ constexpr int prompt_shares(int D, bool cap, bool bias) { return D == 64 && !(cap && bias) ? 3 : 2; }
 // Workgroups where tiles are cut into ranges of keys, at most
-__host__ __device__ constexpr int prompt_ranges(int D) { return 256 * prompt_shares(D, false); }
+__host__ __device__ constexpr int prompt_ranges(int D) { return 256 * prompt_shares(D, false, false); }
 constexpr int kMaxParts = 128;  // ranges of a tile (two tiles of 85 rows × 31072 keys: 23 us with at most 128, 29 with 243)
 
 // The workspace of a launch with ranges: the parts (one a workgroup, of kPromptRows rows), the number of tiles, and for each
@@ -107,9 +108,9 @@ __device__ __forceinline__ int wave_max(int v) {  // (of values of at least 0)
   return __builtin_amdgcn_readlane(v, 63);
 }
 
-// GENERAL: scores may be capped or biased by distance.
-template <class X, class E, int D, bool GENERAL>
-__global__ void __launch_bounds__(256, prompt_shares(D, GENERAL)) paged_prompt_kernel(const PagedAttnArgs A) {
+// CAP, BIAS: scores are capped, biased by distance.
+template <class X, class E, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt_kernel(const PagedAttnArgs A) {
   typedef PromptCfg<D> C;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float row_ml[kPromptRows][2];
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(256, prompt_shares(D, GENERAL)) paged_prompt_k
     // Every tile in ranges of about `each` blocks (a sequence's tiles in as many as its last has), the least with which all
     // fit into the launch: ragged lengths need no other balancing.
     auto cuts_of = [&](int each) { return max(1, min((int)A.splits, (min((len + BKV - 1) / BKV, most) + each - 1) / each)); };
-    int room = 256 * prompt_shares(D, GENERAL) / A.Hkv;
+    int room = 256 * prompt_shares(D, CAP, BIAS) / A.Hkv;
     auto over = [&](auto&& f) {  // the sum of f over the sequences, at most 2^24
       int sum = 0;
       for (int b = 0; b < A.B; b += 64) {
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(256, prompt_shares(D, GENERAL)) paged_prompt_k
   const int w_all_hi = last_key(wq0), w_any_hi = last_key(wq1), w_all_lo = first_key(wq1), w_any_lo = first_key(wq0);
   const int flat = t.row0 + min(32 * wave + (lane & 31), rows - 1), qi = flat / G, h = t.hk * G + (flat - qi * G);
   const int pos = t.pos0 + qi, hi = last_key(qi), lo = first_key(qi);
-  const float slope = GENERAL && A.slopes ? A.slopes[h] * kLog2e : 0.f;
+  const float slope = BIAS ? A.slopes[h] * kLog2e : 0.f;
 
   // Blocks into LDS: a wave-wide load fills 1 KB, the lane that fills chunk position c of row r takes chunk c ^ swz(r).
   // (The swizzle depends on r mod 16, the same for all loads of a lane.)
@@ -350,51 +351,42 @@ __global__ void __launch_bounds__(256, prompt_shares(D, GENERAL)) paged_prompt_k
     }
     // exponents relative to the reference, masked; key of register r: kb + 32 tt + 8 (r / 4) + 4 half + r % 4
     const float ref = m == -INFINITY ? 0.f : m;
-    if constexpr (GENERAL) {
-      const float base = slope * (float)(kb + 4 * half - pos) - ref;
-      auto scores = [&](auto&& bias) {  // (the last operation of every form adds the bias: none costs one for it)
-        if (!(score.cap2 > 0.f)) {
+    // (the last operation of every form adds the bias: none costs one for it)
+    const float base = BIAS ? slope * (float)(kb + 4 * half - pos) - ref : -ref;
+    auto bias = [&](int tt, int r) { return BIAS ? __builtin_fmaf(slope, (float)(32 * tt + 8 * (r >> 2) + (r & 3)), base) : base; };
+    if constexpr (CAP) {
+      // tanh z = z P(z²) to 2^-25 for |z| <= 1/2, a polynomial that interpolates at Chebyshev nodes: 28 cycles a score
+      // instead of 48, in the blocks where no score reaches half the cap (four prompts of up to 2048 tokens 136 -> 120 us)
+      float top = 0.f;
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
+      for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) st[tt][r] = __builtin_fmaf(st[tt][r], score.sl2, bias(tt, r));
-          return;
-        }
-        // tanh z = z P(z²) to 2^-25 for |z| <= 1/2, a polynomial that interpolates at Chebyshev nodes: 28 cycles a score
-        // instead of 48, in the blocks where no score reaches half the cap (four prompts of up to 2048 tokens 136 -> 120 us)
-        float top = 0.f;
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[tt][r]));
+      if (__builtin_amdgcn_ballot_w64(!(top * fabsf(cap_scale) <= 0.5f))) {
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[tt][r]));
-        if (__builtin_amdgcn_ballot_w64(!(top * fabsf(cap_scale) <= 0.5f))) {
+          for (int r = 0; r < 16; ++r) {
+            const float e = __builtin_amdgcn_exp2f(st[tt][r] * score.capz);
+            st[tt][r] = __builtin_fmaf(-2.f * score.cap2, __builtin_amdgcn_rcpf(e + 1.f), score.cap2 + bias(tt, r));
+          }
+      } else {
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
+        for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float e = __builtin_amdgcn_exp2f(st[tt][r] * score.capz);
-              st[tt][r] = __builtin_fmaf(-2.f * score.cap2, __builtin_amdgcn_rcpf(e + 1.f), score.cap2 + bias(tt, r));
-            }
-        } else {
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float z = st[tt][r] * cap_scale, zz = z * z;
-              float p = __builtin_fmaf(zz, 0x1.18d7e8p-6f, -0x1.b2167ep-5f);
-              p = __builtin_fmaf(zz, p, 0x1.10e47ap-3f);
-              p = __builtin_fmaf(zz, p, -0x1.5554a6p-2f);
-              st[tt][r] = __builtin_fmaf(__builtin_fmaf(zz, p, 1.f), z * score.cap2, bias(tt, r));
-            }
-        }
-      };
-      if (A.slopes) scores([&](int tt, int r) { return __builtin_fmaf(slope, (float)(32 * tt + 8 * (r >> 2) + (r & 3)), base); });
-      else scores([&](int, int) { return -ref; });
+          for (int r = 0; r < 16; ++r) {
+            const float z = st[tt][r] * cap_scale, zz = z * z;
+            float p = __builtin_fmaf(zz, 0x1.18d7e8p-6f, -0x1.b2167ep-5f);
+            p = __builtin_fmaf(zz, p, 0x1.10e47ap-3f);
+            p = __builtin_fmaf(zz, p, -0x1.5554a6p-2f);
+            st[tt][r] = __builtin_fmaf(__builtin_fmaf(zz, p, 1.f), z * score.cap2, bias(tt, r));
+          }
+      }
     } else {
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st[tt][r] = __builtin_fmaf(st[tt][r], score.sl2, -ref);
+        for (int r = 0; r < 16; ++r) st[tt][r] = __builtin_fmaf(st[tt][r], score.sl2, bias(tt, r));
     }
     if (kb + BKV - 1 > w_all_hi || kb < w_all_lo) {
 #pragma unroll
@@ -613,8 +605,8 @@ void launch_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) 
     if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("paged_attention LDS attribute: ") + hipGetErrorString(e));
     launch_k(a.splits > 1 ? nullptr : done, kernel, grid, block, lds, stream, a);
   };
-  if (a.softcap > 0.f || a.slopes) go(paged_prompt_kernel<X, E, D, true>);
-  else go(paged_prompt_kernel<X, E, D, false>);
+  if (a.softcap > 0.f) a.slopes ? go(paged_prompt_kernel<X, E, D, true, true>) : go(paged_prompt_kernel<X, E, D, true, false>);
+  else a.slopes ? go(paged_prompt_kernel<X, E, D, false, true>) : go(paged_prompt_kernel<X, E, D, false, false>);
   if (a.splits <= 1) return;
   const unsigned tiles = (unsigned)a.max_tiles, chunks = kPromptRows * D / 4 / 256;
   if (tiles <= 32) launch_k(done, paged_prompt_join_kernel<X, D, 4>, dim3(tiles * chunks * 4), block, 0, stream, a);
