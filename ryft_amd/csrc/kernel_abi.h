@@ -392,10 +392,10 @@ struct PagedAttnArgs {
   // set by paged_attention_plan: the kernel and its split
   int32_t tile_rows;      // rows (query, head of a group) of a tile (0: the kernel for any type and head dim)
   int32_t groups;         // workgroups
-  int32_t min_units;      // least stretch of a workgroup
   int32_t splits;         // ranges of keys of a tile of 128 rows, at most
   int32_t max_tiles;      // counters
   int32_t page_shift;     // key / P = key · page_mul >> page_shift
+  int32_t pad_;
   uint64_t page_mul;
   float* ws;              // partial results; every one that is read was written by the same launch
   int32_t* counters;      // arrivals, one a tile: zero between launches

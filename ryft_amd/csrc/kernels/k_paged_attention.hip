@@ -209,16 +209,17 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
   };
   auto last_lane = [&](int v) { return __builtin_amdgcn_readlane(v, 63); };
   // The whole line's length (paged_attention_plan keeps it below 2^30); workgroup w has [w q + min(w, r), ...) of it, a
-  // unit more where w < r, and none where the stretches would fall below the least and a tile.
+  // unit more where w < r.
   FewSeq seq = sequence(lane);
   int incl = scan(seq.units * seq.tiles), tiles_incl = scan(seq.tiles);
-  int all = last_lane(incl), all_tiles = last_lane(tiles_incl);
+  int all = last_lane(incl);
   for (int b = 64; b < A.B; b += 64) {
     const FewSeq s = sequence(b + lane);
-    all += last_lane(scan(s.units * s.tiles)), all_tiles += last_lane(scan(s.tiles));
+    all += last_lane(scan(s.units * s.tiles));
   }
-  // (a workgroup a tile where they are short: 35 sequences of up to 18 keys took 22 us in 8 stretches, 9 in 35)
-  const int working = uni(max(1, min(W, max(all / A.min_units, min(all, all_tiles)))));
+  // (down to a unit a stretch: with 4 as the least, 16 queries over 5624 keys took 27 us, 17 so, and 35 sequences of up to 18
+  // keys 22 and 9)
+  const int working = uni(max(1, min(W, all)));
   const int q_units = uni(all / working), r_units = all - q_units * working;
   const int w = blockIdx.x;
   if (w >= working) return;
@@ -624,13 +625,12 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
   if (rows > 16 || (tiles128 <= 32 && keys >= (tiles128 >= 16 ? 8192 : 16384))) return paged_prompt_plan(a, ws_floats);
   a.tile_rows = TR;
   const int unit = a.D == 128 ? 128 : 256;
-  a.min_units = 512 / unit;
   const int64_t tiles = (a.T * G / a.tile_rows + a.B) * a.Hkv;
   // (units are counted in 32 bits)
   if (a.T * a.Hq > INT32_MAX || tiles > (1 << 30) / ((int64_t)a.M * a.P / unit + 1)) { a.tile_rows = 0; return; }
   a.max_tiles = (int32_t)tiles;
   // two workgroups a CU, fewer if even the longest sequences have no work for them
-  const int64_t most = tiles * (((int64_t)a.M * a.P + 511) / 512 + 1);
+  const int64_t most = tiles * (((int64_t)a.M * a.P + unit - 1) / unit + 1);
   a.groups = (int32_t)std::max<int64_t>(1, std::min<int64_t>(512, most));
   *ws_floats = 2 * a.groups * paged_part_floats(a.tile_rows, a.D);
   *counters = a.max_tiles;
