@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAtt
 //    are in flight, while the values are weighed the next keys.
 // Scores come transposed, S = K · Qᵀ, so that a lane has one row's scores and the probabilities, rounded and packed, are
 // the second operand of Oᵀ = Vᵀ · Pᵀ as they are; transposing LDS reads give the first. Measured: 64 sequences of 8 to 4096
-// keys, 32 heads on 8 of 128: 110 us (4.9 TB/s; all of 4096: 5.5); 8 x 2 queries over 20000 keys of 8 heads of 64: 70 us
+// keys, 32 heads on 8 of 128: 110 us (4.8 TB/s; all of 4096: 5.5); 8 x 2 queries over 20000 keys of 8 heads of 64: 70 us
 // (4.7 TB/s); one query of 8 heads over 500 keys: 9 us, as any launch from the host.
 constexpr int FEW_WAVES = 4;
 constexpr int TR = 16;  // rows of a tile
@@ -619,8 +619,8 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
   // The other kernel takes tiles of up to 128 rows, and its parts are joined by a second launch of the whole chip, here a
   // tile's by one workgroup. Heads of 128 over 4 x 4 queries of 8 sequences of 16000 keys: 102 us there, 132 here in tiles
   // of 32 rows; 3 x 5 queries of 5 heads of 64 over 12811 keys 25 and 38. With 16 rows or fewer it is the parts of a tile
-  // that decide: one query of 5 heads over 30000 keys of two heads 19 and 30 us, 8 queries of 4 x 4 heads over 9000 keys
-  // 39 and 42, but one over 9000 keys of one head 14 and 12, and 8 of 8 x 4 over 4000 34 and 32.
+  // that decide: one query of 5 heads over 30000 keys of two heads 19 and 38 us, 8 queries of 4 x 4 heads over 9000 keys
+  // 39 and 42, but one over 9000 keys of one head 13 and 12, and 8 of 8 x 4 over 4000 34 and 33.
   const int64_t tiles128 = (a.T * G / kPromptRows + a.B) * a.Hkv, keys = (int64_t)a.M * a.P;
   if (rows > 16 || (tiles128 <= 32 && keys >= (tiles128 >= 16 ? 8192 : 16384))) return paged_prompt_plan(a, ws_floats);
   a.tile_rows = TR;
