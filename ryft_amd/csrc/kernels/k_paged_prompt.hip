@@ -26,7 +26,7 @@ namespace ryft {
 
 namespace {
 
-constexpr int BKV = 64;  // keys a block
+constexpr int BKV = kPromptKeys;
 // Workgroups that share a CU, by registers and LDS (2048 queries of two heads of 64 over 65000 keys: 99 us with three, 111
 // with two; two chunks of 512, biased, 36 and 38). Caps and biases in kernels of their own are what leaves room for it: in
 // one kernel they spilled, 41 us.
@@ -107,6 +107,26 @@ __device__ __forceinline__ int wave_max(int v) {  // (of values of at least 0)
   v = max(v, dpp_int<0x143, 0xc>(v));
   return __builtin_amdgcn_readlane(v, 63);
 }
+
+// prompt_nth_tile's sequences, one a lane.
+struct PromptWave {
+  PromptSeq own;
+  template <class F>
+  __device__ __forceinline__ int sum(F&& f) const { return wave_total(f(own)); }
+  template <class F>
+  __device__ __forceinline__ int largest(F&& f) const { return wave_max(f(own)); }
+  template <class F>
+  __device__ __forceinline__ int first_past(F&& f, int target, int* before) const {
+    const int v = f(own), incl = wave_scan(v);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(incl > target);
+    if (!past) return -1;
+    const int who = __builtin_ctzll(past);
+    *before = __builtin_amdgcn_readlane(incl - v, who);
+    return who;
+  }
+  template <class F>
+  __device__ __forceinline__ int at(int who, F&& f) const { return __builtin_amdgcn_readlane(f(own), who); }
+};
 
 // CAP, BIAS: scores are capped, biased by distance.
 template <class X, class E, int D, bool CAP, bool BIAS>
@@ -196,32 +216,11 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
   } else if (A.B <= 64) {
     // Row tiles in falling order of the blocks of keys they see, over all sequences, so that the chip does not wait for
     // long ones that began late (four causal prompts of 875 to 1824 tokens: the last workgroup ended 26% after the mean).
-    // The place in that order is found without a sort: a sequence a lane, the number of blocks that as many tiles reach by
-    // bisection, then the tile among those of that number.
     sequence(lane);
-    const int all = A.causal ? 0 : tiles;  // (not causal: every tile sees all)
-    auto reach = [&](int c) {  // tiles that see c blocks or more
-      if (c > most) return 0;
-      if (!A.causal) return (len + BKV - 1) / BKV >= c ? all : 0;
-      const int q = BKV * (c - 1) - (len - n);  // the first query that does
-      if (q <= 0) return tiles;
-      return q >= n ? 0 : tiles - (int)(((uint32_t)G * q + kPromptRows) / kPromptRows) + 1;
-    };
-    if (want >= wave_total(tiles)) return;
-    int lo = 0, hi = wave_max(min((len + BKV - 1) / BKV, most)) + 1;  // more than `want` tiles see lo blocks, not more see hi
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (wave_total(reach(mid)) > want) lo = mid;
-      else hi = mid;
-    }
-    const int above = reach(hi), equal = reach(lo) - above;
-    const int incl = wave_scan(equal), rest = want - wave_total(above);
-    const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(incl > rest));
-    t.b = who;
-    t.s0 = __builtin_amdgcn_readlane(s0, who);
-    t.n = __builtin_amdgcn_readlane(n, who);
-    // (the last `above` tiles of a sequence see more, the `equal` before those as many)
-    const int tile = __builtin_amdgcn_readlane(tiles - above - equal + rest - (incl - equal), who);
+    int tile = 0;
+    if (!prompt_nth_tile(PromptWave{PromptSeq{n, len, tiles}}, G, A.causal, most, want, &t.b, &tile)) return;
+    t.s0 = __builtin_amdgcn_readlane(s0, t.b);
+    t.n = __builtin_amdgcn_readlane(n, t.b);
     t.row0 = tile * kPromptRows;
   } else {
     // from the last sequence to the first, 64 at a time, each from its last tile

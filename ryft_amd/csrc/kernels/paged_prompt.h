@@ -2,10 +2,9 @@
 #pragma once
 
 #include "kernels.h"
+#include "prompt_tiles.h"
 
 namespace ryft {
-
-constexpr int kPromptRows = 128;  // rows of a tile (PagedAttnArgs::tile_rows)
 
 void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats);
 void launch_paged_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done);
