@@ -179,17 +179,13 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
   const int G = A.Hq / A.Hkv, W = (int)gridDim.x;
   const PagedScore score(A);
 
-  // rows of no sequence
-  for (int64_t t = blockIdx.x; t < A.T; t += W) {
-    if (t >= paged_start(A, 0) && t < paged_start(A, A.B)) continue;
-    for (int64_t i = tid; i < (int64_t)A.Hq * D; i += 256) ((uint16_t*)A.o)[t * A.Hq * D + i] = 0;
-  }
-
+  bool falls = false;  // of the lane's sequences, one ends before it begins
   auto sequence = [&](int b) {
     FewSeq s{0, 0, 0, 0, 0};
     if (b < A.B) {
       s.s0 = paged_start(A, b);
-      s.n = max(0, paged_start(A, b + 1) - s.s0);
+      s.n = paged_start(A, b + 1) - s.s0;
+      falls |= s.n < 0;
       s.len = paged_length(A, b);
       if (s.n > 0) {
         const int first = A.window > 0 ? (int)max((int64_t)0, (int64_t)s.len - s.n - A.window + 1) / C::KB * C::KB : 0;
@@ -217,6 +213,15 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
     const FewSeq s = sequence(b + lane);
     all += last_lane(scan(s.units * s.tiles));
   }
+  // Rows of no sequence; all of them where starts decrease. Those may name more tiles than there are counters for, and a line
+  // longer than 32 bits count, whose parts would wait for workgroups that never come and leave their counters behind for
+  // the next launch.
+  const bool none = __builtin_amdgcn_ballot_w64(falls) != 0;
+  for (int64_t t = blockIdx.x; t < A.T; t += W) {
+    if (!none && t >= paged_start(A, 0) && t < paged_start(A, A.B)) continue;
+    for (int64_t i = tid; i < (int64_t)A.Hq * D; i += 256) ((uint16_t*)A.o)[t * A.Hq * D + i] = 0;
+  }
+  if (none) return;
   // (down to a unit a stretch: with 4 as the least, 16 queries over 5624 keys took 27 us, 17 so, and 35 sequences of up to 18
   // keys 22 and 9)
   const int working = uni(max(1, min(W, all)));
@@ -231,15 +236,10 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
   const int end = at + q_units + (w < r_units ? 1 : 0);
   if (at >= end) return;
   int b0 = 0, before = 0, tiles_before = 0;  // units and tiles of the sequences before b0
-  auto next_range = [&]() {  // (the same in every wavefront)
+  auto next_range = [&]() {  // (the same in every wavefront; `at` lies on the line)
     FewRange R;
-    R.rows = 0;
     int here = last_lane(incl);
     while (at >= before + here) {
-      if (b0 + 64 >= A.B) {  // (starts that decrease: their sums may have overflowed)
-        at = end;
-        return R;
-      }
       before += here;
       tiles_before += last_lane(tiles_incl);
       b0 += 64;
@@ -341,7 +341,6 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
   int parts = 0;
   u32x4p qf[D / 32];
   FewRange R = next_range();
-  if (R.rows <= 0) return;
   begin(R, qf);
   while (true) {
     const PagedTile t = R.t;
@@ -472,13 +471,10 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
     // The next range's first block is on its way before the wavefronts join this one's rows, where the rows fit beside the
     // ring: waiting for each other, for the workspace and for that block one after the other took as long as two blocks.
     const bool early = rows <= C::STAGE_ROWS;
-    bool more_ranges = at < end;
+    const bool more_ranges = at < end;
     const FewRange cur = R;
     u32x4p qn[D / 32];
-    if (more_ranges) {
-      R = next_range();
-      more_ranges = R.rows > 0;
-    }
+    if (more_ranges) R = next_range();
     if (early && more_ranges) begin(R, qn);
     // staged outputs [wave][rows][OP], summed by all threads
     const bool whole = cur.u0 == 0 && cur.u1 == cur.units;
@@ -560,7 +556,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       }
     }
     few_barrier();
-    if (!whole && cur.index < A.max_tiles) {
+    if (!whole) {
       // (its first range and its last: no workgroup has more parts than two)
       const int w0 = owner(cur.at), w1 = owner(cur.at + cur.units - 1);
       const FewPart P{t, rows, w0, w1 - w0 + 1, cur.index};

@@ -6,7 +6,7 @@ import torch  # noqa: F401  (before the plugin: both then use one HIP runtime)
 
 from oracle import operators as oo
 from oracle import stablehlo as sh
-from ryft_amd import pjrt
+from ryft_amd import operators, pjrt
 from tests import operator_programs as op
 from tests.test_gpu_operators import attention_error, close, device_buffers, span, sync
 
@@ -52,3 +52,34 @@ def test_more_queries_than_keys(gpu_client, name, d, dtype):
     close(got, want, dtype, attention_error(x, dtype), name)
     unseen = ~want.any(axis=(1, 2))
     assert unseen.any() and not got[unseen].any()                     # rows that see nothing are exactly zero
+
+
+# ------------------------------------------------------------------------------------------------ starts that decrease
+@pytest.mark.parametrize("starts, sequences", [([0, 4000] * 1053 + [0], 2106), ([0, 9, 3, 12] + [12] * 400, 403)], ids=["long", "short"])
+def test_starts_that_decrease_leave_nothing_behind(gpu_client, starts, sequences):
+    # a decoding step whose starts name far more rows than there are (the first: so many that a count of their units in 32 bits
+    # ends inside a tile of sequence 311): zeros, and the next call on the same executable gives what the one before gave
+    tokens, pages, size, per = max(starts), 3, 512, 255
+    r = np.random.RandomState(7)
+    lengths = r.randint(1, 3000, sequences)
+    lengths[311] = size * per - 100
+    module = operators.paged_attention_module(tokens=tokens, sequences=sequences, q_heads=32, kv_heads=8, head_dim=64, pages=pages,
+                                              page_size=size, pages_per_sequence=per, scale=0.125)
+    cache, good = (pages, 8, size, 64), np.maximum(0, np.arange(sequences + 1) - (sequences - min(sequences, tokens)))
+    ins = [op.host(r.randn(tokens, 32, 64), "bf16"), op.host(r.randn(*cache), "bf16"), op.host(r.randn(*cache), "bf16"),
+           op.host(r.randint(0, pages, (sequences, per)), "i32"), op.host(good, "i32"), op.host(lengths, "i32")]
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    bufs = device_buffers(gpu_client, ins)
+    bad = device_buffers(gpu_client, [op.host(starts, "i32"), op.host(np.full(sequences, size * per), "i32")])
+    (out,) = device_buffers(gpu_client, [op.host(np.full((tokens, 32, 64), 7.0), "bf16")])
+
+    def execute(args):
+        exe.execute_into([span(b) for b in args], [span(out)])
+        sync()
+        return sh.from_raw(out.to_numpy(), "bf16")
+
+    want = execute(bufs)
+    assert np.isfinite(want).all() and want[:min(sequences, tokens)].any() and not want[sequences:].any()
+    for _ in range(2):
+        assert not execute(bufs[:4] + bad).any()
+        assert np.array_equal(execute(bufs), want)
