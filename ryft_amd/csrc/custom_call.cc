@@ -59,7 +59,7 @@ struct Call {
 };
 
 constexpr int64_t kMaxHeadDim = 256;
-constexpr double kFloatMax = 3.4028234663852886e38;
+constexpr double kFloatMax = 0x1.fffffefffffffp127;  // the largest that rounds to a finite f32
 
 void check_cache(const Call& c, const TensorType& kc, const TensorType& vc, DType dt, int64_t hkv, int64_t d) {
   c.rank("the key cache", kc, 4);
