@@ -386,10 +386,8 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       const bool mask = kb + C::KB - 1 > all_hi || kb < all_lo;
       uint32_t pf[C::KT * 2];
       if (score.cap2 > 0.f) {
-#pragma unroll
-        for (int tt = 0; tt < C::KT; ++tt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) st[tt][i] = score.capped(st[tt][i]);
+        auto at = [&](int i) -> float& { return ((float*)st)[i]; };
+        score.cap<C::KT * 4>(at, [](int) { return 0.f; });
       } else {
 #pragma unroll
         for (int tt = 0; tt < C::KT; ++tt) st[tt] *= score.sl2;

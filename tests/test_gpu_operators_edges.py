@@ -83,3 +83,54 @@ def test_starts_that_decrease_leave_nothing_behind(gpu_client, starts, sequences
     for _ in range(2):
         assert not execute(bufs[:4] + bad).any()
         assert np.array_equal(execute(bufs), want)
+
+
+# ------------------------------------------------------------------------------------------------ caps of any size
+CAPPED = {
+    # a decoding step, prompts, ranges of keys, the kernel for any type and head dim
+    "step": dict(new=[1, 1, 3], lengths=[300, 40, 70], heads=(8, 2, 128)),
+    "step_64": dict(new=[1, 1, 3], lengths=[300, 40, 70], heads=(4, 4, 64), slopes=True),
+    "prompt": dict(new=[150, 9], lengths=[150, 64], heads=(4, 2, 128)),
+    "prompt_64": dict(new=[150, 9], lengths=[150, 64], heads=(4, 2, 64), slopes=True),
+    "ranges": dict(new=[30, 2], lengths=[1500, 700], heads=(4, 1, 64)),
+    "any": dict(new=[1, 30], lengths=[200, 90], heads=(4, 2, 80)),
+}
+
+
+@pytest.mark.parametrize("poison", [False, True], ids=["", "poison"])
+@pytest.mark.parametrize("softcap", [1e-42, 1e-38, 1e-6, 0.25, 1.0, 1e3, 1e5, 1e6, 1e7, 1e9, 1e20, 1e38, 3.4028234663852886e38], ids=str)
+@pytest.mark.parametrize("name", CAPPED)
+def test_caps_of_any_size(gpu_client, name, softcap, poison):
+    # far above the scores a cap changes nothing, far below them every score is the cap's sign; also beside infinite and
+    # NaN keys that nothing sees
+    c = dict(CAPPED[name])
+    new, lengths, heads = (c.pop(k) for k in ("new", "lengths", "heads"))
+    for dtype in ("bf16", "f32") if name == "any" else ("bf16", "f16"):
+        module, ins = op.attention_case(new, lengths, *heads, 16, dtype, seed=17, softcap=softcap, poison=poison, **c)
+        q = op.values(ins)[0]
+        q[-1] = 0.0                                                   # (scores of zero stay so under any cap)
+        ins[0] = op.host(q, dtype)
+        (got,) = run_over(gpu_client, module, ins, [(ins[0].dims, dtype)])
+        x = op.values(ins)
+        want, = oo.paged_attention(x, op.config_of(module))
+        assert np.isfinite(want).all()
+        close(got, want, dtype, attention_error(x, dtype), (name, softcap, dtype))
+
+
+@pytest.mark.parametrize("softcap", [40.0, 300.0, 500.0, 5000.0], ids=str)
+@pytest.mark.parametrize("new, lengths, d", [([1, 2], [300, 70], 128), ([1, 2], [300, 70], 64), ([70], [200], 128), ([70], [200], 64),
+                                             ([3], [90], 80)], ids=str)
+def test_caps_near_scores_of_hundreds(gpu_client, new, lengths, d, softcap):
+    # scores on both sides of half the cap, beside each other in a block; keys past the first of small size, so that scores
+    # near zero are weighed against each other while larger ones of either sign stand among them
+    hkv, tokens = 2, sum(new)
+    module, ins = op.attention_case(new, lengths, 4, hkv, d, 16, "bf16", seed=19, softcap=softcap)
+    q, kc = op.values(ins)[:2]
+    q[:], kc[:] = np.abs(q), kc * 0.01
+    kc[:, :, 3] = -300.0 * np.abs(kc[:, :, 3]) / 0.01 / np.sqrt(d)    # (far below the others, and far past the cap's half)
+    ins[0], ins[1] = op.host(q, "bf16"), op.host(kc, "bf16")
+    (got,) = run_over(gpu_client, module, ins, [(ins[0].dims, "bf16")])
+    x = op.values(ins)
+    want, = oo.paged_attention(x, op.config_of(module))
+    assert np.isfinite(want).all()
+    close(got, want, "bf16", attention_error(x, "bf16"), softcap)
