@@ -403,9 +403,10 @@ struct PagedAttnArgs {
 
 // ryft.sample (k_sample.hip): for each row of logits [B, V], in 64 bits, w_i = exp((x_i - max x) / temperature); of the
 // tokens with w_i > 0, those among the top_k largest (0: all; equal logits: the lower index first), with w_i >= min_p
-// (relative to the largest), and preceded in that order by less than top_p of the weight left so far; then token = the
-// first index whose running sum of kept weights exceeds uniform · their total, logprob = log(w / total). temperature 0
-// is the largest logit. NaN logits are never drawn; a row without any logit above -inf gives token -1, logprob -inf.
+// (relative to the largest; above 1: the first of the largest alone), and preceded in that order by less than top_p of the
+// weight left so far; then token = the first index whose running sum of kept weights exceeds uniform · their total,
+// logprob = log(w / total). temperature 0 is the largest logit. NaN logits are never drawn; a row without any logit above
+// -inf gives token -1, logprob -inf.
 struct SampleArgs {
   const void* logits;
   const float* temperature;

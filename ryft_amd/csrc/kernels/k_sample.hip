@@ -362,7 +362,7 @@ __device__ __attribute__((noinline)) void sample_row(const SampleArgs& A, int64_
   int low_last = V;
   const int k = A.top_k[r];
   auto kept = [&](int i, uint32_t key) {
-    return (key > low || (key == low && i <= low_last)) && (key == top || !(wt.real(key_logit(key)) < minp));
+    return (key > low || (key == low && i <= low_last)) && !(wt.real(key_logit(key)) < minp);
   };
   if (k > 0 && k < V) {
     auto one = [&](int, uint32_t key) -> uint64_t { return key != 0; };
@@ -577,6 +577,9 @@ __device__ __attribute__((noinline)) void list_row(const SampleArgs& A, int64_t 
   }
 }
 
+// Whether a row takes the first of its largest logits: no weight is at least a min_p above 1, and the largest is kept.
+__device__ __forceinline__ bool greedy_row(const SampleArgs& A, int64_t r) { return !(A.temperature[r] > 0.f) || !(A.min_p[r] <= 1.f); }
+
 // What a row asks for.
 struct Wanted {
   bool greedy, by_count, by_weight, by_mass, filtered;
@@ -588,7 +591,7 @@ struct Wanted {
     const float temp = A.temperature[r];
     k = A.top_k[r];
     minp = A.min_p[r], p = A.top_p[r];
-    greedy = !(temp > 0.f);
+    greedy = greedy_row(A, r);
     by_count = k > 0 && k < A.V, by_weight = minp > 0.0, by_mass = p < 1.0;
     filtered = !greedy && (by_count || by_weight || by_mass);
     few = filtered && by_count && k <= kFew;
@@ -810,7 +813,7 @@ __device__ __forceinline__ uint64_t filtered(const SampleArgs& A, int64_t r, uin
   };
   int cut_bin = NB;
   if (want.by_weight) {
-    const uint32_t key = want.minp > 1.0 ? key_top : lowest_of_weight(key_top, ftop, want.c, want.minp);
+    const uint32_t key = lowest_of_weight(key_top, ftop, want.c, want.minp);
     if (bin_of(key) < NB - 1) cut = (uint64_t)key << 32, cut_bin = bin_of(key);
   }
   int count_bin = want.by_count ? first_bin_of([&](int i) { return sh.row_count[i] >= (uint32_t)want.k; }) : NB;
@@ -1006,7 +1009,7 @@ __global__ void __launch_bounds__(ST) sample_whole_kernel(const SampleArgs A) {
     if (tid == 0) A.token[r] = -1, A.logprob[r] = -INFINITY;
     return;
   }
-  if (!(A.temperature[r] > 0.f)) {
+  if (greedy_row(A, r)) {
     const int i = find_index<E>(A, r, 0, V, 0, sh, [&](int, float x) -> uint64_t { return logit_key(x) == top; });
     if (tid == 0) A.token[r] = i, A.logprob[r] = 0.f;
     return;

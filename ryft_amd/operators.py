@@ -19,8 +19,9 @@ are one of bf16, f16, f32):
   logprob [B] f32). The softmax of logits / temperature, computed in 64 bits, cut to the top_k largest (0: all; of equal
   logits the lower index first), to those of at least min_p times the largest, and to the smallest prefix of what is
   left, in falling order, that holds top_p of its weight; the token is where the running sum of what is kept, by index,
-  passes uniform (in [0, 1)) of the total. temperature 0 takes the largest; the largest is always kept; a NaN logit is
-  never drawn; a row with no logit above -inf gives token -1 and logprob -inf.
+  passes uniform (in [0, 1)) of the total. temperature 0 takes the largest; the largest is always kept (of several, by a
+  min_p above 1, the first alone); a NaN logit is never drawn; a row with no logit above -inf gives token -1 and logprob
+  -inf.
 
 The caches are results as well as operands. With `tf.aliasing_output` on the parameters (the modules below have it) and a
 donated argument, or the same address as parameter and result of `execute_into`, only the new tokens are written;

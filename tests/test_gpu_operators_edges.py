@@ -8,7 +8,7 @@ from oracle import operators as oo
 from oracle import stablehlo as sh
 from ryft_amd import operators, pjrt
 from tests import operator_programs as op
-from tests.test_gpu_operators import attention_error, close, device_buffers, span, sync
+from tests.test_gpu_operators import attention_error, check_sample, close, device_buffers, span, sync
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,18 @@ def test_caps_near_scores_of_hundreds(gpu_client, new, lengths, d, softcap):
     want, = oo.paged_attention(x, op.config_of(module))
     assert np.isfinite(want).all()
     close(got, want, "bf16", attention_error(x, "bf16"), softcap)
+
+
+# ------------------------------------------------------------------------------------------------ filters at their ends
+@pytest.mark.parametrize("vocab", [40, 9000, 540000])
+def test_min_p_above_one_keeps_one_token(gpu_client, vocab):
+    # of several largest logits the first, as the largest is always kept and nothing else is; NaN is no bound that any meets
+    x = np.random.RandomState(vocab).randn(6, vocab) - 9
+    x[:, [7, 11, vocab - 1]] = 2.0
+    x[4, 11] = np.inf
+    x[5] = np.nan
+    for min_p in (1.0 + 2.0 ** -23, 2.0, np.inf, np.nan):
+        token = check_sample(gpu_client, x, "f32", min_p=min_p, uniform=[0.0, 0.5, 0.9, 0.99, 0.7, 0.1], top_k=[0, 0, 2, 9, 0, 0],
+                             top_p=[1.0, 0.5, 1.0, 0.9, 1.0, 1.0])
+        assert list(token) == [7, 7, 7, 7, 11, -1]
+    assert len(set(check_sample(gpu_client, x[:3], "f32", min_p=1.0, uniform=[0.1, 0.5, 0.9]))) == 3  # (all three)
