@@ -387,8 +387,9 @@ __device__ __attribute__((noinline)) void sample_row(const SampleArgs& A, int64_
   }
   const uint64_t z = total(mass);
   const double want = (double)A.uniform[r] * (double)z;
-  const uint64_t target = want > 0 ? min((uint64_t)want, z - 1) : 0;
-  const int token = find(mass, target);
+  // (no target: the first token kept that has any weight, however little)
+  const int token = want > 0 ? find(mass, min((uint64_t)want, z - 1))
+                             : find([&](int i, uint32_t key) -> uint64_t { return key && kept(i, key) && wt.real(key_logit(key)) > 0; }, 0);
   if (tid == 0) {
     A.token[r] = token;
     A.logprob[r] = (float)log(wt.real(key_logit(key_at(token))) / __builtin_ldexp((double)z, -wt.bits));
@@ -840,7 +841,10 @@ __device__ __forceinline__ uint64_t filtered(const SampleArgs& A, int64_t r, uin
       }
     }
   }
-  if (crowded || (want.few && first_bin != 0)) {
+  // What top_k or min_p cut off past the bins is less than a sum over the row shows, and is left out of it: only a uniform
+  // number of 0 asks for what is kept of that.
+  const bool past = (want.by_count || want.by_weight) && (cut_bin == NB || (want.few && !want.by_mass && sh.row_count[NB - 2] < (uint32_t)want.k));
+  if (crowded || (want.few && first_bin != 0) || (past && !(uniform > 0))) {
     sample_row<E>(sample_args(), r, key_top, sh);
     return 0;
   }

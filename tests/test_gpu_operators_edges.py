@@ -149,3 +149,20 @@ def test_min_p_above_one_keeps_one_token(gpu_client, vocab):
                              top_p=[1.0, 0.5, 1.0, 0.9, 1.0, 1.0])
         assert list(token) == [7, 7, 7, 7, 11, -1]
     assert len(set(check_sample(gpu_client, x[:3], "f32", min_p=1.0, uniform=[0.1, 0.5, 0.9]))) == 3  # (all three)
+
+
+@pytest.mark.parametrize("vocab, near", [(5000, 100), (5000, 10), (40000, 3), (540000, 100), (30000, 20000)], ids=str)
+def test_uniform_zero_takes_the_first_token_kept(gpu_client, vocab, near):
+    # all but `near` tokens weigh so little that no sum over the row shows them, but some are kept: with a uniform number of 0
+    # the first of those is the token, and never one that a filter has cut off
+    r = np.random.RandomState(vocab + near)
+    x = np.full((8, vocab), -80.0) - 20 * r.rand(8, vocab)
+    for row in range(8):
+        x[row, r.permutation(vocab - 900)[:near] + 900] = r.rand(near) * 1e-3
+    x[:, 0] = -101.0                                                  # (the least of all)
+    x[1, :800] = -800.0                                               # (no weight at all: 0 in 64 bits)
+    token = check_sample(gpu_client, x, "f32", uniform=0.0, top_k=[0, 0, 2000, 4999, 500, 11, 0, 0],
+                         min_p=[0, 0, 0, 0, 0, 0, 1e-40, 1e-36], top_p=1.0)
+    assert token[0] == 0 and (token[2:] > 0).all()
+    check_sample(gpu_client, x, "f32", uniform=0.0, top_k=[0, 0, 2000, 4999, 500, 11, 0, 0], top_p=0.9)
+    check_sample(gpu_client, x, "f32", uniform=0.5, top_k=[0, 0, 2000, 4999, 500, 11, 0, 0], min_p=[0, 0, 0, 0, 0, 0, 1e-40, 1e-36])
