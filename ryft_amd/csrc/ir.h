@@ -128,7 +128,7 @@ struct Graph {
   std::vector<int> param_alias;     // result index or -1
   std::vector<bool> param_donor;
   std::string name = "main";
-  std::vector<std::vector<int>> users() const;
+  std::vector<std::vector<int>> users() const;  // of each node, once for every operand; a custom_call is one user, its first node
   std::string dump() const;
 };
 

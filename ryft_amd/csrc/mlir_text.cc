@@ -141,8 +141,10 @@ bool op_is_elementwise(Op op) {
 
 std::vector<std::vector<int>> Graph::users() const {
   std::vector<std::vector<int>> u(nodes.size());
-  for (size_t i = 0; i < nodes.size(); ++i)
+  for (size_t i = 0; i < nodes.size(); ++i) {
+    if (nodes[i].op == Op::CustomCall && nodes[i].result_index > 0) continue;  // (one user a call: its first result)
     for (int o : nodes[i].operands) u[o].push_back((int)i);
+  }
   return u;
 }
 

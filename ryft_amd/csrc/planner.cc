@@ -179,6 +179,7 @@ class Planner {
   void emit_custom_call(int node, int target);
   View row_view(int node);
   int updated_operand(int operand, int out);
+  int place_of(int result);
   int shared_workspace(int64_t bytes);
   int shared_counters(int64_t count);
   void push_window_step(const char* name, int mode, int src, int dst, const std::vector<int>& idx,
@@ -812,6 +813,20 @@ int Planner::updated_operand(int operand, int out) {
   return out;
 }
 
+// The function result that a custom_call's result is, or becomes by appends alone, each of which is all that reads the one
+// before: a cache that several appends write in turn is then one buffer, whichever of them is planned first. -1: none.
+int Planner::place_of(int result) {
+  for (size_t k = 0; k < g_.results.size(); ++k)
+    if (g_.results[k] == result) return plan_.output_slots[k];
+  if (users_[result].size() != 1) return -1;
+  const int u = users_[result][0];
+  const Node& n = g_.nodes[u];
+  if (n.op != Op::CustomCall || n.call_target != "ryft.rope_append") return -1;
+  for (int i = 1; i < 3; ++i)
+    if (n.operands[5 + i] == result) return place_of(u + i);  // (the nodes of a call follow each other)
+  return -1;
+}
+
 // A [tokens, heads, head dim] operand as rows of contiguous elements at 16-byte aligned addresses: the strided view
 // where its rows are that (a slice of a fused projection), else a contiguous copy. Rows of a contiguous operand that
 // are no multiple of 16 bytes stay as they are; the kernels read those an element at a time.
@@ -856,9 +871,7 @@ void Planner::emit_custom_call(int node, int target) {
     if (g_.nodes[k].op == Op::CustomCall && g_.nodes[k].call == n.call) res.push_back((int)k);
   auto out_slot = [&](int i) {
     const int r = res[i];
-    int slot = r == node ? target : -1;
-    for (size_t k = 0; k < g_.results.size() && slot < 0; ++k)
-      if (g_.results[k] == r) slot = plan_.output_slots[k];
+    int slot = r == node && target >= 0 ? target : place_of(r);
     if (slot < 0) slot = new_slot(Slot::TEMP, g_.nodes[r].type);
     mat_[r] = slot;
     return slot;

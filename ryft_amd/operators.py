@@ -25,7 +25,8 @@ are one of bf16, f16, f32):
 
 The caches are results as well as operands. With `tf.aliasing_output` on the parameters (the modules below have it) and a
 donated argument, or the same address as parameter and result of `execute_into`, only the new tokens are written;
-otherwise the cache is copied first.
+otherwise the cache is copied first. Appends to one cache after each other write one buffer where each is all that reads
+the caches of the one before; a cache between two appends that an attention reads, or that is a result, is copied.
 """
 from __future__ import annotations
 

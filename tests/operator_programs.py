@@ -47,6 +47,32 @@ def append_case(tokens, hq, hkv, d, rot, page, pages, dtype, *, norm, interleave
     return module, ins
 
 
+def append_chain(steps, tokens=3, hq=4, hkv=2, d=64, page=16, pages=2, returns=None, aliased=True, extra="", seed=0):
+    """`steps` appends of other tokens to one pair of caches, each over the one before. `returns`: results by name (%r0#0 ...),
+    all queries and the last caches otherwise; `extra`: more lines."""
+    r = np.random.RandomState(seed)
+    q, k = f"tensor<{tokens}x{hq}x{d}xbf16>", f"tensor<{tokens}x{hkv}x{d}xbf16>"
+    i, f, c = f"tensor<{tokens}xi32>", f"tensor<{d // 2}xf32>", f"tensor<{pages}x{hkv}x{page}x{d}xbf16>"
+    last = steps - 1
+    returns = returns or [f"%r{n}#0" for n in range(steps)] + [f"%r{last}#1", f"%r{last}#2"]
+    kind = [q if n.endswith("#0") else c for n in returns]
+    alias = {"kc": f"%r{last}#1", "vc": f"%r{last}#2"}
+    params, ins, body = [("f", f), ("kc", c), ("vc", c)], [host(10000.0 ** (-np.arange(d // 2) / d), "f32")], ""
+    ins += [host(r.randn(pages, hkv, page, d), "bf16") for _ in range(2)]
+    slots = r.permutation(pages * page)
+    for n in range(steps):
+        params += [(f"q{n}", q), (f"k{n}", k), (f"v{n}", k), (f"p{n}", i), (f"s{n}", i)]
+        ins += [host(r.randn(tokens, h, d), "bf16") for h in (hq, hkv, hkv)]
+        ins += [host(r.randint(0, 1000, tokens), "i32"), host(slots[n * tokens:(n + 1) * tokens], "i32")]
+        caches = ("%kc", "%vc") if n == 0 else (f"%r{n - 1}#1", f"%r{n - 1}#2")
+        body += operators.rope_append(f"%r{n}", [(f"%q{n}", q), (f"%k{n}", k), (f"%v{n}", k), (f"%p{n}", i), (f"%s{n}", i), ("%f", f),
+                                                 (caches[0], c), (caches[1], c)])
+    head = ", ".join(f"%{n}: {t}" + (f" {{tf.aliasing_output = {returns.index(alias[n])} : i32}}"
+                                     if aliased and alias.get(n) in returns else "") for n, t in params)
+    types = ", ".join(kind)
+    return (f"module {{\n  func.func @main({head}) -> ({types}) {{\n{body}{extra}    return {', '.join(returns)} : {types}\n  }}\n}}\n", ins)
+
+
 def attention_case(new, lengths, hq, hkv, d, page, dtype, *, window=0, softcap=0.0, slopes=False, causal=True, spare=0,
                    bad_pages=False, poison=False, seed=0, spread=1.0):
     """`spare`: rows of q that belong to no sequence. bad_pages: a few table entries outside the cache. poison: what no

@@ -166,3 +166,31 @@ def test_uniform_zero_takes_the_first_token_kept(gpu_client, vocab, near):
     assert token[0] == 0 and (token[2:] > 0).all()
     check_sample(gpu_client, x, "f32", uniform=0.0, top_k=[0, 0, 2000, 4999, 500, 11, 0, 0], top_p=0.9)
     check_sample(gpu_client, x, "f32", uniform=0.5, top_k=[0, 0, 2000, 4999, 500, 11, 0, 0], min_p=[0, 0, 0, 0, 0, 0, 1e-40, 1e-36])
+
+
+# ------------------------------------------------------------------------------------------------ chains of appends
+CHAINS = {
+    "two": dict(steps=2), "three": dict(steps=3), "caches_first": dict(steps=2, returns=["%r1#2", "%r1#1", "%r0#0", "%r1#0"]),
+    "between": dict(steps=2, returns=["%r0#1", "%r1#1", "%r1#2"]), "keys_alone": dict(steps=3, returns=["%r2#1"]),
+    "not_aliased": dict(steps=2, aliased=False), "same_cache": dict(steps=1, returns=["%r0#1", "%r0#2"]),
+}
+
+
+@pytest.mark.parametrize("donate", [False, True])
+@pytest.mark.parametrize("name", CHAINS)
+def test_chains_of_appends(gpu_client, name, donate):
+    module, ins = op.append_chain(seed=len(name), **CHAINS[name])
+    if name == "same_cache":
+        c = "tensor<2x2x16x64xbf16>"
+        module = module.replace("%kc, %vc)", "%e, %e)").replace("    %r0:3", f"    %e = stablehlo.add %kc, %vc : {c}\n    %r0:3")
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    want = sh.evaluate(module, op.values(ins))
+    bufs = device_buffers(gpu_client, ins)
+    out = exe.execute([[pjrt.ExecutionInput(b, donatable=donate and i in (1, 2)) for i, b in enumerate(bufs)]])[0]
+    out.done.await_()
+    for n, (b, (w, _)) in enumerate(zip(out.outputs, want)):
+        got = sh.from_raw(b.to_numpy(), "bf16")
+        close(got, w, "bf16", 2.0 ** -8 * np.abs(w) + 2.0 ** -18 * np.abs(w).max(), (name, n))  # (the oracle rounds too)
+    if not donate:                                                    # the operands are as they were
+        for i in (1, 2):
+            assert np.array_equal(sh.from_raw(bufs[i].to_numpy(), "bf16"), op.values(ins)[i])

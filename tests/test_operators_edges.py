@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 from ryft_amd import operators, pjrt
+from tests import operator_programs as op
 
 
 def attention(client, **kw):
@@ -21,3 +22,31 @@ def test_every_finite_f32_is_a_scale_and_a_cap(compile_client):
         with pytest.raises(pjrt.PjrtError) as e:
             attention(compile_client, **kw)
         assert e.value.code == pjrt.ErrorCode.INVALID_ARGUMENT and "out of range" in str(e.value)
+
+
+# ------------------------------------------------------------------------------------------------ chains of appends
+def plan(client, *args, **kw):
+    return client.compile(pjrt.Program.mlir(op.append_chain(*args, **kw)[0])).describe_plan()
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3])
+@pytest.mark.parametrize("first", ["queries", "caches"])
+def test_a_chain_of_appends_is_one_buffer(compile_client, steps, first):
+    # one copy a cache, which an execution that donates it skips, whichever result the plan begins with
+    last = [f"%r{steps - 1}#1", f"%r{steps - 1}#2"]
+    queries = [f"%r{n}#0" for n in range(steps)]
+    text = plan(compile_client, steps, returns=queries + last if first == "queries" else last[::-1] + queries)
+    assert text.count(": rope_append ") == steps and text.count(": copy") == 2
+    assert text.count("(in place)") == 2 and "(own buffer)" not in text
+
+
+def test_what_else_reads_a_cache_keeps_it(compile_client):
+    # the cache between two appends as a result of its own, or one value as both caches: buffers of their own, copied
+    c = "tensor<2x2x16x64xbf16>"
+    text = plan(compile_client, 2, returns=["%r0#1", "%r1#1", "%r1#2"])
+    assert "result 1 <- parameter 1 (own buffer)" in text and "result 2 <- parameter 2 (in place)" in text
+    module, _ = op.append_chain(1, returns=["%r0#1", "%r0#2"])
+    both = module.replace("%kc, %vc)", "%e, %e)").replace("    %r0:3", f"    %e = stablehlo.add %kc, %vc : {c}\n    %r0:3")
+    assert both.count("%e") == 3
+    text = compile_client.compile(pjrt.Program.mlir(both)).describe_plan()
+    assert text.count(": copy") == 2 and "(in place)" not in text
