@@ -36,9 +36,9 @@ __host__ __device__ constexpr int prompt_ranges(int D) { return 256 * prompt_sha
 constexpr int kMaxParts = 128;  // ranges of a tile (two tiles of 85 rows × 31072 keys: 23 us with at most 128, 29 with 243)
 
 // The workspace of a launch with ranges: the parts (one a workgroup, of kPromptRows rows), the number of tiles, and for each
-// tile {first token of its sequence, first flat row, rows + 256 parts, first workgroup}.
+// of max_tiles {first token of its sequence, first flat row, rows + 256 parts, first workgroup}.
 __host__ __device__ inline int64_t prompt_part(int D) { return paged_part_floats(kPromptRows, D); }
-__device__ __forceinline__ int32_t* prompt_head(const PagedAttnArgs& A, int D) { return (int32_t*)(A.ws + (int64_t)prompt_ranges(D) * prompt_part(D)); }
+__device__ __forceinline__ int32_t* prompt_head(const PagedAttnArgs& A, int D) { return (int32_t*)(A.ws + (int64_t)A.groups * prompt_part(D)); }
 
 template <int D>
 struct PromptCfg {
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
     // Every tile in ranges of about `each` blocks (a sequence's tiles in as many as its last has), the least with which all
     // fit into the launch: ragged lengths need no other balancing.
     auto cuts_of = [&](int each) { return max(1, min((int)A.splits, (min((len + BKV - 1) / BKV, most) + each - 1) / each)); };
-    int room = 256 * prompt_shares(D, CAP, BIAS) / A.Hkv;
+    int room = min(256 * prompt_shares(D, CAP, BIAS), A.groups) / A.Hkv;
     auto over = [&](auto&& f) {  // the sum of f over the sequences, at most 2^24
       int sum = 0;
       for (int b = 0; b < A.B; b += 64) {
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
       each = max(2, work / room);
       while (over([&]() { return tiles * cuts_of(each); }) > room) each += max(1, each / 16);
     }
-    if (x == 0 && tid == 0) *prompt_head(A, D) = total <= room ? min(total * A.Hkv, prompt_ranges(D)) : 0;
+    if (x == 0 && tid == 0) *prompt_head(A, D) = total <= room ? min(total * A.Hkv, A.max_tiles) : 0;
     int sum = 0, before = 0, found = -1;
     for (int b = 0; b < A.B && found < 0; b += 64) {
       if (A.B > 64) sequence(b + lane);
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
   const int any_hi = last_key(q_last);
   const int jfirst = first_key(q_first) / BKV, blocks = max(0, any_hi / BKV + (any_hi >= 0 ? 1 : 0) - jfirst);
   const int parts = max(1, min(cuts, blocks / 2));
-  if (A.splits > 1 && split == 0 && tid == 0 && tile_no < prompt_ranges(D)) {  // for the join
+  if (A.splits > 1 && split == 0 && tid == 0 && tile_no < A.max_tiles) {  // for the join
     int32_t* const at = prompt_head(A, D) + 4 + 4 * tile_no;
     at[0] = t.s0, at[1] = t.row0, at[2] = rows + 256 * parts, at[3] = x;
   }
@@ -591,7 +591,6 @@ void launch_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) 
 
 void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats) {
   const int64_t tiles = (a.T * (a.Hq / a.Hkv) / kPromptRows + a.B) * a.Hkv;  // (at most)
-  const int ranges = prompt_ranges((int)a.D);
   if (a.T * a.Hq > INT32_MAX || tiles > INT32_MAX) return;
   a.tile_rows = kPromptRows;
   a.max_tiles = (int32_t)tiles;
@@ -599,8 +598,9 @@ void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats) {
   // of two heads: 76 us in 16 ranges, 23 in 121). Of two blocks at least; under 8 blocks the second launch costs more than
   // they save (300 queries of their own: 16 us, 17 with ranges).
   a.splits = tiles <= 512 && (int64_t)a.M * a.P >= 8 * BKV ? (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (int64_t)a.M * a.P / (2 * BKV))) : 1;
-  a.groups = a.splits > 1 ? ranges : (int32_t)tiles;  // (of ranges, those that the kernel has no room for end at once)
-  if (a.splits > 1) *ws_floats = ranges * prompt_part((int)a.D) + 4 + 4 * ranges;
+  // (of ranges no more than the tiles can be cut into; those that the kernel has no room for end at once)
+  a.groups = (int32_t)(a.splits > 1 ? std::min<int64_t>(prompt_ranges((int)a.D), tiles * a.splits) : tiles);
+  if (a.splits > 1) *ws_floats = a.groups * prompt_part((int)a.D) + 4 + 4 * tiles;
 }
 
 void launch_paged_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {

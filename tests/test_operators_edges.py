@@ -50,3 +50,17 @@ def test_what_else_reads_a_cache_keeps_it(compile_client):
     assert both.count("%e") == 3
     text = compile_client.compile(pjrt.Program.mlir(both)).describe_plan()
     assert text.count(": copy") == 2 and "(in place)" not in text
+
+
+# ------------------------------------------------------------------------------------------------ workspaces
+@pytest.mark.parametrize("d, sequences, heads, keys", [(128, 1, (8, 1), 32768), (64, 1, (4, 2), 32768), (128, 2, (16, 2), 100016), (128, 4, (32, 8), 16384),
+                                                       (64, 9, (16, 4), 2048)], ids=str)
+def test_ranges_of_keys_take_room_for_the_parts_there_can_be(compile_client, d, sequences, heads, keys):
+    # a part is 128 rows of d values, a maximum and a sum; a tile is cut into 128 ranges at most, each of 128 keys at least,
+    # and a launch has two workgroups a CU, three for heads of 64
+    exe = attention(compile_client, tokens=sequences * 5, sequences=sequences, q_heads=heads[0], kv_heads=heads[1], head_dim=d,
+                    pages=8, pages_per_sequence=keys // 16)
+    tiles = (sequences * 5 * (heads[0] // heads[1]) // 128 + sequences) * heads[1]
+    parts = min(512 if d == 128 else 768, tiles * min(128, keys // 128))
+    temp = exe.executable().memory_statistics()["temp_size_in_bytes"]
+    assert 0 <= temp - parts * 128 * (d + 2) * 4 <= 16384, temp
