@@ -1,6 +1,6 @@
 // ryft.paged_attention: attention of a ragged batch of queries over a paged key / value cache (the definition stands at
-// PagedAttnArgs in kernel_abi.h). Scores, softmax statistics and outputs are f32 and rounded once, on store; 16-bit types
-// round the probabilities to their type for the product with the values, and sum what they rounded.
+// PagedAttnArgs in kernel_abi.h). Scores, softmax statistics and outputs are f32 and rounded once, on store; probabilities
+// go to the matrix cores as two terms of a 16-bit type (paged_attention.h).
 //
 // Three kernels: few rows a sequence (here: a decoding step), many (k_paged_prompt.hip), and any type and head dim (here).
 #include <hip/hip_runtime.h>
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAtt
 //  - each wavefront streams blocks of its own (8 KB of keys, 8 KB of values) from the cache straight into its own part
 //    of LDS, and waits for its own loads only: no barriers inside a stretch. While the scores are computed the values
 //    are in flight, while the values are weighed the next keys.
-// Scores come transposed, S = K · Qᵀ, so that a lane has one row's scores and the probabilities, rounded and packed, are
+// Scores come transposed, S = K · Qᵀ, so that a lane has one row's scores and the probabilities, packed, are
 // the second operand of Oᵀ = Vᵀ · Pᵀ as they are; transposing LDS reads give the first. Measured: 64 sequences of 8 to 4096
 // keys, 32 heads on 8 of 128: 110 us (4.8 TB/s; all of 4096: 5.5); 8 x 2 queries over 20000 keys of 8 heads of 64: 70 us
 // (4.7 TB/s); one query of 8 heads over 500 keys: 9 us, as any launch from the host.
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
         fetch(A.k_cache, 0);
       }
       const bool mask = kb + C::KB - 1 > all_hi || kb < all_lo;
-      uint32_t pf[C::KT * 2];
+      uint32_t pf[C::KT * 2], pr[C::KT * 2];  // probabilities: rounded, and what that leaves of them
       if (score.cap2 > 0.f) {
         auto at = [&](int i) -> float& { return ((float*)st)[i]; };
         score.cap<C::KT * 4>(at, [](int) { return 0.f; });
@@ -438,9 +438,9 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
         for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(st[tt][i] - ref);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t w = X::pack(p[2 * i], p[2 * i + 1]);
-          l = X::sum2(w, l);
-          pf[2 * tt + i] = w;
+          l += p[2 * i] + p[2 * i + 1];
+          pf[2 * tt + i] = X::pack(p[2 * i], p[2 * i + 1]);
+          pr[2 * tt + i] = X::rest(pf[2 * tt + i], p[2 * i], p[2 * i + 1]);
         }
       }
       // the values; of what was issued after them, the eight loads of the next keys may still run
@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
           for (int d = 0; d < 4; ++d) {
             const u32x4p vf = {f[2 * d].x, f[2 * d].y, f[2 * d + 1].x, f[2 * d + 1].y};
             o[4 * d4 + d] = X::mma16(vf, u32x4p{pf[4 * s], pf[4 * s + 1], pf[4 * s + 2], pf[4 * s + 3]}, o[4 * d4 + d]);
+            o[4 * d4 + d] = X::mma16(vf, u32x4p{pr[4 * s], pr[4 * s + 1], pr[4 * s + 2], pr[4 * s + 3]}, o[4 * d4 + d]);
           }
         }
       }

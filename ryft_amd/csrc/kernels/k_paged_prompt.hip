@@ -414,8 +414,9 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[tt][r] -= shift;
     }
-    // probabilities of 16 keys a k-step, in the accumulator's key order (16 s + 8 (e / 4) + 4 half + e % 4)
-    u32x4p pf[4];
+    // probabilities of 16 keys a k-step, in the accumulator's key order (16 s + 8 (e / 4) + 4 half + e % 4): rounded, and what
+    // that leaves of them
+    u32x4p pf[4], pr[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
 #pragma unroll
@@ -423,7 +424,8 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
         const float a = __builtin_amdgcn_exp2f(st[s >> 1][8 * (s & 1) + 2 * i]);
         const float b = __builtin_amdgcn_exp2f(st[s >> 1][8 * (s & 1) + 2 * i + 1]);
         pf[s][i] = X::pack(a, b);
-        l = X::sum2(pf[s][i], l);
+        pr[s][i] = X::rest(pf[s][i], a, b);
+        l += a + b;
       }
     }
 #pragma unroll
@@ -440,7 +442,9 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int dt = i % (D / 32), ss = s + i / (D / 32);
-        o[dt] = X::mma32(u32x4p{f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y}, pf[ss], o[dt]);
+        const u32x4p vf = {f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y};
+        o[dt] = X::mma32(vf, pf[ss], o[dt]);
+        o[dt] = X::mma32(vf, pr[ss], o[dt]);
       }
     }
     arrived();

@@ -14,9 +14,13 @@ typedef uint32_t u32x2p __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4p __attribute__((ext_vector_type(4)));
 typedef float f32x16p __attribute__((__vector_size__(16 * sizeof(float))));
 
-// 16-bit matrix operands of one type: products into f32, pairs of probabilities rounded to it (nearest even), and the
-// sum of such a pair. LIFT: the power of two by which probabilities stand above 1 at the running maximum, so that f16
-// keeps its full precision down to 2^-21 of it (and may exceed it by 2^8: below 2^16).
+// 16-bit matrix operands of one type: products into f32, pairs of values rounded to it (nearest even), and what that leaves
+// of them, rounded to it too. Probabilities go to the product with the values as both terms, 2^-17 (f16: 2^-22) off, so that
+// an output is as exact as f32 ones make it. The first term alone added 14 to 26% to its error against 64 bits (prompts of
+// bf16 2.0e-3 of the norm, 1.6e-3 so). The second costs half of the matrix instructions again and three float instructions a
+// score: four prompts of up to 2048 tokens 117 -> 137 us, two chunks of 512 35.6 -> 39.4; decoding steps, which HBM bounds,
+// nothing (64 sequences of up to 4096 keys 111 us). LIFT: the power of two by which probabilities stand above 1 at the
+// running maximum, so that f16 keeps its full precision down to 2^-21 of it (and may exceed it by 2^8: below 2^16).
 struct MmaBF16 {
   typedef __bf16 x8 __attribute__((__vector_size__(8 * sizeof(__bf16))));
   typedef __bf16 x2 __attribute__((ext_vector_type(2)));
@@ -31,8 +35,8 @@ struct MmaBF16 {
     typedef float f2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{lo, hi}, x2));
   }
-  __device__ static __forceinline__ float sum2(uint32_t w, float c) {
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(x2, w), __builtin_bit_cast(x2, 0x3F803F80u), c, false);
+  __device__ static __forceinline__ uint32_t rest(uint32_t w, float lo, float hi) {
+    return pack(lo - __uint_as_float(w << 16), hi - __uint_as_float(w & 0xffff0000u));
   }
 };
 struct MmaF16 {
@@ -49,9 +53,9 @@ struct MmaF16 {
     typedef float f2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{lo, hi}, x2));
   }
-  __device__ static __forceinline__ float sum2(uint32_t w, float c) {
-    typedef _Float16 h2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), __builtin_bit_cast(h2, 0x3C003C00u), c, false);
+  __device__ static __forceinline__ uint32_t rest(uint32_t w, float lo, float hi) {
+    const x2 h = __builtin_bit_cast(x2, w);
+    return pack(lo - (float)h[0], hi - (float)h[1]);
   }
 };
 

@@ -89,8 +89,9 @@ def rows(x, cfg):
 
 def bound(x, cfg, dtype):
     """How far a result may be from the exact one. With probabilities p_j, values v_j and o = Σ p_j v_j, relative errors e_j
-    of the p_j move o by Σ p_j e_j (v_j - o). They are: half a step where probabilities are rounded to 16 bits (f16: not
-    under 2^-32 of the largest, its subnormal numbers' half step at the scale that they are held at); the score's, an f32
+    of the p_j move o by Σ p_j e_j (v_j - o). They are: where probabilities are held as two terms of 16 bits, half a step of
+    half a step (f16: not under 2^-32 of the largest, its subnormal numbers' half step at the scale that they are held
+    at); the score's, an f32
     sum of D products, and its multiples by f32 constants, each a few roundings of it, of the cap and of the bias; an
     exponential, 2^-21. Then f32 sums of n / 4 steps at most and a join's, and the result's own rounding: half a step of it, or
     of its type's subnormal numbers (f16; the others' may be zero)."""
@@ -99,7 +100,7 @@ def bound(x, cfg, dtype):
     tol = np.full(x[0].shape, 2.0 ** -25 if dtype == "f16" else 2.0 ** -126)
     for t, h, seen, p, s, mag, v in rows(x, cfg):
         o = p @ v
-        e = (half if dtype != "f32" else 0.0) + (d + 16) * 2.0 ** -24 * mag + 2.0 ** -22 * (2 * np.abs(s) + cap) + 2.0 ** -21
+        e = (half ** 2 if dtype != "f32" else 0.0) + (d + 16) * 2.0 ** -24 * mag + 2.0 ** -22 * (2 * np.abs(s) + cap) + 2.0 ** -21
         if len(x) > 6:
             e = e + 2.0 ** -22 * np.abs(x[6][h]) * (seen[-1] - seen)
         small = 2.0 ** -32 * p.max() if dtype == "f16" else 0.0
