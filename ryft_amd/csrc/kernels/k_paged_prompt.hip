@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
     }
     tiles = (int)(((uint32_t)n * (uint32_t)G + kPromptRows - 1) / kPromptRows);
   };
-  // blocks of a tile: to its last query's key, at most those of a window and the tile's own queries
+  // blocks of a tile: to its last query's key, at most those of a window and the tile's own queries (an estimate where causality
+  // does not end them: the order and the ranges of tiles go by it, not what they read)
   const int most = A.window > 0 ? A.window / BKV + kPromptRows / G / BKV + 2 : INT32_MAX;
   int split = 0, cuts = 1, tile_no = 0;  // this workgroup's range of the tile, ranges that the tile has at most
   if (A.splits > 1) {

@@ -85,6 +85,30 @@ def test_starts_that_decrease_leave_nothing_behind(gpu_client, starts, sequences
         assert np.array_equal(execute(bufs), want)
 
 
+# ------------------------------------------------------------------------------------------------ windows without causality
+OPEN_WINDOWS = {
+    # a query sees from its window's first key to the sequence's last
+    "step": dict(new=[1, 3], lengths=[900, 200], heads=(8, 2, 128)),
+    "step_64": dict(new=[1, 3], lengths=[900, 200], heads=(4, 4, 64)),
+    "prompt": dict(new=[100, 40], lengths=[100, 200], heads=(4, 2, 128)),
+    "ranges": dict(new=[20, 33], lengths=[3000, 700], heads=(4, 1, 64)),
+    "many": dict(new=[20] * 66, lengths=[40 + 3 * i for i in range(66)], heads=(8, 8, 64)),
+    "any": dict(new=[1, 20], lengths=[300, 90], heads=(4, 2, 80)),
+}
+
+
+@pytest.mark.parametrize("window", [1, 30, 400])
+@pytest.mark.parametrize("name", OPEN_WINDOWS)
+def test_windows_without_causality(gpu_client, name, window):
+    c = dict(OPEN_WINDOWS[name])
+    new, lengths, heads = (c.pop(k) for k in ("new", "lengths", "heads"))
+    module, ins = op.attention_case(new, lengths, *heads, 16, "bf16", seed=23, window=window, causal=False)
+    (got,) = run_over(gpu_client, module, ins, [(ins[0].dims, "bf16")])
+    x = op.values(ins)
+    want, = oo.paged_attention(x, op.config_of(module))
+    close(got, want, "bf16", attention_error(x, "bf16"), name)
+
+
 # ------------------------------------------------------------------------------------------------ caps of any size
 CAPPED = {
     # a decoding step, prompts, ranges of keys, the kernel for any type and head dim
