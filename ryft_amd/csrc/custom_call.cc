@@ -151,16 +151,23 @@ void check_sample(const Call& c, std::map<std::string, double>* config) {
   c.is("result 1", c.results[1], DType::F32, {B});
 }
 
+typedef void (*Check)(const Call&, std::map<std::string, double>*);
+Check check_of(const std::string& target) {
+  if (target == "ryft.rope_append") return check_rope_append;
+  if (target == "ryft.paged_attention") return check_paged_attention;
+  if (target == "ryft.sample") return check_sample;
+  unimplemented("custom_call target '" + target + "' is not provided by the MI355X plugin");
+}
+
 }  // namespace
+
+void custom_call_target(const std::string& target) { check_of(target); }
 
 std::vector<Node> custom_call_nodes(const Graph& g, const Node& proto, const std::string& target,
                                     const std::vector<TensorType>& results) {
   const Call c{g, proto, target, results};
   std::map<std::string, double> config;
-  if (target == "ryft.rope_append") check_rope_append(c, &config);
-  else if (target == "ryft.paged_attention") check_paged_attention(c, &config);
-  else if (target == "ryft.sample") check_sample(c, &config);
-  else unimplemented("custom_call target '" + target + "' is not provided by the MI355X plugin");
+  check_of(target)(c, &config);
   std::vector<Node> nodes;
   for (size_t i = 0; i < results.size(); ++i) {
     Node m = proto;

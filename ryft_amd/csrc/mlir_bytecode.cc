@@ -1065,12 +1065,13 @@ class BytecodeParser {
         for (int64_t v : op.operands) n.operands.push_back(value(v));
         std::vector<TensorType> results;
         for (int t : op.result_types) results.push_back(tensor_type(t));
+        std::string target = need(op, "call_target_name").str;
+        if (target.size() >= 2 && target.front() == '"' && target.back() == '"') target = target.substr(1, target.size() - 2);
+        custom_call_target(target);
         const BAttr* side = get(op, "has_side_effect");
         if (side && (side->kind == BAttr::TEXT ? side->str.rfind("true", 0) == 0 : side->i != 0))
           unimplemented("custom_call with side effects is not supported");
         if (const BAttr* c = get(op, "backend_config")) n.config = call_config(*c);
-        std::string target = need(op, "call_target_name").str;
-        if (target.size() >= 2 && target.front() == '"' && target.back() == '"') target = target.substr(1, target.size() - 2);
         std::vector<Node> nodes = custom_call_nodes(g, n, target, results);
         if (op.results.size() != nodes.size()) invalid("custom_call: result count mismatch");
         for (size_t i = 0; i < nodes.size(); ++i) node_of[op.results[i]] = add(std::move(nodes[i]));

@@ -41,8 +41,11 @@ int mlir_inline_map(Graph& g, const std::vector<int>& inputs, const TensorType& 
                     const Graph& body);
 // backend_config of a custom_call as text: `{eps = 1.0e-06 : f32, interleaved = false}` (numbers and truth values)
 std::map<std::string, double> mlir_config_text(const std::string& raw);
+// Throws UNIMPLEMENTED for a custom_call target that the plugin does not provide; asked first, since what else such a call
+// says has another operator's form.
+void custom_call_target(const std::string& target);
 // The nodes of one custom_call, one per result (`proto` holds the operands and the config), after the checks of the
-// operator that `target` names (custom_call.cc). Throws UNIMPLEMENTED for a target the plugin does not provide.
+// operator that `target` names (custom_call.cc).
 std::vector<Node> custom_call_nodes(const Graph& g, const Node& proto, const std::string& target,
                                     const std::vector<TensorType>& results);
 std::vector<Node> mlir_reduce_nodes(const Graph& g, const Node& proto, const std::vector<TensorType>& results,

@@ -1105,6 +1105,7 @@ class Parser {
       std::string target = get("call_target_name");
       if (!target.empty() && target[0] == '@') target = target.substr(1);
       if (target.size() >= 2 && target.front() == '"' && target.back() == '"') target = target.substr(1, target.size() - 2);
+      custom_call_target(target);
       if (get("has_side_effect").rfind("true", 0) == 0) unimplemented("custom_call with side effects is not supported");
       n.config = mlir_config_text(get("backend_config"));
       std::vector<TensorType> results = os.type.results;

@@ -24,6 +24,23 @@ def test_every_finite_f32_is_a_scale_and_a_cap(compile_client):
         assert e.value.code == pjrt.ErrorCode.INVALID_ARGUMENT and "out of range" in str(e.value)
 
 
+def test_other_targets_are_not_implemented_whatever_their_config(compile_client, monkeypatch):
+    # as a program from another front-end has them: an opaque string, a value that no operator here takes
+    module = operators.sample_module(rows=3, vocab=100)
+    other = module.replace("@ryft.sample", "@Sharding")
+    opaque = [other.replace("api_version = 4 : i32, backend_config = {}", f"api_version = 2 : i32, backend_config = {c}")
+              for c in ('"opaque"', '{shape = [1, 2]}', '{k = "v"}')]
+    for text in [other] + opaque:
+        assert "Sharding" in text
+        with pytest.raises(pjrt.PjrtError) as e:
+            compile_client.compile(pjrt.Program.mlir(text))
+        assert e.value.code == pjrt.ErrorCode.UNIMPLEMENTED and "'Sharding'" in str(e.value)
+    code = op.to_bytecode(other.replace("backend_config = {}", "backend_config = {k = 3 : i64}"), monkeypatch)
+    with pytest.raises(pjrt.PjrtError) as e:
+        compile_client.compile(pjrt.Program.mlir(code))
+    assert e.value.code == pjrt.ErrorCode.UNIMPLEMENTED and "'Sharding'" in str(e.value)
+
+
 # ------------------------------------------------------------------------------------------------ chains of appends
 def plan(client, *args, **kw):
     return client.compile(pjrt.Program.mlir(op.append_chain(*args, **kw)[0])).describe_plan()
