@@ -614,10 +614,14 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
   // The other kernel takes tiles of up to 128 rows, and its parts are joined by a second launch of the whole chip, here a
   // tile's by one workgroup. Heads of 128 over 4 x 4 queries of 8 sequences of 16000 keys: 102 us there, 132 here in tiles
   // of 32 rows; 3 x 5 queries of 5 heads of 64 over 12811 keys 25 and 38. With 16 rows or fewer it is the parts of a tile
-  // that decide: one query of 5 heads over 30000 keys of two heads 19 and 38 us, 8 queries of 4 x 4 heads over 9000 keys
-  // 39 and 42, but one over 9000 keys of one head 13 and 12, and 8 of 8 x 4 over 4000 34 and 33.
+  // that decide, many where tiles are few and long. How long is on the device; the table's room is what is known here. With
+  // the lengths that the room is for: 1 tile of 30000 keys 20 us there and 55 here, 2 tiles 20 and 37, 4 tiles of 100001
+  // keys 51 and 56, 8 of 30000 18 and 22, but 1 of 9000 14 and 12, and 16 of 9000 17 and 19, 32 of 9000 39 and 41. In a
+  // table for 32768 keys, one sequence of 8 tiles: 12 and 9 us for 100 keys, 14 and 11 for 2000, 16 and 14 for 4000, 20 and
+  // 24 for 8000, 23 and 37 for 16000, 36 and 34 for 32768; four sequences 15 and 11 for 500, 24 and 19 for 4000, 58 and 58
+  // for 16000, 104 and 98 for 32768. So 8 tiles at most, which lose 3 us where they are short.
   const int64_t tiles128 = (a.T * G / kPromptRows + a.B) * a.Hkv, keys = (int64_t)a.M * a.P;
-  if (rows > 16 || (tiles128 <= 32 && keys >= (tiles128 >= 16 ? 8192 : 16384))) return paged_prompt_plan(a, ws_floats);
+  if (rows > 16 || (tiles128 <= 8 && keys >= 16384)) return paged_prompt_plan(a, ws_floats);
   a.tile_rows = TR;
   const int unit = a.D == 128 ? 128 : 256;
   const int64_t tiles = (a.T * G / a.tile_rows + a.B) * a.Hkv;

@@ -81,3 +81,14 @@ def test_ranges_of_keys_take_room_for_the_parts_there_can_be(compile_client, d, 
     parts = min(512 if d == 128 else 768, tiles * min(128, keys // 128))
     temp = exe.executable().memory_statistics()["temp_size_in_bytes"]
     assert 0 <= temp - parts * 128 * (d + 2) * 4 <= 16384, temp
+
+
+def test_room_for_long_contexts_leaves_decoding_steps_to_their_kernel(compile_client):
+    # (told by the workspace: two parts of 16 rows a workgroup; ranges of keys, 128 rows, only for the fewest sequences)
+    few = lambda d: 2 * 512 * 16 * (d + 2) * 4  # noqa: E731
+    for d, sequences, heads, keys, want in ((128, 4, (32, 8), 32768, True), (64, 2, (16, 8), 65536, True), (128, 1, (32, 8), 16368, True),
+                                            (128, 1, (32, 8), 16384, False), (64, 4, (8, 2), 131072, False)):
+        exe = attention(compile_client, tokens=sequences, sequences=sequences, q_heads=heads[0], kv_heads=heads[1], head_dim=d,
+                        pages=8, pages_per_sequence=keys // 16)
+        temp = exe.executable().memory_statistics()["temp_size_in_bytes"]
+        assert (temp == few(d)) == want, (d, sequences, heads, keys, temp)
