@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAtt
 //    are in flight, while the values are weighed the next keys.
 // Scores come transposed, S = K · Qᵀ, so that a lane has one row's scores and the probabilities, packed, are
 // the second operand of Oᵀ = Vᵀ · Pᵀ as they are; transposing LDS reads give the first. Measured: 64 sequences of 8 to 4096
-// keys, 32 heads on 8 of 128: 110 us (4.8 TB/s; all of 4096: 5.5); 8 x 2 queries over 20000 keys of 8 heads of 64: 70 us
-// (4.7 TB/s); one query of 8 heads over 500 keys: 9 us, as any launch from the host.
+// keys, 32 heads on 8 of 128: 111 us (4.7 TB/s; all of 4096: 6.0); 8 x 2 queries over 20000 keys of 8 heads of 64: 68 us
+// (4.8 TB/s); one query of 8 heads over 500 keys: 9 us, as any launch from the host.
 constexpr int FEW_WAVES = 4;
 constexpr int TR = 16;  // rows of a tile
 

@@ -9,8 +9,9 @@
 // The matrix products and the exponentials bound it (a wavefront's float instructions and matrix instructions add up):
 // the exponent reference moves only when a block exceeds it by 2^8, and masks are applied only in the blocks that need
 // one. Two or three workgroups share a CU, so that one's waits for LDS are the others' work. Measured, heads of 128 and 64: four
-// prompts of 875 to 1824 tokens, 32 heads, capped, 116 us (550 TFLOP/s); two chunks of 512 with a window of 4096, 36 us;
-// 256 x 4 queries of two sequences of 60000 keys 87 us (720 TFLOP/s); 16 rows over 4 x 8 x 16000 keys 105 us (5.0 TB/s).
+// prompts of 875 to 1824 tokens, 32 heads, capped, 132 us (480 TFLOP/s, counting a product with the values once), uncapped 120;
+// two chunks of 512 with a window of 4096, 40 us; 256 x 4 queries of two sequences of 60000 keys 106 us (590 TFLOP/s); 4 x 5
+// queries each of 8 x 8 tiles over 16000 keys 104 us (5.0 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -27,13 +28,12 @@ namespace ryft {
 namespace {
 
 constexpr int BKV = kPromptKeys;
-// Workgroups that share a CU, by registers and LDS (2048 queries of two heads of 64 over 65000 keys: 99 us with three, 111
-// with two; two chunks of 512, biased, 36 and 38). Caps and biases in kernels of their own are what leaves room for it: in
-// one kernel they spilled, 41 us.
-__host__ __device__ constexpr int prompt_shares(int D, bool cap, bool bias) { return D == 64 && !(cap && bias) ? 3 : 2; }
+// Workgroups that share a CU, by registers and LDS (2048 queries of two heads of 64 over 65000 keys: 128 us with three, 136
+// with two; prompts of heads of 64 capped and biased, which keep 4 registers in scratch for it, 100 and 106).
+__host__ __device__ constexpr int prompt_shares(int D) { return D == 64 ? 3 : 2; }
 // Workgroups where tiles are cut into ranges of keys, at most
-__host__ __device__ constexpr int prompt_ranges(int D) { return 256 * prompt_shares(D, false, false); }
-constexpr int kMaxParts = 128;  // ranges of a tile (two tiles of 85 rows × 31072 keys: 23 us with at most 128, 29 with 243)
+__host__ __device__ constexpr int prompt_ranges(int D) { return 256 * prompt_shares(D); }
+constexpr int kMaxParts = 128;  // ranges of a tile (two tiles of 85 rows × 31072 keys: 24 us with at most 128, 30 with 243)
 
 // The workspace of a launch with ranges: the parts (one a workgroup, of kPromptRows rows), the number of tiles, and for each
 // of max_tiles {first token of its sequence, first flat row, rows + 256 parts, first workgroup}.
@@ -130,7 +130,7 @@ struct PromptWave {
 
 // CAP, BIAS: scores are capped, biased by distance.
 template <class X, class E, int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt_kernel(const PagedAttnArgs A) {
+__global__ void __launch_bounds__(256, prompt_shares(D)) paged_prompt_kernel(const PagedAttnArgs A) {
   typedef PromptCfg<D> C;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float row_ml[kPromptRows][2];
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
     // Every tile in ranges of about `each` blocks (a sequence's tiles in as many as its last has), the least with which all
     // fit into the launch: ragged lengths need no other balancing.
     auto cuts_of = [&](int each) { return max(1, min((int)A.splits, (min((len + BKV - 1) / BKV, most) + each - 1) / each)); };
-    int room = min(256 * prompt_shares(D, CAP, BIAS), A.groups) / A.Hkv;
+    int room = min(prompt_ranges(D), A.groups) / A.Hkv;
     auto over = [&](auto&& f) {  // the sum of f over the sequences, at most 2^24
       int sum = 0;
       for (int b = 0; b < A.B; b += 64) {
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
     if (total <= room) {
       const int work = over([&]() { return (int)min((int64_t)1 << 18, (int64_t)tiles * min((len + BKV - 1) / BKV, most)); });
       // (a third workgroup a CU where that leaves ranges of four blocks: two times 4 x 5 rows over 16000 keys of 4 heads 18
-      // us, 19 with it)
+      // us, 20 with it)
       if (work / room < 4 && total <= 512 / A.Hkv) room = min(room, 512 / A.Hkv);
       each = max(2, work / room);
       while (over([&]() { return tiles * cuts_of(each); }) > room) each += max(1, each / 16);
@@ -354,7 +354,6 @@ __global__ void __launch_bounds__(256, prompt_shares(D, CAP, BIAS)) paged_prompt
     const float base = BIAS ? slope * (float)(kb + 4 * half - pos) - ref : -ref;
     auto bias = [&](int tt, int r) { return BIAS ? __builtin_fmaf(slope, (float)(32 * tt + 8 * (r >> 2) + (r & 3)), base) : base; };
     if constexpr (CAP) {
-      // (by the polynomial 28 cycles a score instead of 48: four prompts of up to 2048 tokens 136 -> 120 us)
       auto at = [&](int i) -> float& { return ((float*)st)[i]; };
       score.cap<32>(at, [&](int i) { return bias(i >> 4, i & 15); });
     } else {
@@ -600,8 +599,8 @@ void paged_prompt_plan(PagedAttnArgs& a, int64_t* ws_floats) {
   a.tile_rows = kPromptRows;
   a.max_tiles = (int32_t)tiles;
   // Ranges of keys where the tiles alone may leave the chip short of two workgroups a CU (one tile of 85 rows × 31072 keys
-  // of two heads: 76 us in 16 ranges, 23 in 121). Of two blocks at least; under 8 blocks the second launch costs more than
-  // they save (300 queries of their own: 16 us, 17 with ranges).
+  // of two heads: 68 us in 16 ranges, 24 in 121). Of two blocks at least; under 8 blocks the second launch costs more than
+  // they save (300 queries of their own: 17.9 us, 18.5 with ranges).
   a.splits = tiles <= 512 && (int64_t)a.M * a.P >= 8 * BKV ? (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (int64_t)a.M * a.P / (2 * BKV))) : 1;
   // (of ranges no more than the tiles can be cut into; those that the kernel has no room for end at once)
   a.groups = (int32_t)(a.splits > 1 ? std::min<int64_t>(prompt_ranges((int)a.D), tiles * a.splits) : tiles);

@@ -71,14 +71,13 @@ __device__ __forceinline__ int page_of(const PagedAttnArgs& A, int key) {
   return (int)(((uint64_t)(uint32_t)key * A.page_mul) >> A.page_shift);
 }
 
-// Scores in the log2 domain, constants of a launch. A cap is held by two forms: with z = s / cap, below half the cap s ·
-// (tanh z / z), tanh z / z by a polynomial in z² that interpolates at Chebyshev nodes (2^-25 off), which leaves a score far
-// below its cap as it is; from there on cap - 2 · cap / (e^(2 z) + 1), which saturates at both ends and is off by 2^-23 of
-// the cap. Each score has its own form only where that matters: up to kFarCap (log2) the second is 2^-14 off anywhere, an
-// eighth of half a step of f16 in a probability, and a block of keys with any score past half the cap takes it for all (four
-// prompts of up to 2048 tokens capped at 2: 118 us, 149 with a choice a score). Constants past f32's range are its largest
-// numbers: a cap that small is reached by every score, one that large by none.
-constexpr float kFarCap = 512.f;
+// Scores in the log2 domain, constants of a launch. A cap is held by two forms, with z = s / cap: cap - 2 · cap / (e^(2 z) + 1),
+// which saturates at both ends and is off by 2^-22 of the cap, for all scores up to a cap of kFarCap (log2; 2^-15 there, a
+// twentieth of half a step of f16 in a probability; four prompts of up to 2048 tokens capped at 50 132 us, 138 with the other
+// form where it would do); and above it where z is past 1/2, below that s · (tanh z / z), tanh z / z by a polynomial in z²
+// that interpolates at Chebyshev nodes (2^-25 off), which leaves a score far below its cap as it is. Constants past f32's
+// range are its largest numbers: a cap that small is reached by every score, one that large by none.
+constexpr float kFarCap = 128.f;
 struct PagedScore {
   float sl2, capr, capz, cap2;  // scale · log2 e; scale / cap; 2 · capr · log2 e; cap · log2 e (0: none)
   __device__ explicit PagedScore(const PagedAttnArgs& A) {
@@ -104,18 +103,20 @@ struct PagedScore {
   // N scores of a block of keys, the bias of score i bias(i)
   template <int N, class S, class B>
   __device__ __forceinline__ void cap(S& st, B&& bias) const {
+    if (cap2 <= kFarCap) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) st(i) = far_cap(st(i), bias(i));
+      return;
+    }
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(st(i)));
-    if (!__builtin_amdgcn_ballot_w64(far(top))) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) st(i) = near_cap(st(i), bias(i));
-    } else if (cap2 <= kFarCap) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) st(i) = far_cap(st(i), bias(i));
-    } else {
+    if (__builtin_amdgcn_ballot_w64(far(top))) {
 #pragma unroll
       for (int i = 0; i < N; ++i) st(i) = far(st(i)) ? far_cap(st(i), bias(i)) : near_cap(st(i), bias(i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) st(i) = near_cap(st(i), bias(i));
     }
   }
 };
