@@ -612,7 +612,7 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
   const int G = a.Hq / a.Hkv;
   const double rows = (double)a.T * G / a.B;  // rows a sequence has of a key head, on average
   // The other kernel takes tiles of up to 128 rows, and its parts are joined by a second launch of the whole chip, here a
-  // tile's by one workgroup. Heads of 128 over 4 x 4 queries of 8 sequences of 16000 keys: 102 us there, 132 here in tiles
+  // tile's by one workgroup. Heads of 128 over 4 x 4 queries of 8 sequences of 16000 keys: 104 us there, 132 here in tiles
   // of 32 rows; 3 x 5 queries of 5 heads of 64 over 12811 keys 25 and 38. With 16 rows or fewer it is the parts of a tile
   // that decide, many where tiles are few and long. How long is on the device; the table's room is what is known here. With
   // the lengths that the room is for: 1 tile of 30000 keys 20 us there and 55 here, 2 tiles 20 and 37, 4 tiles of 100001

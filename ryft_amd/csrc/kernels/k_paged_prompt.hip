@@ -9,8 +9,8 @@
 // The matrix products and the exponentials bound it (a wavefront's float instructions and matrix instructions add up):
 // the exponent reference moves only when a block exceeds it by 2^8, and masks are applied only in the blocks that need
 // one. Two or three workgroups share a CU, so that one's waits for LDS are the others' work. Measured, heads of 128 and 64: four
-// prompts of 875 to 1824 tokens, 32 heads, capped, 132 us (480 TFLOP/s, counting a product with the values once), uncapped 120;
-// two chunks of 512 with a window of 4096, 40 us; 256 x 4 queries of two sequences of 60000 keys 106 us (590 TFLOP/s); 4 x 5
+// prompts of 875 to 1824 tokens, 32 heads, capped, 129 us (490 TFLOP/s, counting a product with the values once), uncapped 117;
+// two chunks of 512 with a window of 4096, 39 us; 256 x 4 queries of two sequences of 60000 keys 106 us (590 TFLOP/s); 4 x 5
 // queries each of 8 x 8 tiles over 16000 keys 104 us (5.0 TB/s).
 #include <hip/hip_runtime.h>
 

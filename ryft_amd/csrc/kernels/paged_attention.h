@@ -18,7 +18,7 @@ typedef float f32x16p __attribute__((__vector_size__(16 * sizeof(float))));
 // of them, rounded to it too. Probabilities go to the product with the values as both terms, 2^-17 (f16: 2^-22) off, so that
 // an output is as exact as f32 ones make it. The first term alone added 14 to 26% to its error against 64 bits (prompts of
 // bf16 2.0e-3 of the norm, 1.6e-3 so). The second costs half of the matrix instructions again and three float instructions a
-// score: four prompts of up to 2048 tokens 117 -> 137 us, two chunks of 512 35.6 -> 39.4; decoding steps, which HBM bounds,
+// score: four prompts of up to 2048 tokens 112 -> 129 us, two chunks of 512 35.5 -> 39.1; decoding steps, which HBM bounds,
 // nothing (64 sequences of up to 4096 keys 111 us). LIFT: the power of two by which probabilities stand above 1 at the
 // running maximum, so that f16 keeps its full precision down to 2^-21 of it (and may exceed it by 2^8: below 2^16).
 struct MmaBF16 {
@@ -73,7 +73,7 @@ __device__ __forceinline__ int page_of(const PagedAttnArgs& A, int key) {
 
 // Scores in the log2 domain, constants of a launch. A cap is held by two forms, with z = s / cap: cap - 2 · cap / (e^(2 z) + 1),
 // which saturates at both ends and is off by 2^-22 of the cap, for all scores up to a cap of kFarCap (log2; 2^-15 there, a
-// twentieth of half a step of f16 in a probability; four prompts of up to 2048 tokens capped at 50 132 us, 138 with the other
+// twentieth of half a step of f16 in a probability; four prompts of up to 2048 tokens capped at 50 129 us, 135 with the other
 // form where it would do); and above it where z is past 1/2, below that s · (tanh z / z), tanh z / z by a polynomial in z²
 // that interpolates at Chebyshev nodes (2^-25 off), which leaves a score far below its cap as it is. Constants past f32's
 // range are its largest numbers: a cap that small is reached by every score, one that large by none.
