@@ -11,10 +11,11 @@
 //    place itself from the bin's tokens: the picks where they reach that far, else one pass over the row. The token is
 //    looked for in the one stretch whose running sum passes the uniform number, or among the picks.
 // Within a chunk weights are summed as integers of the scale 2^48, across chunks in f64 in a fixed order: no sum depends on
-// the order in which lanes, wavefronts or workgroups finish, and a token within one part in 2^45 of a border falls on the
-// side that the 64-bit definition puts it on. Logits are ordered by a 32-bit key (equal for -0 and +0). Rows whose tokens
-// crowd into few bins (more than LDS holds), that have an infinite logit, or temperatures at which f32 logits are too
-// coarse are searched key digit by digit (sample_row).
+// the order in which lanes, wavefronts or workgroups finish. A weight is rounded to within 2^-49 of its chunk's largest, so a
+// sum over a chunk is off by 2^-36 of that at most: a token farther from a border falls on the side that the 64-bit
+// definition puts it on. Logits are ordered by a 32-bit key (equal for -0 and +0). Rows whose tokens crowd into few bins
+// (more than LDS holds), that have an infinite logit, or temperatures at which f32 logits are too coarse are searched key
+// digit by digit (sample_row, in integers of the scale 2^51 or 2^62 / V).
 //
 // Two launches and small code are on purpose: joined by the workgroup that finished last, the chunks kept the registers and
 // LDS of the search and ran two to a CU where four fit; and with every search inlined and unrolled (175 KB) a workgroup
