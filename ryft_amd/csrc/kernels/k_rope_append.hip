@@ -97,9 +97,11 @@ __global__ void __launch_bounds__(256) rope_append_any_kernel(const RopeAppendAr
 // 16-byte loads, the two halves of its pairs (half layout: 8 c and R / 2 + 8 c on; interleaved: 16 c and 16 c + 8 on; past
 // the rotated part the same), so that a rotation needs no other lane, and D / 16 lanes have a head, 64 · 16 / D heads a
 // wavefront. It moves each value in and out once and is bound by HBM where there are many tokens (8192 of 48 heads of 128,
-// half of each rotated, 201 MB: 42 us, 4.8 TB/s; with three times as many heads a wavefront, all loads first, 48; a
-// workgroup a token with a value a lane, 97) and by latency where there are few (256 tokens of the same 10 us and 17). A
-// wavefront turns its lane number into one rotation of its token, and the lanes take theirs from LDS.
+// half of each rotated, 201 MB: 42 us, 4.8 TB/s, where every pass has other tensors, 38 where it writes the queries to the
+// same memory, 32 over all the same again, which the last-level cache holds in part; a torch copy of that size 39 and 28;
+// slots in order change nothing. With three times as many heads a wavefront, all loads first, 48; a workgroup a token with a
+// value a lane, 97) and by latency where there are few (256 tokens of the same 10 us and 17). A wavefront turns its lane
+// number into one rotation of its token, and the lanes take theirs from LDS.
 typedef uint32_t u32x4r __attribute__((ext_vector_type(4)));
 template <class E>
 __global__ void __launch_bounds__(256) rope_append_rows_kernel(const RopeAppendArgs A, int passes) {
