@@ -122,4 +122,72 @@ def sample(ops, _cfg):
     return [np.array(tokens, dtype=np.int64), np.array(logs)]
 
 
-OPERATORS = {"ryft.rope_append": rope_append, "ryft.paged_attention": paged_attention, "ryft.sample": sample}
+def tree_attention(ops, cfg):
+    q, kc, vc, table, starts, lengths, visible = ops
+    out = np.zeros_like(q)
+    tokens, hq, d = q.shape
+    pages, hkv, size, _ = kc.shape
+    cap, window = _f32(cfg.get("softcap", 0)), int(cfg.get("window", 0))
+    scale = _f32(cfg["scale"]) if "scale" in cfg else 1.0 / math.sqrt(d)
+    for b in range(lengths.shape[0]):
+        s0, s1 = (min(max(int(s), 0), tokens) for s in starts[b:b + 2])
+        length = min(max(int(lengths[b]), 0), table.shape[1] * size)
+        first = length - (s1 - s0)  # (below 0: the first nodes have no position)
+        for t in range(s0, s1):
+            nodes = [j for j in range(min(s1 - s0, 32 * visible.shape[1])) if int(visible[t, j // 32]) >> j % 32 & 1]
+            at = first + len(nodes) - 1
+            see = [p for p in range(first) if not window or at - p < window] + [first + j for j in nodes if first + j >= 0]
+            see = [(int(table[b, p // size]), p % size) for p in see]
+            see = [(page, row) for page, row in see if 0 <= page < pages]
+            if not see:
+                continue
+            page, row = (np.array(a) for a in zip(*see))
+            for h in range(hq):
+                s = scale * (kc[page, h * hkv // hq, row] @ q[t, h])
+                if cap > 0:
+                    s = cap * np.tanh(s / cap)
+                p = np.exp(s - s.max())
+                out[t, h] = p @ vc[page, h * hkv // hq, row] / p.sum()
+    return [out]
+
+
+def tree_accept(ops, _cfg):
+    tokens, parents, targets, slots, starts = ops[:5]
+    caches = [c.copy() for c in ops[5:]]
+    total = tokens.shape[0]
+    counts, emitted, path = [], np.full(total, -1), np.full(total, -1)
+    for b in range(starts.shape[0] - 1):
+        s0, s1 = (min(max(int(s), 0), total) for s in starts[b:b + 2])
+        nodes = [0] if s1 > s0 else []
+        while nodes:
+            at = nodes[-1]
+            named = [c for c in range(at + 1, s1 - s0) if parents[s0 + c] == at and tokens[s0 + c] == targets[s0 + at]]
+            if not named:
+                break
+            nodes.append(named[0])
+        counts.append(len(nodes))
+        moves = []
+        for j, node in enumerate(nodes):
+            emitted[s0 + j], path[s0 + j] = targets[s0 + node], node
+            moves.append((int(slots[s0 + node]), int(slots[s0 + j])))
+        for c in caches:
+            pages, _, size, _ = c.shape
+            inside = [(a, z) for a, z in moves if 0 <= a < pages * size and 0 <= z < pages * size]
+            rows = [c[a // size, :, a % size].copy() for a, _ in inside]
+            for (_, z), row in zip(inside, rows):
+                c[z // size, :, z % size] = row
+    return [np.array(counts, dtype=np.int64), emitted, path] + caches
+
+
+def int4_matmul(ops, _cfg):
+    x, weight, scale = ops[:3]
+    n, half = weight.shape
+    w = np.zeros((n, 2 * half))
+    w[:, 0::2], w[:, 1::2] = weight % 16, weight // 16
+    group = 2 * half // scale.shape[1]
+    zero = np.repeat(ops[3], group, axis=1) if len(ops) > 3 else 8
+    return [x @ ((w - zero) * np.repeat(scale, group, axis=1)).T]
+
+
+OPERATORS = {"ryft.rope_append": rope_append, "ryft.paged_attention": paged_attention, "ryft.sample": sample,
+             "ryft.tree_attention": tree_attention, "ryft.tree_accept": tree_accept, "ryft.int4_matmul": int4_matmul}

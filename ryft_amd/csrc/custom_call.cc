@@ -1,9 +1,10 @@
 // The plugin's own operators, reached as `stablehlo.custom_call @ryft.<name>` with a backend_config dictionary (the
 // typed form, api_version 4): operand and result types, and the config's names and ranges, checked when the program is
 // read. The planner turns each call into one step (planner.cc), the kernels are in kernels/k_rope_append.hip,
-// k_paged_attention.hip and k_sample.hip; their definitions stand beside the argument blocks in kernel_abi.h.
+// k_paged_attention.hip, k_sample.hip, k_int4_matmul.hip and k_tree_accept.hip; their definitions stand beside the argument blocks in kernel_abi.h.
 #include <cmath>
 
+#include "kernel_abi.h"
 #include "mlir_common.h"
 
 namespace ryft {
@@ -106,10 +107,8 @@ void check_rope_append(const Call& c, std::map<std::string, double>* config) {
   (*config)["magnitude"] = c.number("magnitude", 1.0, -1e6, 1e6);
 }
 
-// (q, k_cache, v_cache, page_table, starts, lengths[, slopes]) -> o
-void check_paged_attention(const Call& c, std::map<std::string, double>* config) {
-  c.counts(6, 7, 1);
-  c.names({"scale", "softcap", "window", "causal"});
+// The operands that paged_attention and tree_attention share, the result and their config.
+void check_attention(const Call& c, std::map<std::string, double>* config) {
   const TensorType &q = c.operand(0), &kc = c.operand(1), &tab = c.operand(3), &len = c.operand(5);
   c.float16_or_32("q", q);
   c.rank("q", q, 3);
@@ -126,13 +125,32 @@ void check_paged_attention(const Call& c, std::map<std::string, double>* config)
   c.is("starts", c.operand(4), DType::S32, {B + 1});
   c.is("lengths", len, DType::S32, {B});
   if (B > (1 << 20) || tab.shape[1] * kc.shape[2] > INT32_MAX - 65536) c.bad("too many sequences, or too long ones");
-  if (c.n.operands.size() == 7) c.is("slopes", c.operand(6), DType::F32, {hq});
   c.is("the result", c.results[0], q.dtype, q.shape);
   (*config)["scale"] = c.number("scale", 1.0 / std::sqrt((double)d), -kFloatMax, kFloatMax);
   (*config)["softcap"] = c.number("softcap", 0, 0, kFloatMax);
   (*config)["window"] = c.number("window", 0, 0, INT32_MAX);
-  (*config)["causal"] = c.number("causal", 1, 0, 1);
   c.whole("window", (*config)["window"]);
+}
+
+// (q, k_cache, v_cache, page_table, starts, lengths[, slopes]) -> o
+void check_paged_attention(const Call& c, std::map<std::string, double>* config) {
+  c.counts(6, 7, 1);
+  c.names({"scale", "softcap", "window", "causal"});
+  check_attention(c, config);
+  if (c.n.operands.size() == 7) c.is("slopes", c.operand(6), DType::F32, {c.operand(0).shape[1]});
+  (*config)["causal"] = c.number("causal", 1, 0, 1);
+}
+
+// (q, k_cache, v_cache, page_table, starts, lengths, visible) -> o
+void check_tree_attention(const Call& c, std::map<std::string, double>* config) {
+  c.counts(7, 7, 1);
+  c.names({"scale", "softcap", "window"});
+  check_attention(c, config);
+  const TensorType& vis = c.operand(6);
+  c.rank("visible", vis, 2);
+  c.is("visible", vis, DType::S32, {c.operand(0).shape[0], vis.shape[1]});
+  if (vis.shape[1] < 1 || vis.shape[1] > (1 << 16)) c.bad("visible needs 1 to 65536 words a token");
+  (*config)["causal"] = 0;
 }
 
 // (logits, temperature, top_k, top_p, min_p, uniform) -> (token, logprob)
@@ -151,11 +169,69 @@ void check_sample(const Call& c, std::map<std::string, double>* config) {
   c.is("result 1", c.results[1], DType::F32, {B});
 }
 
+// (x, weight, scale[, zero]) -> y
+void check_int4_matmul(const Call& c, std::map<std::string, double>*) {
+  c.counts(3, 4, 1);
+  c.names({});
+  const TensorType &x = c.operand(0), &w = c.operand(1), &s = c.operand(2), &y = c.results[0];
+  c.float16_or_32("x", x);
+  c.float16_or_32("scale", s);
+  c.float16_or_32("the result", y);
+  c.rank("x", x, 2);
+  c.rank("weight", w, 2);
+  c.rank("scale", s, 2);
+  const int64_t T = x.shape[0], K = x.shape[1], N = w.shape[0], groups = s.shape[1];
+  if (K < 2 || K % 2 || K > (1 << 24)) c.bad("x has rows of " + std::to_string(K) + " values: an even number up to 2^24 is needed");
+  if (N < 1 || N > (1 << 24)) c.bad("a weight of " + std::to_string(N) + " rows is out of range (1 to 2^24)");
+  if (T > INT32_MAX) c.bad("too many rows");
+  c.is("weight", w, DType::U8, {N, K / 2});
+  c.is("scale", s, s.dtype, {N, groups});
+  if (s.dtype != x.dtype && s.dtype != DType::F32) c.bad("scale is " + s.str() + " but must have x's element type or f32");
+  if (y.dtype != x.dtype && y.dtype != DType::F32) c.bad("the result is " + y.str() + " but must have x's element type or f32");
+  if (groups < 1 || K % groups || K / groups % 2)
+    c.bad("rows of " + std::to_string(K) + " values are not cut into " + std::to_string(groups) + " groups of an even number of values");
+  if (c.n.operands.size() == 4) c.is("zero", c.operand(3), DType::U8, s.shape);
+  c.is("the result", y, y.dtype, {T, N});
+}
+
+// (tokens, parents, targets, slots, starts, caches...) -> (counts, emitted, path, caches...)
+void check_tree_accept(const Call& c, std::map<std::string, double>*) {
+  const size_t n = c.n.operands.size() < 5 ? 0 : c.n.operands.size() - 5;
+  if (n > (size_t)kMaxTreeCaches) c.bad(std::to_string(n) + " caches: at most " + std::to_string(kMaxTreeCaches));
+  c.counts(5 + n, 5 + n, 3 + n);
+  c.names({});
+  const TensorType &tok = c.operand(0), &st = c.operand(4);
+  c.rank("tokens", tok, 1);
+  c.rank("starts", st, 1);
+  const int64_t T = tok.shape[0], B = st.shape[0] - 1;
+  if (B < 0 || B > (1 << 20) || T > INT32_MAX) c.bad("too many tokens or sequences, or no starts");
+  const char* names[] = {"tokens", "parents", "targets", "slots"};
+  for (int i = 0; i < 4; ++i) c.is(names[i], c.operand(i), DType::S32, {T});
+  c.is("starts", st, DType::S32, {B + 1});
+  for (size_t i = 0; i < n; ++i) {
+    const TensorType& kc = c.operand(5 + i);
+    if (i == 0) {
+      c.float16_or_32("the cache", kc);
+      c.rank("the cache", kc, 4);
+      if (kc.shape[3] < 1 || kc.shape[3] > kMaxHeadDim) c.bad("head dim " + std::to_string(kc.shape[3]) + " is out of range (1 to 256)");
+      check_cache(c, kc, kc, kc.dtype, -1, kc.shape[3]);
+    }
+    c.is("a cache", kc, c.operand(5).dtype, c.operand(5).shape);
+    c.is("a cache's result", c.results[3 + i], kc.dtype, kc.shape);
+  }
+  c.is("result 0", c.results[0], DType::S32, {B});
+  c.is("result 1", c.results[1], DType::S32, {T});
+  c.is("result 2", c.results[2], DType::S32, {T});
+}
+
 typedef void (*Check)(const Call&, std::map<std::string, double>*);
 Check check_of(const std::string& target) {
   if (target == "ryft.rope_append") return check_rope_append;
   if (target == "ryft.paged_attention") return check_paged_attention;
   if (target == "ryft.sample") return check_sample;
+  if (target == "ryft.tree_attention") return check_tree_attention;
+  if (target == "ryft.int4_matmul") return check_int4_matmul;
+  if (target == "ryft.tree_accept") return check_tree_accept;
   unimplemented("custom_call target '" + target + "' is not provided by the MI355X plugin");
 }
 

@@ -374,6 +374,10 @@ struct RopeAppendArgs {
 // softcap) and, with slopes, s += slopes[h] · (p_k - p_q): o = Σ softmax(s) v over the visible keys: p_k < lengths[b],
 // p_k <= p_q (causal), p_q - p_k < window (window > 0), a page inside [0, pages). A query that sees no key, or belongs
 // to no sequence, gets zeros. starts are clamped to [0, T] and lengths to [0, M · P].
+// ryft.tree_attention is the same call with `visible` (causal = 0, no slopes): of the last n_b positions, query t sees
+// those whose bits its row of `visible` has (position lengths[b] - n_b + j: bit j % 32 of word j / 32; what is past W words
+// is not seen), of the earlier ones all, or with a window those with lengths[b] - n_b + depth - p_k < window, where depth
+// + 1 is the number of its bits among the first n_b.
 struct PagedAttnArgs {
   const void* q;        // [T, Hq, D]: unit stride along D, 16-byte aligned rows
   const void* k_cache;
@@ -382,6 +386,7 @@ struct PagedAttnArgs {
   const int32_t* starts;  // [B + 1]
   const int32_t* lengths; // [B]
   const float* slopes;    // [Hq] or null
+  const uint32_t* visible;  // [T, W] or null
   void* o;                // [T, Hq, D] row-major
   int64_t T, pages;
   int64_t qs[2];          // element strides of (token, head)
@@ -395,7 +400,7 @@ struct PagedAttnArgs {
   int32_t splits;         // ranges of keys of a tile of 128 rows, at most
   int32_t max_tiles;      // counters
   int32_t page_shift;     // key / P = key · page_mul >> page_shift
-  int32_t pad_;
+  int32_t W;              // words of a row of `visible`
   uint64_t page_mul;
   float* ws;              // partial results; every one that is read was written by the same launch
   int32_t* counters;      // arrivals, one a tile: zero between launches
@@ -424,6 +429,44 @@ struct SampleArgs {
   int32_t pad_;
   int64_t row0;       // first row of a launch
   void* ws;           // the chunks' results; each one that is read was written by the same call
+};
+
+// ryft.int4_matmul (k_int4_matmul.hip): y[t, n] = Σ_g scale[n, g] · Σ_{k in group g} (w[n, k] - zero[n, g]) · x[t, k], where
+// w[n, k] is the low (k even) or high nibble of byte k / 2 of row n, group g the G values from g · G on, and zero 8 where
+// there is none. Sums in f32, rounded once.
+struct Int4Args {
+  const void* x;        // [T, K], unit stride along K
+  const uint8_t* w;     // [N, K / 2]
+  const void* scale;    // [N, K / G]
+  const uint8_t* zero;  // [N, K / G] or null
+  void* y;              // [T, N] row-major
+  int64_t T, K, N, xs;  // xs: elements from one row of x to the next
+  int32_t G;
+  int32_t x_dtype, scale_dtype, y_dtype;
+  int32_t pad_;
+};
+
+// ryft.tree_accept (k_tree_accept.hip): sequence b's nodes are the rows starts[b] .. starts[b+1]-1, the first its root. From
+// the root on, the path goes to the lowest child c > i of node i (parents[c] == i) with tokens[c] == targets[i]. counts[b]:
+// the path's nodes (0 without any); emitted and path, at the first counts[b] rows of the sequence: the path's targets and
+// node numbers, -1 in every other row. In each cache the row of the path's node j > 0 is copied to the slot of node j. A
+// slot outside the cache is neither read nor written. starts are clamped to [0, T].
+constexpr int kMaxTreeCaches = 256;
+struct TreeAcceptArgs {
+  const int32_t* tokens;   // [T]
+  const int32_t* parents;  // [T]
+  const int32_t* targets;  // [T]
+  const int32_t* slots;    // [T]
+  const int32_t* starts;   // [B + 1]
+  int32_t* counts;         // [B]
+  int32_t* emitted;        // [T]
+  int32_t* path;           // [T]
+  int64_t T, pages;
+  int32_t B, Hkv, P;
+  int32_t row_bytes;       // of one head
+  int32_t n_caches;
+  int32_t pad_;
+  void* caches[kMaxTreeCaches];  // [pages, Hkv, P, row_bytes]
 };
 
 }  // namespace ryft

@@ -1,4 +1,4 @@
-// ryft.paged_attention: attention of a ragged batch of queries over a paged key / value cache (the definition stands at
+// ryft.paged_attention and ryft.tree_attention: attention of a ragged batch of queries over a paged key / value cache (the definition stands at
 // PagedAttnArgs in kernel_abi.h). Scores, softmax statistics and outputs are f32 and rounded once, on store; probabilities
 // go to the matrix cores as two terms of a 16-bit type (paged_attention.h).
 //
@@ -37,7 +37,13 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAtt
     const int len = paged_length(A, b);
     pos = len - (paged_start(A, b + 1) - (int)t);
     last = A.causal ? min(len, pos + 1) : len;
-    if (A.window > 0) first = (int)max((int64_t)0, (int64_t)pos - A.window + 1);
+    if (A.visible) {
+      const int n = paged_start(A, b + 1) - paged_start(A, b);
+      pos = len - n;
+      first = tree_first(A, t, n, pos);
+    } else if (A.window > 0) {
+      first = (int)max((int64_t)0, (int64_t)pos - A.window + 1);
+    }
   }
   float m, l;
   const float x = paged_row<E>(A, b, t, h, pos, first, last, sh, &m, &l);
@@ -167,7 +173,8 @@ struct FewPart {
   int rows, w0, parts, index;
 };
 
-template <class X, class E, int D>
+// TREE: the queries are a tree of drafted tokens (PagedAttnArgs::visible).
+template <class X, class E, int D, bool TREE>
 __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const PagedAttnArgs A) {
   typedef FewCfg<D> C;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -179,6 +186,10 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
   const int G = A.Hq / A.Hkv, W = (int)gridDim.x;
   const PagedScore score(A);
 
+  // a block's first key at or before the first that any query of a sequence sees (of a tree, one that sees no drafted token)
+  auto from_key = [&](int pos0) {
+    return A.window > 0 ? (int)max((int64_t)0, (int64_t)pos0 - A.window + (TREE ? 0 : 1)) / C::KB * C::KB : 0;
+  };
   bool falls = false;  // of the lane's sequences, one ends before it begins
   auto sequence = [&](int b) {
     FewSeq s{0, 0, 0, 0, 0};
@@ -188,8 +199,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       falls |= s.n < 0;
       s.len = paged_length(A, b);
       if (s.n > 0) {
-        const int first = A.window > 0 ? (int)max((int64_t)0, (int64_t)s.len - s.n - A.window + 1) / C::KB * C::KB : 0;
-        s.units = max(1, (s.len - first + C::UNIT - 1) / C::UNIT);
+        s.units = max(1, (s.len - from_key(s.len - s.n) + C::UNIT - 1) / C::UNIT);
         s.tiles = (int)(((uint32_t)s.n * (uint32_t)G + TR - 1) / TR) * A.Hkv;
       }
     }
@@ -266,7 +276,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
     t.hk = tile - group * A.Hkv;
     t.row0 = group * TR;
     R.rows = min(TR, t.n * G - t.row0);
-    R.kfirst = A.window > 0 ? (int)max((int64_t)0, (int64_t)t.pos0 - A.window + 1) / C::KB * C::KB : 0;
+    R.kfirst = from_key(t.pos0);
     return R;
   };
   auto last_key = [&](const PagedTile& t, int q) { return A.causal ? min(t.len - 1, t.pos0 + q) : t.len - 1; };
@@ -347,14 +357,22 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
     const int rows = R.rows;
     // this lane's row
     const int flat = t.row0 + l16, qi = flat / G, pos = t.pos0 + qi;
-    const int hi = l16 < rows ? last_key(t, qi) : -1, lo = first_key(t, qi);
+    const int hi = l16 < rows ? last_key(t, qi) : -1;
+    int lo = first_key(t, qi);
+    if constexpr (TREE) {
+      if (A.window > 0) {
+        lo = l16 < rows ? tree_first(A, t.s0 + qi, t.n, t.pos0) : 0;
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+      }
+    }
     float slope = 0.f;
     if (A.slopes) {
       slope = A.slopes[l16 < rows ? t.hk * G + (flat - qi * G) : 0] * kLog2e;
       __builtin_amdgcn_s_waitcnt(0x0F70);
     }
     // the keys that every row sees
-    const int all_hi = last_key(t, uni(t.row0 / G)), all_lo = first_key(t, uni((t.row0 + rows - 1) / G));
+    const int all_hi = TREE ? t.pos0 - 1 : last_key(t, uni(t.row0 / G));
+    const int all_lo = first_key(t, TREE ? t.n - 1 : uni((t.row0 + rows - 1) / G));
 
     float m = -INFINITY, l = 0.f;
     f32x4p o[D / 16];
@@ -365,6 +383,11 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       const int kb = kstart + j * C::UNIT;
       const bool more = j + 1 < blocks;
       const uint64_t bad_now = bad;
+      const bool mask = kb + C::KB - 1 > all_hi || kb < all_lo;
+      uint64_t vis = ~(uint64_t)0;
+      if constexpr (TREE) {
+        if (kb + C::KB - 1 > all_hi && l16 < rows) vis = tree_bits(A, t.s0 + qi, kb - t.pos0);
+      }
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): the keys are there, the values may be on their way
       asm volatile("" ::: "memory");
@@ -383,7 +406,6 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
         locate(kb + C::UNIT);
         fetch(A.k_cache, 0);
       }
-      const bool mask = kb + C::KB - 1 > all_hi || kb < all_lo;
       uint32_t pf[C::KT * 2], pr[C::KT * 2];  // probabilities: rounded, and what that leaves of them
       if (score.cap2 > 0.f) {
         auto at = [&](int i) -> float& { return ((float*)st)[i]; };
@@ -405,7 +427,8 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int rel = 16 * tt + 4 * g16 + i, key = kb + rel;
-            st[tt][i] = key <= hi && key >= lo ? st[tt][i] : -INFINITY;
+            const bool seen = !TREE || ((uint32_t)(vis >> (16 * tt)) >> (4 * g16 + i) & 1);
+            st[tt][i] = key <= hi && key >= lo && seen ? st[tt][i] : -INFINITY;
           }
       }
       if (bad_now) {
@@ -526,10 +549,11 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       const int r = __builtin_ctz(again);
       again &= again - 1;
       const int flat = t.row0 + r, qi = flat / G;
-      const int64_t first = max((int64_t)cur.kfirst + (int64_t)cur.u0 * C::UNIT, (int64_t)first_key(t, qi));
+      const int64_t first = max((int64_t)cur.kfirst + (int64_t)cur.u0 * C::UNIT,
+                                (int64_t)(TREE ? tree_first(A, t.s0 + qi, t.n, t.pos0) : first_key(t, qi)));
       const int64_t last = min((int64_t)cur.kfirst + (int64_t)cur.u1 * C::UNIT, (int64_t)last_key(t, qi) + 1);
       float rm, rl;
-      const float v = paged_row<E>(A, t.b, t.s0 + qi, t.hk * G + (flat - qi * G), t.pos0 + qi, (int)first, (int)max(last, (int64_t)0),
+      const float v = paged_row<E>(A, t.b, t.s0 + qi, t.hk * G + (flat - qi * G), TREE ? t.pos0 : t.pos0 + qi, (int)first, (int)max(last, (int64_t)0),
                                    *(PagedRowLds*)so, &rm, &rl);
       float* const one = so + sizeof(PagedRowLds) / 4;
       if (tid < D) one[tid] = v;
@@ -581,19 +605,19 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
   }
 }
 
-template <class X, class E, int D>
+template <class X, class E, int D, bool TREE>
 void launch_few(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
   constexpr int lds = FewCfg<D>::LDS;
-  const hipError_t e = hipFuncSetAttribute((const void*)paged_attention_few_kernel<X, E, D>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  const hipError_t e = hipFuncSetAttribute((const void*)paged_attention_few_kernel<X, E, D, TREE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("paged_attention LDS attribute: ") + hipGetErrorString(e));
-  launch_k(done, paged_attention_few_kernel<X, E, D>, dim3((unsigned)a.groups), dim3(256), lds, stream, a);
+  launch_k(done, paged_attention_few_kernel<X, E, D, TREE>, dim3((unsigned)a.groups), dim3(256), lds, stream, a);
 }
 
 template <class X, class E>
 void launch_matrix(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
   if (a.tile_rows == kPromptRows) return launch_paged_prompt(a, stream, done);
-  if (a.D == 128) return launch_few<X, E, 128>(a, stream, done);
-  launch_few<X, E, 64>(a, stream, done);
+  if (a.visible) return a.D == 128 ? launch_few<X, E, 128, true>(a, stream, done) : launch_few<X, E, 64, true>(a, stream, done);
+  a.D == 128 ? launch_few<X, E, 128, false>(a, stream, done) : launch_few<X, E, 64, false>(a, stream, done);
 }
 
 }  // namespace
@@ -638,6 +662,7 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
 void launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
   if (a.D < 1 || a.D > 256 || a.Hkv < 1 || a.Hq < 1 || a.Hq > 65535 || a.Hq % a.Hkv || a.P < 1)
     fail(PJRT_Error_Code_INTERNAL, "paged_attention of a shape the kernels do not take");
+  if (a.W && (!a.visible || a.causal || a.slopes)) fail(PJRT_Error_Code_INTERNAL, "tree_attention without its mask, or with another");
   if (a.T == 0) return record_done(done, stream);
   if (a.tile_rows) {
     if (a.groups < 1 || (a.tile_rows != kPromptRows && (!a.ws || !a.counters))) fail(PJRT_Error_Code_INTERNAL, "paged_attention without a workspace");

@@ -128,8 +128,8 @@ struct PromptWave {
   __device__ __forceinline__ int at(int who, F&& f) const { return __builtin_amdgcn_readlane(f(own), who); }
 };
 
-// CAP, BIAS: scores are capped, biased by distance.
-template <class X, class E, int D, bool CAP, bool BIAS>
+// CAP, BIAS: scores are capped, biased by distance. TREE: the queries are a tree of drafted tokens (PagedAttnArgs::visible).
+template <class X, class E, int D, bool CAP, bool BIAS, bool TREE>
 __global__ void __launch_bounds__(256, prompt_shares(D)) paged_prompt_kernel(const PagedAttnArgs A) {
   typedef PromptCfg<D> C;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -249,7 +249,9 @@ __global__ void __launch_bounds__(256, prompt_shares(D)) paged_prompt_kernel(con
   const int q_first = __builtin_amdgcn_readfirstlane(t.row0 / G), q_last = __builtin_amdgcn_readfirstlane((t.row0 + rows - 1) / G);
   // this range's blocks [j0, j1) of 64 keys
   const int any_hi = last_key(q_last);
-  const int jfirst = first_key(q_first) / BKV, blocks = max(0, any_hi / BKV + (any_hi >= 0 ? 1 : 0) - jfirst);
+  // (a drafted token that sees none of the tree sees one key more of a window than the first query otherwise)
+  const int tree_lo = A.window > 0 ? (int)max((int64_t)0, (int64_t)t.pos0 - A.window) : 0;
+  const int jfirst = (TREE ? tree_lo : first_key(q_first)) / BKV, blocks = max(0, any_hi / BKV + (any_hi >= 0 ? 1 : 0) - jfirst);
   const int parts = max(1, min(cuts, blocks / 2));
   if (A.splits > 1 && split == 0 && tid == 0 && tile_no < A.max_tiles) {  // for the join
     int32_t* const at = prompt_head(A, D) + 4 + 4 * tile_no;
@@ -264,9 +266,10 @@ __global__ void __launch_bounds__(256, prompt_shares(D)) paged_prompt_kernel(con
   const bool wlive = wrows > 0;
   const int wq0 = __builtin_amdgcn_readfirstlane((t.row0 + 32 * wave) / G);
   const int wq1 = __builtin_amdgcn_readfirstlane((t.row0 + 32 * wave + max(wrows, 1) - 1) / G);
-  const int w_all_hi = last_key(wq0), w_any_hi = last_key(wq1), w_all_lo = first_key(wq1), w_any_lo = first_key(wq0);
+  const int w_all_hi = TREE ? t.pos0 - 1 : last_key(wq0), w_any_hi = last_key(wq1);
+  const int w_all_lo = first_key(TREE ? t.n - 1 : wq1), w_any_lo = TREE ? tree_lo : first_key(wq0);
   const int flat = t.row0 + min(32 * wave + (lane & 31), rows - 1), qi = flat / G, h = t.hk * G + (flat - qi * G);
-  const int pos = t.pos0 + qi, hi = last_key(qi), lo = first_key(qi);
+  const int pos = t.pos0 + qi, hi = last_key(qi), lo = TREE ? tree_first(A, t.s0 + qi, t.n, t.pos0) : first_key(qi);
   const float slope = BIAS ? A.slopes[h] * kLog2e : 0.f;
 
   // Blocks into LDS: a wave-wide load fills 1 KB, the lane that fills chunk position c of row r takes chunk c ^ swz(r).
@@ -335,6 +338,10 @@ __global__ void __launch_bounds__(256, prompt_shares(D)) paged_prompt_kernel(con
       arrived();
       continue;
     }
+    uint64_t vis = ~(uint64_t)0;
+    if constexpr (TREE) {
+      if (kb + BKV - 1 > w_all_hi) vis = tree_bits(A, t.s0 + qi, kb - t.pos0) >> (4 * half);
+    }
     const uint32_t sk = lds0 + (j & 1) * C::STAGE, sv = sk + C::KBYTES;
     f32x16p st[2] = {f32x16p{}, f32x16p{}};
 #pragma unroll
@@ -368,7 +375,8 @@ __global__ void __launch_bounds__(256, prompt_shares(D)) paged_prompt_kernel(con
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = kb + 4 * half + 32 * tt + 8 * (r >> 2) + (r & 3);
-          st[tt][r] = key <= hi && key >= lo ? st[tt][r] : -INFINITY;
+          const bool seen = !TREE || ((uint32_t)(vis >> (32 * tt)) >> (8 * (r >> 2) + (r & 3)) & 1);
+          st[tt][r] = key <= hi && key >= lo && seen ? st[tt][r] : -INFINITY;
         }
     }
     if (bad_now) {
@@ -480,9 +488,9 @@ __global__ void __launch_bounds__(256, prompt_shares(D)) paged_prompt_kernel(con
       const int row = 32 * w + __builtin_ctz(again);
       again &= again - 1;
       const int f = t.row0 + row, q = f / G;
-      const int k0 = max(first_key(q), j0 * BKV), k1 = min(last_key(q) + 1, j1 * BKV);
+      const int k0 = max(TREE ? tree_first(A, t.s0 + q, t.n, t.pos0) : first_key(q), j0 * BKV), k1 = min(last_key(q) + 1, j1 * BKV);
       float rm, rl;
-      const float v = paged_row<E>(A, t.b, t.s0 + q, t.hk * G + (f - q * G), t.pos0 + q, k0, max(k1, 0), row_lds, &rm, &rl);
+      const float v = paged_row<E>(A, t.b, t.s0 + q, t.hk * G + (f - q * G), TREE ? t.pos0 : t.pos0 + q, k0, max(k1, 0), row_lds, &rm, &rl);
       if (tid < D) so[row * C::OP + tid] = v;
       if (tid == 0) row_ml[row][0] = rm, row_ml[row][1] = rl;
       __syncthreads();
@@ -583,8 +591,9 @@ void launch_prompt(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) 
     if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("paged_attention LDS attribute: ") + hipGetErrorString(e));
     launch_k(a.splits > 1 ? nullptr : done, kernel, grid, block, lds, stream, a);
   };
-  if (a.softcap > 0.f) a.slopes ? go(paged_prompt_kernel<X, E, D, true, true>) : go(paged_prompt_kernel<X, E, D, true, false>);
-  else a.slopes ? go(paged_prompt_kernel<X, E, D, false, true>) : go(paged_prompt_kernel<X, E, D, false, false>);
+  if (a.visible) a.softcap > 0.f ? go(paged_prompt_kernel<X, E, D, true, false, true>) : go(paged_prompt_kernel<X, E, D, false, false, true>);
+  else if (a.softcap > 0.f) a.slopes ? go(paged_prompt_kernel<X, E, D, true, true, false>) : go(paged_prompt_kernel<X, E, D, true, false, false>);
+  else a.slopes ? go(paged_prompt_kernel<X, E, D, false, true, false>) : go(paged_prompt_kernel<X, E, D, false, false, false>);
   if (a.splits <= 1) return;
   const unsigned tiles = (unsigned)a.max_tiles, chunks = kPromptRows * D / 4 / 256;
   if (tiles <= 32) launch_k(done, paged_prompt_join_kernel<X, D, 4>, dim3(tiles * chunks * 4), block, 0, stream, a);

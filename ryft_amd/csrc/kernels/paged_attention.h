@@ -71,6 +71,26 @@ __device__ __forceinline__ int page_of(const PagedAttnArgs& A, int key) {
   return (int)(((uint64_t)(uint32_t)key * A.page_mul) >> A.page_shift);
 }
 
+// Trees of drafted tokens (PagedAttnArgs::visible). The 64 bits of token t's row from bit `from` on: ones before bit 0, which
+// stand for the tokens before the tree, zeros past the row's end.
+__device__ __forceinline__ uint64_t tree_bits(const PagedAttnArgs& A, int64_t t, int from) {
+  const uint32_t* const row = A.visible + t * A.W;
+  auto word = [&](int i) -> uint32_t { return i < 0 ? 0xffffffffu : i < A.W ? row[i] : 0u; };
+  const int i = from >> 5, s = from & 31;  // (rounded down)
+  const uint64_t lo = (uint64_t)word(i + 1) << 32 | word(i);
+  return s ? lo >> s | (uint64_t)word(i + 2) << (64 - s) : lo;
+}
+// The first key that a token of a tree of n sees, under a window; the tree starts at position pos0.
+__device__ __forceinline__ int tree_first(const PagedAttnArgs& A, int64_t t, int n, int pos0) {
+  if (A.window <= 0) return 0;
+  int seen = 0;
+  for (int i = 0; i < A.W && 32 * i < n; ++i) {
+    const uint32_t w = A.visible[t * A.W + i];
+    seen += __popc(n - 32 * i < 32 ? w & ((1u << (n - 32 * i)) - 1) : w);
+  }
+  return (int)max((int64_t)0, min((int64_t)pos0, (int64_t)pos0 + seen - A.window));
+}
+
 // Scores in the log2 domain, constants of a launch. A cap is held by two forms, with z = s / cap: cap - 2 · cap / (e^(2 z) + 1),
 // which saturates at both ends and is off by 2^-22 of the cap, for all scores up to a cap of kFarCap (log2; 2^-15 there, a
 // twentieth of half a step of f16 in a probability; four prompts of up to 2048 tokens capped at 50 129 us, 135 with the other
@@ -137,7 +157,7 @@ __device__ __forceinline__ float sum_rows16(float v) {
 
 // ------------------------------------------------------------------------------------------------ one row
 // One query and head over the keys [first, last), by a workgroup of 256, for any type, head dim up to 256 and page size;
-// nothing that the query does not see is read. Leaves the maximum (log2), the sum and, at thread d, element d of the
+// nothing that the query does not see is read. pos: the query's position, of a tree that of its first token. Leaves the maximum (log2), the sum and, at thread d, element d of the
 // unnormalised output. Each wavefront takes every fourth block of 64 keys, a lane a key for the scores and an element
 // of the head for the output; the four meet in LDS at the end.
 struct PagedRowLds {
@@ -163,7 +183,7 @@ __device__ __forceinline__ float paged_row(const PagedAttnArgs& A, int b, int64_
     const int key = k0 + wave * 64 + lane;
     float s = -INFINITY;
     int64_t at = -1;
-    if (key < last) {
+    if (key < last && (!A.visible || key < pos || (tree_bits(A, t, key - pos) & 1))) {
       const int pi = page_of(A, key);
       const int page = A.table[(int64_t)b * A.M + pi];
       if (page >= 0 && page < A.pages) {

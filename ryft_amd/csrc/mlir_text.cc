@@ -767,7 +767,7 @@ class Parser {
         std::string nm = c_.sigil_name('%');
         int64_t k = 1;
         if (c_.try_consume(":")) k = c_.integer();
-        if (k < 1 || k > 64) invalid("bad result count for " + nm);
+        if (k < 1 || k > 1024) invalid("bad result count for " + nm);
         if (k == 1) os.results.push_back(nm);
         for (int64_t i = 0; k > 1 && i < k; ++i) os.results.push_back(nm + "#" + std::to_string(i));
       } while (c_.try_consume(","));

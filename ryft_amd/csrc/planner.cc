@@ -180,6 +180,7 @@ class Planner {
   View row_view(int node);
   int updated_operand(int operand, int out);
   int place_of(int result);
+  bool depends_on(int from, int what) const;
   int shared_workspace(int64_t bytes);
   int shared_counters(int64_t count);
   void push_window_step(const char* name, int mode, int src, int dst, const std::vector<int>& idx,
@@ -804,26 +805,65 @@ void Planner::emit_concatenate(int node, int target) {
 }
 
 // The value that a step is about to write parts of, put into the step's result slot `out`: computed straight into it
-// only when nothing else reads it (the write would change it under its other readers); otherwise it gets a slot of its
-// own and is copied. For a parameter that is a copy, which an execution that donates it into `out` skips.
+// only when nothing else reads it (the write would change it under its other readers), or nothing that has not read it yet
+// (place_of); otherwise it gets a slot of its own and is copied. For a parameter that is a copy, which an execution that
+// donates it into `out` skips.
 int Planner::updated_operand(int operand, int out) {
-  if (users_[operand].size() > 1 || results_.count(operand))
-    emit_copy(materialize(operand), 0, out, g_.nodes[operand].type.bytes());
-  else materialize(operand, out);
+  if (users_[operand].size() > 1 || results_.count(operand)) {
+    const int slot = materialize(operand);
+    if (slot != out) emit_copy(slot, 0, out, g_.nodes[operand].type.bytes());
+  } else {
+    materialize(operand, out);
+  }
   return out;
 }
 
+// Whether node `from` is computed from node `what`.
+bool Planner::depends_on(int from, int what) const {
+  std::vector<bool> seen(g_.nodes.size(), false);
+  std::vector<int> todo{from};
+  while (!todo.empty()) {
+    const int k = todo.back();
+    todo.pop_back();
+    if (k == what) return true;
+    if (seen[k]) continue;
+    seen[k] = true;
+    for (int o : g_.nodes[k].operands) todo.push_back(o);
+  }
+  return false;
+}
+
 // The function result that a custom_call's result is, or becomes by appends alone, each of which is all that reads the one
-// before: a cache that several appends write in turn is then one buffer, whichever of them is planned first. -1: none.
+// before: a cache that several appends write in turn is then one buffer, whichever of them is planned first. A tree_accept
+// writes it too, and attention may have read it before: the tree_accept's choices come from that attention, so that its
+// step runs before theirs. -1: none.
 int Planner::place_of(int result) {
   for (size_t k = 0; k < g_.results.size(); ++k)
     if (g_.results[k] == result) return plan_.output_slots[k];
-  if (users_[result].size() != 1) return -1;
-  const int u = users_[result][0];
+  int u = -1;
+  for (int k : users_[result]) {
+    const Node& n = g_.nodes[k];
+    if (n.op == Op::CustomCall && (n.call_target == "ryft.paged_attention" || n.call_target == "ryft.tree_attention")) continue;
+    if (u >= 0) return -1;
+    u = k;
+  }
+  if (u < 0) return -1;
   const Node& n = g_.nodes[u];
-  if (n.op != Op::CustomCall || n.call_target != "ryft.rope_append") return -1;
-  for (int i = 1; i < 3; ++i)
-    if (n.operands[5 + i] == result) return place_of(u + i);  // (the nodes of a call follow each other)
+  if (n.op != Op::CustomCall) return -1;
+  if (n.call_target == "ryft.rope_append" && users_[result].size() == 1) {
+    for (int i = 1; i < 3; ++i)
+      if (n.operands[5 + i] == result) return place_of(u + i);  // (the nodes of a call follow each other)
+  }
+  if (n.call_target == "ryft.tree_accept") {
+    // (what a call reads besides the caches, its choices among it, is computed before the call's caches are written)
+    for (int k : users_[result]) {
+      bool before = k == u;
+      for (int i = 0; i < 5; ++i) before |= depends_on(n.operands[i], k);
+      if (!before) return -1;
+    }
+    for (size_t i = 5; i < n.operands.size(); ++i)
+      if (n.operands[i] == result) return place_of(u + (int)i - 2);
+  }
   return -1;
 }
 
@@ -861,8 +901,8 @@ int Planner::shared_counters(int64_t count) {
 }
 
 // One of the plugin's operators (custom_call.cc): all results of the op written by one step, each straight into the
-// buffer of the function result it is, if it is one. rope_append's caches are copied into their results first and then
-// written at their slots, so that an execution whose cache argument is donated into the result, or is the result's own
+// buffer of the function result it is, if it is one. The caches of rope_append and tree_accept are copied into their
+// results first and then written at their slots, so that an execution whose cache argument is donated into the result, or is the result's own
 // memory, writes the new tokens only.
 void Planner::emit_custom_call(int node, int target) {
   const Node n = g_.nodes[node];
@@ -923,7 +963,7 @@ void Planner::emit_custom_call(int node, int target) {
     st.patches.push_back({offsetof(RopeAppendArgs, v_cache), vo});
     st.bytes = 2.0 * (double)(q.bytes() + 2 * type(1).bytes()) + 8.0 * (double)a.T + 2.0 * a.R + weights;
     st.flops = (double)a.T * (a.Hq + a.Hkv) * (4.0 * a.R + (weights ? 4.0 * a.D : 0.0));
-  } else if (n.call_target == "ryft.paged_attention") {
+  } else if (n.call_target == "ryft.paged_attention" || n.call_target == "ryft.tree_attention") {
     st.kind = Step::PAGED_ATTENTION;
     PagedAttnArgs& a = st.paged;
     const TensorType &q = type(0), &kc = type(1), &tab = type(3);
@@ -946,7 +986,12 @@ void Planner::emit_custom_call(int node, int target) {
     read(offsetof(PagedAttnArgs, table), 3);
     read(offsetof(PagedAttnArgs, starts), 4);
     read(offsetof(PagedAttnArgs, lengths), 5);
-    if (n.operands.size() == 7) read(offsetof(PagedAttnArgs, slopes), 6);
+    if (n.call_target == "ryft.tree_attention") {
+      a.W = (int32_t)type(6).shape[1];
+      read(offsetof(PagedAttnArgs, visible), 6);
+    } else if (n.operands.size() == 7) {
+      read(offsetof(PagedAttnArgs, slopes), 6);
+    }
     st.patches.push_back({offsetof(PagedAttnArgs, o), out_slot(0)});
     int64_t ws = 0, counters = 0;
     paged_attention_plan(a, &ws, &counters);
@@ -954,6 +999,52 @@ void Planner::emit_custom_call(int node, int target) {
     if (counters) st.patches.push_back({offsetof(PagedAttnArgs, counters), shared_counters(counters)});
     // how many keys are read is known on the device only: the queries and the result
     st.bytes = 2.0 * (double)q.bytes();
+  } else if (n.call_target == "ryft.int4_matmul") {
+    st.kind = Step::INT4_MATMUL;
+    Int4Args& a = st.int4;
+    const TensorType &x = type(0), &w = type(1), &s = type(2), &y = g_.nodes[res[0]].type;
+    a.T = x.shape[0];
+    a.K = a.xs = x.shape[1];
+    a.N = w.shape[0];
+    a.G = (int32_t)(a.K / s.shape[1]);
+    a.x_dtype = (int32_t)x.dtype;
+    a.scale_dtype = (int32_t)s.dtype;
+    a.y_dtype = (int32_t)y.dtype;
+    read(offsetof(Int4Args, x), 0);
+    read(offsetof(Int4Args, w), 1);
+    read(offsetof(Int4Args, scale), 2);
+    if (n.operands.size() == 4) read(offsetof(Int4Args, zero), 3);
+    st.patches.push_back({offsetof(Int4Args, y), out_slot(0)});
+    st.bytes = (double)(x.bytes() + w.bytes() + s.bytes() + y.bytes()) + (n.operands.size() == 4 ? (double)type(3).bytes() : 0.0);
+    st.flops = 2.0 * (double)a.T * (double)a.N * (double)a.K;
+  } else if (n.call_target == "ryft.tree_accept") {
+    st.kind = Step::TREE_ACCEPT;
+    TreeAcceptArgs& a = st.accept;
+    a.T = type(0).shape[0];
+    a.B = (int32_t)(type(4).shape[0] - 1);
+    a.n_caches = (int32_t)n.operands.size() - 5;
+    read(offsetof(TreeAcceptArgs, tokens), 0);
+    read(offsetof(TreeAcceptArgs, parents), 1);
+    read(offsetof(TreeAcceptArgs, targets), 2);
+    read(offsetof(TreeAcceptArgs, slots), 3);
+    read(offsetof(TreeAcceptArgs, starts), 4);
+    if (a.n_caches) {
+      const TensorType& kc = type(5);
+      a.pages = kc.shape[0];
+      a.Hkv = (int32_t)kc.shape[1];
+      a.P = (int32_t)kc.shape[2];
+      a.row_bytes = (int32_t)(kc.shape[3] * (int64_t)dtype_size(kc.dtype));
+    }
+    st.patches.push_back({offsetof(TreeAcceptArgs, counts), out_slot(0)});
+    st.patches.push_back({offsetof(TreeAcceptArgs, emitted), out_slot(1)});
+    st.patches.push_back({offsetof(TreeAcceptArgs, path), out_slot(2)});
+    for (int i = 0; i < a.n_caches; ++i) {
+      const int to = out_slot(3 + i);
+      updated_operand(n.operands[5 + i], to);
+      st.patches.push_back({offsetof(TreeAcceptArgs, caches) + i * sizeof(void*), to});
+    }
+    // how many rows move is known on the device only
+    st.bytes = 24.0 * (double)a.T;
   } else {
     st.kind = Step::SAMPLE;
     SampleArgs& a = st.sample;
@@ -2524,7 +2615,12 @@ bool Planner::in_place(int ps, int os) const {
                                 return q.second == ps || (q.second == os && q.first != offsetof(RopeAppendArgs, k_cache) &&
                                                           q.first != offsetof(RopeAppendArgs, v_cache));
                               });
-          if (append) {
+          // and tree_accept, which reads the rows that it moves from the cache it writes
+          const bool accept = w.kind == Step::TREE_ACCEPT &&
+                              std::none_of(w.patches.begin(), w.patches.end(), [&](const std::pair<size_t, int>& q) {
+                                return q.second == ps || (q.second == os && q.first < offsetof(TreeAcceptArgs, caches));
+                              });
+          if (append || accept) {
             if (windows.empty() || windows.back() != (int)i) windows.push_back((int)i);
             continue;
           }
@@ -2625,6 +2721,12 @@ std::string Plan::describe() const {
     } else if (s.kind == Step::PAGED_ATTENTION) {
       os << " tokens=" << s.paged.T << " sequences=" << s.paged.B << " heads=" << s.paged.Hq << "/" << s.paged.Hkv
          << " D=" << s.paged.D << " page=" << s.paged.P << " causal=" << s.paged.causal << " window=" << s.paged.window;
+      if (s.paged.W) os << " words=" << s.paged.W;
+    } else if (s.kind == Step::INT4_MATMUL) {
+      os << " M=" << s.int4.T << " N=" << s.int4.N << " K=" << s.int4.K << " group=" << s.int4.G << " x="
+         << dtype_name((DType)s.int4.x_dtype) << " out=" << dtype_name((DType)s.int4.y_dtype);
+    } else if (s.kind == Step::TREE_ACCEPT) {
+      os << " tokens=" << s.accept.T << " sequences=" << s.accept.B << " caches=" << s.accept.n_caches;
     } else if (s.kind == Step::SAMPLE) {
       os << " rows=" << s.sample.B << " vocab=" << s.sample.V;
     } else if (s.kind == Step::SCATTER) {

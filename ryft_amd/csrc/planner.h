@@ -19,7 +19,7 @@ struct Slot {
 
 struct Step {
   enum Kind { ELEMENTWISE, REDUCE, GEMM, ATTENTION, COPY, ROW, WINDOW, GATHER, REDUCE_BODY, SCATTER, PACK,
-              ROPE_APPEND, PAGED_ATTENTION, SAMPLE } kind;
+              ROPE_APPEND, PAGED_ATTENTION, SAMPLE, INT4_MATMUL, TREE_ACCEPT } kind;
   std::string name;  // kernel family ("gemm_bf16_mfma_256x256", "attention_fwd", ...)
   std::string timing_name;  // label in kernel timings and profiles: the name, or an edge GEMM's own tile and K ranges
   EwProgram ew;
@@ -35,6 +35,8 @@ struct Step {
   RopeAppendArgs rope;
   PagedAttnArgs paged;
   SampleArgs sample;
+  Int4Args int4;
+  TreeAcceptArgs accept;
   struct { int64_t bytes; int64_t src_offset; } copy;  // src_offset: bytes into the source slot
   // Pointer fields inside the args block that refer to slots: (byte offset of the pointer field, slot). The
   // field's initial value is a byte offset into the slot's buffer.
@@ -56,6 +58,8 @@ struct Step {
       case ROPE_APPEND: return &rope;
       case PAGED_ATTENTION: return &paged;
       case SAMPLE: return &sample;
+      case INT4_MATMUL: return &int4;
+      case TREE_ACCEPT: return &accept;
       default: return nullptr;
     }
   }

@@ -694,7 +694,8 @@ bool enqueue_steps(Client* c, const Plan& plan, void* const* ptr, hipStream_t st
   constexpr size_t kBlock = std::max({sizeof(EwProgram), sizeof(ReduceArgs), sizeof(GemmArgs), sizeof(RowArgs),
                                       sizeof(AttnArgs), sizeof(WindowArgs), sizeof(GatherArgs),
                                       sizeof(ReduceBodyArgs), sizeof(ScatterArgs), sizeof(PackArgs),
-                                      sizeof(RopeAppendArgs), sizeof(PagedAttnArgs), sizeof(SampleArgs)});
+                                      sizeof(RopeAppendArgs), sizeof(PagedAttnArgs), sizeof(SampleArgs),
+                                      sizeof(Int4Args), sizeof(TreeAcceptArgs)});
   alignas(64) static thread_local unsigned char block[kBlock + 64];
   bool recorded = false;
   for (size_t si = 0; si < plan.steps.size(); ++si) {
@@ -730,6 +731,8 @@ bool enqueue_steps(Client* c, const Plan& plan, void* const* ptr, hipStream_t st
                   : step.kind == Step::ROPE_APPEND ? sizeof(RopeAppendArgs)
                   : step.kind == Step::PAGED_ATTENTION ? sizeof(PagedAttnArgs)
                   : step.kind == Step::SAMPLE    ? sizeof(SampleArgs)
+                  : step.kind == Step::INT4_MATMUL ? sizeof(Int4Args)
+                  : step.kind == Step::TREE_ACCEPT ? sizeof(TreeAcceptArgs)
                   : step.kind == Step::REDUCE_BODY ? sizeof(ReduceBodyArgs)
                                                  : sizeof(AttnArgs);
       memcpy(block, const_cast<Step&>(step).args_block(), sz);
@@ -751,6 +754,8 @@ bool enqueue_steps(Client* c, const Plan& plan, void* const* ptr, hipStream_t st
         case Step::ROPE_APPEND: launch_rope_append(*(RopeAppendArgs*)block, st, last); break;
         case Step::PAGED_ATTENTION: launch_paged_attention(*(PagedAttnArgs*)block, st, last); break;
         case Step::SAMPLE: launch_sample(*(SampleArgs*)block, st, last); break;
+        case Step::INT4_MATMUL: launch_int4_matmul(*(Int4Args*)block, st, last); break;
+        case Step::TREE_ACCEPT: launch_tree_accept(*(TreeAcceptArgs*)block, st, last); break;
         case Step::REDUCE_BODY: launch_reduce_body(*(ReduceBodyArgs*)block, st, last); break;
         default: recorded = false; break;
       }

@@ -22,6 +22,25 @@ are one of bf16, f16, f32):
   passes uniform (in [0, 1)) of the total. temperature 0 takes the largest; the largest is always kept (of several, by a
   min_p above 1, the first alone); a NaN logit is never drawn; a row with no logit above -inf gives token -1 and logprob
   -inf.
+* ``ryft.tree_attention`` (q, k_cache, v_cache, page_table, starts, lengths as above, visible [T,W] i32) → o [T,Hq,D].
+  Sequence b's queries are a tree of drafted tokens, whose keys and values are the last of its lengths[b] positions, node j
+  at the j-th of them. A query sees every position before those, or, if `window` > 0, the last `window` up to its own place
+  in the text (as many places behind the first drafted token as its row of `visible` has bits, less one); of the tree it
+  sees node j where bit j % 32 of word j / 32 of its row is set (its ancestors and itself; nodes past 32 · W are not seen).
+  `scale`, `softcap`, pages outside the cache and queries that see nothing as in paged_attention.
+* ``ryft.tree_accept`` (tokens, parents, targets, slots [T] i32, starts [B+1] i32, any number of caches up to 256, all
+  [pages,Hkv,page_size,D]) → (counts [B] i32, emitted, path [T] i32, the caches). Sequence b's rows are a tree: the first
+  is its root (the last token that is certain), parents[c] the number of c's parent within the sequence (lower than c;
+  anything else: no node reaches it), tokens the drafted tokens, targets the model's choice after each. The path runs from
+  the root to the lowest child whose token is its parent's target, and on; counts is its length (0 for no rows), and the
+  first counts[b] rows of emitted and path are the targets along it, the sequence's next tokens, and its nodes; the other
+  rows are -1. In each cache the j-th node of the path moves from its slot to that of node j, so that the sequence's
+  positions continue with the path; slots of a call are distinct, one outside the cache is neither read nor written.
+  starts do not decrease.
+* ``ryft.int4_matmul`` (x [T,K], weight [N,K/2] ui8, scale [N,K/G] (, zero [N,K/G] ui8)) → y [T,N]. Value k of a row of
+  the weight is the low (k even) or high four bits of its byte k / 2, less its group's zero (8 without the operand), times
+  its group's scale; groups are G consecutive values, G even. y = x · weightᵀ, summed in 32 bits. scale and y are of x's
+  type or f32.
 
 The caches are results as well as operands. With `tf.aliasing_output` on the parameters (the modules below have it) and a
 donated argument, or the same address as parameter and result of `execute_into`, only the new tokens are written;
@@ -79,6 +98,52 @@ def sample(result: str, operands: Sequence[Tuple[str, str]], rows: int) -> str:
     return _call([f"{result}#0", f"{result}#1"], "ryft.sample", operands, [_t((rows,), "i32"), _t((rows,), "f32")], [])
 
 
+def tree_attention(result: str, operands: Sequence[Tuple[str, str]], *, scale: float, softcap: float = 0.0,
+                   window: int = 0) -> str:
+    """The line `result = custom_call @ryft.tree_attention(...)`."""
+    cfg = [("scale", _f32(scale)), ("softcap", _f32(softcap)), ("window", f"{int(window)} : i64")]
+    return _call([result], "ryft.tree_attention", operands, [operands[0][1]], cfg)
+
+
+def tree_accept(result: str, operands: Sequence[Tuple[str, str]], tokens: int, sequences: int) -> str:
+    """The line `result:3+ = custom_call @ryft.tree_accept(...)`; its results are result#0 (counts), #1 (emitted), #2 (path)
+    and the caches from result#3 on."""
+    types = [_t((sequences,), "i32"), _t((tokens,), "i32"), _t((tokens,), "i32")] + [t for _, t in operands[5:]]
+    return _call([f"{result}#{i}" for i in range(len(types))], "ryft.tree_accept", operands, types, [])
+
+
+def int4_matmul(result: str, operands: Sequence[Tuple[str, str]], type: str) -> str:
+    """The line `result = custom_call @ryft.int4_matmul(...)`, its result of `type`."""
+    return _call([result], "ryft.int4_matmul", operands, [type], [])
+
+
+def pack_int4(values: np.ndarray) -> np.ndarray:
+    """Rows of whole numbers 0 to 15 as int4_matmul's weight: two to a byte, the first in the low four bits."""
+    v = np.asarray(values)
+    if v.shape[-1] % 2 or v.min(initial=0) < 0 or v.max(initial=0) > 15:
+        raise ValueError("int4 weights are whole numbers from 0 to 15, an even number a row")
+    return (v[..., 0::2] | v[..., 1::2] << 4).astype(np.uint8)
+
+
+def quantize_int4(weight: np.ndarray, group: int, zeros: bool = False) -> Tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """weight [N,K] in four bits: (values [N,K/2] for int4_matmul, scales [N,K/group], zeros [N,K/group]). Without `zeros`
+    every zero is 8 and a group's largest magnitude is 7 steps; with them a group's range is 15 steps."""
+    w = np.asarray(weight, dtype=np.float64)
+    if group < 2 or group % 2 or w.shape[1] % group:
+        raise ValueError(f"rows of {w.shape[1]} values are not cut into groups of {group}")
+    g = w.reshape(w.shape[0], -1, group)
+    if zeros:
+        lo, hi = np.minimum(g.min(axis=-1), 0.0), np.maximum(g.max(axis=-1), 0.0)
+        scale = (hi - lo) / 15
+        zero = np.round(np.divide(-lo, scale, out=np.full_like(lo, 8.0), where=scale > 0))
+    else:
+        scale = np.abs(g).max(axis=-1) / 7
+        zero = np.full_like(scale, 8.0)
+    step = np.divide(g, scale[..., None], out=np.zeros_like(g), where=scale[..., None] > 0)
+    q = np.clip(np.round(step) + zero[..., None], 0, 15).astype(np.int64)
+    return pack_int4(q.reshape(w.shape)), scale.astype(np.float32), zero.astype(np.uint8)
+
+
 def rope_append_module(*, tokens: int, q_heads: int, kv_heads: int, head_dim: int, rotary_dim: int, pages: int,
                        page_size: int, dtype: str = "bf16", norm: bool = False, eps: float = 1e-6,
                        interleaved: bool = False, magnitude: float = 1.0) -> str:
@@ -115,6 +180,40 @@ def sample_module(*, rows: int, vocab: int, dtype: str = "f32") -> str:
     params = ", ".join(f"%arg{n}: {t}" for n, t in enumerate(types))
     call = sample("%0", [(f"%arg{n}", t) for n, t in enumerate(types)], rows)
     return f"module {{\n  func.func @main({params}) -> ({i}, {f}) {{\n{call}    return %0#0, %0#1 : {i}, {f}\n  }}\n}}\n"
+
+
+def tree_attention_module(*, tokens: int, sequences: int, q_heads: int, kv_heads: int, head_dim: int, pages: int,
+                          page_size: int, pages_per_sequence: int, words: int, dtype: str = "bf16", scale: float,
+                          softcap: float = 0.0, window: int = 0) -> str:
+    """A module of one tree_attention: its operands are the parameters."""
+    q, c = _t((tokens, q_heads, head_dim), dtype), _t((pages, kv_heads, page_size, head_dim), dtype)
+    types = [q, c, c, _t((sequences, pages_per_sequence), "i32"), _t((sequences + 1,), "i32"), _t((sequences,), "i32"),
+             _t((tokens, words), "i32")]
+    params = ", ".join(f"%arg{n}: {t}" for n, t in enumerate(types))
+    call = tree_attention("%0", [(f"%arg{n}", t) for n, t in enumerate(types)], scale=scale, softcap=softcap, window=window)
+    return f"module {{\n  func.func @main({params}) -> {q} {{\n{call}    return %0 : {q}\n  }}\n}}\n"
+
+
+def tree_accept_module(*, tokens: int, sequences: int, caches: int = 0, pages: int = 1, kv_heads: int = 1, page_size: int = 1,
+                       head_dim: int = 1, dtype: str = "bf16") -> str:
+    """A module of one tree_accept: its operands are the parameters, the caches aliased to their results."""
+    i, c = _t((tokens,), "i32"), _t((pages, kv_heads, page_size, head_dim), dtype)
+    types = [i, i, i, i, _t((sequences + 1,), "i32")] + [c] * caches
+    outs = [_t((sequences,), "i32"), i, i] + [c] * caches
+    params = ", ".join(f"%arg{n}: {t}" + (f" {{tf.aliasing_output = {n - 2} : i32}}" if n >= 5 else "") for n, t in enumerate(types))
+    call = tree_accept("%0", [(f"%arg{n}", t) for n, t in enumerate(types)], tokens, sequences)
+    rets, kinds = ", ".join(f"%0#{n}" for n in range(len(outs))), ", ".join(outs)
+    return f"module {{\n  func.func @main({params}) -> ({kinds}) {{\n{call}    return {rets} : {kinds}\n  }}\n}}\n"
+
+
+def int4_matmul_module(*, rows: int, inner: int, columns: int, group: int, dtype: str = "bf16", scale_dtype: Optional[str] = None,
+                       out_dtype: Optional[str] = None, zeros: bool = False) -> str:
+    """A module of one int4_matmul [rows, inner] x [columns, inner]: its operands are the parameters."""
+    y, g = _t((rows, columns), out_dtype or dtype), (columns, inner // group)
+    types = [_t((rows, inner), dtype), _t((columns, inner // 2), "ui8"), _t(g, scale_dtype or dtype)] + ([_t(g, "ui8")] if zeros else [])
+    params = ", ".join(f"%arg{n}: {t}" for n, t in enumerate(types))
+    call = int4_matmul("%0", [(f"%arg{n}", t) for n, t in enumerate(types)], y)
+    return f"module {{\n  func.func @main({params}) -> {y} {{\n{call}    return %0 : {y}\n  }}\n}}\n"
 
 
 def _rms_norm(p: str, x: str, w: str, rows: int, d: int, eps: float) -> str:
@@ -156,26 +255,42 @@ def _rows(r: str, table: str, index: str, rows: int, d: int, n: int) -> str:
 
 def decoder_module(*, tokens: int, sequences: int, vocab: int, layers: int, d_model: int, q_heads: int, kv_heads: int,
                    head_dim: int, ffn: int, pages: int, page_size: int, pages_per_sequence: int, eps: float = 1e-6,
-                   softcap: float = 0.0, window: int = 0) -> Tuple[str, List[Tuple[str, Tuple[int, ...], str]]]:
+                   softcap: float = 0.0, window: int = 0, int4_group: int = 0,
+                   tree_words: int = 0) -> Tuple[str, List[Tuple[str, Tuple[int, ...], str]]]:
     """One step of a small bf16 decoder over a ragged batch, prompts and single tokens alike: embedding rows, per layer
     RMSNorm, a fused query/key/value projection, rope_append, paged_attention, output projection and a SwiGLU block,
     then the norm and the tied output projection of each sequence's last token (`last`), and sample. Returns the module
     and its parameters as (name, shape, element type); its results are the tokens, their log-probabilities, and every
-    layer's caches, aliased to their parameters."""
+    layer's caches, aliased to their parameters.
+
+    `int4_group` > 0: the layers' projections are int4_matmul with scales for groups of that many values; a weight is then
+    [outputs, inputs / 2] with a second parameter, <name>_scale, of [outputs, inputs / int4_group]. `tree_words` > 0: the
+    tokens are trees of drafted tokens: tree_attention with the parameter `visible` [tokens, tree_words], a choice after
+    every token (the sampling parameters and the first two results have `tokens` rows, and `last` is gone) and, from the
+    parameter `parents`, tree_accept over every layer's caches, whose results counts, emitted and path stand before the
+    caches."""
     t, b, hd = tokens, sequences, head_dim
+    rows = t if tree_words else b  # of the sampler
     wide = (q_heads + 2 * kv_heads) * hd
     cache = (pages, kv_heads, page_size, hd)
     params: List[Tuple[str, Tuple[int, ...], str]] = [
         ("ids", (t,), "i32"), ("positions", (t,), "i32"), ("slots", (t,), "i32"),
         ("table", (b, pages_per_sequence), "i32"), ("starts", (b + 1,), "i32"), ("lengths", (b,), "i32"),
-        ("last", (b,), "i32"), ("temperature", (b,), "f32"), ("top_k", (b,), "i32"), ("top_p", (b,), "f32"),
-        ("min_p", (b,), "f32"), ("uniform", (b,), "f32"), ("inv_freq", (hd // 2,), "f32"),
+        *([("visible", (t, tree_words), "i32"), ("parents", (t,), "i32")] if tree_words else [("last", (b,), "i32")]),
+        ("temperature", (rows,), "f32"), ("top_k", (rows,), "i32"), ("top_p", (rows,), "f32"),
+        ("min_p", (rows,), "f32"), ("uniform", (rows,), "f32"), ("inv_freq", (hd // 2,), "f32"),
         ("embed", (vocab, d_model), "bf16"), ("norm", (d_model,), "bf16")]
+
+    def weight(name: str, k: int, n: int) -> List[Tuple[str, Tuple[int, ...], str]]:
+        if not int4_group:
+            return [(name, (k, n), "bf16")]
+        return [(name, (n, k // 2), "ui8"), (f"{name}_scale", (n, k // int4_group), "bf16")]
+
     for n in range(layers):
-        params += [(f"l{n}_norm1", (d_model,), "bf16"), (f"l{n}_qkv", (d_model, wide), "bf16"),
-                   (f"l{n}_qw", (hd,), "bf16"), (f"l{n}_kw", (hd,), "bf16"), (f"l{n}_o", (q_heads * hd, d_model), "bf16"),
-                   (f"l{n}_norm2", (d_model,), "bf16"), (f"l{n}_gate_up", (d_model, 2 * ffn), "bf16"),
-                   (f"l{n}_down", (ffn, d_model), "bf16"),
+        params += [(f"l{n}_norm1", (d_model,), "bf16"), *weight(f"l{n}_qkv", d_model, wide),
+                   (f"l{n}_qw", (hd,), "bf16"), (f"l{n}_kw", (hd,), "bf16"), *weight(f"l{n}_o", q_heads * hd, d_model),
+                   (f"l{n}_norm2", (d_model,), "bf16"), *weight(f"l{n}_gate_up", d_model, 2 * ffn),
+                   *weight(f"l{n}_down", ffn, d_model),
                    (f"l{n}_k", cache, "bf16"), (f"l{n}_v", cache, "bf16")]
     types = {name: _t(shape, dt) for name, shape, dt in params}
     xt, xf, q3, k3, qt = _t((t, d_model), "bf16"), _t((t, d_model), "f32"), _t((t, q_heads, hd), "bf16"), \
@@ -183,13 +298,19 @@ def decoder_module(*, tokens: int, sequences: int, vocab: int, layers: int, d_mo
     a3, wt, wf, ht, hf = _t((t, q_heads + 2 * kv_heads, hd), "bf16"), _t((t, wide), "bf16"), _t((t, wide), "f32"), \
         _t((t, ffn), "bf16"), _t((t, ffn), "f32")
     arg = lambda n: (f"%{n}", types[n])  # noqa: E731
+
+    def project(r: str, a: str, name: str, k: int, n: int) -> str:
+        if not int4_group:
+            return _dot(r, a, f"%{name}", t, k, n)
+        return int4_matmul(f"%{r}", [(a, _t((t, k), "bf16")), arg(name), arg(f"{name}_scale")], _t((t, n), "f32"))
+
     body = _rows("x", "%embed", "%ids", vocab, d_model, t)
     x = "%x"
     caches = []
     for n in range(layers):
         p = f"l{n}"
         body += _rms_norm(f"{p}a", x, f"%{p}_norm1", t, d_model, eps)
-        body += _dot(f"{p}p", f"%{p}an", f"%{p}_qkv", t, d_model, wide)
+        body += project(f"{p}p", f"%{p}an", f"{p}_qkv", d_model, wide)
         body += f"    %{p}pb = stablehlo.convert %{p}p : ({wf}) -> {wt}\n"
         body += f"    %{p}ph = stablehlo.reshape %{p}pb : ({wt}) -> {a3}\n"
         for name, lo, hi, ty in (("q", 0, q_heads, q3), ("k", q_heads, q_heads + kv_heads, k3),
@@ -198,30 +319,45 @@ def decoder_module(*, tokens: int, sequences: int, vocab: int, layers: int, d_mo
         body += rope_append(f"%{p}r", [(f"%{p}q", q3), (f"%{p}k", k3), (f"%{p}v", k3), arg("positions"), arg("slots"),
                                        arg("inv_freq"), arg(f"{p}_k"), arg(f"{p}_v"), arg(f"{p}_qw"), arg(f"{p}_kw")], eps=eps)
         ct = types[f"{p}_k"]
-        body += paged_attention(f"%{p}t", [(f"%{p}r#0", q3), (f"%{p}r#1", ct), (f"%{p}r#2", ct), arg("table"),
-                                           arg("starts"), arg("lengths")], scale=hd ** -0.5, softcap=softcap, window=window)
+        ops = [(f"%{p}r#0", q3), (f"%{p}r#1", ct), (f"%{p}r#2", ct), arg("table"), arg("starts"), arg("lengths")]
+        if tree_words:
+            body += tree_attention(f"%{p}t", ops + [arg("visible")], scale=hd ** -0.5, softcap=softcap, window=window)
+        else:
+            body += paged_attention(f"%{p}t", ops, scale=hd ** -0.5, softcap=softcap, window=window)
         caches += [f"%{p}r#1", f"%{p}r#2"]
         body += f"    %{p}u = stablehlo.reshape %{p}t : ({q3}) -> {qt}\n"
-        body += _dot(f"{p}w", f"%{p}u", f"%{p}_o", t, q_heads * hd, d_model)
+        body += project(f"{p}w", f"%{p}u", f"{p}_o", q_heads * hd, d_model)
         body += f"    %{p}xf = stablehlo.convert {x} : ({xt}) -> {xf}\n"
         body += f"    %{p}s = stablehlo.add %{p}xf, %{p}w : {xf}\n    %{p}sb = stablehlo.convert %{p}s : ({xf}) -> {xt}\n"
         body += _rms_norm(f"{p}b", f"%{p}sb", f"%{p}_norm2", t, d_model, eps)
-        body += _dot(f"{p}gu", f"%{p}bn", f"%{p}_gate_up", t, d_model, 2 * ffn)
+        body += project(f"{p}gu", f"%{p}bn", f"{p}_gate_up", d_model, 2 * ffn)
         for name, lo, hi in (("g", 0, ffn), ("h", ffn, 2 * ffn)):
             body += f"    %{p}{name} = stablehlo.slice %{p}gu [0:{t}, {lo}:{hi}] : ({_t((t, 2 * ffn), 'f32')}) -> {hf}\n"
         body += f"    %{p}i = stablehlo.logistic %{p}g : {hf}\n    %{p}j = stablehlo.multiply %{p}g, %{p}i : {hf}\n"
         body += f"    %{p}m = stablehlo.multiply %{p}j, %{p}h : {hf}\n    %{p}mb = stablehlo.convert %{p}m : ({hf}) -> {ht}\n"
-        body += _dot(f"{p}d", f"%{p}mb", f"%{p}_down", t, ffn, d_model)
+        body += project(f"{p}d", f"%{p}mb", f"{p}_down", ffn, d_model)
         body += f"    %{p}sf = stablehlo.convert %{p}sb : ({xt}) -> {xf}\n"
         body += f"    %{p}y = stablehlo.add %{p}sf, %{p}d : {xf}\n    %{p}yb = stablehlo.convert %{p}y : ({xf}) -> {xt}\n"
         x = f"%{p}yb"
-    body += _rows("z", x, "%last", t, d_model, b)
-    body += _rms_norm("f", "%z", "%norm", b, d_model, eps)
-    body += _dot("logits", "%fn", "%embed", b, d_model, vocab, "[1] x [1]", types["embed"])
-    body += sample("%out", [("%logits", _t((b, vocab), "f32"))] + [arg(n) for n in ("temperature", "top_k", "top_p", "min_p", "uniform")], b)
-    outs = [_t((b,), "i32"), _t((b,), "f32")] + [types[f"l{n}_k"] for n in range(layers) for _ in range(2)]
-    alias = {f"l{n}_{c}": 2 + 2 * n + i for n in range(layers) for i, c in enumerate("kv")}
+    if not tree_words:
+        body += _rows("z", x, "%last", t, d_model, b)
+        x = "%z"
+    body += _rms_norm("f", x, "%norm", rows, d_model, eps)
+    body += _dot("logits", "%fn", "%embed", rows, d_model, vocab, "[1] x [1]", types["embed"])
+    body += sample("%out", [("%logits", _t((rows, vocab), "f32"))] + [arg(n) for n in ("temperature", "top_k", "top_p", "min_p", "uniform")], rows)
+    outs = [_t((rows,), "i32"), _t((rows,), "f32")]
+    results = ["%out#0", "%out#1"]
+    if tree_words:
+        i = _t((t,), "i32")
+        body += tree_accept("%acc", [arg("ids"), arg("parents"), ("%out#0", i), arg("slots"), arg("starts")]
+                            + [(c, types["l0_k"]) for c in caches], t, b)
+        outs += [_t((b,), "i32"), i, i]
+        results += ["%acc#0", "%acc#1", "%acc#2"]
+        caches = [f"%acc#{3 + n}" for n in range(len(caches))]
+    first = len(outs)
+    outs += [types[f"l{n}_k"] for n in range(layers) for _ in range(2)]
+    alias = {f"l{n}_{c}": first + 2 * n + i for n in range(layers) for i, c in enumerate("kv")}
     head = ", ".join(f"%{n}: {types[n]}" + (f" {{tf.aliasing_output = {alias[n]} : i32}}" if n in alias else "") for n, _, _ in params)
-    rets = ", ".join(["%out#0", "%out#1"] + caches)
+    rets = ", ".join(results + caches)
     return (f"module {{\n  func.func @main({head}) -> ({', '.join(outs)}) {{\n{body}    return {rets} : {', '.join(outs)}\n  }}\n}}\n",
             params)
