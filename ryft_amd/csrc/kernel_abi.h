@@ -443,8 +443,16 @@ struct Int4Args {
   int64_t T, K, N, xs;  // xs: elements from one row of x to the next
   int32_t G;
   int32_t x_dtype, scale_dtype, y_dtype;
+  // set by int4_matmul_plan: the kernel and its split
+  int32_t kernel;       // Int4Kernel
+  int32_t span;         // values whose scale is one, at a time: 32, 64 or 128
+  int32_t tiles_t, tiles_n;  // tiles a wavefront takes along T and N
+  int32_t parts;        // ranges of K of an output tile
   int32_t pad_;
+  float* ws;            // partial sums; every one that is read was written by the same launch
+  int32_t* counters;    // arrivals, one a tile: zero between launches
 };
+enum Int4Kernel : int32_t { INT4_ANY = 0, INT4_FEW = 1, INT4_TILE = 2 };
 
 // ryft.tree_accept (k_tree_accept.hip): sequence b's nodes are the rows starts[b] .. starts[b+1]-1, the first its root. From
 // the root on, the path goes to the lowest child c > i of node i (parents[c] == i) with tokens[c] == targets[i]. counts[b]:

@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
   // their first slot.
   for (int p = 0; p < parts; ++p) {
     const FewPart P = p == 0 ? part[0] : part[1];
-    if (paged_arrive(A.counters + P.index, P.parts, &last_word))
+    if (last_to_arrive(A.counters + P.index, P.parts, &last_word))
       paged_join<X, D, TR>(A, P.t, P.rows, P.parts, [&](int i) { return 2 * (P.w0 + i) + (i == 0 ? 1 : 0); }, (float*)smem);
     __syncthreads();
   }
