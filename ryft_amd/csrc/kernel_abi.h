@@ -448,7 +448,9 @@ struct Int4Args {
   int32_t span;         // values whose scale is one, at a time: 32, 64 or 128
   int32_t tiles_t, tiles_n;  // tiles a wavefront takes along T and N
   int32_t parts;        // ranges of K of an output tile
-  int32_t pad_;
+  int32_t groups;       // K / G
+  int32_t group_spans;  // G / span
+  int32_t steps;        // of the K loop
   float* ws;            // partial sums; every one that is read was written by the same launch
   int32_t* counters;    // arrivals, one a tile: zero between launches
 };

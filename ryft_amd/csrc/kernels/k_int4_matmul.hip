@@ -75,36 +75,47 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 2) int4_few_kernel(const Int4A
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g16 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
-  const int steps = (int)((A.K + FEW_STEP - 1) / FEW_STEP), part = blockIdx.y;
-  const int lo = (int)((int64_t)steps * part / A.parts), hi = (int)((int64_t)steps * (part + 1) / A.parts);
+  const int part = blockIdx.y, K = (int)A.K;
+  int lo, hi;
+  int4_range(A, part, lo, hi);
 
-  const uint8_t* w[NT];
-  int64_t row[NT];
+  const __amdgpu_buffer_rsrc_t wb = int4_buffer(A.w + n0 * (K / 2), (A.N - n0) * (K / 2)), xb = int4_buffer(A.x, A.T * A.xs * 2);
+  const Int4Groups groups(A, n0);
+  uint32_t w[NT], row[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    row[i] = min(n0 + 16 * i + l16, A.N - 1);  // (rows past the last are computed and not stored)
-    w[i] = A.w + row[i] * (A.K / 2) + 16 * g16;
+    const int r = (int)min((int64_t)(16 * i + l16), A.N - 1 - n0);  // (rows past the last are computed and not stored)
+    w[i] = (uint32_t)r * (uint32_t)(K / 2) + 16 * g16;
+    row[i] = (uint32_t)r * (uint32_t)A.groups;
   }
-  const uint16_t* const x = (const uint16_t*)A.x + (l16 < A.T ? l16 : A.T - 1) * A.xs + 8 * g16;
+  const uint32_t x = l16 < A.T ? (uint32_t)(l16 * (int)A.xs + 8 * g16) * 2 : kOutside;
 
   struct Step {
     u32x4p w[NT][2], x[8];
-    float s[NT][SPANS], c[NT][SPANS];
+    Int4Scales<SPAN, SPANS> s[NT];
   };
   auto load = [&](Step& v, int step) {
-    const int64_t k = (int64_t)step * FEW_STEP;
+    const int k = step * FEW_STEP;
+    if (k + FEW_STEP <= K) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        v.w[i][j] = int4_load(k + 128 * j + 32 * g16 < A.K ? w[i] + k / 2 + 64 * j : w[i] - 16 * g16);
+        for (int j = 0; j < 2; ++j) v.w[i][j] = int4_load<kOnce>(wb, w[i], k / 2 + 64 * j);
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      v.x[b] = u32x4p{0, 0, 0, 0};
-      if (k + 32 * b < A.K) v.x[b] = *(const u32x4p*)(x + k + 32 * b);
+      for (int b = 0; b < 8; ++b) v.x[b] = int4_load<0>(xb, x, 2 * (k + 32 * b));
+    } else {
+      // (the row ends within the step)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          v.w[i][j] = int4_load<kOnce>(wb, k + 128 * j + 32 * g16 < K ? w[i] + (uint32_t)(k / 2 + 64 * j) : kOutside, 0);
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+        v.x[b] = int4_load<0>(xb, k + 32 * b < K && x != kOutside ? x + (uint32_t)(2 * (k + 32 * b)) : kOutside, 0);
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i) int4_scales<SPAN, SPANS, X>(A, row[i], k, v.s[i], v.c[i]);
+    for (int i = 0; i < NT; ++i) v.s[i].load(A, groups, row[i], k);
   };
 
   f32x4p y[NT];
@@ -134,16 +145,17 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 2) int4_few_kernel(const Int4A
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
+        const float scale = v.s[i].template scale<X>(A, p), c = -16.f - (float)v.s[i].z[p];
         f32x4p acc;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = v.c[i][p] * sx[r];
+        for (int r = 0; r < 4; ++r) acc[r] = c * sx[r];
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) {
           const int at = p * BLOCKS + b;
           acc = X::mma16(xf[b], int4_operand<X>(q[i][at >> 2][at & 3]), acc);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[i][r] = __builtin_fmaf(v.s[i][p], acc[r], y[i][r]);
+        for (int r = 0; r < 4; ++r) y[i][r] = __builtin_fmaf(scale, acc[r], y[i][r]);
       }
     }
   };
@@ -205,6 +217,7 @@ void few_plan(Int4Args& a, int64_t* ws_floats, int64_t* counters) {
   a.kernel = INT4_FEW;
   a.tiles_t = 1;
   const int64_t steps = (a.K + FEW_STEP - 1) / FEW_STEP;
+  a.steps = (int32_t)steps;
   a.tiles_n = a.N >= 16384 ? 2 : 1;
   const int64_t tiles = (a.N + 16 * a.tiles_n - 1) / (16 * a.tiles_n);
   // ranges of K until there are two workgroups a CU, each with a step for every wavefront
@@ -222,7 +235,11 @@ void int4_matmul_plan(Int4Args& a, int64_t* ws_floats, int64_t* counters) {
   a.kernel = INT4_ANY;
   a.parts = 1;
   if ((a.x_dtype != DT_BF16 && a.x_dtype != DT_F16) || a.G % 32 || a.T == 0) return;
+  // (offsets within a tile's rows are 31 bits)
+  if (a.K > (1 << 22)) return;
   a.span = a.G % 128 == 0 ? 128 : a.G % 64 == 0 ? 64 : 32;
+  a.groups = (int32_t)(a.K / a.G);
+  a.group_spans = a.G / a.span;
   if (a.T <= 16) return few_plan(a, ws_floats, counters);
   int4_tile_plan(a, ws_floats, counters);
 }

@@ -55,9 +55,9 @@ __device__ __forceinline__ u32x4p sum_terms(float s) {
   return u32x4p{a | b << 16, c | a << 16, b | c << 16, 0u};
 }
 template <class X>
-__device__ __forceinline__ u32x4p sum_factors(float c, bool mine) {
+__device__ __forceinline__ u32x4p sum_factors(uint32_t zero, bool mine) {
   if (!mine) return u32x4p{0u, 0u, 0u, 0u};
-  const float z = -16.f - c;  // the zero point
+  const float z = (float)zero;
   const uint32_t a1 = X::put(-16.f * SumTerms<X>::H), b1 = X::put(-16.f), a2 = X::put(-z * SumTerms<X>::H), b2 = X::put(-z);
   return u32x4p{a1 | b1 << 16, b1 | a2 << 16, b2 | b2 << 16, 0u};
 }
@@ -79,42 +79,52 @@ __global__ void __launch_bounds__(256, OCC) int4_tile_kernel(const Int4Args A) {
   const int tiles_n = (int)((A.N + BN - 1) / BN), tiles_t = (int)((A.T + C::BM - 1) / C::BM);
   const int tile = blockIdx.x;
   const int tn = tile / tiles_t, tt = tile - tn * tiles_t, part = blockIdx.y;
-  const int64_t t0 = (int64_t)tt * C::BM, n0 = (int64_t)tn * BN + wave * (32 * NW);
-  const int stages = (int)((A.K + STAGE - 1) / STAGE);
-  const int lo = (int)((int64_t)stages * part / A.parts), hi = (int)((int64_t)stages * (part + 1) / A.parts);
+  const int64_t t0 = (int64_t)tt * C::BM, n0 = (int64_t)tn * BN;
+  const int K = (int)A.K;
+  int lo, hi;
+  int4_range(A, part, lo, hi);
 
-  const uint8_t* w[NW];
-  int64_t row[NW];
+  const __amdgpu_buffer_rsrc_t wb = int4_buffer(A.w + n0 * (K / 2), (A.N - n0) * (K / 2));
+  const __amdgpu_buffer_rsrc_t xb = int4_buffer((const uint16_t*)A.x + t0 * A.xs, (A.T - t0) * A.xs * 2);
+  const Int4Groups groups(A, n0);
+  uint32_t w[NW], row[NW];
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
-    row[i] = min(n0 + 32 * i + l32, A.N - 1);  // (rows past the last are computed and not stored)
-    w[i] = A.w + row[i] * (A.K / 2);
+    const int r = (int)min((int64_t)(wave * (32 * NW) + 32 * i + l32), A.N - 1 - n0);  // (rows past the last are computed and not stored)
+    w[i] = (uint32_t)r * (uint32_t)(K / 2) + 16 * half;
+    row[i] = (uint32_t)r * (uint32_t)A.groups;
   }
-  // chunk j of this thread: row j · 16 + tid / 16 of the tile, values 8 · (tid % 16) on
+  // chunk j of this thread: row 16 j + tid / 16 of the tile, values 8 · (tid % 16) on
   const int xr = tid >> 4, xc = tid & 15;
-  const uint16_t* const x = (const uint16_t*)A.x + 8 * xc;
+  uint32_t x[CH];
+#pragma unroll
+  for (int j = 0; j < CH; ++j)
+    x[j] = t0 + 16 * j + xr < A.T ? (uint32_t)((16 * j + xr) * (int)A.xs + 8 * xc) * 2 : kOutside;
 
   u32x4p xs[CH], q[NW][2];
-  float s[NW][SPANS], c[NW][SPANS];
+  Int4Scales<SPAN, SPANS> sc[NW];
   auto load_x = [&](int stage) {
-    const int64_t k = (int64_t)stage * STAGE;
+    const int k = stage * STAGE;
+    if (k + STAGE <= K) {
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const int64_t t = t0 + 16 * j + xr;
-      xs[j] = u32x4p{0, 0, 0, 0};
-      if (t < A.T && k + 8 * xc < A.K) xs[j] = *(const u32x4p*)(x + t * A.xs + k);
+      for (int j = 0; j < CH; ++j) xs[j] = int4_load<0>(xb, x[j], 2 * k);
+    } else {
+      // (the row ends within the stage)
+#pragma unroll
+      for (int j = 0; j < CH; ++j) xs[j] = int4_load<0>(xb, k + 8 * xc < K && x[j] != kOutside ? x[j] + (uint32_t)(2 * k) : kOutside, 0);
     }
   };
   auto load_w = [&](int stage) {
-    const int64_t k = (int64_t)stage * STAGE;
+    const int k = stage * STAGE;
+    const bool whole = k + STAGE <= K;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int64_t at = k + 64 * j + 32 * half;  // (past the row's end x is 0)
-        q[i][j] = *(const u32x4p*)(w[i] + (at < A.K ? at / 2 : 0));
+        if (whole) q[i][j] = int4_load<0>(wb, w[i], k / 2 + 32 * j);
+        else q[i][j] = int4_load<0>(wb, k + 64 * j + 32 * half < K ? w[i] + (uint32_t)(k / 2 + 32 * j) : kOutside, 0);
       }
-      int4_scales<SPAN, SPANS, X>(A, row[i], k, s[i], c[i]);
+      sc[i].load(A, groups, row[i], k);
     }
   };
   auto store_x = [&](int buffer) {
@@ -131,6 +141,11 @@ __global__ void __launch_bounds__(256, OCC) int4_tile_kernel(const Int4Args A) {
     }
   };
 
+  // where a lane's block f of a stage's first span lies: row l32, chunk 2 f + half (and 32 FR bytes on, by exclusive or, the next)
+  uint32_t chunk[FR];
+#pragma unroll
+  for (int f = 0; f < FR; ++f) chunk[f] = l32 * (STAGE * 2) + 16 * ((2 * f + half) ^ (l32 & 15));
+
   f32x16p y[MT][NW];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -146,7 +161,7 @@ __global__ void __launch_bounds__(256, OCC) int4_tile_kernel(const Int4Args A) {
       const char* const from = smem + ((stage - lo) & 1) * C::LDS1;
       // the words that the matrix instructions take: block f of 16 values, words exchanged between the half-waves
       uint32_t word[NW][8];
-      float sn[NW][SPANS], cn[NW][SPANS];
+      Int4Scales<SPAN, SPANS> now[NW];
 #pragma unroll
       for (int i = 0; i < NW; ++i) {
 #pragma unroll
@@ -155,41 +170,46 @@ __global__ void __launch_bounds__(256, OCC) int4_tile_kernel(const Int4Args A) {
           const auto b = __builtin_amdgcn_permlane32_swap(q[i][j][2], q[i][j][3], false, false);
           word[i][4 * j] = a[0], word[i][4 * j + 1] = b[0], word[i][4 * j + 2] = a[1], word[i][4 * j + 3] = b[1];
         }
-#pragma unroll
-        for (int p = 0; p < SPANS; ++p) sn[i][p] = s[i][p], cn[i][p] = c[i][p];
+        now[i] = sc[i];
       }
       if (stage + 1 < hi) {
         load_x(stage + 1);
         load_w(stage + 1);
       }
-#pragma unroll
+      // (a loop: the compiler would put off the sums of one span behind the products of the next, past the registers)
+#pragma unroll 1
       for (int p = 0; p < SPANS; ++p) {
         u32x4p wf[NW][FR], zf[NW];
+        float scale[NW];
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-          zf[i] = sum_factors<X>(cn[i][p], half == 0);
+          zf[i] = sum_factors<X>(now[i].z[0], half == 0);
+          scale[i] = now[i].template scale<X>(A, 0);
 #pragma unroll
-          for (int f = 0; f < FR; ++f) wf[i][f] = int4_operand<X>(word[i][p * FR + f]);
+          for (int f = 0; f < FR; ++f) wf[i][f] = int4_operand<X>(word[i][f]);
+#pragma unroll
+          for (int f = 0; f + FR < 8; ++f) word[i][f] = word[i][f + FR];  // (the next span's come first)
+#pragma unroll
+          for (int j = 0; j + 1 < SPANS; ++j) now[i].s[j] = now[i].s[j + 1], now[i].z[j] = now[i].z[j + 1];
         }
+        const char* const sums = from + C::XB + (p * C::BM + l32) * 16;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const int r = 32 * m + l32;
           f32x16p acc[NW];
-          const u32x4p sf = *(const u32x4p*)(from + C::XB + (p * C::BM + r) * 16);
+          const u32x4p sf = *(const u32x4p*)(sums + 32 * m * 16);
 #pragma unroll
           for (int i = 0; i < NW; ++i) acc[i] = X::mma32(sf, zf[i], f32x16p{});
 #pragma unroll
           for (int f = 0; f < FR; ++f) {
-            const u32x4p xf = *(const u32x4p*)(from + r * (STAGE * 2) + 16 * ((2 * (p * FR + f) + half) ^ (r & 15)));
+            const u32x4p xf = *(const u32x4p*)(from + (chunk[f] ^ (p * (32 * FR))) + 32 * m * (STAGE * 2));
 #pragma unroll
             for (int i = 0; i < NW; ++i) acc[i] = X::mma32(xf, wf[i][f], acc[i]);
           }
 #pragma unroll
           for (int i = 0; i < NW; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[m][i][e] = __builtin_fmaf(sn[i][p], acc[i][e], y[m][i][e]);
+            for (int e = 0; e < 16; ++e) y[m][i][e] = __builtin_fmaf(scale[i], acc[i][e], y[m][i][e]);
         }
-        __builtin_amdgcn_sched_barrier(0);  // (spans of one stage at once would not fit the registers)
       }
       if (stage + 1 < hi) {
         store_x((stage + 1 - lo) & 1);
@@ -230,7 +250,7 @@ __global__ void __launch_bounds__(256, OCC) int4_tile_kernel(const Int4Args A) {
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-      const int64_t n = n0 + 32 * i + l32;
+      const int64_t n = n0 + wave * (32 * NW) + 32 * i + l32;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int64_t t = t0 + 32 * m + 8 * (e >> 2) + 4 * half + (e & 3);
@@ -272,6 +292,7 @@ void int4_tile_plan(Int4Args& a, int64_t* ws_floats, int64_t* counters) {
   const int64_t bm = 32 * a.tiles_t, bn = 128 * a.tiles_n;
   const int64_t tiles = ((a.T + bm - 1) / bm) * ((a.N + bn - 1) / bn), stages = (a.K + STAGE - 1) / STAGE;
   if (tiles > INT32_MAX) { a.kernel = INT4_ANY; return; }
+  a.steps = (int32_t)stages;
   a.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, stages / 4));
   if (a.parts > 1) {
     *ws_floats = tiles * a.parts * (bm * bn);
