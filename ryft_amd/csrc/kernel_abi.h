@@ -446,13 +446,13 @@ struct Int4Args {
   // set by int4_matmul_plan: the kernel and its split
   int32_t kernel;       // Int4Kernel
   int32_t span;         // values whose scale is one, at a time: 32, 64 or 128
-  int32_t tiles_t, tiles_n;  // tiles a wavefront takes along T and N
+  int32_t tile;         // rows of x a tile, of 32 (INT4_TILE)
+  int32_t x_steps;      // steps of x that a wavefront keeps in registers (INT4_FEW)
   int32_t parts;        // ranges of K of an output tile
   int32_t groups;       // K / G
   int32_t group_spans;  // G / span
   int32_t steps;        // of the K loop
-  float* ws;            // partial sums; every one that is read was written by the same launch
-  int32_t* counters;    // arrivals, one a tile: zero between launches
+  float* ws;            // what INT4_TILE's launches leave for one another
 };
 enum Int4Kernel : int32_t { INT4_ANY = 0, INT4_FEW = 1, INT4_TILE = 2 };
 

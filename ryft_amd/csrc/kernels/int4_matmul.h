@@ -44,78 +44,38 @@ struct Int4F16 {
   __device__ static __forceinline__ uint16_t put(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
 };
 
-// A word's eight values as 16 + q, in the order above.
+// A word's eight values as 16 + q, in the order above. The constants are kept in registers: with a literal, masking and joining
+// are two instructions.
 template <class X>
-__device__ __forceinline__ u32x4p int4_operand(uint32_t w) {
-  auto pair = [](uint32_t v) { return (v & X::MASK) | X::BASE; };
-  u32x4p f;
-  f[0] = pair(w << X::SHIFT);
+struct Int4Operand {
+  uint32_t mask = X::MASK, base = X::BASE;
+  __device__ __forceinline__ Int4Operand() {
+    asm volatile("" : "+s"(mask));
+    asm volatile("" : "+v"(base));
+  }
+  __device__ __forceinline__ u32x4p operator()(uint32_t w) const {
+    u32x4p f;
 #pragma unroll
-  for (int i = 1; i < 4; ++i) f[i] = pair(4 * i > X::SHIFT ? w >> (4 * i - X::SHIFT > 0 ? 4 * i - X::SHIFT : 0) : w << (X::SHIFT - 4 * i > 0 ? X::SHIFT - 4 * i : 0));
-  return f;
-}
+    for (int i = 0; i < 4; ++i) {
+      constexpr int S = X::SHIFT;
+      const uint32_t v = 4 * i >= S ? w >> (4 * i >= S ? 4 * i - S : 0) : w << (4 * i < S ? S - 4 * i : 0);
+      f[i] = (v & mask) | base;
+    }
+    return f;
+  }
+};
 // Eight consecutive values of x in that order.
 __device__ __forceinline__ u32x4p int4_order(const u32x4p& v) {
   return u32x4p{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
                 __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
 }
 
-// Loads through buffer descriptors: one address register a lane for the whole loop, `step` bytes on in it. A lane's place is
-// inside the buffer or kOutside, which reads zeros; `step` alone never passes the buffer's end, so that nothing here depends on
-// whether the hardware's check counts it.
-constexpr uint32_t kOutside = 0x80000000u;
+// Loads go through buffer descriptors: one address register a lane for the whole loop. No lane's place is outside its buffer, so
+// that nothing here depends on the hardware's check.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t int4_buffer(const void* p, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)max((int64_t)0, min(bytes, (int64_t)0x7fffffff)), 0x00020000);
 }
-template <int AUX>
-__device__ __forceinline__ u32x4p int4_load(__amdgpu_buffer_rsrc_t r, uint32_t at, int step) {
-  return __builtin_bit_cast(u32x4p, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, step, AUX));
-}
 constexpr int kOnce = 2;  // nt: read once, past the caches' use for it
-
-// The groups of the rows of a weight from row n0 < N on.
-struct Int4Groups {
-  __amdgpu_buffer_rsrc_t s, z;
-  __device__ __forceinline__ Int4Groups(const Int4Args& A, int64_t n0) {
-    const int es = A.scale_dtype == DT_F32 ? 4 : 2;
-    const int64_t first = n0 * A.groups, rest = (A.N - n0) * A.groups;
-    s = int4_buffer((const char*)A.scale + first * es, rest * es);
-    z = int4_buffer(A.zero ? (const void*)(A.zero + first) : A.scale, A.zero ? rest : 0);
-  }
-};
-// Scales and zero points of `C` consecutive spans from value k on of the row whose groups begin `at` groups into them (spans
-// past the row's end: of its last group), as they lie in memory: nothing waits for them here.
-template <int SPAN, int C>
-struct Int4Scales {
-  uint32_t s[C], z[C];
-  __device__ __forceinline__ void load(const Int4Args& A, const Int4Groups& G, uint32_t at, int k) {
-    int g[C];
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-      g[i] = k / SPAN + i;
-      if (A.group_spans > 1) g[i] = (int)((uint32_t)g[i] / (uint32_t)A.group_spans);
-      g[i] = min(g[i], A.groups - 1);
-    }
-    if (A.scale_dtype == DT_F32) {
-#pragma unroll
-      for (int i = 0; i < C; ++i) s[i] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(G.s, (int)(4 * at), 4 * g[i], 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) s[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(G.s, (int)(2 * at), 2 * g[i], 0);
-    }
-    if (A.zero) {
-#pragma unroll
-      for (int i = 0; i < C; ++i) z[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(G.z, (int)at, g[i], 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) z[i] = 8;
-    }
-  }
-  template <class X>
-  __device__ __forceinline__ float scale(const Int4Args& A, int i) const {
-    return A.scale_dtype == DT_F32 ? __uint_as_float(s[i]) : X::lo(s[i]);
-  }
-};
 
 // A workgroup's range of the K loop's steps.
 __device__ __forceinline__ void int4_range(const Int4Args& A, int part, int& lo, int& hi) {
@@ -125,7 +85,7 @@ __device__ __forceinline__ void int4_range(const Int4Args& A, int part, int& lo,
 }
 
 // k_int4_tile.hip
-void int4_tile_plan(Int4Args& a, int64_t* ws_floats, int64_t* counters);
+void int4_tile_plan(Int4Args& a, int64_t* ws_floats);
 void launch_int4_tile(const Int4Args& a, hipStream_t stream, hipEvent_t done);
 
 }  // namespace ryft

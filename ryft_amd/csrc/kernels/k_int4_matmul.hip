@@ -55,183 +55,414 @@ __global__ void __launch_bounds__(256) int4_matmul_any_kernel(const Int4Args A) 
 }
 
 // ------------------------------------------------------------------------------------------------ up to 16 rows of x
-// bf16 and f16, groups of a multiple of 32: the weight's bytes bound it, so they go from memory into registers once, and
-// nothing else is waited for on their way. A workgroup has NT tiles of 16 rows of the weight, its eight wavefronts take every
-// eighth step of 256 values, and meet in LDS at the end, in one order; where that leaves the chip idle, `parts` workgroups
-// share a tile, and the last of them to arrive adds the parts, in their order too. A step's bytes are on their way while the
-// one before is multiplied.
+// bf16 and f16, groups of a multiple of 32: the weight's bytes bound it. A workgroup takes tiles of 16 rows of the weight, one
+// after the other; its wavefronts take every W-th step of 256 values, and meet in LDS at the tile's end, in one order.
 //
-// Scores the 16 rows of x as the first operand: a lane's four sums are of one row of the weight, so that it needs one scale
-// a group. A lane loads 32 values of a row, four lanes 128 together; the exchange between them leaves each with the values
+// Each wavefront streams its steps, weight, scales and zero points, from memory straight into a ring of its own in LDS, DEPTH
+// steps deep, over the tiles' borders, in whole lines (a lane that loaded its own 16 bytes of a row, as the matrix instructions
+// take them, had each of 16 neighbours on another line: 58 MB took 29 us so, 2.0 TB/s), and waits for its own loads only.
+//
+// x: where the wavefronts' steps of a row are S or fewer each and there is more than a tile a workgroup, every wavefront keeps
+// its part of x in registers for all its tiles. Otherwise x comes through the ring, as the weight does.
+//
+// The products have the 16 rows of x as the first operand: a lane's four sums are of one row of the weight, so that it needs one
+// scale a group. A lane reads 32 values of a row, four lanes 128 together; the exchange between them leaves each with the values
 // that a matrix instruction takes from it. Σ x comes from a product with ones.
-constexpr int FEW_WAVES = 8;
-constexpr int FEW_STEP = 256;
+constexpr int FEW_STEP = 256, CUS = 256;
 
-template <class X, int NT, int SPAN>
-__global__ void __launch_bounds__(64 * FEW_WAVES, 2) int4_few_kernel(const Int4Args A) {
-  constexpr int SPANS = FEW_STEP / SPAN, BLOCKS = SPAN / 32;
-  __shared__ f32x4p sums[FEW_WAVES][NT][64];
-  __shared__ int last;
+// XL: loads of two rows of x each, at least as many as there are rows. S: steps of x in registers, 0: x through the ring.
+template <int SPAN, int XL, int S>
+struct FewCfg {
+  static constexpr int W = S || XL <= 4 ? 8 : 4;     // wavefronts (with 16 rows of x in the rings there is no room for eight)
+  static constexpr int SPANS = FEW_STEP / SPAN;
+  static constexpr int SL = SPANS > 4 ? 2 : 1;       // loads of a tile's scales: SPANS words a row
+  static constexpr int SW = SPANS, ZW = SPANS > 4 ? 4 : 2;  // words a row of scales, of zero points
+  static constexpr int X0 = 2048, S0 = X0 + (S ? 0 : XL * 1024), Z0 = S0 + SL * 256, SLOT = Z0 + 512;
+  static constexpr int SUMS = W * 1024;              // bytes of a tile's sums
+  static constexpr int depth(int shares) { return (160 * 1024 / shares - 256 - 2 * SUMS) / (W * SLOT); }  // with that many on a CU
+  static constexpr int SHARES = !S && depth(2) >= 2 ? 2 : 1;
+  static constexpr int DEPTH = depth(SHARES) < 7 ? depth(SHARES) : 7;
+  static constexpr int LDS = W * DEPTH * SLOT + 2 * SUMS;
+  static constexpr int LOADS = 3 + SL + (S ? 0 : XL);  // of a step
+  static_assert(DEPTH >= 2, "");
+};
+
+typedef __attribute__((address_space(3))) void few_lds;
+
+// LDS reads that the compiler does not order behind the loads on their way: waited for in their statement.
+__device__ __forceinline__ void few_read_x(u32x4p (&f)[8], uint32_t a, uint32_t b) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n ds_read_b128 %1, %9\n ds_read_b128 %2, %8 offset:128\n ds_read_b128 %3, %9 offset:128\n"
+      "ds_read_b128 %4, %8 offset:256\n ds_read_b128 %5, %9 offset:256\n ds_read_b128 %6, %8 offset:384\n ds_read_b128 %7, %9 offset:384\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7])
+      : "v"(a), "v"(b)
+      : "memory");
+}
+// A row's 32 bytes of the weight, and its words of scales and zero points.
+typedef uint32_t u32x2f __attribute__((ext_vector_type(2)));
+template <int SPANS>
+__device__ __forceinline__ void few_read_w(u32x4p (&f)[2], uint32_t (&s)[8], uint32_t (&z)[4], uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  if constexpr (SPANS == 2) {
+    u32x2f u, v;
+    asm volatile("ds_read_b64 %2, %6\n ds_read_b64 %3, %7\n ds_read_b128 %0, %4\n ds_read_b128 %1, %5\n s_waitcnt lgkmcnt(0)"
+                 : "=&v"(f[0]), "=&v"(f[1]), "=&v"(u), "=&v"(v)
+                 : "v"(a), "v"(b), "v"(c), "v"(d)
+                 : "memory");
+    s[0] = u[0], s[1] = u[1], z[0] = v[0], z[1] = v[1];
+  } else if constexpr (SPANS == 4) {
+    u32x4p u;
+    u32x2f v;
+    asm volatile("ds_read_b128 %2, %6\n ds_read_b64 %3, %7\n ds_read_b128 %0, %4\n ds_read_b128 %1, %5\n s_waitcnt lgkmcnt(0)"
+                 : "=&v"(f[0]), "=&v"(f[1]), "=&v"(u), "=&v"(v)
+                 : "v"(a), "v"(b), "v"(c), "v"(d)
+                 : "memory");
+    s[0] = u[0], s[1] = u[1], s[2] = u[2], s[3] = u[3], z[0] = v[0], z[1] = v[1];
+  } else {
+    u32x4p u, w, v;
+    asm volatile("ds_read_b128 %2, %7\n ds_read_b128 %3, %7 offset:16\n ds_read_b128 %4, %8\n ds_read_b128 %0, %5\n ds_read_b128 %1, %6\n s_waitcnt lgkmcnt(0)"
+                 : "=&v"(f[0]), "=&v"(f[1]), "=&v"(u), "=&v"(w), "=&v"(v)
+                 : "v"(a), "v"(b), "v"(c), "v"(d)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = u[i], s[4 + i] = w[i], z[i] = v[i];
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void few_wait() {  // until N loads or fewer are on their way
+  constexpr int n = N > 63 ? 63 : N;
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (n & 15) | (n >> 4) << 14);
+}
+
+template <class X, int SPAN, int XL, int S>
+__global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_kernel(const Int4Args A) {
+  typedef FewCfg<SPAN, XL, S> C;
+  constexpr int SPANS = C::SPANS, BLOCKS = SPAN / 32, W = C::W;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g16 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
-  const int part = blockIdx.y, K = (int)A.K;
-  int lo, hi;
-  int4_range(A, part, lo, hi);
+  const int K = (int)A.K, T = (int)A.T, N = (int)A.N, steps = A.steps;
+  const int tiles = (N + 15) / 16;
 
-  const __amdgpu_buffer_rsrc_t wb = int4_buffer(A.w + n0 * (K / 2), (A.N - n0) * (K / 2)), xb = int4_buffer(A.x, A.T * A.xs * 2);
-  const Int4Groups groups(A, n0);
-  uint32_t w[NT], row[NT];
+  const int es = A.scale_dtype == DT_F32 ? 4 : 2;
+  const __amdgpu_buffer_rsrc_t xb = int4_buffer(A.x, A.T * A.xs * 2);
+  uint32_t x_row[XL];  // position c of row r holds chunk c ^ (r mod 8)
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int r = (int)min((int64_t)(16 * i + l16), A.N - 1 - n0);  // (rows past the last are computed and not stored)
-    w[i] = (uint32_t)r * (uint32_t)(K / 2) + 16 * g16;
-    row[i] = (uint32_t)r * (uint32_t)A.groups;
+  for (int h = 0; h < XL; ++h)
+    x_row[h] = (uint32_t)min(2 * h + (lane >> 5), T - 1) * (uint32_t)(2 * A.xs) + 16 * ((lane & 31) ^ ((2 * h + (lane >> 5)) & 7));
+  const int w_chunk = (lane & 7) ^ (lane >> 3);
+  char* const ring = smem + wave * (C::DEPTH * C::SLOT);
+  const uint32_t ring_at = (uint32_t)(uintptr_t)(few_lds*)ring;
+  if (!A.zero) {
+    // (the zero points that the loads below leave alone)
+#pragma unroll
+    for (int d = 0; d < C::DEPTH; ++d) ((uint32_t*)(ring + d * C::SLOT + C::Z0))[lane] = 0x08080808u;
   }
-  const uint32_t x = l16 < A.T ? (uint32_t)(l16 * (int)A.xs + 8 * g16) * 2 : kOutside;
 
-  struct Step {
-    u32x4p w[NT][2], x[8];
-    Int4Scales<SPAN, SPANS> s[NT];
+  // First group of step `step`, of those that a row has.
+  auto first_group = [&](int step) {
+    int g = step * SPANS;
+    if (A.group_spans > 1) g = (int)((uint32_t)g / (uint32_t)A.group_spans);
+    return min(g, A.groups - 1);
   };
-  auto load = [&](Step& v, int step) {
-    const int k = step * FEW_STEP;
-    if (k + FEW_STEP <= K) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) v.w[i][j] = int4_load<kOnce>(wb, w[i], k / 2 + 64 * j);
-#pragma unroll
-      for (int b = 0; b < 8; ++b) v.x[b] = int4_load<0>(xb, x, 2 * (k + 32 * b));
-    } else {
-      // (the row ends within the step)
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          v.w[i][j] = int4_load<kOnce>(wb, k + 128 * j + 32 * g16 < K ? w[i] + (uint32_t)(k / 2 + 64 * j) : kOutside, 0);
-#pragma unroll
-      for (int b = 0; b < 8; ++b)
-        v.x[b] = int4_load<0>(xb, k + 32 * b < K && x != kOutside ? x + (uint32_t)(2 * (k + 32 * b)) : kOutside, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) v.s[i].load(A, groups, row[i], k);
+  // Steps on one line: of tile blockIdx.x, + gridDim.x, ... one after the other.
+  struct Place {
+    int tile, step;
   };
-
-  f32x4p y[NT];
+  auto rows_of = [&](int tile) { return min(16, N - tile * 16); };  // (rows past the last are computed as it, not stored)
+  // Loads of a step at `ahead`: places of a lane within its tile's rows. A row of the weight has eight chunks of 16 bytes a step,
+  // one of x 32: position c of row r holds chunk c ^ (r mod 8), so that the reads below take different banks. Scales and zero
+  // points come in whole words (a tile's begin with one; the last of an odd number of 16-bit scales lies in one with two bytes that belong to no one, as
+  // the last zero points may). Loads never leave the buffers: of a step that a row ends in, chunks past its end are read from
+  // its beginning, and words past the last as that.
+  Place ahead;
+  uint32_t w_row[2], s_row[C::SL], z_row;
+  __amdgpu_buffer_rsrc_t wb, sb, zb;
+  uint32_t s_last = 0, z_last = 0;
+  const int64_t w_next = (int64_t)16 * (K / 2), s_next = (int64_t)16 * A.groups * es, z_next = (int64_t)16 * A.groups;  // bytes of a tile: whole words
+  auto places = [&](int rows) {
 #pragma unroll
-  for (int i = 0; i < NT; ++i) y[i] = f32x4p{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](const Step& v) {
-    const u32x4p ones = {X::ONES, X::ONES, X::ONES, X::ONES};
-    // word of block b that this lane has: the four words of lane group g are blocks' words, exchanged between the groups
-    u32x4p q[NT][2];
+    for (int h = 0; h < 2; ++h) w_row[h] = (uint32_t)min(8 * h + (lane >> 3), rows - 1) * (uint32_t)(K / 2) + 16 * w_chunk;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int h = 0; h < C::SL; ++h) s_row[h] = (uint32_t)(min((64 * h + lane) / C::SW, rows - 1) * A.groups) * es;
+    z_row = (uint32_t)(min(lane / C::ZW, rows - 1) * A.groups);
+  };
+  auto enter = [&]() {  // `ahead` is at a tile's first step
+    const int rows = rows_of(ahead.tile);
+    const uint32_t s_bytes = (uint32_t)min((int64_t)(N - ahead.tile * 16) * A.groups * es + 3, (int64_t)0x7ffffffc) & ~3u;
+    const uint32_t z_bytes = (uint32_t)min((int64_t)(N - ahead.tile * 16) * A.groups + 3, (int64_t)0x7ffffffc) & ~3u;
+    wb = int4_buffer(A.w + ahead.tile * w_next, (int64_t)rows * (K / 2));
+    sb = int4_buffer((const char*)A.scale + ahead.tile * s_next, s_bytes);
+    zb = A.zero ? int4_buffer(A.zero + ahead.tile * z_next, z_bytes) : sb;
+    s_last = s_bytes - 4, z_last = (A.zero ? z_bytes : s_bytes) - 4;
+    if (rows < 16) places(rows);
+  };
+  const int z_to = A.zero ? C::Z0 : C::Z0 + 256;
+  auto fetch = [&](int slot) {
+    const int step = ahead.step, k = step * FEW_STEP;
+    char* const to = ring + slot * C::SLOT;
+    const bool whole = k + FEW_STEP <= K;
+    if (whole) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const u32x4p d = v.w[i][j];
-        const auto a = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), b = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
-        const auto e = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), f = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-        q[i][j] = u32x4p{e[0], e[1], f[0], f[1]};
+      for (int h = 0; h < 2; ++h) __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (few_lds*)(to + h * 1024), 16, (int)w_row[h], k / 2, 0, kOnce);
+      if constexpr (S == 0) {
+#pragma unroll
+        for (int h = 0; h < XL; ++h) __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (few_lds*)(to + C::X0 + h * 1024), 16, (int)x_row[h], 2 * k, 0, 0);
       }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t at = k + 32 * w_chunk < K ? w_row[h] + k / 2 : w_row[h] - 16 * w_chunk;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (few_lds*)(to + h * 1024), 16, (int)at, 0, 0, kOnce);
+      }
+      if constexpr (S == 0) {
+#pragma unroll
+        for (int h = 0; h < XL; ++h) {
+          const int chunk = (lane & 31) ^ ((2 * h + (lane >> 5)) & 7);
+          const uint32_t at = k + 8 * chunk < K ? x_row[h] + 2 * k : x_row[h] - 16 * chunk;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (few_lds*)(to + C::X0 + h * 1024), 16, (int)at, 0, 0, 0);
+        }
+      }
+    }
+    const uint32_t g = (uint32_t)first_group(step);
+#pragma unroll
+    for (int h = 0; h < C::SL; ++h) {
+      const uint32_t at = ((s_row[h] + g * es) & ~3u) + 4 * ((64 * h + lane) % C::SW);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (few_lds*)(to + C::S0 + h * 256), 4, (int)min(at, s_last), 0, 0, 0);
+    }
+    // (without zero points some of the scales, to a place that no one reads: for the number of loads)
+    const uint32_t z = ((z_row + g) & ~3u) + 4 * (lane % C::ZW);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(zb, (few_lds*)(to + z_to), 4, (int)min(z, z_last), 0, 0, 0);
+    ahead.step += W;
+    if (ahead.step >= steps) {
+      ahead.step = wave, ahead.tile += (int)gridDim.x;
+      if (ahead.tile < tiles) enter();
+    }
+  };
+  // Waits until the oldest of `later` + 1 steps on their way is there.
+  auto arrived = [&](int later) {
+    asm volatile("" ::: "memory");
+    constexpr int L = C::LOADS, D = C::DEPTH - 1;
+    if (later >= D) few_wait<D * L>();
+    else if (D > 4 && later >= 4) few_wait<4 * L>();
+    else if (D > 2 && later >= 2) few_wait<2 * L>();
+    else if (D > 1 && later == 1) few_wait<L>();
+    else few_wait<0>();
+    asm volatile("" ::: "memory");
+  };
+
+  const Int4Operand<X> operand;
+  const u32x4p ones = {X::ONES, X::ONES, X::ONES, X::ONES};
+  f32x4p y;
+  uint32_t row;  // groups before this lane's row of the tile
+  const int xl = min(l16, 2 * XL - 1);  // (rows that there are not: of the last, and not stored)
+  const uint32_t w_at = ring_at + l16 * 128, w_pos = 16 * (g16 ^ (l16 & 7)), x_at = ring_at + C::X0 + xl * 512, x_pos = 16 * (g16 ^ (xl & 7));
+  const uint32_t s_at = ring_at + C::S0 + l16 * (4 * C::SW), z_at = ring_at + C::Z0 + l16 * (4 * C::ZW);
+  // the part of x in registers, in a word's order, and its sums where they are few
+  constexpr bool SUMMED = S > 0 && SPAN == 128;
+  u32x4p x_own[S ? S : 1][8];
+  f32x4p x_sum[SUMMED ? S : 1][SPANS];
+  if constexpr (S > 0) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int at = 0; at < 8; ++at) {
+        const int k = (wave + W * s) * FEW_STEP + 32 * at + 8 * g16;
+        x_own[s][at] = u32x4p{0u, 0u, 0u, 0u};
+        if (k < K) x_own[s][at] = *(const u32x4p*)((const uint16_t*)A.x + (int64_t)min(l16, T - 1) * A.xs + k);
+      }
+  }
+  auto multiply = [&](int step, int slot, const u32x4p (&xo)[8], const f32x4p (&xs)[SPANS]) {
+    const uint32_t off = (uint32_t)slot * C::SLOT;
+    u32x4p xv[8], wv[2];
+    uint32_t sv[8], zv[4];
+    if constexpr (S == 0) few_read_x(xv, x_at + off + x_pos, x_at + off + (x_pos ^ 64));
+    few_read_w<SPANS>(wv, sv, zv, w_at + off + w_pos, w_at + off + (w_pos ^ 64), s_at + off, z_at + off);
+    // scales and zero points of the step's spans (0 past the row's end)
+    float scale[SPANS], c[SPANS];
+    const uint32_t g0 = (uint32_t)first_group(step);
+    const int left = (K - step * FEW_STEP) / SPAN;
+    const uint32_t before = row + g0;
+#pragma unroll
+    for (int p = 0; p < SPANS; p += 4) {
+      const uint32_t z = __builtin_amdgcn_alignbyte(zv[p / 4 + 1], zv[p / 4], A.zero ? before & 3 : 0);
+#pragma unroll
+      for (int e = 0; e < 4 && p + e < SPANS; ++e) c[p + e] = -16.f - (float)(z >> (8 * e) & 255u);
+    }
+    if (es == 4) {
+#pragma unroll
+      for (int p = 0; p < SPANS; ++p) scale[p] = __uint_as_float(sv[p]);
+    } else {
+#pragma unroll
+      for (int p = 0; p < SPANS; p += 2) {
+        const uint32_t w = __builtin_amdgcn_alignbyte(sv[p / 2 + 1], sv[p / 2], 2 * before & 2);
+        scale[p] = X::lo(w & 0xffffu), scale[p + 1] = X::hi(w);
+      }
+    }
+    if (A.group_spans > 1) {
+      // (several spans a group: of the groups that were read, each the one that it lies in)
+      float s1[SPANS], c1[SPANS];
+#pragma unroll
+      for (int p = 0; p < SPANS; ++p) {
+        const int g = (int)((uint32_t)(step * SPANS + p) / (uint32_t)A.group_spans) - (int)g0;
+        s1[p] = scale[0], c1[p] = c[0];
+#pragma unroll
+        for (int j = 1; j < SPANS; ++j) s1[p] = g == j ? scale[j] : s1[p], c1[p] = g == j ? c[j] : c1[p];
+      }
+#pragma unroll
+      for (int p = 0; p < SPANS; ++p) scale[p] = s1[p], c[p] = c1[p];
+    }
+    if (left < SPANS) {
+#pragma unroll
+      for (int p = 1; p < SPANS; ++p)
+        if (p >= left) scale[p] = 0.f;
+    }
+    // word of block b that this lane has: the four words of lane group g are blocks' words, exchanged between the groups
+    u32x4p q[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const u32x4p d = wv[j];
+      const auto a = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), b = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+      const auto e = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), f = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+      q[j] = u32x4p{e[0], e[1], f[0], f[1]};
+    }
 #pragma unroll
     for (int p = 0; p < SPANS; ++p) {
-      u32x4p xf[BLOCKS];
-      f32x4p sx = {0.f, 0.f, 0.f, 0.f};
+      f32x4p sx = {0.f, 0.f, 0.f, 0.f}, acc = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (SUMMED) sx = xs[p];
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
-        xf[b] = int4_order(v.x[p * BLOCKS + b]);
-        sx = X::mma16(xf[b], ones, sx);
+        const int at = p * BLOCKS + b;
+        const u32x4p xf = S ? xo[at] : int4_order(xv[at]);
+        if constexpr (!SUMMED) sx = X::mma16(xf, ones, sx);
+        acc = X::mma16(xf, operand(q[at >> 2][at & 3]), acc);
       }
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const float scale = v.s[i].template scale<X>(A, p), c = -16.f - (float)v.s[i].z[p];
-        f32x4p acc;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = c * sx[r];
-#pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-          const int at = p * BLOCKS + b;
-          acc = X::mma16(xf[b], int4_operand<X>(q[i][at >> 2][at & 3]), acc);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[i][r] = __builtin_fmaf(scale, acc[r], y[i][r]);
-      }
+      for (int r = 0; r < (XL == 1 ? 2 : 4); ++r) y[r] = __builtin_fmaf(scale[p], __builtin_fmaf(c[p], sx[r], acc[r]), y[r]);
     }
   };
-  int step = lo + wave;
-  if (step < hi) {
-    Step a, b;
-    load(a, step);
-    while (true) {
-      if (step + FEW_WAVES < hi) load(b, step + FEW_WAVES);
-      multiply(a);
-      step += FEW_WAVES;
-      if (step >= hi) break;
-      if (step + FEW_WAVES < hi) load(a, step + FEW_WAVES);
-      multiply(b);
-      step += FEW_WAVES;
-      if (step >= hi) break;
+  Place here{(int)blockIdx.x, wave};
+  if (here.step >= steps) here.tile = tiles;  // (a wavefront without steps only takes part in the sums)
+  ahead = here;
+  places(16);
+  if (ahead.tile < tiles) enter();
+  int slot = 0, to = 0, count = 0;  // count: steps on their way
+#pragma unroll 1
+  for (int d = 0; d < C::DEPTH - 1 && ahead.tile < tiles; ++d, ++count, ++to) fetch(to);
+  if constexpr (S > 0) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int at = 0; at < 8; ++at) x_own[s][at] = int4_order(x_own[s][at]);
+    if constexpr (SUMMED) {
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int p = 0; p < SPANS; ++p) {
+          x_sum[s][p] = f32x4p{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int b = 0; b < BLOCKS; ++b) x_sum[s][p] = X::mma16(x_own[s][p * BLOCKS + b], ones, x_sum[s][p]);
+        }
     }
   }
-#pragma unroll
-  for (int i = 0; i < NT; ++i) sums[wave][i][lane] = y[i];
-  __syncthreads();
-  // thread i of the first NT · 64: lane i % 64 of tile i / 64
-  const int i = tid >> 6;
-  f32x4p sum = {0.f, 0.f, 0.f, 0.f};
-  if (i < NT) {
-#pragma unroll
-    for (int u = 0; u < FEW_WAVES; ++u) sum += sums[u][i][lane];
-  }
-  if (A.parts > 1) {
-    const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc((void*)(A.ws + (int64_t)blockIdx.x * A.parts * (NT * 256)), (short)0, -1, 0x00020000);
-    if (i < NT) agent_put4(ws, (uint32_t)(part * NT * 64 + tid) * 16, sum);
-    if (!last_to_arrive(A.counters + blockIdx.x, A.parts, &last)) return;
-    if (i < NT) {
-      sum = f32x4p{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int u = 0; u < A.parts; ++u) sum += agent_get4(ws, (uint32_t)(u * NT * 64 + tid) * 16);
+  int turn = 0;
+  auto forward = [&]() {  // has the next step loaded and waits for the oldest
+    if (ahead.tile < tiles) {
+      fetch(to);
+      ++count;
+      if (++to == C::DEPTH) to = 0;
     }
-  }
-  const int64_t n = n0 + 16 * i + l16;
-  if (i >= NT || n >= A.N) return;
+    arrived(--count);
+  };
+  for (int tile = blockIdx.x; tile < tiles; tile += (int)gridDim.x, ++turn) {
+    y = f32x4p{0.f, 0.f, 0.f, 0.f};
+    row = (uint32_t)(min(l16, rows_of(tile) - 1) * A.groups);
+    if constexpr (S > 0) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int64_t t = 4 * g16 + r;
-    if (t >= A.T) continue;
-    if (A.y_dtype == DT_F32) ((float*)A.y)[t * A.N + n] = sum[r];
-    else ((uint16_t*)A.y)[t * A.N + n] = X::put(sum[r]);
+      for (int s = 0; s < S; ++s) {
+        if (wave + W * s >= steps) break;
+        forward();
+        multiply(wave + W * s, slot, x_own[s], x_sum[SUMMED ? s : 0]);
+        if (++slot == C::DEPTH) slot = 0;
+      }
+    } else {
+#pragma unroll 1
+      while (here.tile == tile) {
+        forward();
+        multiply(here.step, slot, x_own[0], x_sum[0]);
+        if (++slot == C::DEPTH) slot = 0;
+        here.step += W;
+        if (here.step >= steps) here.step = wave, here.tile += (int)gridDim.x;
+      }
+    }
+    // The wavefronts' sums, by turns in one of two places: a wavefront writes one again only after all have passed the barrier
+    // of the tile between.
+    const uint32_t sums = (uint32_t)(uintptr_t)(few_lds*)(smem + W * C::DEPTH * C::SLOT + (turn & 1) * C::SUMS);  // [W][64]
+    asm volatile("ds_write_b128 %0, %1\n s_waitcnt lgkmcnt(0)" ::"v"(sums + (wave * 64 + lane) * 16), "v"(y) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (wave != turn % W) continue;  // (the wavefronts finish tiles by turns)
+    f32x4p sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < W; u += 4) {
+      f32x4p v[4];
+      asm volatile("ds_read_b128 %0, %4\n ds_read_b128 %1, %4 offset:1024\n ds_read_b128 %2, %4 offset:2048\n ds_read_b128 %3, %4 offset:3072\n s_waitcnt lgkmcnt(0)"
+                   : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+                   : "v"(sums + (u * 64 + lane) * 16)
+                   : "memory");
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += v[j];
+    }
+    const int n = tile * 16 + l16;
+    if (n >= N) continue;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int t = 4 * g16 + r;
+      if (t >= T) continue;
+      if (A.y_dtype == DT_F32) ((float*)A.y)[(int64_t)t * N + n] = sum[r];
+      else ((uint16_t*)A.y)[(int64_t)t * N + n] = X::put(sum[r]);
+    }
   }
 }
 
-template <class X, int NT>
+template <class X, int SPAN, int XL, int S>
+void launch_few_of(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
+  typedef FewCfg<SPAN, XL, S> C;
+  const hipError_t e = hipFuncSetAttribute((const void*)int4_few_kernel<X, SPAN, XL, S>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+  if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("int4_matmul LDS attribute: ") + hipGetErrorString(e));
+  const dim3 grid((unsigned)std::min<int64_t>((a.N + 15) / 16, C::SHARES * CUS));
+  launch_k(done, int4_few_kernel<X, SPAN, XL, S>, grid, dim3(64 * C::W), C::LDS, stream, a);
+}
+template <class X, int SPAN>
+void launch_few_span(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
+  if (a.x_steps == 1) launch_few_of<X, SPAN, 8, 1>(a, stream, done);
+  else if (a.x_steps == 2) launch_few_of<X, SPAN, 8, 2>(a, stream, done);
+  else if (a.x_steps == 4) launch_few_of<X, SPAN, 8, 4>(a, stream, done);
+  else if (a.T <= 2) launch_few_of<X, SPAN, 1, 0>(a, stream, done);
+  else if (a.T <= 8) launch_few_of<X, SPAN, 4, 0>(a, stream, done);
+  else launch_few_of<X, SPAN, 8, 0>(a, stream, done);
+}
+template <class X>
 void launch_few(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
-  const dim3 grid((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)a.parts), block(64 * FEW_WAVES);
-  if (a.span == 128) launch_k(done, int4_few_kernel<X, NT, 128>, grid, block, 0, stream, a);
-  else if (a.span == 64) launch_k(done, int4_few_kernel<X, NT, 64>, grid, block, 0, stream, a);
-  else launch_k(done, int4_few_kernel<X, NT, 32>, grid, block, 0, stream, a);
+  if (a.span == 128) launch_few_span<X, 128>(a, stream, done);
+  else if (a.span == 64) launch_few_span<X, 64>(a, stream, done);
+  else launch_few_span<X, 32>(a, stream, done);
 }
 
-void few_plan(Int4Args& a, int64_t* ws_floats, int64_t* counters) {
+void few_plan(Int4Args& a) {
   a.kernel = INT4_FEW;
-  a.tiles_t = 1;
-  const int64_t steps = (a.K + FEW_STEP - 1) / FEW_STEP;
-  a.steps = (int32_t)steps;
-  a.tiles_n = a.N >= 16384 ? 2 : 1;
-  const int64_t tiles = (a.N + 16 * a.tiles_n - 1) / (16 * a.tiles_n);
-  // ranges of K until there are two workgroups a CU, each with a step for every wavefront
-  a.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(512 / tiles, steps / FEW_WAVES));
-  if (a.parts > 1) {
-    *ws_floats = tiles * a.parts * a.tiles_n * 256;
-    *counters = tiles;
-  }
+  a.steps = (int32_t)((a.K + FEW_STEP - 1) / FEW_STEP);
+  // x in registers: 16 rows, 4096 values against 28672 rows of the weight, bf16: 20.5 us, through the ring 29.8; 4 rows against
+  // 12288: 11.2 and 11.6. Not for one or two rows, of which a step's x is an eighth of the weight's bytes (28672 rows: 19.4 and
+  // 17.5), nor with a tile or less a workgroup (4096 x 4096, one row: 6.3 and 5.4).
+  if ((a.N + 15) / 16 > CUS && a.T > 2) a.x_steps = a.steps <= 8 ? 1 : a.steps <= 16 ? 2 : a.steps <= 32 ? 4 : 0;
 }
 
 }  // namespace
 
-void int4_matmul_plan(Int4Args& a, int64_t* ws_floats, int64_t* counters) {
-  *ws_floats = *counters = 0;
+void int4_matmul_plan(Int4Args& a, int64_t* ws_floats) {
+  *ws_floats = 0;
   a.kernel = INT4_ANY;
   a.parts = 1;
   if ((a.x_dtype != DT_BF16 && a.x_dtype != DT_F16) || a.G % 32 || a.T == 0) return;
@@ -240,19 +471,20 @@ void int4_matmul_plan(Int4Args& a, int64_t* ws_floats, int64_t* counters) {
   a.span = a.G % 128 == 0 ? 128 : a.G % 64 == 0 ? 64 : 32;
   a.groups = (int32_t)(a.K / a.G);
   a.group_spans = a.G / a.span;
-  if (a.T <= 16) return few_plan(a, ws_floats, counters);
-  int4_tile_plan(a, ws_floats, counters);
+  // (16 rows, 4096 x 28672: 20.5 us, with tiles 30; 14336 x 4096: 16.7 and 24; 4096 x 4096: 7.2 and 15. From 17 rows on a
+  // second pass over the weight would be needed.)
+  if (a.T <= 16) return few_plan(a);
+  int4_tile_plan(a, ws_floats);
 }
 
 void launch_int4_matmul(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
   if (a.K < 2 || a.K % 2 || a.N < 1 || a.G < 2 || a.G % 2 || a.K % a.G)
     fail(PJRT_Error_Code_INTERNAL, "int4_matmul of a shape the kernels do not take");
   if (a.T == 0) return record_done(done, stream);
-  if (a.kernel != INT4_ANY && a.parts > 1 && (!a.ws || !a.counters)) fail(PJRT_Error_Code_INTERNAL, "int4_matmul without a workspace");
   if (a.kernel == INT4_FEW) {
     if (a.T > 16) fail(PJRT_Error_Code_INTERNAL, "int4_matmul's kernel for few rows with many");
-    if (a.x_dtype == DT_BF16) a.tiles_n == 2 ? launch_few<Int4BF16, 2>(a, stream, done) : launch_few<Int4BF16, 1>(a, stream, done);
-    else a.tiles_n == 2 ? launch_few<Int4F16, 2>(a, stream, done) : launch_few<Int4F16, 1>(a, stream, done);
+    if (a.x_dtype == DT_BF16) launch_few<Int4BF16>(a, stream, done);
+    else launch_few<Int4F16>(a, stream, done);
   } else if (a.kernel == INT4_TILE) {
     launch_int4_tile(a, stream, done);
   } else {

@@ -1,4 +1,14 @@
-// ryft.int4_matmul with more than 16 rows of x, bf16 and f16, groups of a multiple of 32.
+// ryft.int4_matmul with more than a few rows of x, bf16 and f16, groups of a multiple of 32.
+//
+// Two or three launches. The first puts x into the order and the places that the second's LDS has, and sums it over every span
+// of values that share a scale: done by each workgroup of the second for itself it was most of its float and integer
+// instructions (2048 rows against 12288 x 4096: 361 us; 237 and 8 so, 870 TFLOP/s). The second multiplies tiles of 32 MT rows of
+// x, which a workgroup's eight wavefronts share through a ring in LDS, with 32 rows of the weight a wavefront, which come through
+// a ring of its own. A lane's sums are of one row of the weight, 16 rows of x each: one scale a span. Tiles are cut into ranges
+// of K where they leave the chip idle; the third adds the parts in their order.
+//
+// Bound by the issue of instructions around the matrix ones: of 237 us the products themselves take 105, turning 4-bit values
+// into operands and scaling the sums 70, the reads of x from LDS 80, and they overlap in part. Without LDS reads it took 116.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -13,13 +23,17 @@ namespace ryft {
 namespace {
 
 constexpr int STAGE = 128;  // values of x a stage
+constexpr int CUS = 256, LEAST = 4;  // workgroups that run at a time (LDS has room for one a CU); stages a range of K
+constexpr int AHEAD = 5;    // fragments of x on their way from LDS
 
-template <int MT, int SPAN>
-struct TileCfg {
-  static constexpr int BM = 32 * MT, SPANS = STAGE / SPAN;
-  static constexpr int XB = BM * STAGE * 2;         // bytes of a stage's x
-  static constexpr int LDS1 = XB + BM * SPANS * 16;  // and of the terms of its sums
-};
+// x as the second launch has it, for `rows` rows: of stage s and row t 256 bytes at (s · rows + t) · 256, chunk c (eight values,
+// in a word's order) at position c ^ (t mod 16); then of span p and row t 16 bytes at (p · rows + t) · 16: the terms of its sum.
+// A tile of the last rows reads on past them, whatever is there, and stores nothing of it: both parts end with room for that.
+constexpr int MOST_ROWS = 128;
+__host__ __device__ inline int64_t tile_x_bytes(int64_t steps, int64_t rows) { return (steps * rows + MOST_ROWS) * (STAGE * 2); }
+__host__ __device__ inline int64_t tile_ws_bytes(int64_t steps, int64_t rows, int span) {
+  return tile_x_bytes(steps, rows) + (steps * (STAGE / span) * rows + MOST_ROWS) * 16;
+}
 
 // Sum over the lanes of 4, 8 or 16 that have a span's chunks of eight values.
 template <int CTRL>
@@ -35,7 +49,7 @@ __device__ __forceinline__ float span_sum(float v) {
   return v;
 }
 
-// Terms of a span's sum S that a matrix instruction multiplies by -(16 + z): S = a · H + b + c, each rounded to 16 bits (a: a
+// Terms of a span's sum S that a matrix instruction multiplies by -(16 + z): S = a · H + b + c, each rounded to 16 bits (H: a
 // power of two that keeps f16 from overflowing), so that nothing of S's 24 bits is lost.
 template <class X>
 struct SumTerms;
@@ -62,245 +76,373 @@ __device__ __forceinline__ u32x4p sum_factors(uint32_t zero, bool mine) {
   return u32x4p{a1 | b1 << 16, b1 | a2 << 16, b2 | b2 << 16, 0u};
 }
 
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
+template <class X, int SPAN>
+__global__ void __launch_bounds__(256) int4_prepare_kernel(const Int4Args A, int64_t t0, int rows) {
+  const int c = threadIdx.x & 15, K = (int)A.K, t = (int)blockIdx.x * 16 + (threadIdx.x >> 4), stage = blockIdx.y, k = stage * STAGE + 8 * c;
+  if (t >= rows) return;  // (whole groups of 16 lanes)
+  const int64_t st = (int64_t)stage * rows + t;
+  u32x4p v = {0, 0, 0, 0};
+  if (k < K) v = *(const u32x4p*)((const uint16_t*)A.x + (t0 + t) * A.xs + k);
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum += X::lo(v[e]) + X::hi(v[e]);
+  sum = span_sum<SPAN>(sum);
+  char* const ws = (char*)A.ws;
+  *(u32x4p*)(ws + st * (STAGE * 2) + 16 * (c ^ (t & 15))) = int4_order(v);
+  constexpr int CS = SPAN / 8;
+  if (c % CS == 0)
+    *(u32x4p*)(ws + tile_x_bytes(A.steps, rows) + ((int64_t)(stage * (STAGE / SPAN) + c / CS) * rows + t) * 16) = sum_terms<X>(sum);
+}
+
+constexpr int WAVES = 8, BN = 32 * WAVES;  // wavefronts of a workgroup, each with 32 rows of the weight
+
+// Rings in LDS: stages of x and its sums, DX of them, which all wavefronts read; stages of a wavefront's weight, scales and zero
+// points, DW of them, which have further to come.
+template <int MT, int SPAN>
+struct TileCfg {
+  static constexpr int BM = 32 * MT, SPANS = STAGE / SPAN;
+  static constexpr int XB = BM * STAGE * 2;                          // bytes of a stage's x
+  static constexpr int XS = XB + (BM * SPANS * 16 + 1023) / 1024 * 1024;  // and of the terms of its sums
+  static constexpr int SW = SPANS, SL = SPANS > 2 ? 2 : 1;           // words a row of scales, loads of them
+  static constexpr int ZW = SPANS > 1 ? 2 : 1;                       // words a row of zero points
+  static constexpr int S0 = 2048, Z0 = S0 + SL * 256, WS = Z0 + 256;  // of a wavefront's stage
+  static constexpr int DX = MT == 1 ? 3 : 2;
+  static constexpr int ROOM = 160 * 1024 - 1536 - DX * XS;
+  static constexpr int DW = ROOM / (WAVES * WS) < 6 ? ROOM / (WAVES * WS) : 6;
+  static constexpr int YP = BN + 4, YB = 32 * YP * 4;                // 32 rows of the result: pitch, bytes
+  static constexpr int DUMP = DX * XS + WAVES * DW * WS;             // a place for loads that are made for their number alone
+  static constexpr int LDS = DUMP + 1024;
+  static_assert(DW > DX && LDS >= YB);
+};
+
+typedef __attribute__((address_space(3))) void tile_lds;
+
+template <int N>
+__device__ __forceinline__ void tile_wait() {  // until N loads or fewer are on their way, and all LDS accesses are done
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
   asm volatile("" ::: "memory");
 }
 
-template <class X, int MT, int NW, int SPAN, int OCC>
-__global__ void __launch_bounds__(256, OCC) int4_tile_kernel(const Int4Args A) {
+// parts > 1: partial sums as f32 rows, [part][row][N], behind the prepared x.
+// MANY: several spans a group.
+template <class X, int MT, int SPAN, bool MANY>
+__global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args A, int64_t t_base, int x_rows) {
   typedef TileCfg<MT, SPAN> C;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int last;
-  constexpr int BN = 128 * NW, SPANS = C::SPANS, FR = SPAN / 16, CH = C::BM * 16 / 256;
+  constexpr int SPANS = C::SPANS, FR = SPAN / 16, CH = C::BM * 16 / (64 * WAVES);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tiles_n = (int)((A.N + BN - 1) / BN), tiles_t = (int)((A.T + C::BM - 1) / C::BM);
+  const int tiles_t = (x_rows + C::BM - 1) / C::BM;
   const int tile = blockIdx.x;
   const int tn = tile / tiles_t, tt = tile - tn * tiles_t, part = blockIdx.y;
-  const int64_t t0 = (int64_t)tt * C::BM, n0 = (int64_t)tn * BN;
+  const int t0 = tt * C::BM;  // (of the prepared rows)
+  const int64_t n0 = (int64_t)tn * BN;
   const int K = (int)A.K;
   int lo, hi;
   int4_range(A, part, lo, hi);
 
+  // A wavefront's own rows of the weight: four lanes load a row's 64 bytes of a stage, chunk c of 16 bytes of row r to position
+  // c ^ (r / 4 mod 4), so that eight rows' reads take different banks. Scales and zero points come in whole words (the last of
+  // an odd number of 16-bit scales lies in one with two bytes that belong to no one, as the last zero points may). Loads never
+  // leave the buffers: chunks past a row's end are read from its beginning (x is 0 there), rows past the last are read as it
+  // and not stored, and words past the last as that.
+  const int es = A.scale_dtype == DT_F32 ? 4 : 2, most = (int)min(A.N - 1 - n0, (int64_t)(BN - 1));
+  const int64_t first = n0 * A.groups, rest = (A.N - n0) * A.groups;
+  const uint32_t s_off = (uint32_t)(first * es & 3), z_off = (uint32_t)(first & 3);
+  const uint32_t s_bytes = (uint32_t)min(rest * es + s_off + 3, (int64_t)0x7ffffffc) & ~3u;
+  const uint32_t z_bytes = (uint32_t)min(rest + z_off + 3, (int64_t)0x7ffffffc) & ~3u;
   const __amdgpu_buffer_rsrc_t wb = int4_buffer(A.w + n0 * (K / 2), (A.N - n0) * (K / 2));
-  const __amdgpu_buffer_rsrc_t xb = int4_buffer((const uint16_t*)A.x + t0 * A.xs, (A.T - t0) * A.xs * 2);
-  const Int4Groups groups(A, n0);
-  uint32_t w[NW], row[NW];
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    const int r = (int)min((int64_t)(wave * (32 * NW) + 32 * i + l32), A.N - 1 - n0);  // (rows past the last are computed and not stored)
-    w[i] = (uint32_t)r * (uint32_t)(K / 2) + 16 * half;
-    row[i] = (uint32_t)r * (uint32_t)A.groups;
-  }
-  // chunk j of this thread: row 16 j + tid / 16 of the tile, values 8 · (tid % 16) on
-  const int xr = tid >> 4, xc = tid & 15;
-  uint32_t x[CH];
-#pragma unroll
-  for (int j = 0; j < CH; ++j)
-    x[j] = t0 + 16 * j + xr < A.T ? (uint32_t)((16 * j + xr) * (int)A.xs + 8 * xc) * 2 : kOutside;
-
-  u32x4p xs[CH], q[NW][2];
-  Int4Scales<SPAN, SPANS> sc[NW];
-  auto load_x = [&](int stage) {
-    const int k = stage * STAGE;
-    if (k + STAGE <= K) {
-#pragma unroll
-      for (int j = 0; j < CH; ++j) xs[j] = int4_load<0>(xb, x[j], 2 * k);
-    } else {
-      // (the row ends within the stage)
-#pragma unroll
-      for (int j = 0; j < CH; ++j) xs[j] = int4_load<0>(xb, k + 8 * xc < K && x[j] != kOutside ? x[j] + (uint32_t)(2 * k) : kOutside, 0);
-    }
+  const __amdgpu_buffer_rsrc_t sb = int4_buffer((const char*)A.scale + (first * es & ~(int64_t)3), s_bytes);
+  const __amdgpu_buffer_rsrc_t zb = A.zero ? int4_buffer(A.zero + (first & ~(int64_t)3), z_bytes) : sb;
+  const int r0 = 32 * wave, wc = (lane & 3) ^ (lane >> 4);
+  // (kept as they are: the compiler would compute them again in every stage)
+  auto keep = [](uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
   };
-  auto load_w = [&](int stage) {
-    const int k = stage * STAGE;
-    const bool whole = k + STAGE <= K;
+  const uint32_t w0 = keep((uint32_t)min(r0 + (lane >> 2), most) * (uint32_t)(K / 2) + 16 * wc);
+  const uint32_t w1 = keep((uint32_t)min(r0 + 16 + (lane >> 2), most) * (uint32_t)(K / 2) + 16 * wc);
+  uint32_t s_row[C::SL];
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
+  for (int h = 0; h < C::SL; ++h)
+    s_row[h] = keep(s_off + (uint32_t)(min(r0 + min((64 * h + lane) / C::SW, 31), most) * A.groups) * es + 4 * ((64 * h + lane) % C::SW));
+  const uint32_t z_row = keep(z_off + (uint32_t)(min(r0 + min(lane / C::ZW, 31), most) * A.groups) + 4 * (lane % C::ZW));
+  const uint32_t own = keep((uint32_t)(first & 3) + (uint32_t)(min(r0 + l32, most) * A.groups));  // groups before this lane's row, from a whole word on
+  char* const w_ring = smem + C::DX * C::XS + wave * (C::DW * C::WS);
+  if (!A.zero) {
+    // (the zero points that the loads below leave alone)
+#pragma unroll
+    for (int d = 0; d < C::DW; ++d) ((uint32_t*)(w_ring + d * C::WS + C::Z0))[lane] = 0x08080808u;
+  }
+  // x and the terms of its sums, as they lie in the workspace
+  const char* const xp = (const char*)A.ws;
+  const char* const tp = xp + tile_x_bytes(A.steps, x_rows);
+  const __amdgpu_buffer_rsrc_t xb = int4_buffer(xp, tile_x_bytes(A.steps, x_rows));
+  const __amdgpu_buffer_rsrc_t tb = int4_buffer(tp, tile_ws_bytes(A.steps, x_rows, SPAN) - tile_x_bytes(A.steps, x_rows));
+  const uint32_t x_at = keep((uint32_t)t0 * (STAGE * 2) + tid * 16);
+  // (64 rows of a span and wavefront; wavefronts that none is left for load the first again, and let it be)
+  const uint32_t t_to = 64 * wave < C::BM * SPANS ? C::XB + wave * 1024 : (uint32_t)C::DUMP;
+  const int ti = 64 * wave < C::BM * SPANS ? min(tid, C::BM * SPANS - 1) : 0;
+  const uint32_t t_at = keep((uint32_t)(ti / C::BM * x_rows + t0 + ti % C::BM) * 16);
+
+  auto group_of = [&](int span) { return min(MANY ? (int)((uint32_t)span / (uint32_t)A.group_spans) : span, A.groups - 1); };
+  auto load_x = [&](int stage, int slot) {
+    char* const to = smem + slot * C::XS;
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (tile_lds*)(to + j * (1024 * WAVES) + wave * 1024), 16, (int)x_at,
+                                               stage * x_rows * (STAGE * 2) + j * (1024 * WAVES), 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(tb, (tile_lds*)((t_to == C::DUMP ? smem : to) + t_to), 16, (int)t_at, stage * x_rows * (SPANS * 16), 0, 0);
+  };
+  const int z_to = A.zero ? C::Z0 : C::DUMP;
+  auto load_w = [&](int stage, int slot) {
+    const int k = stage * STAGE;
+    char* const to = w_ring + slot * C::WS;
+    if (k + STAGE <= K) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (tile_lds*)to, 16, (int)w0, k / 2, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (tile_lds*)(to + 1024), 16, (int)w1, k / 2, 0, 0);
+    } else {
+      const uint32_t off = k + 32 * wc < K ? (uint32_t)(k / 2) : (uint32_t)(-16 * wc);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (tile_lds*)to, 16, (int)(w0 + off), 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, (tile_lds*)(to + 1024), 16, (int)(w1 + off), 0, 0, 0);
+    }
+    const uint32_t g = (uint32_t)group_of(stage * SPANS);
+#pragma unroll
+    for (int h = 0; h < C::SL; ++h)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (tile_lds*)(to + C::S0 + h * 256), 4, (int)min((s_row[h] + g * es) & ~3u, s_bytes - 4), 0, 0, 0);
+    // (without zero points, some of the scales, for the number of loads)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(zb, (tile_lds*)((A.zero ? to : smem) + z_to), 4, (int)min((z_row + g) & ~3u, (A.zero ? z_bytes : s_bytes) - 4), 0, 0, 0);
+  };
+  // Waits for a stage's loads, by how many were made after them. In the first stage those of DW - 2 weights; later those of DX - 2
+  // stages and of one weight more, for x, whose weight's loads are older. Where there are no more weights to load, for all.
+  auto arrived = [&](int stage) {
+    constexpr int NW = 3 + C::SL, NX = CH + 1;
+    if (stage + C::DW - 2 >= hi) tile_wait<0>();
+    else if (stage == lo) tile_wait<(C::DW - 2) * NW>();
+    else tile_wait<(C::DX - 2) * (NX + NW) + NW>();
+  };
+  // where a lane's first block of a stage lies: row l32, chunk `half` (and by exclusive or with 32 bytes the next, and so on)
+  uint32_t chunk = l32 * (STAGE * 2) + 16 * (half ^ (l32 & 15));
+  const uint32_t w_lane = keep(l32 * 64 + 16 * (half ^ (l32 >> 2 & 3))), sums_at = keep(C::XB + l32 * 16);
+  const uint32_t s_lane = keep(C::S0 + l32 * (4 * C::SW)), z_lane = keep(C::Z0 + (A.zero ? l32 * (4 * C::ZW) : 0));
+  const uint32_t s_step = es == 4 ? 0 : 2, z_step = A.zero ? 3 : 0, s_up = es == 4 ? 0 : 16;
+  const Int4Operand<X> operand;
+
+  f32x16p y[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) y[m] = f32x16p{};
+
+  {
+    int xi = 0, wi = 0, xo = C::DX - 1, wo = C::DW - 1;  // slots of this stage, and of those that are loaded in it
+    for (int d = 0; d < C::DX - 1 && lo + d < hi; ++d) load_x(lo + d, d);
+    for (int d = 0; d < C::DW - 1 && lo + d < hi; ++d) load_w(lo + d, d);
+    for (int stage = lo; stage < hi; ++stage) {
+      arrived(stage);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (stage + C::DX - 1 < hi) load_x(stage + C::DX - 1, xo);
+      if (stage + C::DW - 1 < hi) load_w(stage + C::DW - 1, wo);
+      const char* const from = smem + xi * C::XS;
+      const char* const wf_at = w_ring + wi * C::WS;
+      if (++xi == C::DX) xi = 0;
+      if (++wi == C::DW) wi = 0;
+      if (++xo == C::DX) xo = 0;
+      if (++wo == C::DW) wo = 0;
+      // the words that the matrix instructions take: of block f of 16 values, one for each half-wave
+      uint32_t word[8];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (whole) q[i][j] = int4_load<0>(wb, w[i], k / 2 + 32 * j);
-        else q[i][j] = int4_load<0>(wb, k + 64 * j + 32 * half < K ? w[i] + (uint32_t)(k / 2 + 32 * j) : kOutside, 0);
+        const u32x4p v = *(const u32x4p*)(wf_at + (w_lane ^ (32 * j)));
+        const auto a = __builtin_amdgcn_permlane32_swap(v[0], v[1], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(v[2], v[3], false, false);
+        word[4 * j] = a[0], word[4 * j + 1] = b[0], word[4 * j + 2] = a[1], word[4 * j + 3] = b[1];
       }
-      sc[i].load(A, groups, row[i], k);
-    }
-  };
-  auto store_x = [&](int buffer) {
-    char* const to = smem + buffer * C::LDS1;
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const int r = 16 * j + xr;
-      float v = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v += X::lo(xs[j][e]) + X::hi(xs[j][e]);
-      v = span_sum<SPAN>(v);
-      *(u32x4p*)(to + r * (STAGE * 2) + 16 * (xc ^ (r & 15))) = int4_order(xs[j]);
-      if (xc % (SPAN / 8) == 0) *(u32x4p*)(to + C::XB + (xc / (SPAN / 8) * C::BM + r) * 16) = sum_terms<X>(v);
-    }
-  };
-
-  // where a lane's block f of a stage's first span lies: row l32, chunk 2 f + half (and 32 FR bytes on, by exclusive or, the next)
-  uint32_t chunk[FR];
-#pragma unroll
-  for (int f = 0; f < FR; ++f) chunk[f] = l32 * (STAGE * 2) + 16 * ((2 * f + half) ^ (l32 & 15));
-
-  f32x16p y[MT][NW];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int i = 0; i < NW; ++i) y[m][i] = f32x16p{};
-
-  if (lo < hi) {
-    load_x(lo);
-    load_w(lo);
-    store_x(0);
-    lds_barrier();
-    for (int stage = lo; stage < hi; ++stage) {
-      const char* const from = smem + ((stage - lo) & 1) * C::LDS1;
-      // the words that the matrix instructions take: block f of 16 values, words exchanged between the half-waves
-      uint32_t word[NW][8];
-      Int4Scales<SPAN, SPANS> now[NW];
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const auto a = __builtin_amdgcn_permlane32_swap(q[i][j][0], q[i][j][1], false, false);
-          const auto b = __builtin_amdgcn_permlane32_swap(q[i][j][2], q[i][j][3], false, false);
-          word[i][4 * j] = a[0], word[i][4 * j + 1] = b[0], word[i][4 * j + 2] = a[1], word[i][4 * j + 3] = b[1];
-        }
-        now[i] = sc[i];
-      }
-      if (stage + 1 < hi) {
-        load_x(stage + 1);
-        load_w(stage + 1);
-      }
+      const int g0 = group_of(stage * SPANS);
       // (a loop: the compiler would put off the sums of one span behind the products of the next, past the registers)
 #pragma unroll 1
       for (int p = 0; p < SPANS; ++p) {
-        u32x4p wf[NW][FR], zf[NW];
-        float scale[NW];
+        // (of the words that there are; past the row's end x is 0: its last group's)
+        const int g = group_of(stage * SPANS + p) - g0;
+        const uint32_t s_byte = es == 4 ? 4 * g : ((own + g0) << 1 & s_step) + 2 * g, z_byte = A.zero ? ((own + g0) & z_step) + g : 0;
+        uint32_t s_word = *(const uint32_t*)(wf_at + s_lane + (s_byte & ~3u));
+        s_word >>= s_byte << 3 & s_up;
+        const float scale = es == 4 ? __uint_as_float(s_word) : X::lo(s_word & 0xffffu);
+        const u32x4p zf = sum_factors<X>(*(const uint8_t*)(wf_at + z_lane + z_byte), half == 0);
+        u32x4p wf[FR];
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
-          zf[i] = sum_factors<X>(now[i].z[0], half == 0);
-          scale[i] = now[i].template scale<X>(A, 0);
+        for (int f = 0; f < FR; ++f) wf[f] = operand(word[f]);
 #pragma unroll
-          for (int f = 0; f < FR; ++f) wf[i][f] = int4_operand<X>(word[i][f]);
+        for (int f = 0; f + FR < 8; ++f) word[f] = word[f + FR];  // (the next span's come first)
+        asm volatile("" : "+v"(chunk));  // (or all its neighbours would be kept in registers over the stages)
+        const char* const sums = from + sums_at + p * (C::BM * 16);
+        // Fragments of x are read AHEAD matrix instructions before they are multiplied, and 32 rows' sums are scaled while the
+        // next 32 rows' products run: the order is forced, since the compiler's own reads each one, waits and multiplies.
+        constexpr int F1 = FR + 1, ALL = MT * F1;
+        u32x4p ring[AHEAD + 1];
+        f32x16p acc[2];
+        auto read = [&](int at) {
+          const int m = at / F1, f = at % F1;
+          if (f == 0) return *(const u32x4p*)(sums + 32 * m * 16);
+          return *(const u32x4p*)(from + (chunk ^ (32 * (p * FR + f - 1))) + 32 * m * (STAGE * 2));
+        };
 #pragma unroll
-          for (int f = 0; f + FR < 8; ++f) word[i][f] = word[i][f + FR];  // (the next span's come first)
-#pragma unroll
-          for (int j = 0; j + 1 < SPANS; ++j) now[i].s[j] = now[i].s[j + 1], now[i].z[j] = now[i].z[j + 1];
-        }
-        const char* const sums = from + C::XB + (p * C::BM + l32) * 16;
+        for (int at = 0; at < AHEAD && at < ALL; ++at) ring[at] = read(at);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          f32x16p acc[NW];
-          const u32x4p sf = *(const u32x4p*)(sums + 32 * m * 16);
 #pragma unroll
-          for (int i = 0; i < NW; ++i) acc[i] = X::mma32(sf, zf[i], f32x16p{});
+          for (int f = 0; f < F1; ++f) {
+            const int at = m * F1 + f;
+            if (at + AHEAD < ALL) ring[(at + AHEAD) % (AHEAD + 1)] = read(at + AHEAD);
+            const u32x4p x = ring[at % (AHEAD + 1)];
+            acc[m & 1] = f == 0 ? X::mma32(x, zf, f32x16p{}) : X::mma32(x, wf[f > 0 ? f - 1 : 0], acc[m & 1]);
+          }
+          if (m > 0) {
 #pragma unroll
-          for (int f = 0; f < FR; ++f) {
-            const u32x4p xf = *(const u32x4p*)(from + (chunk[f] ^ (p * (32 * FR))) + 32 * m * (STAGE * 2));
-#pragma unroll
-            for (int i = 0; i < NW; ++i) acc[i] = X::mma32(xf, wf[i][f], acc[i]);
+            for (int e = 0; e < 16; ++e) y[m - 1][e] = __builtin_fmaf(scale, acc[(m - 1) & 1][e], y[m - 1][e]);
+            asm volatile("" : "+v"(y[m - 1]));  // (or they would be put off past all products)
           }
 #pragma unroll
-          for (int i = 0; i < NW; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[m][i][e] = __builtin_fmaf(scale[i], acc[i][e], y[m][i][e]);
+          for (int f = 0; f < F1; ++f) {
+            if (m * F1 + f + AHEAD < ALL) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (m > 0) __builtin_amdgcn_sched_group_barrier(0x002, (16 + F1 - 1) / F1, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-      }
-      if (stage + 1 < hi) {
-        store_x((stage + 1 - lo) & 1);
-        lds_barrier();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[MT - 1][e] = __builtin_fmaf(scale, acc[(MT - 1) & 1][e], y[MT - 1][e]);
       }
     }
   }
-  if (A.parts > 1) {
-    // (partial sums as they lie in the registers: 16 bytes a lane)
-    constexpr int PART = MT * NW * 4096;  // floats of a workgroup's tile
-    const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc((void*)(A.ws + (int64_t)tile * A.parts * PART), (short)0, -1, 0x00020000);
-    auto at = [&](int u, int m, int i, int e) { return (uint32_t)((u * (MT * NW * 4) + (m * NW + i) * 4 + e) * 256 + tid) * 16; };
+  // The tile's rows, 32 at a time, through LDS: a thread stores 16 bytes of a row together where rows begin at such places.
+  const bool whole = A.parts == 1;
+  const int ys = whole && A.y_dtype != DT_F32 ? 2 : 4, per = 16 / ys;
+  const bool wide = A.N % per == 0;
+  const int n_here = (int)min((int64_t)BN, A.N - n0);
+  char* const out = whole ? (char*)A.y + (t_base + t0) * A.N * ys
+                          : (char*)A.ws + tile_ws_bytes(A.steps, x_rows, SPAN) + ((int64_t)part * x_rows + t0) * A.N * 4;
+  float* const rows_at = (float*)smem;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m) {
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NW; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) agent_put4(ws, at(part, m, i, e), f32x4p{y[m][i][4 * e], y[m][i][4 * e + 1], y[m][i][4 * e + 2], y[m][i][4 * e + 3]});
-    if (!last_to_arrive(A.counters + tile, A.parts, &last)) return;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < NW; ++i) y[m][i] = f32x16p{};
-    for (int u = 0; u < A.parts; ++u) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < NW; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const f32x4p v = agent_get4(ws, at(u, m, i, e));
-#pragma unroll
-            for (int f = 0; f < 4; ++f) y[m][i][4 * e + f] += v[f];
-          }
-    }
-  }
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int64_t n = n0 + wave * (32 * NW) + 32 * i + l32;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t t = t0 + 32 * m + 8 * (e >> 2) + 4 * half + (e & 3);
-        if (n < A.N && t < A.T) {
-          if (A.y_dtype == DT_F32) ((float*)A.y)[t * A.N + n] = y[m][i][e];
-          else ((uint16_t*)A.y)[t * A.N + n] = X::put(y[m][i][e]);
+    for (int e = 0; e < 16; ++e) rows_at[(8 * (e >> 2) + 4 * half + (e & 3)) * C::YP + 32 * wave + l32] = y[m][e];
+    __syncthreads();
+    const int t_here = min(32, x_rows - t0 - 32 * m);
+    char* const to = out + ((int64_t)32 * m * A.N + n0) * ys;
+    if (wide) {
+      const int chunks = BN / per;
+      for (int i = tid; i < 32 * chunks; i += 64 * WAVES) {
+        const int r = i / chunks, c = (i - r * chunks) * per;
+        if (r >= t_here || c >= n_here) continue;
+        const f32x4p a = *(const f32x4p*)(rows_at + r * C::YP + c);
+        char* const at = to + ((int64_t)r * A.N + c) * ys;
+        if (ys == 4) {
+          *(f32x4p*)at = a;
+        } else {
+          const f32x4p b = *(const f32x4p*)(rows_at + r * C::YP + c + 4);
+          *(u32x4p*)at = u32x4p{X::put(a[0]) | (uint32_t)X::put(a[1]) << 16, X::put(a[2]) | (uint32_t)X::put(a[3]) << 16,
+                                X::put(b[0]) | (uint32_t)X::put(b[1]) << 16, X::put(b[2]) | (uint32_t)X::put(b[3]) << 16};
         }
       }
+    } else {
+      for (int i = tid; i < 32 * BN; i += 64 * WAVES) {
+        const int r = i / BN, c = i % BN;
+        if (r >= t_here || c >= n_here) continue;
+        const float v = rows_at[r * C::YP + c];
+        char* const at = to + ((int64_t)r * A.N + c) * ys;
+        if (ys == 4) *(float*)at = v;
+        else *(uint16_t*)at = X::put(v);
+      }
     }
+  }
 }
 
-template <class X, int MT, int NW, int OCC>
+// Adds the parts of `count` elements, in their order, from `parts` (of the workspace) into y from element `at` on.
+template <class X>
+__global__ void __launch_bounds__(256) int4_join_kernel(const Int4Args A, const float* parts, int64_t at, int64_t count) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= count) return;
+  const bool wide = count % 4 == 0 && at % 4 == 0;  // (every part begins at 16 bytes, and every four elements of y at theirs)
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const int n = (int)min((int64_t)4, count - i);
+  if (wide) {
+#pragma unroll 8
+    for (int p = 0; p < A.parts; ++p) {
+      const f32x4p u = *(const f32x4p*)(parts + p * count + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += u[e];
+    }
+  } else {
+    for (int p = 0; p < A.parts; ++p)
+      for (int e = 0; e < n; ++e) v[e] += parts[p * count + i + e];
+  }
+  for (int e = 0; e < n; ++e) {
+    if (A.y_dtype == DT_F32) ((float*)A.y)[at + i + e] = v[e];
+    else ((uint16_t*)A.y)[at + i + e] = X::put(v[e]);
+  }
+}
+
+// Rows of x that are prepared and multiplied at a time: as many as a workspace of 24 MiB holds (allocation-free executions have
+// 64 MiB for all steps), at least a tile.
+int64_t rows_at_a_time(const Int4Args& a) {
+  const int64_t row = (int64_t)a.steps * (STAGE * 2 + STAGE / a.span * 16), most = std::max<int64_t>(1, (24ll << 20) / (row * 128)) * 128;
+  return std::min(a.T, most);
+}
+
+template <class X, int MT, int SPAN>
+void launch_tile_span(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
+  typedef TileCfg<MT, SPAN> C;
+  const auto kernel = a.group_spans > 1 ? int4_tile_kernel<X, MT, SPAN, true> : int4_tile_kernel<X, MT, SPAN, false>;
+  const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+  if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("int4_matmul LDS attribute: ") + hipGetErrorString(e));
+  const int64_t each = rows_at_a_time(a);
+  for (int64_t t0 = 0; t0 < a.T; t0 += each) {
+    const int rows = (int)std::min(each, a.T - t0);
+    hipEvent_t const end = t0 + each >= a.T ? done : nullptr;
+    launch_k(nullptr, int4_prepare_kernel<X, SPAN>, dim3((unsigned)((rows + 15) / 16), (unsigned)a.steps), dim3(256), 0, stream, a, t0, rows);
+    const int64_t tiles = ((int64_t)(rows + C::BM - 1) / C::BM) * ((a.N + BN - 1) / BN);
+    launch_k(a.parts > 1 ? nullptr : end, kernel, dim3((unsigned)tiles, (unsigned)a.parts), dim3(64 * WAVES), C::LDS, stream, a, t0, rows);
+    if (a.parts == 1) continue;
+    const int64_t count = rows * a.N;
+    launch_k(end, int4_join_kernel<X>, dim3((unsigned)((count + 1023) / 1024)), dim3(256), 0, stream, a,
+             (const float*)((char*)a.ws + tile_ws_bytes(a.steps, rows, SPAN)), t0 * a.N, count);
+  }
+}
+template <class X, int MT>
 void launch_tile(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
-  const int64_t tiles = ((a.T + 32 * MT - 1) / (32 * MT)) * ((a.N + 128 * NW - 1) / (128 * NW));
-  if (tiles > INT32_MAX) fail(PJRT_Error_Code_INTERNAL, "int4_matmul of too many tiles");
-  const dim3 grid((unsigned)tiles, (unsigned)a.parts), block(256);
-  auto go = [&](auto kernel, int lds) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("int4_matmul LDS attribute: ") + hipGetErrorString(e));
-    launch_k(done, kernel, grid, block, lds, stream, a);
-  };
-  if (a.span == 128) go(int4_tile_kernel<X, MT, NW, 128, OCC>, 2 * TileCfg<MT, 128>::LDS1);
-  else if (a.span == 64) go(int4_tile_kernel<X, MT, NW, 64, OCC>, 2 * TileCfg<MT, 64>::LDS1);
-  else go(int4_tile_kernel<X, MT, NW, 32, OCC>, 2 * TileCfg<MT, 32>::LDS1);
+  if (a.span == 128) launch_tile_span<X, MT, 128>(a, stream, done);
+  else if (a.span == 64) launch_tile_span<X, MT, 64>(a, stream, done);
+  else launch_tile_span<X, MT, 32>(a, stream, done);
 }
 template <class X>
 void launch_type(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
-  if (a.tiles_t == 1) return launch_tile<X, 1, 1, 4>(a, stream, done);
-  if (a.tiles_t == 2) return launch_tile<X, 2, 1, 3>(a, stream, done);
-  launch_tile<X, 4, 2, 1>(a, stream, done);
+  if (a.tile == 1) launch_tile<X, 1>(a, stream, done);
+  else if (a.tile == 2) launch_tile<X, 2>(a, stream, done);
+  else launch_tile<X, 4>(a, stream, done);
 }
 
 }  // namespace
 
-void int4_tile_plan(Int4Args& a, int64_t* ws_floats, int64_t* counters) {
-  a.kernel = INT4_TILE;
-  a.tiles_t = a.T <= 32 ? 1 : a.T <= 64 ? 2 : 4;
-  a.tiles_n = a.tiles_t == 4 ? 2 : 1;
-  const int64_t bm = 32 * a.tiles_t, bn = 128 * a.tiles_n;
-  const int64_t tiles = ((a.T + bm - 1) / bm) * ((a.N + bn - 1) / bn), stages = (a.K + STAGE - 1) / STAGE;
-  if (tiles > INT32_MAX) { a.kernel = INT4_ANY; return; }
+void int4_tile_plan(Int4Args& a, int64_t* ws_floats) {
+  const int64_t stages = (a.K + STAGE - 1) / STAGE;
   a.steps = (int32_t)stages;
-  a.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, stages / 4));
-  if (a.parts > 1) {
-    *ws_floats = tiles * a.parts * (bm * bn);
-    *counters = tiles;
-  }
+  // Taller tiles turn the weight into operands less often: 2048 rows against 12288 x 4096, bf16: 237 us with 128 rows a tile, 299
+  // with 64, 415 with 32; 128 rows against 12288 x 4096: 24, 28 and 36; 64 rows against 28672 x 4096: 40, 29 and 37; 16 rows
+  // against the same: 40, 28 and 23.
+  a.tile = a.T <= 32 ? 1 : a.T <= 64 ? 2 : 4;
+  const int64_t rows = rows_at_a_time(a), bm = 32 * a.tile;
+  const int64_t tiles = ((rows + bm - 1) / bm) * ((a.N + BN - 1) / BN);
+  if (tiles > INT32_MAX || stages > 65535 || rows * a.N / 1024 >= INT32_MAX) return;
+  a.kernel = INT4_TILE;
+  a.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(CUS / tiles, stages / LEAST));
+  *ws_floats = tile_ws_bytes(stages, rows, a.span) / 4 + (a.parts > 1 ? a.parts * rows * a.N : 0);
 }
 
 void launch_int4_tile(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
+  if (!a.ws) fail(PJRT_Error_Code_INTERNAL, "int4_matmul without a workspace");
   if (a.x_dtype == DT_BF16) launch_type<Int4BF16>(a, stream, done);
   else launch_type<Int4F16>(a, stream, done);
 }

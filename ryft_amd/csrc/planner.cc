@@ -1015,10 +1015,9 @@ void Planner::emit_custom_call(int node, int target) {
     read(offsetof(Int4Args, scale), 2);
     if (n.operands.size() == 4) read(offsetof(Int4Args, zero), 3);
     st.patches.push_back({offsetof(Int4Args, y), out_slot(0)});
-    int64_t ws = 0, counters = 0;
-    int4_matmul_plan(a, &ws, &counters);
+    int64_t ws = 0;
+    int4_matmul_plan(a, &ws);
     if (ws) st.patches.push_back({offsetof(Int4Args, ws), shared_workspace(4 * ws)});
-    if (counters) st.patches.push_back({offsetof(Int4Args, counters), shared_counters(counters)});
     st.bytes = (double)(x.bytes() + w.bytes() + s.bytes() + y.bytes()) + (n.operands.size() == 4 ? (double)type(3).bytes() : 0.0);
     st.flops = 2.0 * (double)a.T * (double)a.N * (double)a.K;
   } else if (n.call_target == "ryft.tree_accept") {
@@ -2730,7 +2729,7 @@ std::string Plan::describe() const {
       os << " M=" << s.int4.T << " N=" << s.int4.N << " K=" << s.int4.K << " group=" << s.int4.G << " x="
          << dtype_name((DType)s.int4.x_dtype) << " out=" << dtype_name((DType)s.int4.y_dtype);
       if (s.int4.kernel == INT4_FEW) os << " few";
-      else if (s.int4.kernel == INT4_TILE) os << " tile=" << 32 * s.int4.tiles_t << "x" << 128 * s.int4.tiles_n;
+      else if (s.int4.kernel == INT4_TILE) os << " tile=" << 32 * s.int4.tile;
       if (s.int4.parts > 1) os << " parts=" << s.int4.parts;
     } else if (s.kind == Step::TREE_ACCEPT) {
       os << " tokens=" << s.accept.T << " sequences=" << s.accept.B << " caches=" << s.accept.n_caches;
