@@ -174,6 +174,56 @@ def test_int4_matmul_keeps_infinities_in_their_rows(gpu_client, rows, inner):
     close(got[clean], want[clean], "bf16", vp.int4_error([x[0][clean], *x[1:]]), "others")
 
 
+# more tiles of the weight than workgroups, steps of x in registers or not, and rows that are prepared in two goes
+MORE_SIZES = [
+    (1, 1024, 8201, 64), (2, 4096, 8230, 128), (3, 2048, 4300, 32), (4, 1152, 4500, 96), (5, 2304, 4200, 768), (9, 8192, 4111, 64),
+    (16, 4000, 4128, 32), (16, 4096, 8300, 128), (7, 5152, 4333, 32), (13, 8224, 4111, 32), (8, 160, 12321, 32), (300, 32768, 70, 128),
+    (270, 30752, 33, 32), (40, 20480, 300, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True], ids=["eight", "zeros"])
+@pytest.mark.parametrize("size", MORE_SIZES, ids=str)
+def test_int4_matmul_of_more_tiles(gpu_client, size, zeros, dtype):
+    module, ins = vp.int4_case(*size, dtype, zeros=zeros, out_dtype="f32", exact=True, seed=sum(size) + zeros)
+    (got,), _ = run(gpu_client, module, ins, ["f32"])
+    assert np.array_equal(got, oo.int4_matmul(vp.values(ins), {})[0])
+
+
+@pytest.mark.parametrize("dtype, factor", [("bf16", 2.0 ** 100), ("bf16", 2.0 ** -100), ("f16", 2.0 ** 14), ("f16", 2.0 ** -24)])
+@pytest.mark.parametrize("size", [(1, 4096, 300, 128), (16, 2304, 4200, 64), (3, 2048, 4300, 32), (40, 512, 300, 64), (300, 640, 129, 128)], ids=str)
+def test_int4_matmul_of_large_and_small_values(gpu_client, size, dtype, factor):
+    # whole numbers times a power of two: as exact as they are, f16's subnormal numbers among them
+    module, ins = vp.int4_case(*size, dtype, zeros=True, out_dtype="f32", exact=True, seed=sum(size))
+    ins[0] = op.host(vp.values(ins)[0] * factor, dtype)
+    (got,), _ = run(gpu_client, module, ins, ["f32"])
+    assert np.array_equal(got, oo.int4_matmul(vp.values(ins), {})[0])
+
+
+def test_int4_matmul_of_slices(gpu_client):
+    # rows of the weight, scales and zero points that begin anywhere within larger tensors, and a slice of x
+    r = np.random.RandomState(4)
+    x, w = r.randint(-3, 4, (9, 200)), r.randint(0, 256, (41, 80))
+    scale, zero = 2.0 ** r.randint(-2, 3, (41, 5)), r.randint(0, 16, (41, 5))
+    module = """
+module @slices {
+  func.func public @main(%x: tensor<9x200xf16>, %w: tensor<41x80xui8>, %s: tensor<41x5xf16>, %z: tensor<41x5xui8>) -> tensor<5x33xf32> {
+    %0 = stablehlo.slice %x [3:8, 7:167] : (tensor<9x200xf16>) -> tensor<5x160xf16>
+    %1 = stablehlo.slice %w [5:38, 0:80] : (tensor<41x80xui8>) -> tensor<33x80xui8>
+    %2 = stablehlo.slice %s [5:38, 0:5] : (tensor<41x5xf16>) -> tensor<33x5xf16>
+    %3 = stablehlo.slice %z [5:38, 0:5] : (tensor<41x5xui8>) -> tensor<33x5xui8>
+    %4 = stablehlo.custom_call @ryft.int4_matmul(%0, %1, %2, %3) {api_version = 4 : i32, backend_config = {}} : (tensor<5x160xf16>, tensor<33x80xui8>, tensor<33x5xf16>, tensor<33x5xui8>) -> tensor<5x33xf32>
+    return %4 : tensor<5x33xf32>
+  }
+}
+"""
+    ins = [op.host(x, "f16"), vp.host(w, "ui8"), op.host(scale, "f16"), vp.host(zero, "ui8")]
+    (got,), _ = run(gpu_client, module, ins, ["f32"])
+    want, = oo.int4_matmul([x[3:8, 7:167].astype(float), w[5:38], scale[5:38], zero[5:38]], {})
+    assert np.array_equal(got, want)
+
+
 def test_int4_matmul_of_no_rows(gpu_client):
     module, ins = vp.int4_case(0, 64, 10, 32, "bf16")
     (got,), _ = run(gpu_client, module, ins, ["bf16"])
