@@ -448,6 +448,7 @@ struct Int4Args {
   int32_t span;         // values whose scale is one, at a time: 32, 64 or 128
   int32_t tile;         // rows of x a tile, of 32 (INT4_TILE)
   int32_t x_steps;      // steps of x that a wavefront keeps in registers (INT4_FEW)
+  int32_t rows;         // rows of x that are prepared and multiplied at a time (INT4_TILE)
   int32_t parts;        // ranges of K of an output tile
   int32_t groups;       // K / G
   int32_t group_spans;  // G / span

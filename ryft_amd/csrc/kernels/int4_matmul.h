@@ -85,7 +85,7 @@ __device__ __forceinline__ void int4_range(const Int4Args& A, int part, int& lo,
 }
 
 // k_int4_tile.hip
-void int4_tile_plan(Int4Args& a, int64_t* ws_floats);
+void int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats);
 void launch_int4_tile(const Int4Args& a, hipStream_t stream, hipEvent_t done);
 
 }  // namespace ryft

@@ -461,7 +461,7 @@ void few_plan(Int4Args& a) {
 
 }  // namespace
 
-void int4_matmul_plan(Int4Args& a, int64_t* ws_floats) {
+void int4_matmul_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   *ws_floats = 0;
   a.kernel = INT4_ANY;
   a.parts = 1;
@@ -474,7 +474,7 @@ void int4_matmul_plan(Int4Args& a, int64_t* ws_floats) {
   // (16 rows, 4096 x 28672: 20.5 us, with tiles 30; 14336 x 4096: 16.7 and 24; 4096 x 4096: 7.2 and 15. From 17 rows on a
   // second pass over the weight would be needed.)
   if (a.T <= 16) return few_plan(a);
-  int4_tile_plan(a, ws_floats);
+  int4_tile_plan(a, room, ws_floats);
 }
 
 void launch_int4_matmul(const Int4Args& a, hipStream_t stream, hipEvent_t done) {

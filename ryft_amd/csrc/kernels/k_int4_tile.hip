@@ -387,20 +387,13 @@ __global__ void __launch_bounds__(256) int4_join_kernel(const Int4Args A, const 
   }
 }
 
-// Rows of x that are prepared and multiplied at a time: as many as a workspace of 24 MiB holds (allocation-free executions have
-// 64 MiB for all steps), at least a tile.
-int64_t rows_at_a_time(const Int4Args& a) {
-  const int64_t row = (int64_t)a.steps * (STAGE * 2 + STAGE / a.span * 16), most = std::max<int64_t>(1, (24ll << 20) / (row * 128)) * 128;
-  return std::min(a.T, most);
-}
-
 template <class X, int MT, int SPAN>
 void launch_tile_span(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
   typedef TileCfg<MT, SPAN> C;
   const auto kernel = a.group_spans > 1 ? int4_tile_kernel<X, MT, SPAN, true> : int4_tile_kernel<X, MT, SPAN, false>;
   const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
   if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("int4_matmul LDS attribute: ") + hipGetErrorString(e));
-  const int64_t each = rows_at_a_time(a);
+  const int64_t each = a.rows;
   for (int64_t t0 = 0; t0 < a.T; t0 += each) {
     const int rows = (int)std::min(each, a.T - t0);
     hipEvent_t const end = t0 + each >= a.T ? done : nullptr;
@@ -428,19 +421,23 @@ void launch_type(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
 
 }  // namespace
 
-void int4_tile_plan(Int4Args& a, int64_t* ws_floats) {
+void int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   const int64_t stages = (a.K + STAGE - 1) / STAGE;
   a.steps = (int32_t)stages;
   // Taller tiles turn the weight into operands less often: 2048 rows against 12288 x 4096, bf16: 237 us with 128 rows a tile, 299
   // with 64, 415 with 32; 128 rows against 12288 x 4096: 24, 28 and 36; 64 rows against 28672 x 4096: 40, 29 and 37; 16 rows
   // against the same: 40, 28 and 23.
   a.tile = a.T <= 32 ? 1 : a.T <= 64 ? 2 : 4;
-  const int64_t rows = rows_at_a_time(a), bm = 32 * a.tile;
+  // Rows at a time: as many as 24 MiB hold, a tile's at least.
+  const int64_t row = stages * (STAGE * 2 + STAGE / a.span * 16), x_most = std::min<int64_t>(24ll << 20, room);
+  const int64_t rows = std::min(a.T, std::max<int64_t>(1, x_most / (row * MOST_ROWS)) * MOST_ROWS), bm = 32 * a.tile;
   const int64_t tiles = ((rows + bm - 1) / bm) * ((a.N + BN - 1) / BN);
   if (tiles > INT32_MAX || stages > 65535 || rows * a.N / 1024 >= INT32_MAX) return;
   a.kernel = INT4_TILE;
-  a.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(CUS / tiles, stages / LEAST));
-  *ws_floats = tile_ws_bytes(stages, rows, a.span) / 4 + (a.parts > 1 ? a.parts * rows * a.N : 0);
+  a.rows = (int32_t)rows;
+  const int64_t x_bytes = tile_ws_bytes(stages, rows, a.span), part = rows * a.N * 4;
+  a.parts = (int32_t)std::max<int64_t>(1, std::min({CUS / tiles, stages / LEAST, (room - x_bytes) / part}));
+  *ws_floats = (x_bytes + (a.parts > 1 ? a.parts * part : 0)) / 4;
 }
 
 void launch_int4_tile(const Int4Args& a, hipStream_t stream, hipEvent_t done) {

@@ -1016,7 +1016,7 @@ void Planner::emit_custom_call(int node, int target) {
     if (n.operands.size() == 4) read(offsetof(Int4Args, zero), 3);
     st.patches.push_back({offsetof(Int4Args, y), out_slot(0)});
     int64_t ws = 0;
-    int4_matmul_plan(a, &ws);
+    int4_matmul_plan(a, opts_.int4_workspace, &ws);
     if (ws) st.patches.push_back({offsetof(Int4Args, ws), shared_workspace(4 * ws)});
     st.bytes = (double)(x.bytes() + w.bytes() + s.bytes() + y.bytes()) + (n.operands.size() == 4 ? (double)type(3).bytes() : 0.0);
     st.flops = 2.0 * (double)a.T * (double)a.N * (double)a.K;
@@ -2729,7 +2729,7 @@ std::string Plan::describe() const {
       os << " M=" << s.int4.T << " N=" << s.int4.N << " K=" << s.int4.K << " group=" << s.int4.G << " x="
          << dtype_name((DType)s.int4.x_dtype) << " out=" << dtype_name((DType)s.int4.y_dtype);
       if (s.int4.kernel == INT4_FEW) os << " few";
-      else if (s.int4.kernel == INT4_TILE) os << " tile=" << 32 * s.int4.tile;
+      else if (s.int4.kernel == INT4_TILE) os << " tile=" << 32 * s.int4.tile << " rows=" << s.int4.rows;
       if (s.int4.parts > 1) os << " parts=" << s.int4.parts;
     } else if (s.kind == Step::TREE_ACCEPT) {
       os << " tokens=" << s.accept.T << " sequences=" << s.accept.B << " caches=" << s.accept.n_caches;
@@ -2755,8 +2755,18 @@ size_t Plan::temp_bytes() const {
   return n;
 }
 
-Plan build_plan(const Graph& g, const PlanOptions& opts) {
+Plan build_plan(const Graph& g, const PlanOptions& asked) {
+  PlanOptions opts = asked;
   Plan plan = Planner(g, opts).run();
+  // A plan that does not fit the allocation-free scratch gives products with 4-bit weights less of it: their rows go through it
+  // in more goes, and K in fewer ranges (1024 rows against 14336 x 4096 in f32 with 58.7 MB of other temporaries).
+  for (const int64_t room : {16ll << 20, 4ll << 20}) {
+    const auto tiles = [](const Step& st) { return st.kind == Step::INT4_MATMUL && st.int4.kernel == INT4_TILE; };
+    if (plan.temp_bytes() <= kNoAllocScratchBytes || std::none_of(plan.steps.begin(), plan.steps.end(), tiles)) break;
+    opts.int4_workspace = std::min(asked.int4_workspace, (int64_t)room);
+    Plan p = Planner(g, opts).run();
+    if (p.temp_bytes() < plan.temp_bytes()) plan = std::move(p);
+  }
   // Edge GEMMs take the number of K ranges that is estimated fastest. Where it is their partial sums that would keep the
   // plan from the allocation-free scratch, they get as many as leave it room, down to none: 16 products of 2432 × 11520 ×
   // 128 need no temporaries unsplit (152 µs), 76 MiB in the 4 ranges estimated (125).

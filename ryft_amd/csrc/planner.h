@@ -88,6 +88,7 @@ constexpr size_t kNoAllocScratchBytes = (size_t)64 << 20;
 
 struct PlanOptions {
   bool fast_paths = true;  // recognise programs that specialised kernels compute (row norm); false: interpret them
+  int64_t int4_workspace = INT64_MAX;  // bytes of workspace that a product with 4-bit weights may take
   int64_t edge_partials = INT64_MAX;  // most bytes of partial sums that one edge GEMM may take
 };
 Plan build_plan(const Graph& g, const PlanOptions& opts = PlanOptions());

@@ -118,6 +118,24 @@ def test_caches_are_moved_in_place(compile_client):
     assert plan.index(": tree_accept ") > plan.rindex(": tree_attention ") and plan.index(": tree_accept ") > plan.index(": sample ")
 
 
+def test_int4_matmul_leaves_room_for_other_temporaries(compile_client):
+    # allocation-free executions have 64 MiB for all temporaries: beside a large one a product takes less, in more goes
+    def plan(rows, columns):
+        x, w, s = f"tensor<{rows}x4096xbf16>", f"tensor<{columns}x2048xui8>", f"tensor<{columns}x32xbf16>"
+        y, v, t = f"tensor<{rows}x{columns}xf32>", f"tensor<8x{columns // 2}xui8>", f"tensor<8x{columns // 128}xf32>"
+        z = f"tensor<{rows}x8xf32>"
+        exe = compile_client.compile(pjrt.Program.mlir(
+            f"module {{\n  func.func @main(%x: {x}, %w: {w}, %s: {s}, %v: {v}, %t: {t}) -> {z} {{\n"
+            + operators.int4_matmul("%y", [("%x", x), ("%w", w), ("%s", s)], y)
+            + operators.int4_matmul("%z", [("%y", y), ("%v", v), ("%t", t)], z) + f"    return %z : {z}\n  }}\n}}\n"))
+        return exe.describe_plan(), exe.executable().memory_statistics()["temp_size_in_bytes"]
+
+    text, temp = plan(1024, 14336)
+    assert " tile=128 rows=384" in text and 58_720_256 < temp <= 64 << 20
+    text, temp = plan(1024, 4096)
+    assert " tile=128 rows=1024 parts=2" in text and temp <= 64 << 20
+
+
 def test_a_cache_read_after_the_move_is_copied(compile_client):
     # the attention does not feed the choices: it may come after the move, so the move gets a buffer of its own
     c, q, i, s, w = "tensor<3x2x16x64xbf16>", "tensor<5x4x64xbf16>", "tensor<5xi32>", "tensor<2xi32>", "tensor<5x1xi32>"
