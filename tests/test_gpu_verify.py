@@ -261,6 +261,32 @@ def test_tree_accept(gpu_client, name):
         assert np.array_equal(g, w), what
 
 
+def test_tree_accept_of_many_caches(gpu_client):
+    # as many results as a call may have
+    module, ins = vp.accept_case([20, 9], 256, 1, 8, 16, "f16", vocab=1, wide=True, seed=6)
+    got, _ = run(gpu_client, module, ins, ["i32"] * 3 + ["f16"] * 256)
+    want = oo.tree_accept(vp.values(ins), {})
+    for n, (g, w) in enumerate(zip(got, want)):
+        assert np.array_equal(g, w), n
+
+
+def test_tree_accept_of_one_cache_twice(gpu_client):
+    # each result gets its own copy; donated, the parameter's memory becomes the first one's
+    module, ins = vp.accept_case([30, 20], 2, 2, 64, 16, "bf16", vocab=1, wide=True, seed=2)
+    module = module.replace("%arg6)", "%arg5)")
+    x = vp.values(ins)
+    want = oo.tree_accept(x[:6] + [x[5]], {})
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    for donated in (False, True):
+        bufs = device_buffers(gpu_client, ins)
+        out = exe.execute([[pjrt.ExecutionInput(b, donatable=donated and n == 5) for n, b in enumerate(bufs)]])[0]
+        out.done.await_()
+        for n, (g, w) in enumerate(zip(out.outputs, want)):
+            got = sh.from_raw(g.to_numpy(), "i32" if n < 3 else "bf16")
+            assert np.array_equal(got, w), (donated, n)
+        assert bufs[5].is_deleted() == donated
+
+
 def test_tree_accept_bad_starts_stay_in_bounds(gpu_client):
     module, ins = vp.accept_case([20, 20, 20], 2, 2, 64, 16, "bf16", vocab=2, seed=2)
     for starts in ([-5, 30, 20, 60], [60, 0, 60, 0], [10, 20, 5, 2 ** 31 - 1], [-2 ** 31, -1, -1, -1]):
