@@ -8,9 +8,10 @@
 // of K where they leave the chip idle; the third adds the parts in their order.
 //
 // 870 TFLOP/s is 0.62 of what a library product of 16-bit weights reaches on a large square (1396). The matrix instructions are
-// 9/8 of a product's, for the zero points: 166 us at that rate. The rest is the stage's beginning, where no wavefront has
-// operands yet. Wavefronts of 64 x 64, which read half as much of x from LDS and make each operand twice, took 263 us; waiting for
-// fewer loads at the ranges' ends changed nothing.
+// 9/8 of a product's, for the zero points: 166 us at that rate. What is beside them is traffic through LDS: of 213 us (at the
+// card's clock under load) 208 are left without scaling, 213 without making operands, 169 without reading more of x than the
+// first block, 169 without loads, 137 without both. Wavefronts of 64 x 64, which read half as much of x and make each operand
+// twice, take 223 us; words and groups read a stage ahead, or waits for fewer loads at the ranges' ends, change nothing.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -424,19 +425,24 @@ void launch_type(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
 void int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   const int64_t stages = (a.K + STAGE - 1) / STAGE;
   a.steps = (int32_t)stages;
-  // Taller tiles turn the weight into operands less often: 2048 rows against 12288 x 4096, bf16: 237 us with 128 rows a tile, 299
-  // with 64, 415 with 32; 128 rows against 12288 x 4096: 24, 28 and 36; 64 rows against 28672 x 4096: 40, 29 and 37; 16 rows
-  // against the same: 40, 28 and 23.
-  a.tile = a.T <= 32 ? 1 : a.T <= 64 ? 2 : 4;
   // Rows at a time: as many as 24 MiB hold, a tile's at least.
   const int64_t row = stages * (STAGE * 2 + STAGE / a.span * 16), x_most = std::min<int64_t>(24ll << 20, room);
-  const int64_t rows = std::min(a.T, std::max<int64_t>(1, x_most / (row * MOST_ROWS)) * MOST_ROWS), bm = 32 * a.tile;
-  const int64_t tiles = ((rows + bm - 1) / bm) * ((a.N + BN - 1) / BN);
+  const int64_t rows = std::min(a.T, std::max<int64_t>(1, x_most / (row * MOST_ROWS)) * MOST_ROWS);
+  const int64_t x_bytes = tile_ws_bytes(stages, rows, a.span), part = rows * a.N * 4;
+  // Taller tiles turn the weight into operands less often: 2048 rows against 12288 x 4096, bf16: 237 us with 128 rows a tile, 299
+  // with 64, 415 with 32; 128 rows against 12288 x 4096: 24, 28 and 36; 64 rows against 28672 x 4096: 40, 29 and 37; 16 rows
+  // against the same: 40, 28 and 23. Lower ones where taller leave half the chip idle or more: 33 rows against 7001 x 2080: 20
+  // with 64 rows, 17 with 32; 128 against 1024 x 1024: 13.6 with 128 rows, 7.9 with 32; 100 against 8192 x 608: 20 and 12.
+  // Ranges of at least four stages: of two, the parts' sum takes what they save (33 rows: 17.4 and 6.4 for 17.2 and 4.2).
+  int64_t tiles = 0;
+  for (a.tile = a.T <= 32 ? 1 : a.T <= 64 ? 2 : 4;; a.tile /= 2) {
+    tiles = ((rows + 32 * a.tile - 1) / (32 * a.tile)) * ((a.N + BN - 1) / BN);
+    a.parts = (int32_t)std::max<int64_t>(1, std::min({CUS / tiles, stages / LEAST, (room - x_bytes) / part}));
+    if (a.tile == 1 || tiles * a.parts > CUS / 2) break;
+  }
   if (tiles > INT32_MAX || stages > 65535 || rows * a.N / 1024 >= INT32_MAX) return;
   a.kernel = INT4_TILE;
   a.rows = (int32_t)rows;
-  const int64_t x_bytes = tile_ws_bytes(stages, rows, a.span), part = rows * a.N * 4;
-  a.parts = (int32_t)std::max<int64_t>(1, std::min({CUS / tiles, stages / LEAST, (room - x_bytes) / part}));
   *ws_floats = (x_bytes + (a.parts > 1 ? a.parts * part : 0)) / 4;
 }
 
