@@ -97,6 +97,9 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(const Int4Args A, int
     *(u32x4p*)(ws + tile_x_bytes(A.steps, rows) + ((int64_t)(stage * (STAGE / SPAN) + c / CS) * rows + t) * 16) = sum_terms<X>(sum);
 }
 
+// Floats from one part of `count` results to the next: parts begin at 16 bytes.
+__host__ __device__ inline int64_t part_floats(int64_t count) { return (count + 3) & ~(int64_t)3; }
+
 constexpr int WAVES = 8, BN = 32 * WAVES;  // wavefronts of a workgroup, each with 32 rows of the weight
 
 // Rings in LDS: stages of x and its sums, DX of them, which all wavefronts read; stages of a wavefront's weight, scales and zero
@@ -127,7 +130,7 @@ __device__ __forceinline__ void tile_wait() {  // until N loads or fewer are on 
   asm volatile("" ::: "memory");
 }
 
-// parts > 1: partial sums as f32 rows, [part][row][N], behind the prepared x.
+// parts > 1: partial sums as f32 rows, [part][row][N], part_floats() from part to part, behind the prepared x.
 // MANY: several spans a group.
 template <class X, int MT, int SPAN, bool MANY>
 __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args A, int64_t t_base, int x_rows) {
@@ -262,61 +265,61 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
         word[4 * j] = a[0], word[4 * j + 1] = b[0], word[4 * j + 2] = a[1], word[4 * j + 3] = b[1];
       }
       const int g0 = group_of(stage * SPANS);
-      // (a loop: the compiler would put off the sums of one span behind the products of the next, past the registers)
-#pragma unroll 1
+      // scales and zero points (of the groups that there are; past the row's end x is 0: its last one's)
+      float scale[SPANS];
+      u32x4p zf[SPANS];
+#pragma unroll
       for (int p = 0; p < SPANS; ++p) {
-        // (of the words that there are; past the row's end x is 0: its last group's)
         const int g = group_of(stage * SPANS + p) - g0;
         const uint32_t s_byte = es == 4 ? 4 * g : ((own + g0) << 1 & s_step) + 2 * g, z_byte = A.zero ? ((own + g0) & z_step) + g : 0;
         uint32_t s_word = *(const uint32_t*)(wf_at + s_lane + (s_byte & ~3u));
         s_word >>= s_byte << 3 & s_up;
-        const float scale = es == 4 ? __uint_as_float(s_word) : X::lo(s_word & 0xffffu);
-        const u32x4p zf = sum_factors<X>(*(const uint8_t*)(wf_at + z_lane + z_byte), half == 0);
-        u32x4p wf[FR];
-#pragma unroll
-        for (int f = 0; f < FR; ++f) wf[f] = operand(word[f]);
-#pragma unroll
-        for (int f = 0; f + FR < 8; ++f) word[f] = word[f + FR];  // (the next span's come first)
-        asm volatile("" : "+v"(chunk));  // (or all its neighbours would be kept in registers over the stages)
-        const char* const sums = from + sums_at + p * (C::BM * 16);
-        // Fragments of x are read AHEAD matrix instructions before they are multiplied, and 32 rows' sums are scaled while the
-        // next 32 rows' products run: the order is forced, since the compiler's own reads each one, waits and multiplies.
-        constexpr int F1 = FR + 1, ALL = MT * F1;
-        u32x4p ring[AHEAD + 1];
-        f32x16p acc[2];
-        auto read = [&](int at) {
-          const int m = at / F1, f = at % F1;
-          if (f == 0) return *(const u32x4p*)(sums + 32 * m * 16);
-          return *(const u32x4p*)(from + (chunk ^ (32 * (p * FR + f - 1))) + 32 * m * (STAGE * 2));
-        };
-#pragma unroll
-        for (int at = 0; at < AHEAD && at < ALL; ++at) ring[at] = read(at);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-          for (int f = 0; f < F1; ++f) {
-            const int at = m * F1 + f;
-            if (at + AHEAD < ALL) ring[(at + AHEAD) % (AHEAD + 1)] = read(at + AHEAD);
-            const u32x4p x = ring[at % (AHEAD + 1)];
-            acc[m & 1] = f == 0 ? X::mma32(x, zf, f32x16p{}) : X::mma32(x, wf[f > 0 ? f - 1 : 0], acc[m & 1]);
-          }
-          if (m > 0) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[m - 1][e] = __builtin_fmaf(scale, acc[(m - 1) & 1][e], y[m - 1][e]);
-            asm volatile("" : "+v"(y[m - 1]));  // (or they would be put off past all products)
-          }
-#pragma unroll
-          for (int f = 0; f < F1; ++f) {
-            if (m * F1 + f + AHEAD < ALL) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (m > 0) __builtin_amdgcn_sched_group_barrier(0x002, (16 + F1 - 1) / F1, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) y[MT - 1][e] = __builtin_fmaf(scale, acc[(MT - 1) & 1][e], y[MT - 1][e]);
+        scale[p] = es == 4 ? __uint_as_float(s_word) : X::lo(s_word & 0xffffu);
+        zf[p] = sum_factors<X>(*(const uint8_t*)(wf_at + z_lane + z_byte), half == 0);
       }
+      u32x4p wf[8];
+#pragma unroll
+      for (int f = 0; f < 8; ++f) wf[f] = operand(word[f]);
+      asm volatile("" : "+v"(chunk));  // (or all its neighbours would be kept in registers over the stages)
+      const char* const sums = from + sums_at;
+      // Blocks of a span and 32 rows of x, one after the other. Fragments of x are read AHEAD matrix instructions before they are
+      // multiplied, and a block's sums are scaled while the next one's products run: the order is forced, since the compiler's own
+      // reads each one, waits and multiplies.
+      constexpr int F1 = FR + 1, BLOCKS = SPANS * MT, ALL = BLOCKS * F1;
+      u32x4p ring[AHEAD + 1];
+      f32x16p acc[2];
+      auto read = [&](int at) {
+        const int b = at / F1, f = at % F1, p = b / MT, m = b % MT;
+        if (f == 0) return *(const u32x4p*)(sums + (p * C::BM + 32 * m) * 16);
+        return *(const u32x4p*)(from + (chunk ^ (32 * (p * FR + f - 1))) + 32 * m * (STAGE * 2));
+      };
+      auto add = [&](int b) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[b % MT][e] = __builtin_fmaf(scale[b / MT], acc[b & 1][e], y[b % MT][e]);
+        asm volatile("" : "+v"(y[b % MT]));  // (or they would be put off past all products)
+      };
+#pragma unroll
+      for (int at = 0; at < AHEAD && at < ALL; ++at) ring[at] = read(at);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+        for (int f = 0; f < F1; ++f) {
+          const int at = b * F1 + f;
+          if (at + AHEAD < ALL) ring[(at + AHEAD) % (AHEAD + 1)] = read(at + AHEAD);
+          const u32x4p x = ring[at % (AHEAD + 1)];
+          acc[b & 1] = f == 0 ? X::mma32(x, zf[b / MT], f32x16p{}) : X::mma32(x, wf[b / MT * FR + (f > 0 ? f - 1 : 0)], acc[b & 1]);
+        }
+        if (b > 0) add(b - 1);
+#pragma unroll
+        for (int f = 0; f < F1; ++f) {
+          if (b * F1 + f + AHEAD < ALL) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (b > 0) __builtin_amdgcn_sched_group_barrier(0x002, (16 + F1 - 1) / F1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      add(BLOCKS - 1);
     }
   }
   // The tile's rows, 32 at a time, through LDS: a thread stores 16 bytes of a row together where rows begin at such places.
@@ -325,7 +328,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
   const bool wide = A.N % per == 0;
   const int n_here = (int)min((int64_t)BN, A.N - n0);
   char* const out = whole ? (char*)A.y + (t_base + t0) * A.N * ys
-                          : (char*)A.ws + tile_ws_bytes(A.steps, x_rows, SPAN) + ((int64_t)part * x_rows + t0) * A.N * 4;
+                          : (char*)A.ws + tile_ws_bytes(A.steps, x_rows, SPAN) + (part * part_floats(x_rows * A.N) + t0 * A.N) * 4;
   float* const rows_at = (float*)smem;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -363,28 +366,23 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
   }
 }
 
-// Adds the parts of `count` elements, in their order, from `parts` (of the workspace) into y from element `at` on.
+// Adds the parts of `count` elements, in their order, from `parts` (of the workspace, part_floats() apart) into y from element
+// `at` on, a multiple of four: four elements a thread.
 template <class X>
 __global__ void __launch_bounds__(256) int4_join_kernel(const Int4Args A, const float* parts, int64_t at, int64_t count) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= count) return;
-  const bool wide = count % 4 == 0 && at % 4 == 0;  // (every part begins at 16 bytes, and every four elements of y at theirs)
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  const int n = (int)min((int64_t)4, count - i);
-  if (wide) {
+  f32x4p v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int p = 0; p < A.parts; ++p) {
-      const f32x4p u = *(const f32x4p*)(parts + p * count + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += u[e];
-    }
+  for (int p = 0; p < A.parts; ++p) v += *(const f32x4p*)(parts + p * part_floats(count) + i);
+  if (count - i >= 4) {
+    if (A.y_dtype == DT_F32) *(f32x4p*)((float*)A.y + at + i) = v;
+    else *(uint2*)((uint16_t*)A.y + at + i) = uint2{X::put(v[0]) | (uint32_t)X::put(v[1]) << 16, X::put(v[2]) | (uint32_t)X::put(v[3]) << 16};
   } else {
-    for (int p = 0; p < A.parts; ++p)
-      for (int e = 0; e < n; ++e) v[e] += parts[p * count + i + e];
-  }
-  for (int e = 0; e < n; ++e) {
-    if (A.y_dtype == DT_F32) ((float*)A.y)[at + i + e] = v[e];
-    else ((uint16_t*)A.y)[at + i + e] = X::put(v[e]);
+    for (int e = 0; e < (int)(count - i); ++e) {
+      if (A.y_dtype == DT_F32) ((float*)A.y)[at + i + e] = v[e];
+      else ((uint16_t*)A.y)[at + i + e] = X::put(v[e]);
+    }
   }
 }
 
@@ -425,22 +423,31 @@ void launch_type(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
 void int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   const int64_t stages = (a.K + STAGE - 1) / STAGE;
   a.steps = (int32_t)stages;
-  // Rows at a time: as many as 24 MiB hold, a tile's at least.
-  const int64_t row = stages * (STAGE * 2 + STAGE / a.span * 16), x_most = std::min<int64_t>(24ll << 20, room);
-  const int64_t rows = std::min(a.T, std::max<int64_t>(1, x_most / (row * MOST_ROWS)) * MOST_ROWS);
-  const int64_t x_bytes = tile_ws_bytes(stages, rows, a.span), part = rows * a.N * 4;
-  // Taller tiles turn the weight into operands less often: 2048 rows against 12288 x 4096, bf16: 237 us with 128 rows a tile, 299
-  // with 64, 415 with 32; 128 rows against 12288 x 4096: 24, 28 and 36; 64 rows against 28672 x 4096: 40, 29 and 37; 16 rows
-  // against the same: 40, 28 and 23. Lower ones where taller leave half the chip idle or more: 33 rows against 7001 x 2080: 20
-  // with 64 rows, 17 with 32; 128 against 1024 x 1024: 13.6 with 128 rows, 7.9 with 32; 100 against 8192 x 608: 20 and 12.
-  // Ranges of at least four stages: of two, the parts' sum takes what they save (33 rows: 17.4 and 6.4 for 17.2 and 4.2).
-  int64_t tiles = 0;
-  for (a.tile = a.T <= 32 ? 1 : a.T <= 64 ? 2 : 4;; a.tile /= 2) {
-    tiles = ((rows + 32 * a.tile - 1) / (32 * a.tile)) * ((a.N + BN - 1) / BN);
-    a.parts = (int32_t)std::max<int64_t>(1, std::min({CUS / tiles, stages / LEAST, (room - x_bytes) / part}));
-    if (a.tile == 1 || tiles * a.parts > CUS / 2) break;
+  // Rows at a time: equal shares, in whole tiles, of at most 32 MiB (838 rows of 13248 values against 3518 rows, once 768 and 70 at
+  // a time: 226 us).
+  const int64_t row = stages * (STAGE * 2 + STAGE / a.span * 16);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(32ll << 20, room) / (row * MOST_ROWS)) * MOST_ROWS;
+  const int64_t goes = (a.T + most - 1) / most, each = (a.T + goes - 1) / goes;
+  const int64_t rows = std::min(a.T, (each + MOST_ROWS - 1) / MOST_ROWS * MOST_ROWS);
+  const int64_t x_bytes = tile_ws_bytes(stages, rows, a.span), part = 4 * part_floats(rows * a.N);
+  // Tile and ranges of K by what they are estimated to take, in us: 4 for the launch, 3 for a tile's way to its stages and from
+  // them, a stage's time by rows of the tile and values of a span (2048 rows against 12288 x 4096: 219, 267 and 389 us with 128, 64
+  // and 32 rows in spans of 128, 256, 320 and 468 of 64, 324, 406 and 593 of 32), 4 for the third launch and 0.3 a MB of parts,
+  // written and read. Estimated and measured with 128, 64 and 32 rows: 256 rows against 4096 x 4096 30, 27, 29 and 27, 24, 28; 234
+  // against 13226 x 1472 in spans of 64 34, 27, 37 and 33, 27, 38; 373 against 940 x 9216 27, 26, 27 and 24, 24, 27; 100 against
+  // 8192 x 608 in spans of 32 24, 18, 15 and 20, 13, 12.
+  static constexpr double STAGE_US[3][3] = {{0.95, 1.37, 2.2}, {1.13, 1.65, 2.6}, {1.5, 2.1, 3.3}};
+  if (stages > 65535 || rows * ((a.N + 31) / 32) >= INT32_MAX) return;  // (the grids' limits)
+  double best = 1e30;
+  for (int tile = 1; tile <= 4; tile *= 2) {
+    const double stage = STAGE_US[a.span == 128 ? 0 : a.span == 64 ? 1 : 2][tile / 2];
+    const int64_t tiles = ((rows + 32 * tile - 1) / (32 * tile)) * ((a.N + BN - 1) / BN);
+    for (int64_t parts = 1; parts == 1 || (parts * tiles <= CUS && parts <= stages / LEAST && x_bytes + parts * part <= room); ++parts) {
+      double us = 4 + (double)((tiles * parts + CUS - 1) / CUS) * (3 + stage * (double)((stages + parts - 1) / parts));
+      if (parts > 1) us += 4 + 0.3e-6 * (double)(parts * part);
+      if (us < best) best = us, a.tile = tile, a.parts = (int32_t)parts;
+    }
   }
-  if (tiles > INT32_MAX || stages > 65535 || rows * a.N / 1024 >= INT32_MAX) return;
   a.kernel = INT4_TILE;
   a.rows = (int32_t)rows;
   *ws_floats = (x_bytes + (a.parts > 1 ? a.parts * part : 0)) / 4;
