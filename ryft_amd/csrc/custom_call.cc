@@ -1,7 +1,8 @@
 // The plugin's own operators, reached as `stablehlo.custom_call @ryft.<name>` with a backend_config dictionary (the
 // typed form, api_version 4): operand and result types, and the config's names and ranges, checked when the program is
 // read. The planner turns each call into one step (planner.cc), the kernels are in kernels/k_rope_append.hip,
-// k_paged_attention.hip, k_sample.hip, k_int4_matmul.hip and k_tree_accept.hip; their definitions stand beside the argument blocks in kernel_abi.h.
+// k_paged_attention.hip, k_sample.hip, k_int4_matmul.hip and k_tree_accept.hip; their definitions stand beside the argument
+// blocks in kernel_abi.h.
 #include <cmath>
 
 #include "kernel_abi.h"

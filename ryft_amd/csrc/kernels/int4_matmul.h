@@ -2,8 +2,8 @@
 // values as matrix operands, and the scales of their groups.
 //
 // A value q becomes 16 + q in x's own 16-bit type, exactly: four bits of the mantissa under a fixed exponent, for two values
-// in a shift, and one instruction that masks and joins. What that adds, and the zero point, is taken off where a group's sum begins: (q - z) · x
-// summed over a group = Σ (16 + q) x - (16 + z) Σ x. The group's scale multiplies the finished sum, in f32.
+// in a shift, and one instruction that masks and joins. What that adds, and the zero point, is taken off where a group's sum
+// begins: (q - z) · x summed over a group = Σ (16 + q) x - (16 + z) Σ x. The group's scale multiplies the finished sum, in f32.
 //
 // The eight values of a word come out in the order 0 4, 1 5, 2 6, 3 7; x is put into that order.
 #pragma once

@@ -120,7 +120,8 @@ __device__ __forceinline__ void few_read_w(u32x4p (&f)[2], uint32_t (&s)[8], uin
     s[0] = u[0], s[1] = u[1], s[2] = u[2], s[3] = u[3], z[0] = v[0], z[1] = v[1];
   } else {
     u32x4p u, w, v;
-    asm volatile("ds_read_b128 %2, %7\n ds_read_b128 %3, %7 offset:16\n ds_read_b128 %4, %8\n ds_read_b128 %0, %5\n ds_read_b128 %1, %6\n s_waitcnt lgkmcnt(0)"
+    asm volatile("ds_read_b128 %2, %7\n ds_read_b128 %3, %7 offset:16\n ds_read_b128 %4, %8\n"
+                 "ds_read_b128 %0, %5\n ds_read_b128 %1, %6\n s_waitcnt lgkmcnt(0)"
                  : "=&v"(f[0]), "=&v"(f[1]), "=&v"(u), "=&v"(w), "=&v"(v)
                  : "v"(a), "v"(b), "v"(c), "v"(d)
                  : "memory");
@@ -407,7 +408,8 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
 #pragma unroll
     for (int u = 0; u < W; u += 4) {
       f32x4p v[4];
-      asm volatile("ds_read_b128 %0, %4\n ds_read_b128 %1, %4 offset:1024\n ds_read_b128 %2, %4 offset:2048\n ds_read_b128 %3, %4 offset:3072\n s_waitcnt lgkmcnt(0)"
+      asm volatile("ds_read_b128 %0, %4\n ds_read_b128 %1, %4 offset:1024\n ds_read_b128 %2, %4 offset:2048\n"
+                   "ds_read_b128 %3, %4 offset:3072\n s_waitcnt lgkmcnt(0)"
                    : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
                    : "v"(sums + (u * 64 + lane) * 16)
                    : "memory");

@@ -2,16 +2,16 @@
 //
 // Two or three launches. The first puts x into the order and the places that the second's LDS has, and sums it over every span
 // of values that share a scale: done by each workgroup of the second for itself it was most of its float and integer
-// instructions (2048 rows against 12288 x 4096: 361 us; 237 and 8 so, 870 TFLOP/s). The second multiplies tiles of 32 MT rows of
-// x, which a workgroup's eight wavefronts share through a ring in LDS, with 32 rows of the weight a wavefront, which come through
-// a ring of its own. A lane's sums are of one row of the weight, 16 rows of x each: one scale a span. Tiles are cut into ranges
-// of K where they leave the chip idle; the third adds the parts in their order.
+// instructions (2048 rows against 12288 x 4096: 361 us; 205 to 222 and 8 so, with the card's clock: 0.93 to 1.0 PFLOP/s). The
+// second multiplies tiles of 32 MT rows of x, which a workgroup's eight wavefronts share through a ring in LDS, with 32 rows of
+// the weight a wavefront, which come through a ring of its own. A lane's sums are of one row of the weight, 16 rows of x each: one
+// scale a span. Tiles are cut into ranges of K where they leave the chip idle; the third adds the parts in their order.
 //
-// 870 TFLOP/s is 0.62 of what a library product of 16-bit weights reaches on a large square (1396). The matrix instructions are
-// 9/8 of a product's, for the zero points: 166 us at that rate. What is beside them is traffic through LDS: of 213 us (at the
-// card's clock under load) 208 are left without scaling, 213 without making operands, 169 without reading more of x than the
-// first block, 169 without loads, 137 without both. Wavefronts of 64 x 64, which read half as much of x and make each operand
-// twice, take 223 us; words and groups read a stage ahead, or waits for fewer loads at the ranges' ends, change nothing.
+// At 2048 rows that is 0.67 to 0.72 of what a library product of 16-bit weights reaches on a large square (1.40). The matrix
+// instructions are 9/8 of a product's, for the zero points: 166 us at that rate. What is beside them is traffic through LDS: of
+// 213 us 208 are left without scaling, 213 without making operands, 169 without reading more of x than the first block, 169
+// without loads, 137 without both. Wavefronts of 64 x 64, which read half as much of x and make each operand twice, take 223 us;
+// words and groups read a stage ahead, or waits for fewer loads at the ranges' ends, change nothing.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
   for (int h = 0; h < C::SL; ++h)
     s_row[h] = keep(s_off + (uint32_t)(min(r0 + min((64 * h + lane) / C::SW, 31), most) * A.groups) * es + 4 * ((64 * h + lane) % C::SW));
   const uint32_t z_row = keep(z_off + (uint32_t)(min(r0 + min(lane / C::ZW, 31), most) * A.groups) + 4 * (lane % C::ZW));
-  const uint32_t own = keep((uint32_t)(first & 3) + (uint32_t)(min(r0 + l32, most) * A.groups));  // groups before this lane's row, from a whole word on
+  // groups before this lane's row, from a whole word on
+  const uint32_t own = keep((uint32_t)(first & 3) + (uint32_t)(min(r0 + l32, most) * A.groups));
   char* const w_ring = smem + C::DX * C::XS + wave * (C::DW * C::WS);
   if (!A.zero) {
     // (the zero points that the loads below leave alone)
@@ -199,7 +200,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
     for (int j = 0; j < CH; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, (tile_lds*)(to + j * (1024 * WAVES) + wave * 1024), 16, (int)x_at,
                                                stage * x_rows * (STAGE * 2) + j * (1024 * WAVES), 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(tb, (tile_lds*)((t_to == C::DUMP ? smem : to) + t_to), 16, (int)t_at, stage * x_rows * (SPANS * 16), 0, 0);
+    char* const t_base = t_to == C::DUMP ? smem : to;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(tb, (tile_lds*)(t_base + t_to), 16, (int)t_at, stage * x_rows * (SPANS * 16), 0, 0);
   };
   const int z_to = A.zero ? C::Z0 : C::DUMP;
   auto load_w = [&](int stage, int slot) {
@@ -215,10 +217,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
     }
     const uint32_t g = (uint32_t)group_of(stage * SPANS);
 #pragma unroll
-    for (int h = 0; h < C::SL; ++h)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (tile_lds*)(to + C::S0 + h * 256), 4, (int)min((s_row[h] + g * es) & ~3u, s_bytes - 4), 0, 0, 0);
+    for (int h = 0; h < C::SL; ++h) {
+      const uint32_t at = min((s_row[h] + g * es) & ~3u, s_bytes - 4);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (tile_lds*)(to + C::S0 + h * 256), 4, (int)at, 0, 0, 0);
+    }
     // (without zero points, some of the scales, for the number of loads)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(zb, (tile_lds*)((A.zero ? to : smem) + z_to), 4, (int)min((z_row + g) & ~3u, (A.zero ? z_bytes : s_bytes) - 4), 0, 0, 0);
+    const uint32_t z = min((z_row + g) & ~3u, (A.zero ? z_bytes : s_bytes) - 4);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(zb, (tile_lds*)((A.zero ? to : smem) + z_to), 4, (int)z, 0, 0, 0);
   };
   // Waits for a stage's loads, by how many were made after them. In the first stage those of DW - 2 weights; later those of DX - 2
   // stages and of one weight more, for x, whose weight's loads are older. Where there are no more weights to load, for all.

@@ -1,5 +1,5 @@
-// ryft.paged_attention and ryft.tree_attention: attention of a ragged batch of queries over a paged key / value cache (the definition stands at
-// PagedAttnArgs in kernel_abi.h). Scores, softmax statistics and outputs are f32 and rounded once, on store; probabilities
+// ryft.paged_attention and ryft.tree_attention: attention of a ragged batch of queries over a paged key / value cache (the
+// definitions stand at PagedAttnArgs in kernel_abi.h). Scores, softmax statistics and outputs are f32 and rounded once, on store; probabilities
 // go to the matrix cores as two terms of a 16-bit type (paged_attention.h).
 //
 // Three kernels: few rows a sequence (here: a decoding step), many (k_paged_prompt.hip), and any type and head dim (here).

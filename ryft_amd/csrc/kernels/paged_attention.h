@@ -154,8 +154,8 @@ __device__ __forceinline__ float sum_rows16(float v) {
 
 // ------------------------------------------------------------------------------------------------ one row
 // One query and head over the keys [first, last), by a workgroup of 256, for any type, head dim up to 256 and page size;
-// nothing that the query does not see is read. pos: the query's position, of a tree that of its first token. Leaves the maximum (log2), the sum and, at thread d, element d of the
-// unnormalised output. Each wavefront takes every fourth block of 64 keys, a lane a key for the scores and an element
+// nothing that the query does not see is read. pos: the query's position, of a tree that of its first token. Leaves the
+// maximum (log2), the sum and, at thread d, element d of the unnormalised output. Each wavefront takes every fourth block of 64 keys, a lane a key for the scores and an element
 // of the head for the output; the four meet in LDS at the end.
 struct PagedRowLds {
   int64_t base[4][64];

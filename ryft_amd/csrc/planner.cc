@@ -902,8 +902,8 @@ int Planner::shared_counters(int64_t count) {
 
 // One of the plugin's operators (custom_call.cc): all results of the op written by one step, each straight into the
 // buffer of the function result it is, if it is one. The caches of rope_append and tree_accept are copied into their
-// results first and then written at their slots, so that an execution whose cache argument is donated into the result, or is the result's own
-// memory, writes the new tokens only.
+// results first and then written at their slots, so that an execution whose cache argument is donated into the result, or is
+// the result's own memory, writes the new tokens only.
 void Planner::emit_custom_call(int node, int target) {
   const Node n = g_.nodes[node];
   std::vector<int> res;  // the op's result nodes
