@@ -408,10 +408,10 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
 #pragma unroll
     for (int u = 0; u < W; u += 4) {
       f32x4p v[4];
-      asm volatile("ds_read_b128 %0, %4\n ds_read_b128 %1, %4 offset:1024\n ds_read_b128 %2, %4 offset:2048\n"
-                   "ds_read_b128 %3, %4 offset:3072\n s_waitcnt lgkmcnt(0)"
+      asm volatile("ds_read_b128 %0, %4\n ds_read_b128 %1, %4 offset:%5\n ds_read_b128 %2, %4 offset:%6\n"
+                   "ds_read_b128 %3, %4 offset:%7\n s_waitcnt lgkmcnt(0)"
                    : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
-                   : "v"(sums + (u * 64 + lane) * 16)
+                   : "v"(sums + (u * 64 + lane) * 16), "i"(1024), "i"(2 * 1024), "i"(3 * 1024)
                    : "memory");
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum += v[j];
