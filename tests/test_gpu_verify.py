@@ -119,6 +119,32 @@ def test_tree_attention_bad_starts_stay_in_bounds(gpu_client, starts, lengths, h
     assert np.isfinite(got).all() and np.abs(got).max() <= np.abs(vp.values(ins)[2]).max()
 
 
+@pytest.mark.parametrize("nodes", [[4, 2], [50, 40]], ids=str)
+def test_tree_attention_past_32_bits(gpu_client, nodes):
+    # pages of caches of 4.6 GB each, their last among them, against the same pages in small caches
+    pages, hkv, page, d, lengths = 140_000, 8, 16, 128, [300, 90]
+    _, ins = vp.tree_case(nodes, lengths, 16, hkv, d, page, "bf16", seed=4)
+    small = [torch.from_numpy(np.array(i.data).view(np.int16 if i.data.dtype == np.uint16 else i.data.dtype)).cuda() for i in ins]
+    few = small[1].shape[0]
+    to = torch.linspace(0, pages - 1, few, device="cuda").round().long()
+    big = list(small)
+    for n in (1, 2):
+        big[n] = torch.zeros((pages, hkv, page, d), dtype=small[n].dtype, device="cuda")
+        big[n][to] = small[n]
+    big[3] = torch.where((small[3] >= 0) & (small[3] < few), to[small[3].clamp(0, few - 1).long()].int(), small[3])
+    got = []
+    for x, count in ((small, few), (big, pages)):
+        module = operators.tree_attention_module(
+            tokens=sum(nodes), sequences=2, q_heads=16, kv_heads=hkv, head_dim=d, pages=count, page_size=page,
+            pages_per_sequence=x[3].shape[1], words=x[6].shape[1], dtype="bf16", scale=d ** -0.5)
+        exe = gpu_client.compile(pjrt.Program.mlir(module))
+        out = torch.zeros_like(x[0])
+        exe.execute_into([(t.data_ptr(), t.nbytes) for t in x], [(out.data_ptr(), out.nbytes)], torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        got.append(out)
+    assert int((got[0] != 0).sum()) > 0 and torch.equal(got[0], got[1])
+
+
 # ------------------------------------------------------------------------------------------------ int4_matmul
 SIZES = [
     # rows, inner, columns, group
@@ -224,6 +250,28 @@ module @slices {
     assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("rows", [1, 5, 20])
+def test_int4_matmul_past_32_bits(gpu_client, rows):
+    # a weight of 8.6 GB that is 0 but for its last rows and some between
+    inner, columns, group = 16384, (1 << 20) + 3, 128
+    weight = torch.full((columns, inner // 2), 0x88, dtype=torch.uint8, device="cuda")
+    scale = torch.ones((columns, inner // group), dtype=torch.bfloat16, device="cuda")
+    some = [0, 1 << 19, 700_001, columns - 2, columns - 1]
+    for k, n in enumerate(some):
+        weight[n] = 0x99 + 0x11 * k
+    x = torch.arange(rows, device="cuda").bfloat16()[:, None].expand(rows, inner).contiguous() + 1
+    y = torch.full((rows, columns), 7.0, dtype=torch.float32, device="cuda")
+    exe = gpu_client.compile(pjrt.Program.mlir(operators.int4_matmul_module(rows=rows, inner=inner, columns=columns, group=group,
+                                                                            out_dtype="f32")))
+    exe.execute_into([(t.data_ptr(), t.nbytes) for t in (x, weight, scale)], [(y.data_ptr(), y.nbytes)],
+                     torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want = torch.zeros_like(y)
+    for k, n in enumerate(some):
+        want[:, n] = x[:, 0].float() * (k + 1) * inner
+    assert torch.equal(y, want)
+
+
 def test_int4_matmul_of_no_rows(gpu_client):
     module, ins = vp.int4_case(0, 64, 10, 32, "bf16")
     (got,), _ = run(gpu_client, module, ins, ["bf16"])
@@ -287,6 +335,27 @@ def test_tree_accept_of_one_cache_twice(gpu_client):
         assert bufs[5].is_deleted() == donated
 
 
+def test_tree_accept_past_32_bits(gpu_client):
+    # a cache of 4.6 GB, moved in place: rows at its end, the path 0, 2, 3 of a tree whose every choice is token 1
+    pages, hkv, page, d = 140_000, 8, 16, 128
+    cache = torch.zeros((pages, hkv, page, d), dtype=torch.bfloat16, device="cuda")
+    slots = [pages * page - 1 - 37 * i for i in range(4)]
+    for i, slot in enumerate(slots):
+        cache[slot // page, :, slot % page] = i + 1
+    module = operators.tree_accept_module(tokens=4, sequences=1, caches=1, pages=pages, kv_heads=hkv, page_size=page, head_dim=d)
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    words = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    ins = [words(0, 2, 1, 1), words(-1, 0, 0, 2), words(1, 1, 1, 7), words(*slots), words(0, 4), cache]
+    outs = [words(9), words(9, 9, 9, 9), words(9, 9, 9, 9)]
+    exe.execute_into([(t.data_ptr(), t.nbytes) for t in ins], [(t.data_ptr(), t.nbytes) for t in outs + [cache]],
+                     torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert [o.tolist() for o in outs] == [[3], [1, 1, 7, -1], [0, 2, 3, -1]]
+    for slot, want in zip(slots, (1, 3, 4, 4)):
+        assert (cache[slot // page, :, slot % page] == want).all(), slot
+    assert int((cache[:70_000] != 0).sum()) == 0
+
+
 def test_tree_accept_bad_starts_stay_in_bounds(gpu_client):
     module, ins = vp.accept_case([20, 20, 20], 2, 2, 64, 16, "bf16", vocab=2, seed=2)
     for starts in ([-5, 30, 20, 60], [60, 0, 60, 0], [10, 20, 5, 2 ** 31 - 1], [-2 ** 31, -1, -1, -1]):
@@ -328,6 +397,30 @@ def test_replayed_from_a_graph(gpu_client, name):
         again = exe.execute([bufs])[0]
         again.done.await_()
         assert np.array_equal(again.outputs[0].to_numpy(), want), i
+
+
+@pytest.mark.parametrize("names", [("int4_some", "int4_many"), ("tree_few", "int4_some"), ("tree_ranges", "int4_many")], ids=str)
+def test_two_graphs_in_turn(gpu_client, names):
+    # they share the scratch memory; each replay leaves nothing of it for the next
+    made = []
+    for name in names:
+        module, ins = PROGRAMS[name]()
+        exe = gpu_client.compile(pjrt.Program.mlir(module))
+        bufs = device_buffers(gpu_client, ins)
+        ref = exe.execute([bufs])[0]
+        ref.done.await_()
+        out = gpu_client.uninitialized_buffer(ref.outputs[0].element_type(), ref.outputs[0].dimensions())
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            exe.execute_into([span(b) for b in bufs], [span(out)], torch.cuda.current_stream().cuda_stream)
+        made.append((graph, out, ref.outputs[0].to_numpy(), exe, bufs))
+    for i in range(4):
+        for graph, *_ in made:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, *_ in made:
+            assert np.array_equal(out.to_numpy(), want), i
 
 
 def test_tree_accept_replayed_in_place(gpu_client):
