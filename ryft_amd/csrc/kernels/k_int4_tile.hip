@@ -9,7 +9,7 @@
 //
 // At 2048 rows that is 0.67 to 0.72 of what a library product of 16-bit weights reaches on a large square (1.40). The matrix
 // instructions are 9/8 of a product's, for the zero points: 166 us at that rate. What is beside them is traffic through LDS: of
-// 213 us 208 are left without scaling, 213 without making operands, 169 without reading more of x than the first block, 169
+// 213 us 208 are left without scaling, 218 without making operands, 169 without reading more of x than the first block, 169
 // without loads, 137 without both. Wavefronts of 64 x 64, which read half as much of x and make each operand twice, take 223 us;
 // words and groups read a stage ahead, or waits for fewer loads at the ranges' ends, change nothing.
 #include <hip/hip_runtime.h>
