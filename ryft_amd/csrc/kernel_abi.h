@@ -433,7 +433,7 @@ struct SampleArgs {
 
 // ryft.int4_matmul (k_int4_matmul.hip): y[t, n] = Σ_g scale[n, g] · Σ_{k in group g} (w[n, k] - zero[n, g]) · x[t, k], where
 // w[n, k] is the low (k even) or high nibble of byte k / 2 of row n, group g the G values from g · G on, and zero 8 where
-// there is none. Sums in f32, rounded once.
+// there is none. Sums in f32, rounded once; one that is not finite in f32 is summed again in 64 bits.
 struct Int4Args {
   const void* x;        // [T, K], unit stride along K
   const uint8_t* w;     // [N, K / 2]

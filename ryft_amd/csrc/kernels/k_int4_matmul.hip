@@ -24,6 +24,21 @@ __device__ __forceinline__ void write_any(void* p, int64_t i, int dtype, float v
   else ((float*)p)[i] = v;
 }
 
+// y[t, n] in 64 bits, by a wavefront: for a sum that left f32's range.
+__device__ __forceinline__ float any_again(const Int4Args& A, int64_t t, int64_t n) {
+  double sum = 0;
+#pragma unroll 1
+  for (uint32_t j = threadIdx.x & 63; j < (uint32_t)(A.K / 2); j += 64) {
+    const int64_t g = n * ((uint32_t)A.K / (uint32_t)A.G) + 2 * j / (uint32_t)A.G;
+    const double s = read_any(A.scale, g, A.scale_dtype);
+    const int z = A.zero ? A.zero[g] : 8, b = A.w[n * (A.K / 2) + j];
+    sum = __builtin_fma(s * (double)((b & 15) - z), (double)read_any(A.x, t * A.xs + 2 * j, A.x_dtype), sum);
+    sum = __builtin_fma(s * (double)((b >> 4) - z), (double)read_any(A.x, t * A.xs + 2 * j + 1, A.x_dtype), sum);
+  }
+  for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m, 64);
+  return (float)sum;
+}
+
 // Any types and groups: a wavefront a row of the weight and up to eight rows of x, a byte (two values) a lane at a time. Float and
 // integer instructions bound it, two products and an address a value and row: 16 rows, 28672 x 4096: 0.85 ms in f32, 1.06 in bf16
 // with groups of 16 (with the group divided for in 64 bits 1.14 and 1.52).
@@ -53,6 +68,7 @@ __global__ void __launch_bounds__(256) int4_matmul_any_kernel(const Int4Args A) 
 #pragma unroll
     for (int r = 0; r < ANY_ROWS; ++r) {
       for (int x = 32; x; x >>= 1) acc[r] += __shfl_xor(acc[r], x, 64);
+      if (t0 + r < A.T && !int4_finite(acc[r])) acc[r] = any_again(A, t0 + r, n);
       if (lane == 0 && t0 + r < A.T) write_any(A.y, (t0 + r) * A.N + n, A.y_dtype, acc[r]);
     }
   }
@@ -372,6 +388,7 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
     }
   }
   int turn = 0;
+  uint64_t odd = 0;  // whether a sum of the tiles that this wavefront has finished is not finite
   auto forward = [&]() {  // has the next step loaded and waits for the oldest
     if (ahead.tile < tiles) {
       fetch(to);
@@ -421,6 +438,7 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
       for (int j = 0; j < 4; ++j) sum += v[j];
     }
     const int n = tile * 16 + l16;
+    odd |= __ballot(!int4_finite(sum[0]) || !int4_finite(sum[1]) || !int4_finite(sum[2]) || !int4_finite(sum[3]));
     if (n >= N) continue;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -429,6 +447,14 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
       if (A.y_dtype == DT_F32) ((float*)A.y)[(int64_t)t * N + n] = sum[r];
       else ((uint16_t*)A.y)[(int64_t)t * N + n] = X::put(sum[r]);
     }
+  }
+  if (!odd) return;
+  turn = 0;
+#pragma unroll 1
+  for (int tile = blockIdx.x; tile < tiles; tile += (int)gridDim.x, ++turn) {
+    if (wave != turn % W) continue;
+#pragma unroll 1
+    for (int t = 4 * g16; t < 4 * g16 + 4; ++t) int4_mend_stored<X>(A, t < T && tile * 16 + l16 < N, t, tile * 16 + l16);
   }
 }
 

@@ -337,11 +337,24 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
   float* const rows_at = (float*)smem;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
+    const int t_here = min(32, x_rows - t0 - 32 * m);
+    bool odd = false;
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) rows_at[(8 * (e >> 2) + 4 * half + (e & 3)) * C::YP + 32 * wave + l32] = y[m][e];
+    for (int e = 0; e < 16; ++e) {
+      rows_at[(8 * (e >> 2) + 4 * half + (e & 3)) * C::YP + 32 * wave + l32] = y[m][e];
+      odd |= !int4_finite(y[m][e]);
+    }
+    if (whole && __any(odd)) {
+      // (two rows of the wavefront's own columns at a time; parts are looked at when they are added)
+#pragma unroll 1
+      for (int r = half; r < 32; r += 2) {
+        float* const at = rows_at + r * C::YP + 32 * wave + l32;
+        const int c = 32 * wave + l32;
+        *at = int4_mend<X>(A, !int4_finite(*at) && r < t_here && c < n_here, t_base + t0 + 32 * m + r, n0 + c, *at);
+      }
+    }
     __syncthreads();
-    const int t_here = min(32, x_rows - t0 - 32 * m);
     char* const to = out + ((int64_t)32 * m * A.N + n0) * ys;
     if (wide) {
       const int chunks = BN / per;
@@ -376,10 +389,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
 template <class X>
 __global__ void __launch_bounds__(256) int4_join_kernel(const Int4Args A, const float* parts, int64_t at, int64_t count) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= count) return;
+  if (i - 4 * (threadIdx.x & 63) >= count) return;  // (whole wavefronts)
   f32x4p v = {0.f, 0.f, 0.f, 0.f};
+  if (i < count) {
 #pragma unroll 8
-  for (int p = 0; p < A.parts; ++p) v += *(const f32x4p*)(parts + p * part_floats(count) + i);
+    for (int p = 0; p < A.parts; ++p) v += *(const f32x4p*)(parts + p * part_floats(count) + i);
+  }
   if (count - i >= 4) {
     if (A.y_dtype == DT_F32) *(f32x4p*)((float*)A.y + at + i) = v;
     else *(uint2*)((uint16_t*)A.y + at + i) = uint2{X::put(v[0]) | (uint32_t)X::put(v[1]) << 16, X::put(v[2]) | (uint32_t)X::put(v[3]) << 16};
@@ -388,6 +403,12 @@ __global__ void __launch_bounds__(256) int4_join_kernel(const Int4Args A, const 
       if (A.y_dtype == DT_F32) ((float*)A.y)[at + i + e] = v[e];
       else ((uint16_t*)A.y)[at + i + e] = X::put(v[e]);
     }
+  }
+  if (!__any(!int4_finite(v[0]) || !int4_finite(v[1]) || !int4_finite(v[2]) || !int4_finite(v[3]))) return;
+#pragma unroll 1
+  for (int e = 0; e < 4; ++e) {
+    const int64_t t = (at + i + e) / A.N;
+    int4_mend_stored<X>(A, i + e < count, t, at + i + e - t * A.N);
   }
 }
 

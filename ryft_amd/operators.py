@@ -39,8 +39,8 @@ are one of bf16, f16, f32):
   starts do not decrease.
 * ``ryft.int4_matmul`` (x [T,K], weight [N,K/2] ui8, scale [N,K/G] (, zero [N,K/G] ui8)) → y [T,N]. Value k of a row of
   the weight is the low (k even) or high four bits of its byte k / 2, less its group's zero (8 without the operand), times
-  its group's scale; groups are G consecutive values, G even. y = x · weightᵀ, summed in 32 bits. scale and y are of x's
-  type or f32.
+  its group's scale; groups are G consecutive values, G even. y = x · weightᵀ, summed in 32 bits, in 64 where that is not
+  finite. scale and y are of x's type or f32.
 
 The caches are results as well as operands. With `tf.aliasing_output` on the parameters (the modules below have it) and a
 donated argument, or the same address as parameter and result of `execute_into`, only the new tokens are written;

@@ -1,0 +1,118 @@
+"""The operators that verify drafted tokens on the GPU at the ends of what their definitions allow: infinities, sums that
+leave f32's range on the way, calls without tokens, starts that are no starts.
+
+int4_matmul's sums carry a bias of 16 beside each value, so that an infinity of x, or a large finite one, can make them
+infinite or NaN where the definition is not; such results are summed again in 64 bits. Where the definition is infinite or
+NaN the results are that exactly. Finite results: `int4_error` and half a step of the type, as in test_gpu_verify.py; results
+summed again are nearer (64 bits, rounded to f32 and to the type)."""
+import numpy as np
+import pytest
+import torch  # (before the plugin: both then use one HIP runtime)
+
+from oracle import operators as oo
+from tests import operator_programs as op
+from tests import verify_programs as vp
+from tests.test_gpu_operators import close, run
+
+pytestmark = pytest.mark.gpu
+
+# one of each way through the kernels: rows through the ring and in registers, with more tiles than workgroups, tiles in one
+# range of K and in several, results of a number that is no multiple of four, and the kernel for any type and group
+PATHS = {
+    "one": (1, 512, 40, 128, "bf16"),
+    "ring": (5, 4096, 70, 64, "f16"),
+    "registers": (16, 512, 4100, 32, "bf16"),
+    "registers_4": (3, 8192, 4200, 128, "bf16"),
+    "more_tiles": (2, 256, 8230, 64, "bf16"),
+    "tile": (70, 256, 300, 128, "bf16"),
+    "tile_f16": (70, 256, 301, 32, "f16"),
+    "tiles_of_128": (300, 160, 3000, 32, "bf16"),
+    "parts": (40, 4096, 257, 128, "bf16"),
+    "parts_odd": (33, 2080, 71, 32, "f16"),
+    "other_groups": (20, 480, 33, 48, "bf16"),
+    "f32": (20, 512, 33, 64, "f32"),
+}
+
+
+def definition(x):
+    with np.errstate(invalid="ignore", over="ignore"):
+        return oo.int4_matmul(x, {})[0]
+
+
+@pytest.mark.parametrize("zeros", [False, True], ids=["eight", "zeros"])
+@pytest.mark.parametrize("out", ["f32", "same"])
+@pytest.mark.parametrize("name", PATHS)
+def test_int4_matmul_of_infinities(gpu_client, name, out, zeros):
+    # an infinity is ±inf by the sign of its weight, NaN where that is zero or another infinity has the other sign
+    rows, inner, columns, group, dtype = PATHS[name]
+    out = dtype if out == "same" else out
+    module, ins = vp.int4_case(rows, inner, columns, group, dtype, zeros=zeros, out_dtype=out, seed=rows + inner)
+    x = vp.values(ins)
+    x[0][0, 7] = np.inf
+    if rows > 1:
+        x[0][rows - 1, inner - 1] = -np.inf
+    if rows > 2:
+        x[0][1, 3], x[0][1, inner - 2] = np.inf, -np.inf
+    if rows > 4:
+        x[0][2, inner // 2], x[0][3, 0], x[0][3, 1] = np.nan, np.inf, np.nan
+    if rows > 16:
+        x[0][16:rows:9, inner // 3] = np.inf
+    ins[0] = op.host(x[0], dtype)
+    (got,), _ = run(gpu_client, module, ins, [out])
+    want = definition(vp.values(ins))
+    odd = ~np.isfinite(x[0]).all(axis=1)
+    assert np.isinf(want[0]).any() and (np.isnan(want[0]).any() or columns < 50)
+    assert np.array_equal(got[odd], want[odd], equal_nan=True)
+    close(got[~odd], want[~odd], out, vp.int4_error([x[0][~odd], *x[1:]]) + 2.0 ** -25, "others")
+
+
+@pytest.mark.parametrize("power", [108, 114, 120, 125])
+@pytest.mark.parametrize("name", [n for n in PATHS if PATHS[n][4] != "f16"])
+def test_int4_matmul_of_the_largest_values(gpu_client, name, power):
+    # zero points up to 255 and values up to 2^127: sums of (16 + z) x pass f32's range, results are around 2^(power - 20)
+    rows, inner, columns, group, dtype = PATHS[name]
+    module, ins = vp.int4_case(rows, inner, columns, group, dtype, zeros=True, scale_dtype="f32", out_dtype="f32", seed=power + rows)
+    r = np.random.RandomState(power)
+    ins[0] = op.host(r.uniform(-3.9, 3.9, (rows, inner)) * 2.0 ** power, dtype)
+    ins[2] = op.host(r.uniform(0.5, 1, ins[2].dims) * 2.0 ** -35, "f32")
+    ins[3] = vp.host(r.randint(0, 256, ins[3].dims), "ui8")
+    (got,), _ = run(gpu_client, module, ins, ["f32"])
+    x = vp.values(ins)
+    want = definition(x)
+    assert np.isfinite(want.astype(np.float32)).all()
+    close(got, want, "f32", vp.int4_error(x), "y")
+
+
+@pytest.mark.parametrize("name", [n for n in PATHS if PATHS[n][4] != "f16"])
+def test_int4_matmul_of_sums_that_come_back(gpu_client, name):
+    # the second half of a row takes off what the first has put beyond f32's largest value: what is left is one value of x, a
+    # power of two, times the column's number, exactly
+    rows, inner, columns, group, dtype = PATHS[name]
+    half = inner // 2 // group * group
+    module, ins = vp.int4_case(rows, inner, columns, group, dtype, out_dtype="f32", scale_dtype="f32", seed=2)
+    x, q = np.zeros((rows, inner)), np.full((columns, inner), 8)
+    x[:, :half] = 2.0 ** 127
+    x[:, half:2 * half] = -2.0 ** 127
+    x[:, half] = -2.0 ** 120
+    q[:, :2 * half] = 11
+    q[:, 0], q[:, half] = 8, 8 + np.arange(columns) % 8
+    ins[0] = op.host(x, dtype)
+    ins[1] = vp.host(q[:, 0::2] | q[:, 1::2] << 4, "ui8")
+    ins[2] = op.host(np.ones(ins[2].dims), "f32")
+    (got,), _ = run(gpu_client, module, ins, ["f32"])
+    assert np.array_equal(got, np.broadcast_to(-2.0 ** 120 * (np.arange(columns) % 8), got.shape))
+
+
+@pytest.mark.parametrize("name", PATHS)
+def test_int4_matmul_of_scales_that_are_not_finite(gpu_client, name):
+    rows, inner, columns, group, dtype = PATHS[name]
+    module, ins = vp.int4_case(rows, inner, columns, group, dtype, scale_dtype="f32", out_dtype="f32", seed=9)
+    x = vp.values(ins)
+    groups = inner // group
+    x[2][3, groups - 1], x[2][columns - 1, 0], x[2][20, groups // 2] = np.nan, np.inf, -np.inf
+    ins[2] = op.host(x[2], "f32")
+    (got,), _ = run(gpu_client, module, ins, ["f32"])
+    want = definition(x)
+    odd = ~np.isfinite(x[2]).all(axis=1)
+    assert odd.sum() == 3 and np.array_equal(got[:, odd], want[:, odd], equal_nan=True)
+    close(got[:, ~odd], want[:, ~odd], "f32", vp.int4_error([x[0], x[1][~odd], x[2][~odd]]), "others")
