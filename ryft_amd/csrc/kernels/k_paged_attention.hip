@@ -662,8 +662,8 @@ void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counter
 void launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream, hipEvent_t done) {
   if (a.D < 1 || a.D > 256 || a.Hkv < 1 || a.Hq < 1 || a.Hq > 65535 || a.Hq % a.Hkv || a.P < 1)
     fail(PJRT_Error_Code_INTERNAL, "paged_attention of a shape the kernels do not take");
+  if (a.T == 0) return record_done(done, stream);  // (the mask of no tokens has the address 0)
   if (a.W && (!a.visible || a.causal || a.slopes)) fail(PJRT_Error_Code_INTERNAL, "tree_attention without its mask, or with another");
-  if (a.T == 0) return record_done(done, stream);
   if (a.tile_rows) {
     if (a.groups < 1 || (a.tile_rows != kPromptRows && (!a.ws || !a.counters))) fail(PJRT_Error_Code_INTERNAL, "paged_attention without a workspace");
     if (a.dtype == DT_BF16) launch_matrix<MmaBF16, ElemBF16>(a, stream, done);

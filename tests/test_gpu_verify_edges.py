@@ -10,6 +10,7 @@ import pytest
 import torch  # (before the plugin: both then use one HIP runtime)
 
 from oracle import operators as oo
+from ryft_amd import operators, pjrt
 from tests import operator_programs as op
 from tests import verify_programs as vp
 from tests.test_gpu_operators import close, run
@@ -116,3 +117,42 @@ def test_int4_matmul_of_scales_that_are_not_finite(gpu_client, name):
     odd = ~np.isfinite(x[2]).all(axis=1)
     assert odd.sum() == 3 and np.array_equal(got[:, odd], want[:, odd], equal_nan=True)
     close(got[:, ~odd], want[:, ~odd], "f32", vp.int4_error([x[0], x[1][~odd], x[2][~odd]]), "others")
+
+
+# ------------------------------------------------------------------------------------------------ no tokens
+def empty_modules():
+    tree = operators.tree_attention_module(tokens=0, sequences=3, q_heads=4, kv_heads=2, head_dim=64, pages=5, page_size=16,
+                                           pages_per_sequence=4, words=2, scale=0.125)
+    accept = operators.tree_accept_module(tokens=0, sequences=3, caches=2, pages=5, kv_heads=2, page_size=16, head_dim=64)
+    int4 = operators.int4_matmul_module(rows=0, inner=64, columns=10, group=32)
+    cache = ((5, 2, 16, 64), "bf16")
+    words = lambda *shape: (shape, "i32")  # noqa: E731
+    return {
+        "tree_attention": (tree, [((0, 4, 64), "bf16"), cache, cache, words(3, 4), words(4), words(3), words(0, 2)],
+                           [((0, 4, 64), "bf16")]),
+        "tree_accept": (accept, [words(0)] * 4 + [words(4), cache, cache], [words(3), words(0), words(0), cache, cache]),
+        "int4_matmul": (int4, [((0, 64), "bf16"), ((10, 32), "ui8"), ((10, 2), "bf16")], [((0, 10), "bf16")]),
+    }
+
+
+@pytest.mark.parametrize("into", [False, True], ids=["execute", "execute_into"])
+@pytest.mark.parametrize("name", ["tree_attention", "tree_accept", "int4_matmul"])
+def test_no_tokens(gpu_client, name, into):
+    # a tensor of no elements has the address 0
+    module, ins, outs = empty_modules()[name]
+    kind = {"bf16": torch.bfloat16, "i32": torch.int32, "ui8": torch.uint8}
+    given = [torch.ones(s, dtype=kind[t], device="cuda") if t == "bf16" else torch.zeros(s, dtype=kind[t], device="cuda") for s, t in ins]
+    if not into:
+        host = [vp.host(g.cpu().float().numpy(), t) for g, (_, t) in zip(given, ins)]
+        got, _ = run(gpu_client, module, host, [t for _, t in outs])
+    else:
+        exe = gpu_client.compile(pjrt.Program.mlir(module))
+        made = [torch.full(s, 7, dtype=kind[t], device="cuda") for s, t in outs]
+        assert given[0].data_ptr() == 0
+        exe.execute_into([(g.data_ptr(), g.nbytes) for g in given], [(m.data_ptr(), m.nbytes) for m in made],
+                         torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        got = [m.cpu().float().numpy() for m in made]
+    assert [g.shape for g in got] == [s for s, _ in outs]
+    if name == "tree_accept":
+        assert not got[0].any() and all((g == 1).all() for g in got[3:])
