@@ -150,7 +150,7 @@ __device__ __forceinline__ void int4_mend_stored(const Int4Args& A, bool mine, i
 }
 
 // k_int4_tile.hip
-void int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats);
+bool int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats);  // false: not with that workspace
 void launch_int4_tile(const Int4Args& a, hipStream_t stream, hipEvent_t done);
 
 }  // namespace ryft

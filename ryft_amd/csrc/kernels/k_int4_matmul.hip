@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) int4_matmul_any_kernel(const Int4Args A) 
   }
 }
 
-// ------------------------------------------------------------------------------------------------ up to 16 rows of x
+// ------------------------------------------------------------------------------------------------ 16 rows of x at a time
 // bf16 and f16, groups of a multiple of 32: the weight's bytes bound it. A workgroup takes tiles of 16 rows of the weight, one
 // after the other; its wavefronts take every W-th step of 256 values, and meet in LDS at the tile's end, in one order.
 //
@@ -464,7 +464,14 @@ void launch_few_of(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
   const hipError_t e = hipFuncSetAttribute((const void*)int4_few_kernel<X, SPAN, XL, S>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
   if (e != hipSuccess) fail(PJRT_Error_Code_INTERNAL, std::string("int4_matmul LDS attribute: ") + hipGetErrorString(e));
   const dim3 grid((unsigned)std::min<int64_t>((a.N + 15) / 16, C::SHARES * CUS));
-  launch_k(done, int4_few_kernel<X, SPAN, XL, S>, grid, dim3(64 * C::W), C::LDS, stream, a);
+  const int ys = a.y_dtype == DT_F32 ? 4 : 2;
+  for (int64_t t0 = 0; t0 < a.T; t0 += 16) {
+    Int4Args b = a;
+    b.x = (const char*)a.x + t0 * a.xs * 2;
+    b.y = (char*)a.y + t0 * a.N * ys;
+    b.T = std::min<int64_t>(16, a.T - t0);
+    launch_k(t0 + 16 >= a.T ? done : nullptr, int4_few_kernel<X, SPAN, XL, S>, grid, dim3(64 * C::W), C::LDS, stream, b);
+  }
 }
 template <class X, int SPAN>
 void launch_few_span(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
@@ -506,7 +513,9 @@ void int4_matmul_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   // (16 rows, 4096 x 28672: 20.5 us, with tiles 30; 14336 x 4096: 16.7 and 24; 4096 x 4096: 7.2 and 15. From 17 rows on a
   // second pass over the weight would be needed.)
   if (a.T <= 16) return few_plan(a);
-  int4_tile_plan(a, room, ws_floats);
+  // Rows too long for tiles in that workspace go 16 at a time: 32 rows of 2^20 values take 71 MB or more, 17 of 2^22 151 or more,
+  // and the scratch of allocation-free executions is 64 MiB.
+  if (!int4_tile_plan(a, room, ws_floats)) few_plan(a);
 }
 
 void launch_int4_matmul(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
@@ -514,7 +523,6 @@ void launch_int4_matmul(const Int4Args& a, hipStream_t stream, hipEvent_t done) 
     fail(PJRT_Error_Code_INTERNAL, "int4_matmul of a shape the kernels do not take");
   if (a.T == 0) return record_done(done, stream);
   if (a.kernel == INT4_FEW) {
-    if (a.T > 16) fail(PJRT_Error_Code_INTERNAL, "int4_matmul's kernel for few rows with many");
     if (a.x_dtype == DT_BF16) launch_few<Int4BF16>(a, stream, done);
     else launch_few<Int4F16>(a, stream, done);
   } else if (a.kernel == INT4_TILE) {

@@ -446,15 +446,19 @@ void launch_type(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
 
 }  // namespace
 
-void int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
+bool int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   const int64_t stages = (a.K + STAGE - 1) / STAGE;
   a.steps = (int32_t)stages;
   // Rows at a time: equal shares, in whole tiles, of at most 32 MiB (838 rows of 13248 values against 3518 rows, once 768 and 70 at
   // a time: 226 us).
   const int64_t row = stages * (STAGE * 2 + STAGE / a.span * 16);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(32ll << 20, room) / (row * MOST_ROWS)) * MOST_ROWS;
+  int64_t most = std::max<int64_t>(1, std::min<int64_t>(32ll << 20, room) / (row * MOST_ROWS)) * MOST_ROWS, unit = MOST_ROWS;
+  if (tile_ws_bytes(stages, std::min(a.T, most), a.span) > room) {  // (fewer rows than the highest tile has)
+    most = (room - tile_ws_bytes(stages, 0, a.span)) / row / 32 * 32, unit = 32;
+    if (most < 32) return false;
+  }
   const int64_t goes = (a.T + most - 1) / most, each = (a.T + goes - 1) / goes;
-  const int64_t rows = std::min(a.T, (each + MOST_ROWS - 1) / MOST_ROWS * MOST_ROWS);
+  const int64_t rows = std::min(a.T, (each + unit - 1) / unit * unit);
   const int64_t x_bytes = tile_ws_bytes(stages, rows, a.span), part = 4 * part_floats(rows * a.N);
   // Tile and ranges of K by what they are estimated to take, in us: 4 for the launch, 3 for a tile's way to its stages and from
   // them, a stage's time by rows of the tile and values of a span (2048 rows against 12288 x 4096: 219, 267 and 389 us with 128, 64
@@ -463,7 +467,7 @@ void int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   // against 13226 x 1472 in spans of 64 34, 27, 37 and 33, 27, 38; 373 against 940 x 9216 27, 26, 27 and 24, 24, 27; 100 against
   // 8192 x 608 in spans of 32 24, 18, 15 and 20, 13, 12.
   static constexpr double STAGE_US[3][3] = {{0.95, 1.37, 2.2}, {1.13, 1.65, 2.6}, {1.5, 2.1, 3.3}};
-  if (stages > 65535 || rows * ((a.N + 31) / 32) >= INT32_MAX) return;  // (the grids' limits)
+  if (stages > 65535 || rows * ((a.N + 31) / 32) >= INT32_MAX) return false;  // (the grids' limits)
   double best = 1e30;
   for (int tile = 1; tile <= 4; tile *= 2) {
     const double stage = STAGE_US[a.span == 128 ? 0 : a.span == 64 ? 1 : 2][tile / 2];
@@ -477,6 +481,7 @@ void int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   a.kernel = INT4_TILE;
   a.rows = (int32_t)rows;
   *ws_floats = (x_bytes + (a.parts > 1 ? a.parts * part : 0)) / 4;
+  return true;
 }
 
 void launch_int4_tile(const Int4Args& a, hipStream_t stream, hipEvent_t done) {

@@ -63,7 +63,7 @@ int attention_plan_splits(const AttnArgs& a);
 // Chooses the kernel of a paged_attention and its split from the sizes (the operands' pointers are not looked at):
 // floats of workspace and zeroed counters that its launch needs.
 void paged_attention_plan(PagedAttnArgs& a, int64_t* ws_floats, int64_t* counters);
-// The kernel of an int4_matmul and its split, with at most `room` bytes of workspace, more only where a tile's rows need it:
+// The kernel of an int4_matmul and its split, with at most `room` bytes of workspace:
 // floats of workspace that its launches need.
 void int4_matmul_plan(Int4Args& a, int64_t room, int64_t* ws_floats);
 // The split of a sample: bytes of workspace that its launches need.

@@ -156,3 +156,36 @@ def test_no_tokens(gpu_client, name, into):
     assert [g.shape for g in got] == [s for s, _ in outs]
     if name == "tree_accept":
         assert not got[0].any() and all((g == 1).all() for g in got[3:])
+
+
+# ------------------------------------------------------------------------------------------------ the longest rows
+@pytest.mark.parametrize("rows, inner, columns, group", [(40, 1 << 20, 20, 128), (33, (1 << 20) + 2080, 7, 32)])
+def test_int4_matmul_of_long_rows(gpu_client, rows, inner, columns, group):
+    # rows too long for tiles in the scratch of allocation-free executions; as exact as whole numbers below 2^24 are
+    module, ins = vp.int4_case(rows, inner, columns, group, "bf16", zeros=True, out_dtype="f32", exact=True, seed=rows)
+    given = [torch.from_numpy(np.array(i.data).view(np.int16 if i.data.dtype == np.uint16 else i.data.dtype)).cuda() for i in ins]
+    y = torch.full((rows, columns), 7.0, device="cuda")
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    assert " few" in exe.describe_plan()
+    exe.execute_into([(g.data_ptr(), g.nbytes) for g in given], [(y.data_ptr(), y.nbytes)], torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert np.array_equal(y.double().cpu().numpy(), oo.int4_matmul(vp.values(ins), {})[0])
+
+
+def test_int4_matmul_of_the_longest_rows(gpu_client):
+    rows, inner, columns = 17, 1 << 22, 33
+    weight = torch.full((columns, inner // 2), 0x88, dtype=torch.uint8, device="cuda")
+    weight[::4, -1] = 0x98                                            # the last value 1, the others 0
+    weight[1::4] = 0x89                                               # 1, 0, 1, 0, ...
+    x = torch.arange(1, rows + 1, device="cuda").bfloat16()[:, None].expand(rows, inner).contiguous()
+    x[:, -1] = 5
+    scale = torch.full((columns, inner // 32), 0.5, dtype=torch.bfloat16, device="cuda")
+    y = torch.full((rows, columns), 7.0, device="cuda")
+    exe = gpu_client.compile(pjrt.Program.mlir(operators.int4_matmul_module(rows=rows, inner=inner, columns=columns, group=32, out_dtype="f32")))
+    exe.execute_into([(g.data_ptr(), g.nbytes) for g in (x, weight, scale)], [(y.data_ptr(), y.nbytes)],
+                     torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want = torch.zeros_like(y)
+    want[:, ::4] = 2.5
+    want[:, 1::4] = torch.arange(1, rows + 1, device="cuda").float()[:, None] * (inner // 4)
+    assert torch.equal(y, want)
