@@ -450,9 +450,9 @@ bool int4_tile_plan(Int4Args& a, int64_t room, int64_t* ws_floats) {
   const int64_t stages = (a.K + STAGE - 1) / STAGE;
   a.steps = (int32_t)stages;
   // Rows at a time: equal shares, in whole tiles, of at most 32 MiB (838 rows of 13248 values against 3518 rows, once 768 and 70 at
-  // a time: 226 us).
+  // a time: 226 us) and half of the room: parts may take as much (a tile of 128 KiB for each of 256 workgroups).
   const int64_t row = stages * (STAGE * 2 + STAGE / a.span * 16);
-  int64_t most = std::max<int64_t>(1, std::min<int64_t>(32ll << 20, room) / (row * MOST_ROWS)) * MOST_ROWS, unit = MOST_ROWS;
+  int64_t most = std::max<int64_t>(1, std::min<int64_t>(32ll << 20, room / 2) / (row * MOST_ROWS)) * MOST_ROWS, unit = MOST_ROWS;
   if (tile_ws_bytes(stages, std::min(a.T, most), a.span) > room) {  // (fewer rows than the highest tile has)
     most = (room - tile_ws_bytes(stages, 0, a.span)) / row / 32 * 32, unit = 32;
     if (most < 32) return false;

@@ -181,7 +181,7 @@ class Planner {
   int updated_operand(int operand, int out);
   int place_of(int result);
   bool depends_on(int from, int what) const;
-  int shared_workspace(int64_t bytes);
+  int shared_workspace(int64_t bytes, bool int4 = false);
   int shared_counters(int64_t count);
   void push_window_step(const char* name, int mode, int src, int dst, const std::vector<int>& idx,
                         const TensorType& big, const std::vector<int64_t>& win, DType idx_dtype);
@@ -203,6 +203,7 @@ class Planner {
   Plan plan_;
   std::map<int, int> mat_;  // node → slot holding it contiguously (row-major)
   int workspace_ = -1, counters_ = -1;  // slots that the operators' steps share
+  int64_t fixed_workspace_ = 0;         // bytes of it that they cannot do without
 };
 
 // ------------------------------------------------------------------------------------------------ ExprBuilder
@@ -884,11 +885,16 @@ View Planner::row_view(int node) {
   return v;
 }
 
-// The workspace of the operators' steps, which run one after the other: one slot, as large as the largest needs.
-int Planner::shared_workspace(int64_t bytes) {
+// The workspace of the operators' steps, which run one after the other: one slot, as large as the largest needs. int4: a
+// product's with 4-bit weights, which could do with less.
+int Planner::shared_workspace(int64_t bytes, bool int4) {
   if (workspace_ < 0) workspace_ = new_slot(Slot::TEMP, TensorType{DType::U8, {0}});
   int64_t& n = plan_.slots[workspace_].type.shape[0];
   n = std::max(n, bytes);
+  if (!int4) fixed_workspace_ = std::max(fixed_workspace_, bytes);
+  const auto whole = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
+  plan_.workspace_bytes = whole(n);
+  plan_.int4_bytes = whole(n) - whole(fixed_workspace_);
   return workspace_;
 }
 // Their arrival counters: part of the executable, zeroed once when it is loaded; each launch leaves them at zero.
@@ -1017,7 +1023,7 @@ void Planner::emit_custom_call(int node, int target) {
     st.patches.push_back({offsetof(Int4Args, y), out_slot(0)});
     int64_t ws = 0;
     int4_matmul_plan(a, opts_.int4_workspace, &ws);
-    if (ws) st.patches.push_back({offsetof(Int4Args, ws), shared_workspace(4 * ws)});
+    if (ws) st.patches.push_back({offsetof(Int4Args, ws), shared_workspace(4 * ws, true)});
     st.bytes = (double)(x.bytes() + w.bytes() + s.bytes() + y.bytes()) + (n.operands.size() == 4 ? (double)type(3).bytes() : 0.0);
     st.flops = 2.0 * (double)a.T * (double)a.N * (double)a.K;
   } else if (n.call_target == "ryft.tree_accept") {
@@ -2755,29 +2761,30 @@ size_t Plan::temp_bytes() const {
   return n;
 }
 
-Plan build_plan(const Graph& g, const PlanOptions& asked) {
-  PlanOptions opts = asked;
+// A plan whose temporaries pass the allocation-free scratch is made again where less of them would do: edge GEMMs and
+// products with 4-bit weights are split as is estimated fastest, but can do with fewer partial sums, the latter also with
+// fewer rows at a time. A plan that does not fit in the end stays as it was: only executions that allocate run it.
+Plan build_plan(const Graph& g, const PlanOptions& opts) {
   Plan plan = Planner(g, opts).run();
-  // A plan that does not fit the allocation-free scratch gives products with 4-bit weights less of it: their rows go through it
-  // in more goes, and K in fewer ranges (1024 rows against 14336 x 4096 in f32 with 58.7 MB of other temporaries).
-  for (const int64_t room : {16ll << 20, 4ll << 20}) {
-    const auto tiles = [](const Step& st) { return st.kind == Step::INT4_MATMUL && st.int4.kernel == INT4_TILE; };
-    if (plan.temp_bytes() <= kNoAllocScratchBytes || std::none_of(plan.steps.begin(), plan.steps.end(), tiles)) break;
-    opts.int4_workspace = std::min(asked.int4_workspace, (int64_t)room);
-    Plan p = Planner(g, opts).run();
-    if (p.temp_bytes() < plan.temp_bytes()) plan = std::move(p);
-  }
-  // Edge GEMMs take the number of K ranges that is estimated fastest. Where it is their partial sums that would keep the
-  // plan from the allocation-free scratch, they get as many as leave it room, down to none: 16 products of 2432 × 11520 ×
-  // 128 need no temporaries unsplit (152 µs), 76 MiB in the 4 ranges estimated (125).
-  const size_t need = plan.temp_bytes(), partials = (size_t)plan.edge_partial_bytes;
-  if (need <= kNoAllocScratchBytes || need - partials > kNoAllocScratchBytes) return plan;
-  for (int64_t room = (int64_t)(kNoAllocScratchBytes - (need - partials)); ; room = room > 1 << 20 ? room / 2 : 0) {
-    PlanOptions tight = opts;
+  constexpr int64_t kLimit = (int64_t)kNoAllocScratchBytes;
+  const int64_t need = (int64_t)plan.temp_bytes(), fixed = need - plan.edge_partial_bytes - plan.int4_bytes;
+  if (need <= kLimit || fixed > kLimit) return plan;
+  // First products with 4-bit weights get what the others leave (256 rows against 14336 x 4096 beside 29 MB: ranges of K for 38
+  // MB); then edge GEMMs as many partial sums as leave room, down to none: 16 products of 2432 × 11520 × 128 need no
+  // temporaries unsplit (152 µs), 76 MiB in the 4 ranges estimated (125).
+  PlanOptions tight = opts;
+  for (int64_t room = plan.int4_bytes ? INT64_MAX : kLimit - fixed;;
+       room = room == INT64_MAX ? kLimit - fixed : room > 1 << 20 ? room / 2 : 0) {
     tight.edge_partials = std::min(opts.edge_partials, room);
+    tight.int4_workspace = opts.int4_workspace;
     Plan p = Planner(g, tight).run();
-    if (p.temp_bytes() <= kNoAllocScratchBytes) return p;
-    if (room == 0) return plan;
+    const int64_t others = (int64_t)p.temp_bytes() - p.workspace_bytes;
+    if ((int64_t)p.temp_bytes() > kLimit && p.int4_bytes && others < kLimit) {
+      tight.int4_workspace = std::min(opts.int4_workspace, kLimit - others);
+      p = Planner(g, tight).run();
+    }
+    if ((int64_t)p.temp_bytes() <= kLimit) return p;
+    if (room == 0 || !plan.edge_partial_bytes) return plan;
   }
 }
 

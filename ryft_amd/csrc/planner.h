@@ -78,6 +78,7 @@ struct Plan {
   std::vector<bool> output_in_place;
   double total_flops = 0, total_bytes = 0;
   int64_t edge_partial_bytes = 0;  // temporaries that hold the partial sums of split edge GEMMs
+  int64_t workspace_bytes = 0, int4_bytes = 0;  // the operators' workspace; what products with 4-bit weights alone ask of it
   // Device memory of the temporaries, each at a 256-byte aligned offset (the alignment the steps assume of a slot).
   size_t temp_bytes() const;
   std::string describe() const;
