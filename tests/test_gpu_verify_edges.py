@@ -13,7 +13,7 @@ from oracle import operators as oo
 from ryft_amd import operators, pjrt
 from tests import operator_programs as op
 from tests import verify_programs as vp
-from tests.test_gpu_operators import close, run
+from tests.test_gpu_operators import attention_error, close, run
 
 pytestmark = pytest.mark.gpu
 
@@ -156,6 +156,83 @@ def test_no_tokens(gpu_client, name, into):
     assert [g.shape for g in got] == [s for s, _ in outs]
     if name == "tree_accept":
         assert not got[0].any() and all((g == 1).all() for g in got[3:])
+
+
+# ------------------------------------------------------------------------------------------------ starts that are no starts
+def guarded(shape, dtype, value):
+    """A tensor between 64 KiB that no one may write, and what checks that."""
+    n = int(np.prod(shape)) * torch.empty((), dtype=dtype).element_size()
+    room = -(-n // 256) * 256
+    whole = torch.full((room + (1 << 17),), 0x5A, dtype=torch.uint8, device="cuda")
+    inner = whole[1 << 16:(1 << 16) + n].view(dtype).reshape(shape)
+    inner.copy_(value)
+    return inner, lambda: bool((whole[:1 << 16] == 0x5A).all() and (whole[(1 << 16) + n:] == 0x5A).all())
+
+
+BAD_STARTS = [
+    ([-5, 30, 20, 60], True),                      # (0 to 30, none, 20 to 60: the last two share rows)
+    ([60, 0, 60, 0], False), ([0, 20, 20, 60], False), ([-2 ** 31, -1, -1, -1], False), ([61, 70, 2 ** 31 - 1, 60], False),
+    ([2 ** 31 - 1, 40, 40, 60], False), ([10, 20, 5, 2 ** 31 - 1], True),
+]
+
+
+@pytest.mark.parametrize("starts, shared", BAD_STARTS, ids=str)
+@pytest.mark.parametrize("page, heads, dtype", [(16, (2, 64), "bf16"), (5, (3, 7), "bf16"), (16, (1, 4), "f32")], ids=str)
+def test_tree_accept_of_any_starts(gpu_client, starts, shared, page, heads, dtype):
+    """What the definition gives where no row is in two sequences. Rows in two are written by both: counts are still those of
+    each sequence alone, the results are node numbers and targets of some sequence, or -1, and rows of no sequence are -1."""
+    module, ins = vp.accept_case([20, 20, 20], 2, *heads, page, dtype, vocab=1, wide=True, seed=2, bad_slots=page == 5)
+    ins[4] = op.host(starts, "i32")
+    x = vp.values(ins)
+    kind = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    words = lambda a: torch.from_numpy(np.asarray(a).astype(np.int32))  # noqa: E731
+    given = [guarded(a.shape, torch.int32, words(a)) for a in x[:5]] + \
+            [guarded(a.shape, kind, torch.from_numpy(a).to(kind)) for a in x[5:]]
+    made = [guarded(s, torch.int32, torch.tensor(77)) for s in ((3,), (60,), (60,))] + [guarded(a.shape, kind, torch.tensor(0)) for a in x[5:]]
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    exe.execute_into([(g.data_ptr(), g.nbytes) for g, _ in given], [(m.data_ptr(), m.nbytes) for m, _ in made],
+                     torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert all(whole() for _, whole in given + made)
+    for (g, _), a in zip(given, x):                                    # (operands are as they were)
+        assert np.array_equal(g.double().cpu().numpy(), a)
+    counts, emitted, path, *caches = (m.double().cpu().numpy() for m, _ in made)
+    want = oo.tree_accept(x, {})
+    assert np.array_equal(counts, want[0])
+    if not shared:
+        for got, w in zip((emitted, path, *caches), want[1:]):
+            assert np.array_equal(got, w)
+        return
+    clamped = np.clip(starts, 0, 60)
+    inside = [b for b in range(3) if clamped[b] < clamped[b + 1]]
+    rows = np.zeros(60, dtype=bool)
+    for b in inside:
+        rows[clamped[b]:clamped[b + 1]] = True
+    alone = [oo.tree_accept([*x[:4], np.array([clamped[b], clamped[b + 1]])], {}) for b in inside]
+    for got, k in ((emitted, 1), (path, 2)):
+        assert (got[~rows] == -1).all()
+        assert np.any([got == w[k] for w in alone] + [got == -1], axis=0).all()
+    named = {int(s) for s in x[3][rows]}
+    for got, before in zip(caches, x[5:]):
+        for slot in range(before.shape[0] * page):
+            if slot not in named:
+                assert np.array_equal(got[slot // page, :, slot % page], before[slot // page, :, slot % page]), slot
+
+
+@pytest.mark.parametrize("starts", [s for s, shared in BAD_STARTS if not shared], ids=str)
+@pytest.mark.parametrize("tokens, heads, dtype", [(15, (4, 2, 64), "bf16"), (60, (4, 2, 128), "f16"), (60, (2, 2, 64), "f32")], ids=str)
+def test_tree_attention_of_any_starts(gpu_client, starts, tokens, heads, dtype):
+    # starts do not decrease; where they do, a row's heads have what its sequence's range gives, or zeros (15 tokens, with starts
+    # of a quarter: the kernel for few rows, which gives zeros to all)
+    n = tokens // 3
+    module, ins = vp.tree_case([n, n, n], [300, 200, 90], *heads, 16, dtype, seed=4, masks="random", words=2)
+    ins[4] = op.host([s if abs(s) > 60 else s * tokens // 60 for s in starts], "i32")
+    (got,), _ = run(gpu_client, module, ins, [dtype])
+    x = vp.values(ins)
+    want, = oo.tree_attention(x, op.config_of(module))
+    zeros = ~got.any(axis=2) & (np.diff(starts) < 0).any()
+    close(got[~zeros], want[~zeros], dtype, attention_error(x, dtype), str(starts))
+    assert not got[~want.any(axis=(1, 2))].any()
 
 
 # ------------------------------------------------------------------------------------------------ the longest rows
