@@ -117,6 +117,12 @@ def int4_matmul(result: str, operands: Sequence[Tuple[str, str]], type: str) -> 
     return _call([result], "ryft.int4_matmul", operands, [type], [])
 
 
+def _groups(inner: int, group: int) -> int:
+    if group < 2 or group % 2 or inner % group:
+        raise ValueError(f"rows of {inner} values are not cut into groups of {group}: an even number that divides them is needed")
+    return inner // group
+
+
 def pack_int4(values: np.ndarray) -> np.ndarray:
     """Rows of whole numbers 0 to 15 as int4_matmul's weight: two to a byte, the first in the low four bits."""
     v = np.asarray(values)
@@ -209,7 +215,7 @@ def tree_accept_module(*, tokens: int, sequences: int, caches: int = 0, pages: i
 def int4_matmul_module(*, rows: int, inner: int, columns: int, group: int, dtype: str = "bf16", scale_dtype: Optional[str] = None,
                        out_dtype: Optional[str] = None, zeros: bool = False) -> str:
     """A module of one int4_matmul [rows, inner] x [columns, inner]: its operands are the parameters."""
-    y, g = _t((rows, columns), out_dtype or dtype), (columns, inner // group)
+    y, g = _t((rows, columns), out_dtype or dtype), (columns, _groups(inner, group))
     types = [_t((rows, inner), dtype), _t((columns, inner // 2), "ui8"), _t(g, scale_dtype or dtype)] + ([_t(g, "ui8")] if zeros else [])
     params = ", ".join(f"%arg{n}: {t}" for n, t in enumerate(types))
     call = int4_matmul("%0", [(f"%arg{n}", t) for n, t in enumerate(types)], y)
@@ -270,6 +276,8 @@ def decoder_module(*, tokens: int, sequences: int, vocab: int, layers: int, d_mo
     parameter `parents`, tree_accept over every layer's caches, whose results counts, emitted and path stand before the
     caches."""
     t, b, hd = tokens, sequences, head_dim
+    if tree_words < 0:
+        raise ValueError(f"masks of {tree_words} words")
     rows = t if tree_words else b  # of the sampler
     wide = (q_heads + 2 * kv_heads) * hd
     cache = (pages, kv_heads, page_size, hd)
@@ -284,7 +292,7 @@ def decoder_module(*, tokens: int, sequences: int, vocab: int, layers: int, d_mo
     def weight(name: str, k: int, n: int) -> List[Tuple[str, Tuple[int, ...], str]]:
         if not int4_group:
             return [(name, (k, n), "bf16")]
-        return [(name, (n, k // 2), "ui8"), (f"{name}_scale", (n, k // int4_group), "bf16")]
+        return [(name, (n, k // 2), "ui8"), (f"{name}_scale", (n, _groups(k, int4_group)), "bf16")]
 
     for n in range(layers):
         params += [(f"l{n}_norm1", (d_model,), "bf16"), *weight(f"l{n}_qkv", d_model, wide),

@@ -31,6 +31,23 @@ def test_one_product_fits_the_scratch(compile_client, rows, inner, columns, grou
     assert " tile=" in text and 0 < temp <= SCRATCH
 
 
+# ------------------------------------------------------------------------------------------------ groups that do not fit
+@pytest.mark.parametrize("inner, group", [(128, 48), (100, 33), (64, 128), (64, 3), (96, 0), (96, -32), (96, 1)])
+def test_modules_refuse_groups_that_rows_are_not_cut_into(inner, group):
+    # (128 values in groups of 48 would become a program with two groups of 64)
+    with pytest.raises(ValueError, match="groups"):
+        operators.int4_matmul_module(rows=2, inner=inner, columns=10, group=group)
+
+
+@pytest.mark.parametrize("what, size", [("int4_group", 96), ("int4_group", 31), ("int4_group", -32), ("ffn", 200), ("tree_words", -1)])
+def test_decoders_refuse_groups_that_rows_are_not_cut_into(what, size):
+    cfg = dict(tokens=4, sequences=2, vocab=64, layers=1, d_model=128, q_heads=2, kv_heads=1, head_dim=64, ffn=192, pages=2, page_size=16,
+               pages_per_sequence=1, int4_group=32)
+    operators.decoder_module(**cfg)
+    with pytest.raises(ValueError, match="groups|words"):
+        operators.decoder_module(**{**cfg, what: size})
+
+
 # ------------------------------------------------------------------------------------------------ beside other temporaries
 def beside(rows, inner, columns, group, other, dtype="bf16", product=True):
     """A product and a temporary of `other` f32 rows of 4096 beside it: a matrix product that another one reads. Or that alone."""
