@@ -135,9 +135,11 @@ def quantize_int4(weight: np.ndarray, group: int, zeros: bool = False) -> Tuple[
     """weight [N,K] in four bits: (values [N,K/2] for int4_matmul, scales [N,K/group], zeros [N,K/group]). Without `zeros`
     every zero is 8 and a group's largest magnitude is 7 steps; with them a group's range is 15 steps."""
     w = np.asarray(weight, dtype=np.float64)
-    if group < 2 or group % 2 or w.shape[1] % group:
-        raise ValueError(f"rows of {w.shape[1]} values are not cut into groups of {group}")
-    g = w.reshape(w.shape[0], -1, group)
+    if w.ndim != 2:
+        raise ValueError(f"a weight has rows and columns; this has the shape {w.shape}")
+    if not (np.abs(w) <= np.finfo(np.float32).max).all():
+        raise ValueError("int4 weights are of values that are finite in 32 bits")
+    g = w.reshape(w.shape[0], _groups(w.shape[1], group), group)
     if zeros:
         lo, hi = np.minimum(g.min(axis=-1), 0.0), np.maximum(g.max(axis=-1), 0.0)
         scale = (hi - lo) / 15

@@ -1,5 +1,6 @@
 """Plans of programs with int4_matmul and the workspace that they take, without a GPU: allocation-free executions have 64 MiB
 for all temporaries of a program."""
+import numpy as np
 import pytest
 
 from ryft_amd import operators, pjrt
@@ -46,6 +47,21 @@ def test_decoders_refuse_groups_that_rows_are_not_cut_into(what, size):
     operators.decoder_module(**cfg)
     with pytest.raises(ValueError, match="groups|words"):
         operators.decoder_module(**{**cfg, what: size})
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 1e40])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantize_refuses_what_is_not_finite(zeros, bad):
+    w = np.ones((2, 8))
+    w[1, 3] = bad
+    with pytest.raises(ValueError, match="finite"):
+        operators.quantize_int4(w, 4, zeros)
+
+
+def test_quantize_refuses_what_is_no_matrix():
+    for w in (np.ones(8), np.ones((2, 2, 8))):
+        with pytest.raises(ValueError):
+            operators.quantize_int4(w, 4)
 
 
 # ------------------------------------------------------------------------------------------------ beside other temporaries
