@@ -25,8 +25,9 @@ are one of bf16, f16, f32):
 * ``ryft.tree_attention`` (q, k_cache, v_cache, page_table, starts, lengths as above, visible [T,W] i32) → o [T,Hq,D].
   Sequence b's queries are a tree of drafted tokens, whose keys and values are the last of its lengths[b] positions, node j
   at the j-th of them. A query sees every position before those, or, if `window` > 0, the last `window` up to its own place
-  in the text (as many places behind the first drafted token as its row of `visible` has bits, less one); of the tree it
-  sees node j where bit j % 32 of word j / 32 of its row is set (its ancestors and itself; nodes past 32 · W are not seen).
+  in the text (as many places behind the first drafted token as it sees nodes of the tree, less one); of the tree it sees
+  node j where bit j % 32 of word j / 32 of its row is set (its ancestors and itself; nodes past 32 · W are not seen, and
+  bits past the tree's last node stand for nothing).
   `scale`, `softcap`, pages outside the cache and queries that see nothing as in paged_attention.
 * ``ryft.tree_accept`` (tokens, parents, targets, slots [T] i32, starts [B+1] i32, any number of caches up to 256, all
   [pages,Hkv,page_size,D]) → (counts [B] i32, emitted, path [T] i32, the caches). Sequence b's rows are a tree: the first

@@ -235,6 +235,21 @@ def test_tree_attention_of_any_starts(gpu_client, starts, tokens, heads, dtype):
     assert not got[~want.any(axis=(1, 2))].any()
 
 
+@pytest.mark.parametrize("nodes, heads, dtype", [([5, 3], (2, 2, 64), "bf16"), ([40, 70], (4, 2, 128), "f16"), ([20, 9], (2, 1, 64), "f32")],
+                         ids=str)
+def test_bits_past_the_last_node_stand_for_nothing(gpu_client, nodes, heads, dtype):
+    # neither keys nor, under a window, a query's place in the text
+    module, ins = vp.tree_case(nodes, [n + 200 for n in nodes], *heads, 16, dtype, words=4, window=60, seed=sum(nodes))
+    (want,), _ = run(gpu_client, module, ins, [dtype])
+    bits = vp.values(ins)[6]
+    past = np.concatenate([np.broadcast_to([sum(1 << j for j in range(32) if 32 * w + j >= n) for w in range(4)], (n, 4)) for n in nodes])
+    ins[6] = op.host((bits.astype(np.int64) & 0xffffffff | past).astype(np.uint32).view(np.int32), "i32")
+    (got,), _ = run(gpu_client, module, ins, [dtype])
+    assert (vp.values(ins)[6] != bits).any() and want.any() and np.array_equal(got, want)
+    oracle, = oo.tree_attention(vp.values(ins), op.config_of(module))
+    close(got, oracle, dtype, attention_error(vp.values(ins), dtype), "y")
+
+
 # ------------------------------------------------------------------------------------------------ the longest rows
 @pytest.mark.parametrize("rows, inner, columns, group", [(40, 1 << 20, 20, 128), (33, (1 << 20) + 2080, 7, 32)])
 def test_int4_matmul_of_long_rows(gpu_client, rows, inner, columns, group):
