@@ -435,12 +435,12 @@ struct SampleArgs {
 // w[n, k] is the low (k even) or high nibble of byte k / 2 of row n, group g the G values from g · G on, and zero 8 where
 // there is none. Sums in f32, rounded once; one that is not finite in f32 is summed again in 64 bits.
 struct Int4Args {
-  const void* x;        // [T, K], unit stride along K
+  const void* x;        // [T, K]
   const uint8_t* w;     // [N, K / 2]
   const void* scale;    // [N, K / G]
   const uint8_t* zero;  // [N, K / G] or null
   void* y;              // [T, N] row-major
-  int64_t T, K, N, xs;  // xs: elements from one row of x to the next
+  int64_t T, K, N;
   int32_t G;
   int32_t x_dtype, scale_dtype, y_dtype;
   // set by int4_matmul_plan: the kernel and its split

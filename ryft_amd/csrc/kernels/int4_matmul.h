@@ -93,7 +93,7 @@ __device__ __forceinline__ bool int4_finite(float v) { return (__float_as_uint(v
 // y[t, n] from its definition, eight values a lane at a time; `nan`: whether row t of x has a NaN, of which every result is NaN.
 template <class X>
 __device__ __forceinline__ float int4_again(const Int4Args& A, int64_t t, int64_t n, bool& nan) {
-  const uint16_t* const x = (const uint16_t*)A.x + t * A.xs;
+  const uint16_t* const x = (const uint16_t*)A.x + t * A.K;
   const uint32_t* const w = (const uint32_t*)(A.w + n * (A.K / 2));
   const int64_t g0 = n * A.groups;
   double sum = 0;

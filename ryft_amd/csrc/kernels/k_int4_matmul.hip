@@ -32,8 +32,8 @@ __device__ __forceinline__ float any_again(const Int4Args& A, int64_t t, int64_t
     const int64_t g = n * ((uint32_t)A.K / (uint32_t)A.G) + 2 * j / (uint32_t)A.G;
     const double s = read_any(A.scale, g, A.scale_dtype);
     const int z = A.zero ? A.zero[g] : 8, b = A.w[n * (A.K / 2) + j];
-    sum = __builtin_fma(s * (double)((b & 15) - z), (double)read_any(A.x, t * A.xs + 2 * j, A.x_dtype), sum);
-    sum = __builtin_fma(s * (double)((b >> 4) - z), (double)read_any(A.x, t * A.xs + 2 * j + 1, A.x_dtype), sum);
+    sum = __builtin_fma(s * (double)((b & 15) - z), (double)read_any(A.x, t * A.K + 2 * j, A.x_dtype), sum);
+    sum = __builtin_fma(s * (double)((b >> 4) - z), (double)read_any(A.x, t * A.K + 2 * j + 1, A.x_dtype), sum);
   }
   for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m, 64);
   return (float)sum;
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) int4_matmul_any_kernel(const Int4Args A) 
 #pragma unroll
       for (int r = 0; r < ANY_ROWS; ++r)
         if (t0 + r < A.T) {
-          const int64_t at = (t0 + r) * A.xs + 2 * j;
+          const int64_t at = (t0 + r) * A.K + 2 * j;
           acc[r] = __builtin_fmaf(w0, read_any(A.x, at, A.x_dtype), acc[r]);
           acc[r] = __builtin_fmaf(w1, read_any(A.x, at + 1, A.x_dtype), acc[r]);
         }
@@ -167,11 +167,11 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
   const int tiles = (N + 15) / 16;
 
   const int es = A.scale_dtype == DT_F32 ? 4 : 2;
-  const __amdgpu_buffer_rsrc_t xb = int4_buffer(A.x, A.T * A.xs * 2);
+  const __amdgpu_buffer_rsrc_t xb = int4_buffer(A.x, A.T * A.K * 2);
   uint32_t x_row[XL];  // position c of row r holds chunk c ^ (r mod 8)
 #pragma unroll
   for (int h = 0; h < XL; ++h)
-    x_row[h] = (uint32_t)min(2 * h + (lane >> 5), T - 1) * (uint32_t)(2 * A.xs) + 16 * ((lane & 31) ^ ((2 * h + (lane >> 5)) & 7));
+    x_row[h] = (uint32_t)min(2 * h + (lane >> 5), T - 1) * (uint32_t)(2 * A.K) + 16 * ((lane & 31) ^ ((2 * h + (lane >> 5)) & 7));
   const int w_chunk = (lane & 7) ^ (lane >> 3);
   char* const ring = smem + wave * (C::DEPTH * C::SLOT);
   const uint32_t ring_at = (uint32_t)(uintptr_t)(few_lds*)ring;
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
       for (int at = 0; at < 8; ++at) {
         const int k = (wave + W * s) * FEW_STEP + 32 * at + 8 * g16;
         x_own[s][at] = u32x4p{0u, 0u, 0u, 0u};
-        if (k < K) x_own[s][at] = *(const u32x4p*)((const uint16_t*)A.x + (int64_t)min(l16, T - 1) * A.xs + k);
+        if (k < K) x_own[s][at] = *(const u32x4p*)((const uint16_t*)A.x + (int64_t)min(l16, T - 1) * A.K + k);
       }
   }
   auto multiply = [&](int step, int slot, const u32x4p (&xo)[8], const f32x4p (&xs)[SPANS]) {
@@ -467,7 +467,7 @@ void launch_few_of(const Int4Args& a, hipStream_t stream, hipEvent_t done) {
   const int ys = a.y_dtype == DT_F32 ? 4 : 2;
   for (int64_t t0 = 0; t0 < a.T; t0 += 16) {
     Int4Args b = a;
-    b.x = (const char*)a.x + t0 * a.xs * 2;
+    b.x = (const char*)a.x + t0 * a.K * 2;
     b.y = (char*)a.y + t0 * a.N * ys;
     b.T = std::min<int64_t>(16, a.T - t0);
     launch_k(t0 + 16 >= a.T ? done : nullptr, int4_few_kernel<X, SPAN, XL, S>, grid, dim3(64 * C::W), C::LDS, stream, b);

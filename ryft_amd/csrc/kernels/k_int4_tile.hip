@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(const Int4Args A, int
   if (t >= rows) return;  // (whole groups of 16 lanes)
   const int64_t st = (int64_t)stage * rows + t;
   u32x4p v = {0, 0, 0, 0};
-  if (k < K) v = *(const u32x4p*)((const uint16_t*)A.x + (t0 + t) * A.xs + k);
+  if (k < K) v = *(const u32x4p*)((const uint16_t*)A.x + (t0 + t) * A.K + k);
   float sum = 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) sum += X::lo(v[e]) + X::hi(v[e]);

@@ -239,6 +239,38 @@ struct PagedTile {
   int hk, row0;   // key head, first flat row
 };
 
+// Partial results move between workgroups of one launch past the XCDs' L2s (agent scope: sc1).
+constexpr int kAgent = 16;
+typedef uint32_t u32x4w __attribute__((__vector_size__(16)));
+typedef uint32_t u32x2w __attribute__((__vector_size__(8)));
+__device__ __forceinline__ void agent_put4(__amdgpu_buffer_rsrc_t r, uint32_t byte, f32x4p v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4w, v), r, (int)byte, 0, kAgent);
+}
+__device__ __forceinline__ f32x4p agent_get4(__amdgpu_buffer_rsrc_t r, uint32_t byte) {
+  return __builtin_bit_cast(f32x4p, __builtin_amdgcn_raw_buffer_load_b128(r, (int)byte, 0, kAgent));
+}
+__device__ __forceinline__ void agent_put2(__amdgpu_buffer_rsrc_t r, uint32_t byte, float x, float y) {
+  __builtin_amdgcn_raw_buffer_store_b64(u32x2w{__float_as_uint(x), __float_as_uint(y)}, r, (int)byte, 0, kAgent);
+}
+__device__ __forceinline__ float2 agent_get2(__amdgpu_buffer_rsrc_t r, uint32_t byte) {
+  const u32x2w v = __builtin_amdgcn_raw_buffer_load_b64(r, (int)byte, 0, kAgent);
+  return float2{__uint_as_float(v[0]), __uint_as_float(v[1])};
+}
+
+// Whether this workgroup is the last of `parts` to arrive at a counter, once all its own stores are complete. Every
+// thread calls it; `last`: a word of LDS. The counter is back at zero when the last has arrived.
+__device__ __forceinline__ bool last_to_arrive(int32_t* counter, int parts, int* last) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int arrived = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+    if (arrived == parts) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *last = arrived == parts;
+  }
+  __syncthreads();
+  return *(volatile int*)last != 0;
+}
+
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t paged_ws(const PagedAttnArgs& A) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)A.ws, (short)0, -1, 0x00020000);
 }

@@ -1010,7 +1010,7 @@ void Planner::emit_custom_call(int node, int target) {
     Int4Args& a = st.int4;
     const TensorType &x = type(0), &w = type(1), &s = type(2), &y = g_.nodes[res[0]].type;
     a.T = x.shape[0];
-    a.K = a.xs = x.shape[1];
+    a.K = x.shape[1];
     a.N = w.shape[0];
     a.G = (int32_t)(a.K / s.shape[1]);
     a.x_dtype = (int32_t)x.dtype;
