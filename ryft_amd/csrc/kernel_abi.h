@@ -386,7 +386,6 @@ struct PagedAttnArgs {
   const int32_t* starts;  // [B + 1]
   const int32_t* lengths; // [B]
   const float* slopes;    // [Hq] or null
-  const uint32_t* visible;  // [T, W] or null
   void* o;                // [T, Hq, D] row-major
   int64_t T, pages;
   int64_t qs[2];          // element strides of (token, head)
@@ -404,6 +403,7 @@ struct PagedAttnArgs {
   uint64_t page_mul;
   float* ws;              // partial results; every one that is read was written by the same launch
   int32_t* counters;      // arrivals, one a tile: zero between launches
+  const uint32_t* visible;  // [T, W] or null
 };
 
 // ryft.sample (k_sample.hip): for each row of logits [B, V], in 64 bits, w_i = exp((x_i - max x) / temperature); of the

@@ -18,8 +18,10 @@ namespace ryft {
 
 namespace {
 
-// Any type and head dim up to 256: a workgroup a query and head.
-template <class E>
+// Any type and head dim up to 256: a workgroup a query and head. TREE: the queries are a tree of drafted tokens
+// (PagedAttnArgs::visible); asked of each key at run time that took 1 to 2% (2 x 500 queries of 16 heads of 64 in f32: 273 to 279
+// us), so every kernel is made for either.
+template <class E, bool TREE>
 __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAttnArgs A) {
   __shared__ PagedRowLds sh;
   const int64_t t = blockIdx.x;
@@ -37,7 +39,7 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAtt
     const int len = paged_length(A, b);
     pos = len - (paged_start(A, b + 1) - (int)t);
     last = A.causal ? min(len, pos + 1) : len;
-    if (A.visible) {
+    if (TREE) {
       const int n = paged_start(A, b + 1) - paged_start(A, b);
       pos = len - n;
       first = tree_first(A, t, n, pos);
@@ -46,7 +48,7 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedAtt
     }
   }
   float m, l;
-  const float x = paged_row<E>(A, b, t, h, pos, first, last, sh, &m, &l);
+  const float x = paged_row<E, TREE>(A, b, t, h, pos, first, last, sh, &m, &l);
   if (tid < D) ((typename E::raw*)A.o)[(t * A.Hq + h) * D + tid] = E::put(l == 0.f ? 0.f : x / l);
 }
 
@@ -173,7 +175,6 @@ struct FewPart {
   int rows, w0, parts, index;
 };
 
-// TREE: the queries are a tree of drafted tokens (PagedAttnArgs::visible).
 template <class X, class E, int D, bool TREE>
 __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const PagedAttnArgs A) {
   typedef FewCfg<D> C;
@@ -383,7 +384,6 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
       const int kb = kstart + j * C::UNIT;
       const bool more = j + 1 < blocks;
       const uint64_t bad_now = bad;
-      const bool mask = kb + C::KB - 1 > all_hi || kb < all_lo;
       uint64_t vis = ~(uint64_t)0;
       if constexpr (TREE) {
         if (kb + C::KB - 1 > all_hi && l16 < rows) vis = tree_bits(A, t.s0 + qi, kb - t.pos0);
@@ -406,6 +406,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
         locate(kb + C::UNIT);
         fetch(A.k_cache, 0);
       }
+      const bool mask = kb + C::KB - 1 > all_hi || kb < all_lo;
       uint32_t pf[C::KT * 2], pr[C::KT * 2];  // probabilities: rounded, and what that leaves of them
       if (score.cap2 > 0.f) {
         auto at = [&](int i) -> float& { return ((float*)st)[i]; };
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(256, 2) paged_attention_few_kernel(const Paged
                                 (int64_t)(TREE ? tree_first(A, t.s0 + qi, t.n, t.pos0) : first_key(t, qi)));
       const int64_t last = min((int64_t)cur.kfirst + (int64_t)cur.u1 * C::UNIT, (int64_t)last_key(t, qi) + 1);
       float rm, rl;
-      const float v = paged_row<E>(A, t.b, t.s0 + qi, t.hk * G + (flat - qi * G), TREE ? t.pos0 : t.pos0 + qi, (int)first, (int)max(last, (int64_t)0),
+      const float v = paged_row<E, TREE>(A, t.b, t.s0 + qi, t.hk * G + (flat - qi * G), TREE ? t.pos0 : t.pos0 + qi, (int)first, (int)max(last, (int64_t)0),
                                    *(PagedRowLds*)so, &rm, &rl);
       float* const one = so + sizeof(PagedRowLds) / 4;
       if (tid < D) one[tid] = v;
@@ -670,7 +671,8 @@ void launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream, hipEvent
     else launch_matrix<MmaF16, ElemF16>(a, stream, done);
   } else {
     with_elem(a.dtype, [&](auto e) {
-      launch_k(done, paged_attention_any_kernel<decltype(e)>, dim3((unsigned)a.T, (unsigned)a.Hq), dim3(256), 0, stream, a);
+      const auto kernel = a.visible ? paged_attention_any_kernel<decltype(e), true> : paged_attention_any_kernel<decltype(e), false>;
+      launch_k(done, kernel, dim3((unsigned)a.T, (unsigned)a.Hq), dim3(256), 0, stream, a);
     });
   }
   const hipError_t e = hipGetLastError();

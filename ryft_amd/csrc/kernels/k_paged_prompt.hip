@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(256, prompt_shares(D)) paged_prompt_kernel(con
       const int f = t.row0 + row, q = f / G;
       const int k0 = max(TREE ? tree_first(A, t.s0 + q, t.n, t.pos0) : first_key(q), j0 * BKV), k1 = min(last_key(q) + 1, j1 * BKV);
       float rm, rl;
-      const float v = paged_row<E>(A, t.b, t.s0 + q, t.hk * G + (f - q * G), TREE ? t.pos0 : t.pos0 + q, k0, max(k1, 0), row_lds, &rm, &rl);
+      const float v = paged_row<E, TREE>(A, t.b, t.s0 + q, t.hk * G + (f - q * G), TREE ? t.pos0 : t.pos0 + q, k0, max(k1, 0), row_lds, &rm, &rl);
       if (tid < D) so[row * C::OP + tid] = v;
       if (tid == 0) row_ml[row][0] = rm, row_ml[row][1] = rl;
       __syncthreads();

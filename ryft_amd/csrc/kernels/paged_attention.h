@@ -163,7 +163,7 @@ struct PagedRowLds {
   float q[256];
   float part[4][256 + 2];
 };
-template <class E>
+template <class E, bool TREE>
 __device__ __forceinline__ float paged_row(const PagedAttnArgs& A, int b, int64_t t, int h, int pos, int first, int last,
                                            PagedRowLds& sh, float* m_out, float* l_out) {
   typedef typename E::raw raw;
@@ -180,7 +180,7 @@ __device__ __forceinline__ float paged_row(const PagedAttnArgs& A, int b, int64_
     const int key = k0 + wave * 64 + lane;
     float s = -INFINITY;
     int64_t at = -1;
-    if (key < last && (!A.visible || key < pos || (tree_bits(A, t, key - pos) & 1))) {
+    if (key < last && (!TREE || key < pos || (tree_bits(A, t, key - pos) & 1))) {
       const int pi = page_of(A, key);
       const int page = A.table[(int64_t)b * A.M + pi];
       if (page >= 0 && page < A.pages) {
