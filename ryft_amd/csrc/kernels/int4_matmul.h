@@ -86,8 +86,9 @@ __device__ __forceinline__ void int4_range(const Int4Args& A, int part, int& lo,
 
 // Results that are not finite, summed again by a wavefront in 64 bits. The sums above carry 16 + q and 16 + z: an infinity of x is
 // in both of them, and they may pass f32's range where the result does not (x from 2^112 on). What that leaves is infinite or NaN
-// to the end, so that finite results need nothing more than the look at them (16 rows against 28672 x 4096: 20.4 us for 20.0; 2048
-// against 12288 x 4096: 224 for 223). With a NaN in every row the two take 91 us and 1.9 ms, with an infinity 1.5 and 70 ms.
+// to the end, so that finite results need nothing more than the look at them, a product with 0 each (16 rows against 28672 x 4096:
+// 20.0 us with and without; 2048 against 12288 x 4096: 221.5 and 220). With a NaN in every row the two take 0.1 and 2 ms, with an
+// infinity 1.6 and 58 ms, with an infinity in one row 0.14 and 3.6 ms.
 __device__ __forceinline__ bool int4_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
 // y[t, n] from its definition, eight values a lane at a time; `nan`: whether row t of x has a NaN, of which every result is NaN.
@@ -134,6 +135,14 @@ __device__ __forceinline__ float int4_mend(const Int4Args& A, bool bad, int64_t 
     todo &= todo - 1;
   }
   return v;
+}
+
+// The kernel's first argument, read again: so that what the seldom taken way needs of it is not kept in registers on the other
+// (16 rows against 28672 x 4096: 20.4 us where it was).
+__device__ __forceinline__ const Int4Args& int4_args_again() {
+  const void* p = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Int4Args*)p;
 }
 
 // The same for y[t, n] where it lies, by the lane that has written it: at the end of a kernel, for registers that are free there.

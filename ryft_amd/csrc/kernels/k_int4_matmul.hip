@@ -388,7 +388,7 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
     }
   }
   int turn = 0;
-  uint64_t odd = 0;  // whether a sum of the tiles that this wavefront has finished is not finite
+  float odd = 0.f;  // NaN where a sum of the tiles that this wavefront has finished is not finite (in a vector register: those are left)
   auto forward = [&]() {  // has the next step loaded and waits for the oldest
     if (ahead.tile < tiles) {
       fetch(to);
@@ -438,7 +438,8 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
       for (int j = 0; j < 4; ++j) sum += v[j];
     }
     const int n = tile * 16 + l16;
-    odd |= __ballot(!int4_finite(sum[0]) || !int4_finite(sum[1]) || !int4_finite(sum[2]) || !int4_finite(sum[3]));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) odd = __builtin_fmaf(sum[r], 0.f, odd);
     if (n >= N) continue;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -448,13 +449,14 @@ __global__ void __launch_bounds__((64 * FewCfg<SPAN, XL, S>::W), 2) int4_few_ker
       else ((uint16_t*)A.y)[(int64_t)t * N + n] = X::put(sum[r]);
     }
   }
-  if (!odd) return;
+  if (!__any(odd != odd)) return;
+  const Int4Args& B = int4_args_again();
   turn = 0;
 #pragma unroll 1
-  for (int tile = blockIdx.x; tile < tiles; tile += (int)gridDim.x, ++turn) {
+  for (int64_t n0 = (int64_t)blockIdx.x * 16; n0 < B.N; n0 += (int64_t)gridDim.x * 16, ++turn) {
     if (wave != turn % W) continue;
 #pragma unroll 1
-    for (int t = 4 * g16; t < 4 * g16 + 4; ++t) int4_mend_stored<X>(A, t < T && tile * 16 + l16 < N, t, tile * 16 + l16);
+    for (int t = 4 * g16; t < 4 * g16 + 4; ++t) int4_mend_stored<X>(B, t < B.T && n0 + l16 < B.N, t, n0 + l16);
   }
 }
 

@@ -335,26 +335,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
   char* const out = whole ? (char*)A.y + (t_base + t0) * A.N * ys
                           : (char*)A.ws + tile_ws_bytes(A.steps, x_rows, SPAN) + (part * part_floats(x_rows * A.N) + t0 * A.N) * 4;
   float* const rows_at = (float*)smem;
+  float odd = 0.f;  // NaN where a value that this thread stores is not finite
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int t_here = min(32, x_rows - t0 - 32 * m);
-    bool odd = false;
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      rows_at[(8 * (e >> 2) + 4 * half + (e & 3)) * C::YP + 32 * wave + l32] = y[m][e];
-      odd |= !int4_finite(y[m][e]);
-    }
-    if (whole && __any(odd)) {
-      // (two rows of the wavefront's own columns at a time; parts are looked at when they are added)
-#pragma unroll 1
-      for (int r = half; r < 32; r += 2) {
-        float* const at = rows_at + r * C::YP + 32 * wave + l32;
-        const int c = 32 * wave + l32;
-        *at = int4_mend<X>(A, !int4_finite(*at) && r < t_here && c < n_here, t_base + t0 + 32 * m + r, n0 + c, *at);
-      }
-    }
+    for (int e = 0; e < 16; ++e) rows_at[(8 * (e >> 2) + 4 * half + (e & 3)) * C::YP + 32 * wave + l32] = y[m][e];
     __syncthreads();
+    const int t_here = min(32, x_rows - t0 - 32 * m);
     char* const to = out + ((int64_t)32 * m * A.N + n0) * ys;
     if (wide) {
       const int chunks = BN / per;
@@ -363,10 +351,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
         if (r >= t_here || c >= n_here) continue;
         const f32x4p a = *(const f32x4p*)(rows_at + r * C::YP + c);
         char* const at = to + ((int64_t)r * A.N + c) * ys;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd = __builtin_fmaf(a[e], 0.f, odd);
         if (ys == 4) {
           *(f32x4p*)at = a;
         } else {
           const f32x4p b = *(const f32x4p*)(rows_at + r * C::YP + c + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd = __builtin_fmaf(b[e], 0.f, odd);
           *(u32x4p*)at = u32x4p{X::put(a[0]) | (uint32_t)X::put(a[1]) << 16, X::put(a[2]) | (uint32_t)X::put(a[3]) << 16,
                                 X::put(b[0]) | (uint32_t)X::put(b[1]) << 16, X::put(b[2]) | (uint32_t)X::put(b[3]) << 16};
         }
@@ -377,17 +369,27 @@ __global__ void __launch_bounds__(64 * WAVES, 2) int4_tile_kernel(const Int4Args
         if (r >= t_here || c >= n_here) continue;
         const float v = rows_at[r * C::YP + c];
         char* const at = to + ((int64_t)r * A.N + c) * ys;
+        odd = __builtin_fmaf(v, 0.f, odd);
         if (ys == 4) *(float*)at = v;
         else *(uint16_t*)at = X::put(v);
       }
     }
+  }
+  if (!whole || !__any(odd != odd)) return;  // (parts are looked at when they are added)
+  const Int4Args& B = int4_args_again();
+  const int each = wide ? per : 1, chunks = BN / each;
+#pragma unroll 1
+  for (int i = tid; i < C::BM * chunks; i += 64 * WAVES) {  // what this thread has stored; the wavefront together
+    const int r = i / chunks, c = (i - r * chunks) * each;
+#pragma unroll 1
+    for (int e = 0; e < each; ++e) int4_mend_stored<X>(B, t0 + r < x_rows && c + e < n_here, t_base + t0 + r, n0 + c + e);
   }
 }
 
 // Adds the parts of `count` elements, in their order, from `parts` (of the workspace, part_floats() apart) into y from element
 // `at` on, a multiple of four: four elements a thread.
 template <class X>
-__global__ void __launch_bounds__(256) int4_join_kernel(const Int4Args A, const float* parts, int64_t at, int64_t count) {
+__global__ void __launch_bounds__(256, 6) int4_join_kernel(const Int4Args A, const float* parts, int64_t at, int64_t count) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i - 4 * (threadIdx.x & 63) >= count) return;  // (whole wavefronts)
   f32x4p v = {0.f, 0.f, 0.f, 0.f};
