@@ -205,7 +205,8 @@ void check_tree_accept(const Call& c, std::map<std::string, double>*) {
   c.rank("tokens", tok, 1);
   c.rank("starts", st, 1);
   const int64_t T = tok.shape[0], B = st.shape[0] - 1;
-  if (B < 0 || B > (1 << 20) || T > INT32_MAX) c.bad("too many tokens or sequences, or no starts");
+  // (the kernel counts nodes in 32 bits, a workgroup's 256 at a time)
+  if (B < 0 || B > (1 << 20) || T > (1 << 30)) c.bad("too many tokens or sequences, or no starts");
   const char* names[] = {"tokens", "parents", "targets", "slots"};
   for (int i = 0; i < 4; ++i) c.is(names[i], c.operand(i), DType::S32, {T});
   c.is("starts", st, DType::S32, {B + 1});

@@ -37,7 +37,7 @@ are one of bf16, f16, f32):
   first counts[b] rows of emitted and path are the targets along it, the sequence's next tokens, and its nodes; the other
   rows are -1. In each cache the j-th node of the path moves from its slot to that of node j, so that the sequence's
   positions continue with the path; slots of a call are distinct, one outside the cache is neither read nor written.
-  starts do not decrease.
+  starts do not decrease. At most 2^30 tokens.
 * ``ryft.int4_matmul`` (x [T,K], weight [N,K/2] ui8, scale [N,K/G] (, zero [N,K/G] ui8)) → y [T,N]. Value k of a row of
   the weight is the low (k even) or high four bits of its byte k / 2, less its group's zero (8 without the operand), times
   its group's scale; groups are G consecutive values, G even. y = x · weightᵀ, summed in 32 bits, in 64 where that is not

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from ryft_amd import operators, pjrt
+from tests.test_operators import INVALID, refused
 
 SCRATCH = 64 << 20
 
@@ -62,6 +63,16 @@ def test_quantize_refuses_what_is_no_matrix():
     for w in (np.ones(8), np.ones((2, 2, 8))):
         with pytest.raises(ValueError):
             operators.quantize_int4(w, 4)
+
+
+# ------------------------------------------------------------------------------------------------ trees that are too large
+def test_tree_accept_refuses_trees_that_steps_of_a_workgroup_would_leave(compile_client):
+    # nodes are counted in 32 bits, 256 at a time: a tree of 2^31 - 1 would be counted past that
+    most = 1 << 30
+    text, _ = planned(compile_client, operators.tree_accept_module(tokens=most, sequences=1))
+    assert f"tokens={most}" in text
+    for tokens in (most + 1, (1 << 31) - 1):
+        refused(compile_client, operators.tree_accept_module(tokens=tokens, sequences=1), INVALID, "too many tokens")
 
 
 # ------------------------------------------------------------------------------------------------ beside other temporaries
