@@ -10,6 +10,7 @@ import pytest
 import torch  # (before the plugin: both then use one HIP runtime)
 
 from oracle import operators as oo
+from oracle import stablehlo as sh
 from ryft_amd import operators, pjrt
 from tests import operator_programs as op
 from tests import verify_programs as vp
@@ -117,6 +118,56 @@ def test_int4_matmul_of_scales_that_are_not_finite(gpu_client, name):
     odd = ~np.isfinite(x[2]).all(axis=1)
     assert odd.sum() == 3 and np.array_equal(got[:, odd], want[:, odd], equal_nan=True)
     close(got[:, ~odd], want[:, ~odd], "f32", vp.int4_error([x[0], x[1][~odd], x[2][~odd]]), "others")
+
+
+@pytest.mark.parametrize("rows, inner, columns, group", [(1400, 13248, 6144, 64), (300, 32768, 70, 128), (40, 1 << 20, 20, 128)], ids=str)
+def test_int4_matmul_of_infinities_in_later_goes(gpu_client, rows, inner, columns, group):
+    # rows that are prepared, or multiplied, in several goes: results that are summed again are those of their own rows
+    module, ins = vp.int4_case(rows, inner, columns, group, "bf16", zeros=True, out_dtype="f32", seed=rows)
+    raw = np.array(ins[0].data).reshape(rows, inner)
+    some = [0, rows // 2 - 1, rows // 2, rows - 2, rows - 1]
+    for n, t in enumerate(some[1:4]):
+        raw[t, 11 * n], raw[t, inner - 1 - n] = (0x7F80, 0xFF80, 0x7FC0)[n], 0x7F80  # (inf, -inf, NaN; inf)
+    ins[0] = type(ins[0])(raw, ins[0].type, ins[0].dims)
+    given = [torch.from_numpy(np.array(i.data).view(np.int16 if i.data.dtype == np.uint16 else i.data.dtype)).cuda() for i in ins]
+    y = torch.full((rows, columns), 7.0, device="cuda")
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    exe.execute_into([(g.data_ptr(), g.nbytes) for g in given], [(y.data_ptr(), y.nbytes)], torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    got = y[some].double().cpu().numpy()
+    x = [sh.from_raw(raw[some], "bf16")] + vp.values(ins[1:])
+    want = definition(x)
+    assert np.array_equal(got[1:4], want[1:4], equal_nan=True) and not np.isfinite(want[1:4]).any()
+    close(got[[0, 4]], want[[0, 4]], "f32", vp.int4_error([x[0][[0, 4]], *x[1:]]), "others")
+    assert int((~torch.isfinite(y)).any(dim=1).sum()) == 3
+
+
+@pytest.mark.parametrize("name", ["one", "registers", "tile", "parts", "f32"])
+def test_int4_matmul_of_infinities_in_a_replayed_graph(gpu_client, name):
+    # the inputs change between replays: finite, with infinities and NaN, and finite again
+    rows, inner, columns, group, dtype = PATHS[name]
+    module, ins = vp.int4_case(rows, inner, columns, group, dtype, out_dtype="f32", seed=4)
+    given = [torch.from_numpy(np.array(i.data).view(np.int16 if i.data.dtype == np.uint16 else i.data.dtype)).cuda() for i in ins]
+    y = torch.full((rows, columns), 7.0, device="cuda")
+    exe = gpu_client.compile(pjrt.Program.mlir(module))
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        exe.execute_into([(g.data_ptr(), g.nbytes) for g in given], [(y.data_ptr(), y.nbytes)], torch.cuda.current_stream().cuda_stream)
+    x = vp.values(ins)
+    odd = x[0].copy()
+    odd[rows - 1, 5], odd[0, inner - 1] = np.inf, -np.inf
+    if rows > 2:
+        odd[1, 9] = np.nan
+    for now in (x[0], odd, x[0], odd):
+        raw = op.host(now, dtype)
+        given[0].copy_(torch.from_numpy(np.array(raw.data).view(np.int16) if dtype != "f32" else np.array(raw.data)).reshape(given[0].shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        got, want = y.double().cpu().numpy(), definition([now, *x[1:]])
+        some = np.isfinite(now).all(axis=1)
+        assert np.array_equal(got[~some], want[~some], equal_nan=True)
+        close(got[some], want[some], "f32", vp.int4_error([now[some], *x[1:]]), name)
 
 
 # ------------------------------------------------------------------------------------------------ no tokens
