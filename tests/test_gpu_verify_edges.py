@@ -170,6 +170,15 @@ def test_int4_matmul_of_infinities_in_a_replayed_graph(gpu_client, name):
         close(got[some], want[some], "f32", vp.int4_error([now[some], *x[1:]]), name)
 
 
+@pytest.mark.parametrize("rows, inner, columns, group, dtype", [(250_001, 64, 33, 32, "bf16"), (110_000, 32, 300, 32, "f16"), (70_003, 2, 5, 2, "f32"),
+                                                                (600_000, 48, 3, 48, "bf16")], ids=str)
+def test_int4_matmul_of_many_rows(gpu_client, rows, inner, columns, group, dtype):
+    # in several goes, and past the number of workgroups that one axis of a grid has; as exact as whole numbers are
+    module, ins = vp.int4_case(rows, inner, columns, group, dtype, zeros=True, out_dtype="f32", exact=True, seed=rows)
+    (got,), _ = run(gpu_client, module, ins, ["f32"])
+    assert np.array_equal(got, oo.int4_matmul(vp.values(ins), {})[0])
+
+
 # ------------------------------------------------------------------------------------------------ no tokens
 def empty_modules():
     tree = operators.tree_attention_module(tokens=0, sequences=3, q_heads=4, kv_heads=2, head_dim=64, pages=5, page_size=16,
@@ -299,6 +308,19 @@ def test_bits_past_the_last_node_stand_for_nothing(gpu_client, nodes, heads, dty
     assert (vp.values(ins)[6] != bits).any() and want.any() and np.array_equal(got, want)
     oracle, = oo.tree_attention(vp.values(ins), op.config_of(module))
     close(got, oracle, dtype, attention_error(vp.values(ins), dtype), "y")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("masks, window", [("tree", 0), ("tree", 40), ("random", 900)])
+def test_tree_attention_of_large_trees(gpu_client, masks, window, dtype):
+    # trees of many words, larger than the window, most of a sequence, or all of it
+    nodes = [1100, 700, 33]
+    module, ins = vp.tree_case(nodes, [1300, 700, 900], 2, 1, 64, 16, dtype, masks=masks, window=window, seed=window + 5)
+    (got,), _ = run(gpu_client, module, ins, [dtype])
+    x = vp.values(ins)
+    want, = oo.tree_attention(x, op.config_of(module))
+    close(got, want, dtype, attention_error(x, dtype), masks)
+    assert not got[~want.any(axis=(1, 2))].any()
 
 
 # ------------------------------------------------------------------------------------------------ the longest rows
